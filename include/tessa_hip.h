@@ -931,6 +931,128 @@ tessa_status tessa_probe_mfma_rate(uint32_t workgroups, uint32_t chains, uint64_
 void tessa_overflow_labels(uint64_t flags, char *buf, size_t len);
 uint32_t tessa_abi_version(void);
 
+/* ---- paged key-value cache: attention over rows that a search finds --------
+ * A cache holds keys and values in pages of page_rows rows (a power of two);
+ * row j of sequence b lies in page table[b][j / page_rows], slot j % page_rows.
+ * A row is head_dim values (a multiple of 16, at most 256) for each of `heads`
+ * heads: bf16, fp16, or SQ8 codes with one f32 scale (value = scale * code, scale
+ * = max|x| * (1/127), code = x / scale rounded half away from zero).  Strides are between pages, heads and rows, in
+ * elements; rows are contiguous and 16-byte aligned.  Nothing here allocates,
+ * waits for the device or keeps anything between calls: results are queued on
+ * `stream`, scratch is the caller's, and the calls may be captured in a graph.
+ *
+ * No counterpart in the reference: its search ends with the ids
+ * (tessa_graph_search); these operators attend over the rows that they name. */
+enum tessa_kv_type { TESSA_KV_BF16 = 1, TESSA_KV_F16 = 2, TESSA_KV_SQ8 = 3 };
+#define TESSA_KV_ALL 0xffffffffu /* tessa_kv_attend.window: every row is visible */
+
+typedef struct tessa_kv_cache {
+    void *keys;
+    void *values;
+    float *key_scales;   /* SQ8 only */
+    float *value_scales;
+    uint64_t key_strides[3], value_strides[3];             /* elements: page, head, row */
+    uint64_t key_scale_strides[3], value_scale_strides[3]; /* floats */
+    uint32_t type;       /* enum tessa_kv_type */
+    uint32_t pages, heads, page_rows, head_dim;
+    uint32_t reserved;
+} tessa_kv_cache;
+
+/* Page ids outside [0, pages) name no page: their rows are neither read nor
+ * written and weigh nothing.  Lengths are clipped to [0, max_length]. */
+typedef struct tessa_kv_sequences {
+    const int32_t *table;    /* batch x table_stride */
+    const int32_t *lengths;  /* batch: rows of each sequence */
+    uint64_t table_stride;
+    uint32_t batch;
+    uint32_t columns;        /* page ids of a sequence */
+    uint32_t max_length;     /* no length is larger; at most columns * page_rows */
+    uint32_t reserved;
+} tessa_kv_sequences;
+
+/* New rows.  Token t of sequence b (offsets[b] <= t < offsets[b + 1]; without
+ * offsets one token for each sequence) becomes row lengths[b] + t - offsets[b]:
+ * here `lengths` are the rows before the call.  k and v: tokens x heads rows of
+ * bf16 or fp16 (`type`; the cache's own type unless that is SQ8), strides in
+ * elements, 16-byte aligned.  An SQ8 row with a value that is not finite gets the
+ * scale NaN. */
+typedef struct tessa_kv_tokens {
+    const void *k;
+    const void *v;
+    uint64_t k_strides[2], v_strides[2];  /* elements: token, head */
+    const int32_t *offsets;               /* batch + 1, or null */
+    uint64_t tokens;
+    uint32_t max_new;                     /* no sequence has more new tokens */
+    uint32_t type;
+} tessa_kv_tokens;
+tessa_status tessa_kv_append(const tessa_kv_cache *cache, const tessa_kv_sequences *seq,
+                             const tessa_kv_tokens *tokens, void *stream);
+
+/* Attention of query heads h * (q_heads / heads) .. over head h of the cache:
+ *   out = sum_j p_j v_j,  p = softmax(scale * q . k_j),  lse = log sum_j exp(scale * q . k_j).
+ * A query at row p sees rows j <= p with j < sinks or j > p - window (all with
+ * TESSA_KV_ALL).  A query that sees nothing has out 0 and lse -inf; a row whose
+ * logit is -inf weighs nothing.
+ *   tessa_kv_attend_token: one query for each sequence, at its last row; `tokens`
+ *     = batch, no offsets.  listed: rows visible besides the window, listed_count
+ *     for each (sequence, head), e.g. a search's results; entries that are
+ *     negative, past the length or already visible are skipped, others should
+ *     be distinct (a row listed twice counts twice).  weights: f32 accumulator,
+ *     weights[b][h][j] += p_j summed over the head's queries.
+ *   tessa_kv_attend_prompt: the new tokens of each sequence, its last rows;
+ *     offsets as in tessa_kv_append, no list, no weights. */
+typedef struct tessa_kv_attend {
+    const void *q;
+    void *out;
+    float *lse;                            /* tokens x q_heads */
+    uint64_t q_strides[2], out_strides[2]; /* elements: token, head; 16-byte aligned rows */
+    uint32_t type;                         /* of q and out; the cache's own unless that is SQ8 */
+    uint32_t q_heads;
+    float scale;
+    uint32_t sinks, window;
+    uint32_t listed_count;
+    const int32_t *listed;
+    float *weights;
+    uint64_t weight_strides[2];            /* floats: sequence, head; rows contiguous */
+    const int32_t *offsets;
+    uint64_t tokens;
+    uint32_t max_new;
+    uint32_t reserved;
+} tessa_kv_attend;
+tessa_status tessa_kv_attend_token_scratch(const tessa_kv_cache *cache, const tessa_kv_sequences *seq,
+                                           const tessa_kv_attend *a, uint64_t *bytes);
+tessa_status tessa_kv_attend_token(const tessa_kv_cache *cache, const tessa_kv_sequences *seq,
+                                   const tessa_kv_attend *a, void *scratch, uint64_t bytes, void *stream);
+tessa_status tessa_kv_attend_prompt_scratch(const tessa_kv_cache *cache, const tessa_kv_sequences *seq,
+                                            const tessa_kv_attend *a, uint64_t *bytes);
+tessa_status tessa_kv_attend_prompt(const tessa_kv_cache *cache, const tessa_kv_sequences *seq,
+                                    const tessa_kv_attend *a, void *scratch, uint64_t bytes, void *stream);
+
+/* Eviction: of each (sequence, head) with more than `keep` rows, the first
+ * `sinks`, the last `recent` and of the others the keep - sinks - recent with
+ * the largest weights stay (equal weights: the lower row; NaN below everything),
+ * in ascending order as rows 0.. of `into` (page ids as in the sequences' table;
+ * null: in place).  In place, no page may belong to two sequences; other pages
+ * must not be among those read.  new_weights (batch x heads x weight_rows,
+ * contiguous, not the weights themselves) gets the kept rows' weights and zeros
+ * after them, kept (batch x heads x keep) the kept rows and -1 after them,
+ * new_lengths min(length, keep). */
+typedef struct tessa_kv_eviction {
+    const float *weights;
+    uint64_t weight_strides[2];  /* floats: sequence, head */
+    float *new_weights;
+    int32_t *kept;
+    int32_t *new_lengths;
+    const int32_t *into;
+    uint64_t into_stride;
+    uint32_t into_columns;
+    uint32_t weight_rows;        /* >= keep */
+    uint32_t keep, sinks, recent;
+    uint32_t reserved;
+} tessa_kv_eviction;
+tessa_status tessa_kv_evict(const tessa_kv_cache *cache, const tessa_kv_sequences *seq, const tessa_kv_eviction *e,
+                            void *stream);
+
 #ifdef __cplusplus
 }
 #endif

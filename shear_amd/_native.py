@@ -313,6 +313,43 @@ class TierLiftStats(C.Structure):
         return {f: getattr(self, f) for f, _ in self._fields_}
 
 
+KV_BF16, KV_F16, KV_SQ8 = 1, 2, 3
+KV_ALL = 0xFFFFFFFF
+
+
+class KvCache(C.Structure):
+    _fields_ = [("keys", C.c_void_p), ("values", C.c_void_p), ("key_scales", C.c_void_p),
+                ("value_scales", C.c_void_p), ("key_strides", C.c_uint64 * 3), ("value_strides", C.c_uint64 * 3),
+                ("key_scale_strides", C.c_uint64 * 3), ("value_scale_strides", C.c_uint64 * 3), ("type", C.c_uint32),
+                ("pages", C.c_uint32), ("heads", C.c_uint32), ("page_rows", C.c_uint32), ("head_dim", C.c_uint32),
+                ("reserved", C.c_uint32)]
+
+
+class KvSequences(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("lengths", C.c_void_p), ("table_stride", C.c_uint64), ("batch", C.c_uint32),
+                ("columns", C.c_uint32), ("max_length", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class KvTokens(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_strides", C.c_uint64 * 2), ("v_strides", C.c_uint64 * 2),
+                ("offsets", C.c_void_p), ("tokens", C.c_uint64), ("max_new", C.c_uint32), ("type", C.c_uint32)]
+
+
+class KvAttend(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p), ("q_strides", C.c_uint64 * 2),
+                ("out_strides", C.c_uint64 * 2), ("type", C.c_uint32), ("q_heads", C.c_uint32), ("scale", C.c_float),
+                ("sinks", C.c_uint32), ("window", C.c_uint32), ("listed_count", C.c_uint32), ("listed", C.c_void_p),
+                ("weights", C.c_void_p), ("weight_strides", C.c_uint64 * 2), ("offsets", C.c_void_p),
+                ("tokens", C.c_uint64), ("max_new", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class KvEviction(C.Structure):
+    _fields_ = [("weights", C.c_void_p), ("weight_strides", C.c_uint64 * 2), ("new_weights", C.c_void_p),
+                ("kept", C.c_void_p), ("new_lengths", C.c_void_p), ("into", C.c_void_p), ("into_stride", C.c_uint64),
+                ("into_columns", C.c_uint32), ("weight_rows", C.c_uint32), ("keep", C.c_uint32), ("sinks", C.c_uint32),
+                ("recent", C.c_uint32), ("reserved", C.c_uint32)]
+
+
 # Every symbol include/tessa_hip.h declares, with its ctypes signature.
 _P = C.c_void_p
 _U32 = C.c_uint32
@@ -407,6 +444,16 @@ SIGNATURES = {
     "tessa_graph_search": (TessaStatus, [_P, _U32, _U32, _P, _P, _U32, _U32, _P, _U32, _U32, _U32, _P, _P, _P, _P]),
     "tessa_graph_search_sq8": (TessaStatus, [_P, _P, _U32, _U32, _U32, _P, _P, _U32, _U32, _P, _U32, _U32, _U32, _P, _P,
                                              _P, _P]),
+    "tessa_kv_append": (TessaStatus, [C.POINTER(KvCache), C.POINTER(KvSequences), C.POINTER(KvTokens), _P]),
+    "tessa_kv_attend_token_scratch": (TessaStatus, [C.POINTER(KvCache), C.POINTER(KvSequences), C.POINTER(KvAttend),
+                                                    C.POINTER(_U64)]),
+    "tessa_kv_attend_token": (TessaStatus, [C.POINTER(KvCache), C.POINTER(KvSequences), C.POINTER(KvAttend), _P, _U64,
+                                            _P]),
+    "tessa_kv_attend_prompt_scratch": (TessaStatus, [C.POINTER(KvCache), C.POINTER(KvSequences), C.POINTER(KvAttend),
+                                                     C.POINTER(_U64)]),
+    "tessa_kv_attend_prompt": (TessaStatus, [C.POINTER(KvCache), C.POINTER(KvSequences), C.POINTER(KvAttend), _P, _U64,
+                                             _P]),
+    "tessa_kv_evict": (TessaStatus, [C.POINTER(KvCache), C.POINTER(KvSequences), C.POINTER(KvEviction), _P]),
 }
 
 _lib = None

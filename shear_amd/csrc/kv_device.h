@@ -1,0 +1,140 @@
+// kv_device.h -- device helpers of the attention kernels over the paged
+// key-value cache: 16-bit element types on the matrix instructions, exchanges
+// between the 16- and 32-lane groups of a wave, the table lookup.
+#pragma once
+
+#include "kv_kernels.h"
+
+namespace tessa {
+
+using kv_f4 = float __attribute__((ext_vector_type(4)));
+using kv_f16 = float __attribute__((ext_vector_type(16)));
+using kv_u4 = uint32_t __attribute__((ext_vector_type(4)));
+using kv_u2 = uint32_t __attribute__((ext_vector_type(2)));
+
+// A running maximum before any visible row: below every finite logit, and
+// exp2(-inf - kKvNone) is 0 where exp2(-inf - -inf) would be NaN.
+constexpr float kKvNone = -3.0e38f;
+// The running maximum follows a larger logit only when that is more than
+// 2^kKvLag times as large: the weights stay below 2^kKvLag (far from either
+// type's largest value), and almost no tile pays for rescaling the output.
+constexpr float kKvLag = 8.0f;
+// The smallest scale of SQ8 values: below it (values under 1.3e-28) the sum of
+// w_j / v_j could leave f32's range, and such values count as if they had it.
+constexpr float kKvLeastScale = 1.0e-30f;
+
+template <typename T>
+struct KvElem;
+
+template <>
+struct KvElem<__bf16> {
+    using v8 = __bf16 __attribute__((ext_vector_type(8)));
+    using v2 = __bf16 __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ kv_f4 mma16(kv_u4 a, kv_u4 b, kv_f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ kv_f16 mma32(kv_u4 a, kv_u4 b, kv_f16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        const v2 x = {(__bf16)lo, (__bf16)hi};
+        return __builtin_bit_cast(uint32_t, x);
+    }
+    static __device__ __forceinline__ float low(uint32_t x) { return __uint_as_float(x << 16); }
+    static __device__ __forceinline__ float high(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+    // two whole numbers of at most 8 bits: their bf16 is the upper half of the f32
+    static __device__ __forceinline__ uint32_t pack_codes(float lo, float hi) {
+        return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+    }
+    static constexpr uint32_t kExponent = 0x7f80u;  // all ones: infinity or NaN
+};
+
+template <>
+struct KvElem<_Float16> {
+    using v8 = _Float16 __attribute__((ext_vector_type(8)));
+    using v2 = _Float16 __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ kv_f4 mma16(kv_u4 a, kv_u4 b, kv_f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ kv_f16 mma32(kv_u4 a, kv_u4 b, kv_f16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        const v2 x = {(_Float16)lo, (_Float16)hi};
+        return __builtin_bit_cast(uint32_t, x);
+    }
+    static __device__ __forceinline__ float low(uint32_t x) { return (float)__builtin_bit_cast(v2, x)[0]; }
+    static __device__ __forceinline__ float high(uint32_t x) { return (float)__builtin_bit_cast(v2, x)[1]; }
+    static __device__ __forceinline__ uint32_t pack_codes(float lo, float hi) { return pack(lo, hi); }
+    static constexpr uint32_t kExponent = 0x7c00u;
+};
+
+// byte e of x as a signed code
+__device__ __forceinline__ float kv_code(uint32_t x, int e) { return (float)(int8_t)(x >> (8 * e)); }
+
+__device__ __forceinline__ float kv_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// max / sum of x over the lanes that differ in bit 5, in bits 4 and 5
+__device__ __forceinline__ float kv_max32(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float kv_sum32(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float kv_max16(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return kv_max32(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float kv_sum16(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return kv_sum32(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// Orders a wave's LDS writes before its own later reads by other lanes.
+__device__ __forceinline__ void kv_wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Rows of sequence b: its length, clipped to what the tables can hold.
+__device__ __forceinline__ uint32_t kv_length(const KvCacheParams &c, uint32_t b) {
+    const int32_t n = c.lengths[b];
+    return n <= 0 ? 0u : min((uint32_t)n, c.max_length);
+}
+
+// Place of a row in 16-byte units (without the head), or kKvNoOffset where the
+// table names no page of the cache.
+__device__ __forceinline__ uint32_t kv_place(const KvCacheParams &c, const KvArray &a, int32_t page, uint32_t row) {
+    if ((uint32_t)page >= c.pages) return kKvNoOffset;
+    return (uint32_t)page * a.page_units + (row & ((1u << c.page_shift) - 1u)) * a.row_units;
+}
+
+__device__ __forceinline__ uint64_t kv_scale_place(const KvCacheParams &c, const KvArray &a, int32_t page, uint32_t row,
+                                                   uint32_t head) {
+    return (uint64_t)(uint32_t)page * a.scale_page + (uint64_t)head * a.scale_head +
+           (uint64_t)(row & ((1u << c.page_shift) - 1u)) * a.scale_row;
+}
+
+// The visible rows of a single token: [0, first), [last_begin, length) and the
+// listed ones strictly between; index i of [0, count) names one of them.
+struct KvVisible {
+    uint32_t first, last_begin, before_list, count;
+};
+
+__device__ __forceinline__ KvVisible kv_visible(const KvAttendParams &p, uint32_t length) {
+    KvVisible v;
+    if (p.window == 0xffffffffu) {
+        v.first = 0;
+        v.last_begin = 0;
+    } else {
+        v.first = min(p.sinks, length);
+        v.last_begin = max(v.first, length > p.window ? length - p.window : 0u);
+    }
+    v.before_list = v.first + (length - v.last_begin);
+    v.count = v.before_list + (length ? p.listed_count : 0u);
+    return v;
+}
+
+}  // namespace tessa

@@ -1,0 +1,274 @@
+// kv_evict.hip -- eviction from the paged cache by accumulated attention weight.
+//
+// Of the n rows of a (sequence, head) with n > keep, the first `sinks` and the
+// last `recent` stay, and of the others the keep - sinks - recent with the
+// largest weights, equal weights by the lower row, NaN below everything.  The
+// kept rows, in ascending order, become rows 0.. of the destination pages.
+//
+// kv_select_kernel: one workgroup per (sequence, head).  The weights, as
+// integers of the same order, go through three histograms in LDS (11, 11 and 10
+// bits from the top); the last leaves the exact value of the last kept row and
+// how many rows of that value are kept.  A wave owns a contiguous range of rows, so
+// ballots and one sum over the waves give each kept row its place, in order
+// and without a sort.  Up to 32,768 candidates stay in registers from one read
+// (a chain of passes over few bytes: latency-bound).
+//
+// kv_move_kernel: copy-bound.  Into other pages, workgroups share the kept rows
+// out; in place, the destination of a row is never after its source, so one
+// workgroup walks the rows of one 64-byte column of a (sequence, head) in order,
+// reading a batch of rows into registers, waiting for all of it, and writing:
+// what a batch writes lies before every source of the later ones.  Columns
+// are independent, which is where the parallelism comes from.
+#include "kv_device.h"
+
+namespace tessa {
+
+namespace {
+
+constexpr int kSelThreads = 1024;
+constexpr int kSelWaves = kSelThreads / 64;
+constexpr int kSelPer = 32;       // candidates of a lane held in registers
+constexpr int kSelGroup = 8;      // loads in flight where they are not held
+constexpr int kBins = 2048;
+constexpr int kMoveThreads = 256;
+constexpr int kMovePer = 8;       // rows of a thread in flight
+
+// An integer that orders as the weight does; NaN is 0.
+__device__ __forceinline__ uint32_t order_of(float w) {
+    uint32_t u = __float_as_uint(w);
+    if (w != w) return 0u;
+    if (w == 0.0f) u = 0u;  // -0 and 0 are equal
+    return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+}
+
+template <bool kHeld>
+__device__ __forceinline__ void select_rows(const KvEvictParams &p, const float *w, uint32_t n, int32_t *kept, float *out,
+                                            uint32_t *hist, uint32_t (*sh_wave)[kSelWaves], uint32_t *sh_pick) {
+    const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6;
+    const uint32_t candidates = n - p.sinks - p.recent;
+    const uint32_t need = p.keep - p.sinks - p.recent;
+    // contiguous rows of a wave, whole groups of 64
+    const uint32_t span = ((candidates + kSelWaves - 1) / kSelWaves + 63u) / 64u * 64u;
+    const uint32_t lo = wave * span, hi = min(lo + span, candidates);
+    const uint32_t steps = lo < hi ? (hi - lo + 63u) / 64u : 0u;
+    const float *mine = w + p.sinks + lo + lane;
+    auto load = [&](uint32_t s) { return lo + s * 64u + lane < hi ? mine[s * 64u] : 0.0f; };
+    auto inside = [&](uint32_t s) { return lo + s * 64u + lane < hi; };
+    float held[kHeld ? kSelPer : 1];
+    if constexpr (kHeld) {
+#pragma unroll
+        for (int s = 0; s < kSelPer; ++s) held[s] = load(s);
+    }
+    // f(step, weight) for each of the lane's candidates
+    auto each = [&](auto &&f) {
+        if constexpr (kHeld) {
+#pragma unroll
+            for (int s = 0; s < kSelPer; ++s)
+                if ((uint32_t)s < steps) f((uint32_t)s, held[s]);
+        } else {
+            for (uint32_t s0 = 0; s0 < steps; s0 += kSelGroup) {
+                float x[kSelGroup];
+#pragma unroll
+                for (int s = 0; s < kSelGroup; ++s) x[s] = s0 + s < steps ? load(s0 + s) : 0.0f;
+#pragma unroll
+                for (int s = 0; s < kSelGroup; ++s)
+                    if (s0 + s < steps) f(s0 + s, x[s]);
+            }
+        }
+    };
+
+    // the need-th largest value: three digits from the top
+    uint32_t prefix = 0, known = 0, left = need;  // bits known so far, kept rows still to place among them
+    if (need) {
+#pragma unroll 1
+        for (int pass = 0; pass < 3; ++pass) {
+            const int bits = pass == 2 ? 10 : 11, shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+            for (uint32_t i = t; i < kBins; i += kSelThreads) hist[i] = 0u;
+            __syncthreads();
+            each([&](uint32_t s, float x) {
+                const uint32_t u = order_of(x);
+                if (inside(s) && (known == 0 || (u >> (32 - known)) == prefix)) atomicAdd(&hist[(u >> shift) & ((1u << bits) - 1u)], 1u);
+            });
+            __syncthreads();
+            // bins from the top: thread t has bins 2047 - 2t and 2046 - 2t
+            const uint32_t a = hist[kBins - 1 - 2 * t], c = hist[kBins - 2 - 2 * t];
+            uint32_t sum = a + c;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const uint32_t y = __shfl_up(sum, off);
+                if (lane >= (uint32_t)off) sum += y;
+            }
+            if (lane == 63u) sh_wave[0][wave] = sum;
+            __syncthreads();
+            uint32_t before = sum - a - c;
+            for (uint32_t i = 0; i < wave; ++i) before += sh_wave[0][i];
+            if (before < left && left <= before + a + c) {
+                const bool first = left <= before + a;
+                sh_pick[0] = kBins - 1 - 2 * t - (first ? 0u : 1u);
+                sh_pick[1] = left - before - (first ? 0u : a);
+            }
+            __syncthreads();
+            prefix = (prefix << bits) | sh_pick[0];
+            left = sh_pick[1];
+            known += bits;
+            __syncthreads();
+        }
+    }
+    const uint32_t least = need ? prefix : 0xffffffffu;  // nothing is as large as this
+    // rows above it, and equal to it, before each wave's
+    uint32_t above = 0, equal = 0;
+    if (need) {
+        each([&](uint32_t s, float x) {
+            const uint32_t u = order_of(x);
+            above += __popcll(__ballot(inside(s) && u > least));
+            equal += __popcll(__ballot(inside(s) && u == least));
+        });
+        if (lane == 0) {
+            sh_wave[0][wave] = above;
+            sh_wave[1][wave] = equal;
+        }
+        __syncthreads();
+        uint32_t place = p.sinks, equal_before = 0;
+        for (uint32_t i = 0; i < wave; ++i) {
+            const uint32_t e = sh_wave[1][i], room = left > equal_before ? left - equal_before : 0u;
+            place += sh_wave[0][i] + min(e, room);
+            equal_before += e;
+        }
+        uint32_t room = left > equal_before ? left - equal_before : 0u;
+        const uint64_t below = (1ull << lane) - 1ull;
+        each([&](uint32_t s, float x) {
+            const uint32_t u = order_of(x);
+            const uint64_t ties = __ballot(inside(s) && u == least);
+            const bool tie = inside(s) && u == least && (uint32_t)__popcll(ties & below) < room;
+            const bool keep = tie || (inside(s) && u > least);
+            const uint64_t all = __ballot(keep);
+            if (keep) {
+                const uint32_t at = place + (uint32_t)__popcll(all & below);
+                kept[at] = (int32_t)(p.sinks + lo + s * 64u + lane);
+                out[at] = x;
+            }
+            place += (uint32_t)__popcll(all);
+            const uint32_t used = (uint32_t)__popcll(ties);
+            room = room > used ? room - used : 0u;
+        });
+    }
+    for (uint32_t i = t; i < p.sinks; i += kSelThreads) {
+        kept[i] = (int32_t)i;
+        out[i] = w[i];
+    }
+    for (uint32_t i = t; i < p.recent; i += kSelThreads) {
+        kept[p.keep - p.recent + i] = (int32_t)(n - p.recent + i);
+        out[p.keep - p.recent + i] = w[n - p.recent + i];
+    }
+}
+
+__global__ __launch_bounds__(kSelThreads) void kv_select_kernel(KvEvictParams p) {
+    __shared__ uint32_t hist[kBins];
+    __shared__ uint32_t sh_wave[2][kSelWaves];
+    __shared__ uint32_t sh_pick[2];
+    const uint32_t h = blockIdx.x, b = blockIdx.y, t = threadIdx.x;
+    const uint32_t n = kv_length(p.c, b);
+    const uint64_t bh = (uint64_t)b * p.c.heads + h;
+    const float *w = p.weights + (uint64_t)b * p.weight_batch + (uint64_t)h * p.weight_head;
+    int32_t *kept = p.kept + bh * p.keep;
+    float *out = p.new_weights + bh * p.weight_rows;
+    const uint32_t count = min(n, p.keep);
+    if (h == 0 && t == 0) p.new_lengths[b] = (int32_t)count;
+    for (uint32_t i = count + t; i < p.keep; i += kSelThreads) kept[i] = -1;
+    for (uint32_t i = count + t; i < p.weight_rows; i += kSelThreads) out[i] = 0.0f;
+    if (n <= p.keep) {
+        for (uint32_t i = t; i < n; i += kSelThreads) {
+            kept[i] = (int32_t)i;
+            out[i] = w[i];
+        }
+        return;
+    }
+    if (n - p.sinks - p.recent <= (uint32_t)(kSelThreads * kSelPer))
+        select_rows<true>(p, w, n, kept, out, hist, sh_wave, sh_pick);
+    else
+        select_rows<false>(p, w, n, kept, out, hist, sh_wave, sh_pick);
+}
+
+// units: 16-byte pieces of a row that the workgroup moves, from piece `column *
+// units` on, by 2^lanes_log2 lanes; span: rows of a workgroup (in place: all).
+__global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(KvEvictParams p, uint32_t row_units, uint32_t columns, uint32_t units,
+                                                               uint32_t lanes_log2, uint32_t span, bool in_place) {
+    const KvCacheParams &c = p.c;
+    const uint32_t h = blockIdx.y / (2 * columns), rest = blockIdx.y - h * 2 * columns;
+    const uint32_t b = blockIdx.z, t = threadIdx.x;
+    const uint32_t column = rest >> 1;
+    const KvArray &a = (rest & 1u) ? c.values : c.keys;
+    const uint32_t n = kv_length(c, b), count = min(n, p.keep);
+    const uint32_t first = blockIdx.x * span, last = min(first + span, count);
+    if (first >= last || (in_place && n <= p.keep)) return;
+    const int32_t *kept = p.kept + ((uint64_t)b * c.heads + h) * p.keep;
+    const int32_t *from = c.table + (uint64_t)b * c.table_stride, *to = p.into + (uint64_t)b * p.into_stride;
+    const uint32_t lane = t & ((1u << lanes_log2) - 1u), per = kMoveThreads >> lanes_log2;
+    const uint32_t unit = column * units + lane;
+    const bool mine = lane < units && unit < row_units;
+    const bool scales = a.scales != nullptr && unit == 0;
+    char *base = a.rows + ((uint64_t)h * a.head_units + unit) * 16u;
+    const uint32_t into_rows = p.into_columns << c.page_shift;
+    for (uint32_t j0 = first; j0 < last; j0 += per * kMovePer) {
+        kv_u4 x[kMovePer];
+        float sx[kMovePer];
+        uint32_t dst[kMovePer];
+        uint64_t sdst[kMovePer];
+#pragma unroll
+        for (int i = 0; i < kMovePer; ++i) {
+            const uint32_t j = j0 + i * per + (t >> lanes_log2);
+            dst[i] = kKvNoOffset;
+            sdst[i] = 0;
+            sx[i] = 0.0f;
+            x[i] = kv_u4{0, 0, 0, 0};
+            if (j < last && j < into_rows) {
+                const uint32_t row = (uint32_t)kept[j];
+                if (!(in_place && row == j)) {
+                    const int32_t src_page = from[row >> c.page_shift], dst_page = to[j >> c.page_shift];
+                    const uint32_t src = kv_place(c, a, src_page, row);
+                    dst[i] = src == kKvNoOffset ? kKvNoOffset : kv_place(c, a, dst_page, j);
+                    if (dst[i] != kKvNoOffset) {
+                        if (mine) x[i] = *reinterpret_cast<const kv_u4 *>(base + (uint64_t)src * 16u);
+                        if (scales) {
+                            sx[i] = a.scales[kv_scale_place(c, a, src_page, row, h)];
+                            sdst[i] = kv_scale_place(c, a, dst_page, j, h);
+                        }
+                    }
+                }
+            }
+        }
+        if (in_place) {
+            // every row of the batch has arrived before any is written
+#pragma unroll
+            for (int i = 0; i < kMovePer; ++i) asm volatile("" : "+v"(x[i]), "+v"(sx[i]));
+            __syncthreads();
+        }
+#pragma unroll
+        for (int i = 0; i < kMovePer; ++i) {
+            if (dst[i] != kKvNoOffset) {
+                if (mine) *reinterpret_cast<kv_u4 *>(base + (uint64_t)dst[i] * 16u) = x[i];
+                if (scales) a.scales[sdst[i]] = sx[i];
+            }
+        }
+    }
+}
+
+}  // namespace
+
+int launch_kv_evict(const KvEvictParams &p, uint32_t type, hipStream_t stream) {
+    if (p.c.batch == 0) return 0;
+    kv_select_kernel<<<dim3(p.c.heads, p.c.batch), kSelThreads, 0, stream>>>(p);
+    if (hipGetLastError() != hipSuccess) return -1;
+    const bool in_place = p.into == p.c.table;
+    const uint32_t row_units = p.c.dim * (type == kKvSq8 ? 1u : 2u) / 16u;
+    const uint32_t units = in_place ? 4u : row_units;  // 64-byte columns in place, else whole rows
+    const uint32_t columns = (row_units + units - 1) / units;
+    uint32_t lanes_log2 = 0;
+    while ((1u << lanes_log2) < units) ++lanes_log2;
+    const uint32_t span = in_place ? p.keep : (uint32_t)(kMoveThreads >> lanes_log2) * kMovePer;
+    const dim3 grid((p.keep + span - 1) / span, p.c.heads * 2 * columns, p.c.batch);
+    kv_move_kernel<<<grid, kMoveThreads, 0, stream>>>(p, row_units, columns, units, lanes_log2, span, in_place);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+}  // namespace tessa

@@ -1,0 +1,473 @@
+// kv_prompt.hip -- attention of prompts over the paged cache: the new tokens of
+// each sequence, its last rows, attend causally over all of its rows, or over
+// the first `sinks` and the last `window` of them.
+//
+// Per head h of the cache the queries are the pairs (token, one of the G query
+// heads), token-major, 128 to a workgroup and 32 to a wave, so that the heads
+// of a group share every K and V tile and a short prompt still fills the
+// instructions' columns.  Tiles of 64 rows (32 at 256 dims) are staged in LDS twice over: while
+// one is worked on, the next comes from memory into registers (its page ids
+// were read a tile earlier) and goes to the other half afterwards.
+//  * S^T = K Q^T on 32x32x16 instructions (rows are the tile's, columns the
+//    queries): a lane has half of the logits of one query, its partner lane (+- 32) the other
+//    half, so the running maximum and sum cost one exchange a tile.
+//  * O^T = V^T P^T: the logits' registers are the P^T operand as they
+//    stand; V^T comes from LDS by transposing reads of 4 rows x 16 values.
+//  * The maximum follows only a logit 2^8 times as large (kKvLag), and tiles that
+//    every query of the workgroup sees in full carry no mask.
+//  * P is rounded to the queries' type once (an error of the size of the
+//    result's own rounding); sums are in f32.
+//  * SQ8 rows become 16-bit whole numbers on the way into LDS, exactly; scales
+//    enter as in kv_token.hip.
+//  * A row that only some queries see may hold infinities or NaN, which would
+//    reach the others as 0 * inf.  In tiles with a mask such values go to LDS as zeros,
+//    and add_special() adds them to the queries that see them.
+#include "kernel_attr.h"
+#include "kv_device.h"
+
+namespace tessa {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr uint32_t kQueries = 128;  // of a workgroup
+
+typedef short kv_s4 __attribute__((ext_vector_type(4)));
+
+// Piece (16 bytes) of an LDS row in which piece c of row r lies: the K reads
+// (16 rows, one piece) and the V reads (4 rows, 64 bytes) then meet all banks.
+template <int DP>
+__device__ __forceinline__ uint32_t k_piece(uint32_t r, uint32_t c) {
+    return DP == 64 ? c ^ ((r >> 1) & 7u) : c ^ (r & 15u);
+}
+template <int DP>
+__device__ __forceinline__ uint32_t v_piece(uint32_t r, uint32_t c) {
+    return DP == 64 ? c ^ (((r >> 1) & 1u) << 2) : c ^ ((r & 3u) << 2);
+}
+
+template <typename T>
+__device__ __forceinline__ bool special_half(uint32_t x) {
+    return (x & KvElem<T>::kExponent) == KvElem<T>::kExponent;
+}
+
+// Rows of a tile: at 256 dims half as many, for the registers' sake.
+template <int DP>
+constexpr uint32_t prompt_rows() {
+    return DP == 256 ? 32u : 64u;
+}
+
+template <bool kSq8, int DP>
+struct PromptLds {
+    static constexpr uint32_t kRows = prompt_rows<DP>();
+    alignas(16) char k[2][kRows * DP * 2];
+    alignas(16) char v[2][kRows * DP * 2];
+    alignas(16) float scale[kSq8 ? 2 : 1][3][kSq8 ? kRows : 4];
+    // of tile i at i % 4: whether a value was replaced, and the rows without a page.
+    // Cleared two tiles ahead, when nothing reads or sets them.
+    uint32_t marks[4][1 + kRows / 32];
+};
+
+template <typename T, bool kSq8, int DP>
+__global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(KvAttendParams p, uint32_t query_tiles) {
+    using E = KvElem<T>;
+    using Lds = PromptLds<kSq8, DP>;
+    constexpr uint32_t kRows = Lds::kRows;
+    constexpr int kSubs = (int)kRows / 32;       // 32 rows of logits each
+    constexpr int kSteps = DP / 16;              // instructions along the dims
+    constexpr int kBlocks = DP / 32;             // blocks of 32 dims of the output
+    constexpr int kPieces = kSq8 ? DP / 16 : DP / 8;  // 16-byte pieces of a row in memory
+    constexpr int kLoads = (int)kRows * kPieces / kThreads;  // of a thread, for K and for V each
+    constexpr int kRowsPer = kThreads / kPieces;  // rows of one load of the workgroup
+    extern __shared__ __align__(16) char smem[];
+    Lds &lds = *reinterpret_cast<Lds *>(smem);
+
+    const KvCacheParams &c = p.c;
+    const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6;
+    const uint32_t n = lane & 31u, half = lane >> 5;
+    const uint32_t split = blockIdx.x % p.chunks, query_tile = query_tiles - 1u - blockIdx.x / p.chunks;
+    const uint32_t h = blockIdx.y, b = blockIdx.z;
+    const uint32_t length = kv_length(c, b);
+    const int64_t first_token = p.offsets[b];
+    int64_t new64 = (int64_t)p.offsets[b + 1] - first_token;
+    if (first_token < 0 || new64 <= 0 || first_token + new64 > (int64_t)p.tokens) return;
+    const uint32_t fresh = min((uint32_t)min(new64, (int64_t)0x7fffffff), p.max_new);
+    const uint32_t queries = fresh * p.group;
+    const uint32_t q0 = query_tile * kQueries;
+    if (q0 >= queries) return;
+    // a token's row: those of a sequence are its last; before row 0 (fewer rows than tokens) nothing is seen
+    const int32_t row0 = (int32_t)length - (int32_t)fresh;
+    const uint32_t my_q = q0 + wave * 32u + n;
+    const bool query_ok = my_q < queries;
+    const uint32_t my_token = min(my_q, queries - 1u) / p.group;
+    const uint32_t my_head = h * p.group + min(my_q, queries - 1u) - my_token * p.group;
+    const int32_t pos = row0 + (int32_t)my_token;
+    const int32_t pos_first = row0 + (int32_t)(q0 / p.group);
+    const int32_t pos_last = row0 + (int32_t)((min(q0 + kQueries, queries) - 1u) / p.group);
+    const int32_t wave_last = row0 + (int32_t)(min(q0 + wave * 32u + 31u, queries - 1u) / p.group);
+    // rows [0, sinks) and (pos - window, pos]
+    const bool windowed = p.window != 0xffffffffu;
+    const int32_t window = windowed ? (int32_t)p.window : 0;
+    const int32_t sinks = windowed ? (int32_t)p.sinks : 0;
+    const int32_t row_end = max(0, pos_last + 1);
+    const int32_t row_begin = windowed ? max(0, pos_first - window + 1) : 0;
+    const uint32_t sink_tiles = ((uint32_t)min(sinks, row_end) + kRows - 1u) / kRows;
+    const uint32_t window_tile = max(sink_tiles, (uint32_t)row_begin / kRows);
+    const uint32_t end_tile = ((uint32_t)row_end + kRows - 1u) / kRows;
+    const uint32_t all_tiles = sink_tiles + (end_tile > window_tile ? end_tile - window_tile : 0u);
+    const uint32_t first_it = (uint32_t)((uint64_t)all_tiles * split / p.chunks);
+    const uint32_t last_it = (uint32_t)((uint64_t)all_tiles * (split + 1u) / p.chunks);
+    auto tile_row = [&](uint32_t it) { return (it < sink_tiles ? it : window_tile + it - sink_tiles) * kRows; };
+    auto masked = [&](uint32_t r0) {  // whether some query of the workgroup does not see all of the tile
+        const int32_t lo = (int32_t)r0, hi = lo + (int32_t)kRows - 1;
+        return hi > pos_first || (windowed && hi >= sinks && lo <= pos_last - window);
+    };
+
+    const int32_t *table = c.table + (uint64_t)b * c.table_stride;
+    const char *kbase = c.keys.rows + (uint64_t)h * c.keys.head_units * 16u;
+    const char *vbase = c.values.rows + (uint64_t)h * c.values.head_units * 16u;
+    const uint32_t piece = t % kPieces, piece_row = t / kPieces;
+    const bool piece_ok = piece * (kSq8 ? 16u : 8u) < c.dim;
+
+    kv_u4 qf[kSteps];
+    {
+        const char *q = p.q + (uint64_t)(first_token + my_token) * p.q_token + (uint64_t)my_head * p.q_head;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const uint32_t d = (uint32_t)s * 16u + half * 8u;
+            const kv_u4 zero = {0, 0, 0, 0};
+            qf[s] = query_ok && d < c.dim ? *reinterpret_cast<const kv_u4 *>(q + 2u * d) : zero;
+        }
+    }
+    float m = kKvNone, l = 0.0f;
+    kv_f16 acc[kBlocks];
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][e] = 0.0f;
+
+    int32_t pages[kLoads];
+    kv_u4 kr[kLoads], vr[kLoads];
+    float ks = 0.0f, vs = 1.0f;
+    uint32_t missing = 0;  // loads of the thread whose row has no page
+    const kv_u4 zero4 = {0, 0, 0, 0};
+
+    auto read_pages = [&](uint32_t it) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const uint32_t row = tile_row(it) + (uint32_t)i * kRowsPer + piece_row;
+            pages[i] = it < last_it && row < length ? table[row >> c.page_shift] : -1;
+        }
+    };
+    auto read_rows = [&](uint32_t it) {
+        const uint32_t r0 = tile_row(it);
+        missing = 0;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const uint32_t row = r0 + (uint32_t)i * kRowsPer + piece_row;
+            if (row < length && (uint32_t)pages[i] >= c.pages) missing |= 1u << i;
+            const uint32_t kp = kv_place(c, c.keys, pages[i], row), vp = kv_place(c, c.values, pages[i], row);
+            const bool ok = piece_ok && kp != kKvNoOffset;
+            kr[i] = ok ? *reinterpret_cast<const kv_u4 *>(kbase + ((uint64_t)kp + piece) * 16u) : zero4;
+            vr[i] = ok ? *reinterpret_cast<const kv_u4 *>(vbase + ((uint64_t)vp + piece) * 16u) : zero4;
+        }
+        if constexpr (kSq8) {
+            if (t < kRows) {
+                const uint32_t row = r0 + t;
+                const int32_t page = row < length ? table[row >> c.page_shift] : -1;
+                ks = 0.0f;
+                vs = 1.0f;
+                if ((uint32_t)page < c.pages) {
+                    ks = c.keys.scales[kv_scale_place(c, c.keys, page, row, h)];
+                    vs = c.values.scales[kv_scale_place(c, c.values, page, row, h)];
+                }
+            }
+        }
+    };
+    auto write_rows = [&](uint32_t it, uint32_t buf) {
+        const uint32_t r0 = tile_row(it);
+        const bool watch = masked(r0);
+        uint32_t *marks = lds.marks[it & 3u];
+        if (piece == 0) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const uint32_t r = (uint32_t)i * kRowsPer + piece_row;
+                if (missing >> i & 1u) atomicOr(&marks[1 + r / 32u], 1u << (r & 31u));
+            }
+        }
+        if constexpr (!kSq8) {
+            if (watch) {  // infinities and NaN: zeros here, add_special() adds them
+                bool found = false;
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const bool lo = special_half<T>(vr[i][w]), hi = special_half<T>(vr[i][w] >> 16);
+                        if (lo) vr[i][w] &= 0xffff0000u;
+                        if (hi) vr[i][w] &= 0xffffu;
+                        found |= lo | hi;
+                    }
+                if (found) marks[0] = 1u;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const uint32_t r = (uint32_t)i * kRowsPer + piece_row;
+            if constexpr (kSq8) {
+#pragma unroll
+                for (int part = 0; part < 2; ++part) {
+                    kv_u4 k4, v4;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t kw = kr[i][2 * part + e / 2], vw = vr[i][2 * part + e / 2];
+                        k4[e] = E::pack_codes(kv_code(kw, 2 * (e & 1)), kv_code(kw, 2 * (e & 1) + 1));
+                        v4[e] = E::pack_codes(kv_code(vw, 2 * (e & 1)), kv_code(vw, 2 * (e & 1) + 1));
+                    }
+                    const uint32_t to = 2u * piece + (uint32_t)part;
+                    *reinterpret_cast<kv_u4 *>(&lds.k[buf][r * DP * 2 + k_piece<DP>(r, to) * 16u]) = k4;
+                    *reinterpret_cast<kv_u4 *>(&lds.v[buf][r * DP * 2 + v_piece<DP>(r, to) * 16u]) = v4;
+                }
+            } else {
+                *reinterpret_cast<kv_u4 *>(&lds.k[buf][r * DP * 2 + k_piece<DP>(r, piece) * 16u]) = kr[i];
+                *reinterpret_cast<kv_u4 *>(&lds.v[buf][r * DP * 2 + v_piece<DP>(r, piece) * 16u]) = vr[i];
+            }
+        }
+        if constexpr (kSq8) {
+            if (t < kRows) {
+                // a NaN scale: its row is NaN to those that see it, which the logit alone carries
+                const bool bad = vs != vs;
+                const float s = bad ? 1.0f : vs < kKvLeastScale ? kKvLeastScale : vs;
+                lds.scale[buf][0][t] = bad ? vs : ks * p.scale_log2;
+                lds.scale[buf][1][t] = log2f(s);
+                lds.scale[buf][2][t] = 1.0f / s;
+            }
+        }
+    };
+    auto sees = [&](int32_t row) { return row <= pos && (!windowed || row < sinks || row > pos - window); };
+    auto add_special = [&](uint32_t r0) {
+        for (uint32_t r = 0; r < kRows; ++r) {
+            const uint32_t row = r0 + r;
+            if (row >= length) break;
+            const int32_t page = table[row >> c.page_shift];
+            const uint32_t place = kv_place(c, c.values, page, row);
+            if (place == kKvNoOffset) continue;
+            const bool seen = sees((int32_t)row);
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const uint32_t d = (uint32_t)i * 32u + 8u * (e / 4) + 4u * half;
+                    if (d < c.dim) {
+                        const kv_u2 x = *reinterpret_cast<const kv_u2 *>(vbase + (uint64_t)place * 16u + 2u * d);
+                        if (seen) {
+                            if (special_half<T>(x[0])) acc[i][e] += E::low(x[0]);
+                            if (special_half<T>(x[0] >> 16)) acc[i][e + 1] += E::high(x[0]);
+                            if (special_half<T>(x[1])) acc[i][e + 2] += E::low(x[1]);
+                            if (special_half<T>(x[1] >> 16)) acc[i][e + 3] += E::high(x[1]);
+                        }
+                    }
+                }
+        }
+    };
+
+    if (first_it < last_it) {
+        if (t < 4u * (1u + kRows / 32u)) lds.marks[0][t] = 0u;
+        read_pages(first_it);
+        read_rows(first_it);
+        read_pages(first_it + 1);
+        __syncthreads();  // the marks are cleared
+        write_rows(first_it, 0);
+        __syncthreads();
+    }
+    for (uint32_t it = first_it; it < last_it; ++it) {
+        const uint32_t buf = (it - first_it) & 1u;
+        const uint32_t r0 = tile_row(it);
+        const bool more = it + 1 < last_it;
+        if (more) {
+            read_rows(it + 1);
+            read_pages(it + 2);
+        }
+        const bool mask = masked(r0);
+        const uint32_t *marks = lds.marks[it & 3u];
+        if (t < 1u + kRows / 32u) lds.marks[(it + 2u) & 3u][t] = 0u;
+        if ((int32_t)r0 <= wave_last) {  // else the wave's queries see nothing of it
+            // logits of rows 32 u + 8 (e / 4) + 4 half + e % 4
+            kv_f16 x[kSubs];
+#pragma unroll
+            for (int u = 0; u < kSubs; ++u) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[u][e] = 0.0f;
+                const uint32_t r = 32u * u + n;
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s) {
+                    const kv_u4 a = *reinterpret_cast<const kv_u4 *>(&lds.k[buf][r * DP * 2 + k_piece<DP>(r, 2u * s + half) * 16u]);
+                    x[u] = E::mma32(a, qf[s], x[u]);
+                }
+            }
+            if constexpr (kSq8) {
+#pragma unroll
+                for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        const uint32_t r = 32u * u + 2u * e + 4u * half;
+                        const kv_f4 k4 = *reinterpret_cast<const kv_f4 *>(&lds.scale[buf][0][r]);
+                        const kv_f4 v4 = *reinterpret_cast<const kv_f4 *>(&lds.scale[buf][1][r]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) x[u][e + i] = fmaf(x[u][e + i], k4[i], v4[i]);
+                    }
+            }
+            const float factor = kSq8 ? 1.0f : p.scale_log2;
+            if (mask) {
+#pragma unroll
+                for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int32_t row = (int32_t)r0 + 32 * u + 8 * (e / 4) + 4 * (int32_t)half + e % 4;
+                        if (!sees(row)) x[u][e] = -INFINITY;
+                    }
+            }
+#pragma unroll
+            for (int u = 0; u < kSubs; ++u) {
+                const uint32_t gone = marks[1 + u];
+                if (gone) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (gone >> (8u * (e / 4) + 4u * half + e % 4) & 1u) x[u][e] = -INFINITY;
+                }
+            }
+            float top = x[0][0] * factor;
+#pragma unroll
+            for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, x[u][e] * factor);
+            top = kv_max32(fmaxf(top, kKvNone));
+            if (__any(top > m + kKvLag)) {
+                const float higher = fmaxf(m, top);
+                const float f = kv_exp2(m - higher);
+                m = higher;
+                l *= f;
+#pragma unroll
+                for (int i = 0; i < kBlocks; ++i) acc[i] *= f;
+            }
+            kv_u4 pf[2 * kSubs];  // P^T operands of 16 rows each
+            float sum = 0.0f;
+#pragma unroll
+            for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) {
+                    const float w0 = kv_exp2(fmaf(x[u][e], factor, -m)), w1 = kv_exp2(fmaf(x[u][e + 1], factor, -m));
+                    if constexpr (kSq8) {
+                        const uint32_t r = 32u * u + 8u * (e / 4) + 4u * half + e % 4;
+                        sum = fmaf(w0, lds.scale[buf][2][r], sum);
+                        sum = fmaf(w1, lds.scale[buf][2][r + 1], sum);
+                    } else {
+                        sum += w0 + w1;
+                    }
+                    pf[2 * u + e / 8][(e % 8) / 2] = E::pack(w0, w1);
+                }
+            l += sum;
+            // V^T of dims 32 i + n: rows 16 k + 4 half + {0..3}, + 8
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i) {
+#pragma unroll
+                for (int k = 0; k < 2 * kSubs; ++k) {
+                    kv_u4 a;
+#pragma unroll
+                    for (int part = 0; part < 2; ++part) {
+                        // of its 16-lane group, lane 4 j + q reads values 4 q .. of row j
+                        const uint32_t r = 16u * k + 8u * part + 4u * half + ((lane & 15u) >> 2);
+                        const uint32_t d = 32u * i + 16u * ((lane >> 4) & 1u) + 4u * (lane & 3u);
+                        const char *src = &lds.v[buf][r * DP * 2 + v_piece<DP>(r, d / 8u) * 16u + (d & 7u) * 2u];
+                        const kv_s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (__attribute__((address_space(3))) kv_s4 *)const_cast<char *>(src));
+                        const kv_u2 y2 = __builtin_bit_cast(kv_u2, y);
+                        a[2 * part] = y2[0];
+                        a[2 * part + 1] = y2[1];
+                    }
+                    acc[i] = E::mma32(a, pf[k], acc[i]);
+                }
+            }
+            if constexpr (!kSq8)
+                if (mask && marks[0]) add_special(r0);
+        }
+        if (more) {
+            write_rows(it + 1, buf ^ 1u);
+            __syncthreads();
+        }
+    }
+    l = kv_sum32(l);
+
+    if (!query_ok) return;
+    const uint64_t token = (uint64_t)first_token + my_token;
+    const uint64_t query = token * p.q_heads + my_head;
+    if (p.chunks > 1) {
+        float *o = p.part_o + (query * p.chunks + split) * DP;
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+                *reinterpret_cast<kv_f4 *>(o + 32 * i + 2 * e + 4 * half) =
+                    kv_f4{acc[i][e], acc[i][e + 1], acc[i][e + 2], acc[i][e + 3]};
+        if (half == 0) {
+            p.part_ml[(query * p.chunks + split) * 2] = m;
+            p.part_ml[(query * p.chunks + split) * 2 + 1] = l;
+        }
+        return;
+    }
+    const float r = l == 0.0f ? 0.0f : 1.0f / l;
+    char *o = p.out + token * p.out_token + (uint64_t)my_head * p.out_head;
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const uint32_t d = 32u * i + 2u * e + 4u * half;
+            if (d < c.dim) {
+                const kv_u2 y = {E::pack(acc[i][e] * r, acc[i][e + 1] * r), E::pack(acc[i][e + 2] * r, acc[i][e + 3] * r)};
+                *reinterpret_cast<kv_u2 *>(o + 2u * d) = y;
+            }
+        }
+    if (half == 0) p.lse[query] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
+}
+
+template <typename T, bool kSq8, int DP>
+int launch(const KvAttendParams &p, hipStream_t stream) {
+    const uint32_t tiles = (uint32_t)(((uint64_t)p.max_new * p.group + kQueries - 1) / kQueries);
+    const int lds = (int)sizeof(PromptLds<kSq8, DP>);
+    auto *kernel = &kv_prompt_kernel<T, kSq8, DP>;
+    if (ensure_lds_limit(reinterpret_cast<const void *>(kernel), lds) != 0) return -1;
+    kernel<<<dim3(tiles * p.chunks, p.c.heads, p.c.batch), kThreads, lds, stream>>>(p, tiles);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+template <typename T, bool kSq8>
+int launch_dim(const KvAttendParams &p, hipStream_t stream) {
+    switch (kv_padded_dim(p.c.dim)) {
+        case 64: return launch<T, kSq8, 64>(p, stream);
+        case 128: return launch<T, kSq8, 128>(p, stream);
+        default: return launch<T, kSq8, 256>(p, stream);
+    }
+}
+
+}  // namespace
+
+// One workgroup for all rows of its queries where the queries fill the card;
+// else the rows are split until there are two workgroups a compute unit, with
+// at least 256 rows (4 tiles) each, and the partial results joined.
+void kv_prompt_split(KvAttendParams &p) {
+    const uint64_t tiles = ((uint64_t)p.max_new * p.group + kQueries - 1) / kQueries * p.c.heads * p.c.batch;
+    const uint32_t visible = p.window == 0xffffffffu
+                                 ? p.c.max_length
+                                 : (uint32_t)min((uint64_t)p.c.max_length, (uint64_t)p.sinks + p.window + kQueries / p.group);
+    uint64_t chunks = tiles ? ((uint64_t)kv_compute_units() * 2 + tiles - 1) / tiles : 1;
+    const uint32_t most = visible / 256u;
+    chunks = chunks < most ? chunks : most;
+    p.chunks = chunks ? (uint32_t)chunks : 1u;
+    p.chunk = 0;
+}
+
+int launch_kv_prompt(const KvAttendParams &p, uint32_t type, bool sq8, hipStream_t stream) {
+    if (p.tokens == 0 || p.max_new == 0 || p.c.batch == 0) return 0;
+    if (type == kKvBf16) return sq8 ? launch_dim<__bf16, true>(p, stream) : launch_dim<__bf16, false>(p, stream);
+    return sq8 ? launch_dim<_Float16, true>(p, stream) : launch_dim<_Float16, false>(p, stream);
+}
+
+}  // namespace tessa

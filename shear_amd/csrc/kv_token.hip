@@ -1,0 +1,502 @@
+// kv_token.hip -- attention of one new token for each sequence over the paged
+// cache, split over the cache's rows and joined.
+//
+// For head h of the cache and its G query heads:
+//   s_j = scale * q . k_j,  p_j = exp(s_j - m),  out = sum p_j v_j / sum p_j
+// over the visible rows j, in base 2 throughout (scale * log2(e) is one factor).
+// Each wave keeps a running maximum m, sum l and output O; the waves of a
+// workgroup are joined through LDS, workgroups of one (sequence, head) by
+// kv_finish_kernel.
+//
+// Every visible row is read once for up to 16 query heads, so the cache's
+// bytes bound it; nothing is staged in LDS but row places.
+//  * S^T = K Q^T on 16x16x32 instructions: the K operand is 16 bytes of a row
+//    per lane, straight from memory.  Query heads are the columns, so a lane
+//    holds logits of one head and the maximum, sum and rescaling are its own.
+//  * O^T = V^T P^T: the sum over rows may run in any order as long as both
+//    operands agree, so the logits' registers are the P^T operand as they
+//    stand.  V comes as whole rows (16 lanes a row, head_dim / 16 values each,
+//    eight rows a lane); the operand of instruction c is value c of each of
+//    the eight, one byte permute per two values.
+//  * P is given to the matrix instructions as the sum of two 16-bit parts (the
+//    rounded value and the rounded rest), because a single rounding of P would
+//    add an error as large as that of rounding the result; the instructions
+//    it costs are idle otherwise.
+//  * SQ8 rows: codes are whole numbers that both 16-bit types hold exactly.
+//    The key's scale multiplies the logit.  The value's scale v_j enters as
+//    w_j = exp2(s_j + log2 v_j - m), with m the running maximum of that sum, so w_j stays
+//    in range whatever the scales are; l sums w_j / v_j.
+//  * A row that the table leaves without a page, and a place of the list that
+//    names no further visible row, weighs nothing; its values are replaced by zeros
+//    (0 * NaN would be NaN).
+#include "kv_device.h"
+
+namespace tessa {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr uint32_t kTile = 32;  // rows of a wave's step
+
+template <int N>
+struct KvWords;  // N 32-bit words in one load
+template <>
+struct KvWords<1> {
+    uint32_t w[1];
+};
+template <>
+struct alignas(8) KvWords<2> {
+    uint32_t w[2];
+};
+template <>
+struct alignas(16) KvWords<4> {
+    uint32_t w[4];
+};
+template <>
+struct alignas(16) KvWords<8> {
+    uint32_t w[8];
+};
+
+// Row id of visible index i < v.count, or -1 (a place of the list that names no further row).
+__device__ __forceinline__ int32_t visible_row(const KvVisible &v, uint32_t i, const int32_t *list) {
+    if (i < v.first) return (int32_t)i;
+    if (i < v.before_list) return (int32_t)(v.last_begin + (i - v.first));
+    const int32_t r = list[i - v.before_list];
+    return r >= (int32_t)v.first && r < (int32_t)v.last_begin ? r : -1;
+}
+
+template <typename T, bool kSq8, int DP>
+__global__ __launch_bounds__(kThreads) void kv_token_kernel(KvAttendParams p) {
+    using E = KvElem<T>;
+    constexpr int kSteps = DP / 32;                 // matrix instructions of 16 logits
+    constexpr int kPer = DP / 16;                   // values of a row that a lane holds
+    constexpr int kKWords = kSq8 ? DP / 16 : DP / 8;  // words of a K row that a lane holds
+    constexpr int kVWords = kSq8 ? kPer / 4 : kPer / 2;
+    constexpr int kKLoads = kKWords / 4;
+    __shared__ uint32_t sh_place[kWaves][2][kTile];
+    __shared__ float sh_scale[kSq8 ? kWaves : 1][3][kTile];
+    __shared__ float sh_ml[kWaves][2][16];
+    extern __shared__ __align__(16) float sh_out[];  // [waves][heads of the block][DP]
+
+    const KvCacheParams &c = p.c;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t n = lane & 15u, g = lane >> 4;
+    const uint32_t blocks = (p.group + 15u) / 16u;
+    const uint32_t h = blockIdx.y / blocks, first_q = (blockIdx.y - h * blocks) * 16u, b = blockIdx.z;
+    const uint32_t heads = min(16u, p.group - first_q);
+    const KvVisible vis = kv_visible(p, kv_length(c, b));
+    const uint32_t begin = blockIdx.x * p.chunk, end = min(begin + p.chunk, vis.count);
+    if (begin >= vis.count && p.chunks > 1) return;  // the join counts the chunks by itself
+    const uint32_t rows = end > begin ? end - begin : 0u;
+    const uint32_t tiles = (rows + kTile - 1) / kTile;
+    const int32_t *list = p.listed ? p.listed + ((uint64_t)b * c.heads + h) * p.listed_count : nullptr;
+    const int32_t *table = c.table + (uint64_t)b * c.table_stride;
+
+    // Q operand: heads are columns; dims of step s as K's lanes hold them
+    const bool head_ok = n < heads;
+    kv_u4 qf[kSteps];
+    {
+        const char *q = p.q + (uint64_t)b * p.q_token + (uint64_t)(h * p.group + first_q + (head_ok ? n : 0u)) * p.q_head;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const uint32_t d = kSq8 ? (uint32_t)(s / 2) * 64u + g * 16u + (uint32_t)(s & 1) * 8u : (uint32_t)s * 32u + g * 8u;
+            const kv_u4 zero = {0, 0, 0, 0};
+            qf[s] = head_ok && d < c.dim ? *reinterpret_cast<const kv_u4 *>(q + 2u * d) : zero;
+        }
+    }
+    const char *kbase = c.keys.rows + (uint64_t)h * c.keys.head_units * 16u;
+    const char *vbase = c.values.rows + (uint64_t)h * c.values.head_units * 16u;
+    // byte of the lane's values in a row (lanes past the row repeat its start; their outputs are not stored)
+    const uint32_t vbyte = (n * kPer < c.dim ? n * kPer : 0u) * (kSq8 ? 1u : 2u);
+
+    float m = kKvNone, l = 0.0f;
+    kv_f4 acc[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) acc[i] = kv_f4{0, 0, 0, 0};
+
+    // row of the tile after next, page of the next tile: each load waits a whole step
+    const uint32_t l32 = lane & 31u;
+    auto row_of = [&](uint32_t tile) -> int32_t {
+        const uint32_t i = tile * kTile + l32;
+        return i < rows ? visible_row(vis, begin + i, list) : -1;
+    };
+    auto page_of = [&](int32_t row) -> int32_t { return row >= 0 ? table[(uint32_t)row >> c.page_shift] : -1; };
+    int32_t row = row_of(wave);
+    int32_t page = page_of(row);
+    int32_t next_row = row_of(wave + kWaves);
+
+    for (uint32_t tile = wave; tile < tiles; tile += kWaves) {
+        const uint32_t kplace = kv_place(c, c.keys, page, (uint32_t)row);
+        const uint32_t vplace = kv_place(c, c.values, page, (uint32_t)row);
+        const bool mine = kplace != kKvNoOffset;
+        const uint32_t valid = (uint32_t)__ballot(mine);  // lanes 32..63 repeat 0..31
+        if constexpr (kSq8) {
+            if (lane < kTile) {
+                float ks = 0.0f, vs = 1.0f;
+                if (mine) {
+                    ks = c.keys.scales[kv_scale_place(c, c.keys, page, (uint32_t)row, h)];
+                    vs = c.values.scales[kv_scale_place(c, c.values, page, (uint32_t)row, h)];
+                }
+                sh_scale[wave][0][lane] = ks * p.scale_log2;
+                vs = vs < kKvLeastScale ? kKvLeastScale : vs;  // a NaN stays
+                sh_scale[wave][1][lane] = log2f(vs);
+                sh_scale[wave][2][lane] = 1.0f / vs;
+            }
+        }
+        sh_place[wave][lane >> 5][l32] = mine ? (lane < kTile ? kplace : vplace) : 0u;  // row 0 of page 0 is there to read
+        kv_wave_sync();
+        row = next_row;
+        page = page_of(row);
+        next_row = row_of(tile + 2 * kWaves);
+
+        // K: rows n and 16 + n
+        KvWords<4> kw[2][kKLoads];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const char *src = kbase + (uint64_t)sh_place[wave][0][16 * t + n] * 16u;
+#pragma unroll
+            for (int s = 0; s < kKLoads; ++s) {
+                const uint32_t d = kSq8 ? (uint32_t)s * 64u + g * 16u : (uint32_t)s * 32u + g * 8u;
+                kw[t][s] = *reinterpret_cast<const KvWords<4> *>(src + (d < c.dim ? d : 0u) * (kSq8 ? 1u : 2u));
+            }
+        }
+        // V: rows 16 (j / 4) + 4 g + j % 4
+        KvWords<kVWords> vw[8];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const kv_u4 place = *reinterpret_cast<const kv_u4 *>(&sh_place[wave][1][16 * t + 4 * g]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                vw[4 * t + j] = *reinterpret_cast<const KvWords<kVWords> *>(vbase + (uint64_t)place[j] * 16u + vbyte);
+        }
+        if (DP != c.dim) {  // dims past the row meet zeros of Q and must be finite
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int s = 0; s < kKLoads; ++s) {
+                    const uint32_t d = kSq8 ? (uint32_t)s * 64u + g * 16u : (uint32_t)s * 32u + g * 8u;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) kw[t][s].w[w] = d < c.dim ? kw[t][s].w[w] : 0u;
+                }
+        }
+        // logits of rows 16 t + 4 g + i
+        float x[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            kv_f4 sacc = {0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                kv_u4 a;
+                if constexpr (kSq8) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t word = kw[t][s / 2].w[2 * (s & 1) + e / 2];
+                        a[e] = E::pack_codes(kv_code(word, 2 * (e & 1)), kv_code(word, 2 * (e & 1) + 1));
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) a[e] = kw[t][s].w[e];
+                }
+                sacc = E::mma16(a, qf[s], sacc);
+            }
+            if constexpr (kSq8) {
+                const kv_f4 ks = *reinterpret_cast<const kv_f4 *>(&sh_scale[wave][0][16 * t + 4 * g]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[t][i] = sacc[i] * ks[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[t][i] = sacc[i] * p.scale_log2;
+            }
+        }
+        if (valid != 0xffffffffu) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool ok = valid >> (16 * t + 4 * g + i) & 1u;
+                    if (!ok) x[t][i] = -INFINITY;
+#pragma unroll
+                    for (int w = 0; w < kVWords; ++w) vw[4 * t + i].w[w] = ok ? vw[4 * t + i].w[w] : 0u;
+                }
+        }
+        if (p.logits) {
+            float *at = p.logits + (((uint64_t)b * c.heads + h) * p.max_visible + begin + tile * kTile) * p.group + first_q + n;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t r = 16 * t + 4 * g + i;
+                    if (head_ok && tile * kTile + r < rows) at[(uint64_t)r * p.group] = x[t][i];
+                }
+        }
+        float inv[2][4];
+        if constexpr (kSq8) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const kv_f4 lv = *reinterpret_cast<const kv_f4 *>(&sh_scale[wave][1][16 * t + 4 * g]);
+                const kv_f4 iv = *reinterpret_cast<const kv_f4 *>(&sh_scale[wave][2][16 * t + 4 * g]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[t][i] += lv[i];
+                    inv[t][i] = iv[i];
+                }
+            }
+        }
+        float top = kKvNone;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, x[t][i]);
+        top = kv_max16(top);
+        if (__any(top > m + kKvLag)) {
+            const float higher = fmaxf(m, top);
+            const float f = kv_exp2(m - higher);
+            m = higher;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) acc[i] *= f;
+        }
+        kv_u4 hi, lo;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                const float w0 = kv_exp2(x[t][i] - m), w1 = kv_exp2(x[t][i + 1] - m);
+                if constexpr (kSq8)
+                    l = fmaf(w1, inv[t][i + 1], fmaf(w0, inv[t][i], l));
+                else
+                    l += w0 + w1;
+                const uint32_t r = E::pack(w0, w1);
+                hi[2 * t + i / 2] = r;
+                lo[2 * t + i / 2] = E::pack(w0 - E::low(r), w1 - E::high(r));
+            }
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            kv_u4 a;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (kSq8)
+                    a[j] = E::pack_codes(kv_code(vw[2 * j].w[e / 4], e & 3), kv_code(vw[2 * j + 1].w[e / 4], e & 3));
+                else
+                    a[j] = __builtin_amdgcn_perm(vw[2 * j + 1].w[e / 2], vw[2 * j].w[e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+            }
+            acc[e] = E::mma16(a, hi, acc[e]);
+            acc[e] = E::mma16(a, lo, acc[e]);
+        }
+    }
+    l = kv_sum16(l);
+
+    // join the waves: sums relative to the largest maximum
+    if (g == 0) {
+        sh_ml[wave][0][n] = m;
+        sh_ml[wave][1][n] = l;
+    }
+    __syncthreads();
+    float top = sh_ml[0][0][n];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sh_ml[w][0][n]);
+    const float f = kv_exp2(m - top);
+    if (head_ok) {
+        // the lane's values are dims kPer * 4 g .. of head n, in the order of the rows of the accumulators
+        float *o = sh_out + ((uint64_t)wave * heads + n) * DP + kPer * 4 * g;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < kPer; e += 4)
+                *reinterpret_cast<kv_f4 *>(o + kPer * i + e) =
+                    kv_f4{acc[e][i] * f, acc[e + 1][i] * f, acc[e + 2][i] * f, acc[e + 3][i] * f};
+    }
+    __syncthreads();
+    const uint64_t q0 = (uint64_t)b * p.q_heads + h * p.group + first_q;
+    for (uint32_t at = threadIdx.x; at < heads * (DP / 4); at += kThreads) {
+        const uint32_t head = at / (DP / 4), d = (at % (DP / 4)) * 4;
+        kv_f4 o = {0, 0, 0, 0};
+        float big = kKvNone, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            o += *reinterpret_cast<const kv_f4 *>(sh_out + ((uint64_t)w * heads + head) * DP + d);
+            big = fmaxf(big, sh_ml[w][0][head]);
+        }
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) sum += sh_ml[w][1][head] * kv_exp2(sh_ml[w][0][head] - big);
+        if (p.chunks > 1 || p.part_o) {
+            *reinterpret_cast<kv_f4 *>(p.part_o + ((q0 + head) * p.chunks + blockIdx.x) * DP + d) = o;
+            if (d == 0) {
+                p.part_ml[((q0 + head) * p.chunks + blockIdx.x) * 2] = big;
+                p.part_ml[((q0 + head) * p.chunks + blockIdx.x) * 2 + 1] = sum;
+            }
+        } else {
+            const float r = sum == 0.0f ? 0.0f : 1.0f / sum;
+            if (d < c.dim) {
+                const kv_u2 y = {E::pack(o[0] * r, o[1] * r), E::pack(o[2] * r, o[3] * r)};
+                *reinterpret_cast<kv_u2 *>(p.out + (uint64_t)b * p.out_token + (uint64_t)(h * p.group + first_q + head) * p.out_head +
+                                           2u * d) = y;
+            }
+            if (d == 0) p.lse[q0 + head] = sum == 0.0f ? -INFINITY : (big + log2f(sum)) * 0.69314718056f;
+        }
+    }
+}
+
+// Joins the partial results of a query: blocks below `joins` one (query) each,
+// out = sum_c exp2(m_c - m) O_c / sum_c exp2(m_c - m) l_c.  With weights the
+// other blocks turn the logits of 256 visible rows into weights and add them,
+// summed over the group's heads, to the caller's.
+constexpr int kJoinGroups = 8;  // partial results read side by side
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, uint32_t dp, uint32_t joins, uint32_t row_blocks,
+                                                             bool prompt) {
+    using E = KvElem<T>;
+    const KvCacheParams &c = p.c;
+    __shared__ float sh[kJoinGroups][256];
+    __shared__ float sh_m[kThreads], sh_l[kThreads];
+    const uint32_t t = threadIdx.x;
+    auto join_ml = [&](uint64_t query, uint32_t count, uint32_t first, uint32_t step, float &m, float &l) {
+        m = kKvNone;
+        for (uint32_t i = first; i < count; i += step) m = fmaxf(m, p.part_ml[(query * p.chunks + i) * 2]);
+        l = 0.0f;
+        for (uint32_t i = first; i < count; i += step) {
+            const float *ml = p.part_ml + (query * p.chunks + i) * 2;
+            l += ml[1] * kv_exp2(ml[0] - m);
+        }
+    };
+    if (blockIdx.x < joins) {
+        const uint64_t query = blockIdx.x;
+        const uint32_t token = (uint32_t)(query / p.q_heads), head = (uint32_t)(query - (uint64_t)token * p.q_heads);
+        uint32_t count = p.chunks;
+        if (!prompt) {
+            const uint32_t visible = kv_visible(p, kv_length(c, token)).count;
+            count = (visible + p.chunk - 1) / p.chunk;
+            if (p.chunks == 1) count = 1;
+        }
+        float m, l;
+        join_ml(query, count, t & 63u, 64, m, l);
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const float m2 = __shfl_xor(m, off), l2 = __shfl_xor(l, off);
+            const float big = fmaxf(m, m2);
+            l = l * kv_exp2(m - big) + l2 * kv_exp2(m2 - big);
+            m = big;
+        }
+        const uint32_t lanes = dp / 4, groups = min((uint32_t)kJoinGroups, (uint32_t)kThreads / lanes);
+        const uint32_t grp = t / lanes, d = (t % lanes) * 4;
+        kv_f4 o = {0, 0, 0, 0};
+        if (grp < groups) {
+            for (uint32_t i = grp; i < count; i += groups) {
+                const uint64_t at = query * p.chunks + i;
+                const float f = kv_exp2(p.part_ml[at * 2] - m);
+                o += *reinterpret_cast<const kv_f4 *>(p.part_o + at * dp + d) * f;
+            }
+            *reinterpret_cast<kv_f4 *>(&sh[grp][d]) = o;
+        }
+        __syncthreads();
+        if (t < lanes && d < c.dim) {
+            for (uint32_t i = 1; i < groups; ++i) o += *reinterpret_cast<const kv_f4 *>(&sh[i][d]);
+            const float r = l == 0.0f ? 0.0f : 1.0f / l;
+            const kv_u2 y = {E::pack(o[0] * r, o[1] * r), E::pack(o[2] * r, o[3] * r)};
+            *reinterpret_cast<kv_u2 *>(p.out + (uint64_t)token * p.out_token + (uint64_t)head * p.out_head + 2u * d) = y;
+        }
+        if (t == 0) p.lse[query] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
+        return;
+    }
+    // weights of 256 visible rows of one (sequence, head)
+    const uint32_t item = blockIdx.x - joins;
+    const uint32_t part = item % row_blocks, bh = item / row_blocks;
+    const uint32_t b = bh / c.heads, h = bh - b * c.heads;
+    const KvVisible vis = kv_visible(p, kv_length(c, b));
+    if (part * kThreads >= vis.count) return;
+    const uint32_t count = p.chunks == 1 ? 1u : (vis.count + p.chunk - 1) / p.chunk;
+    // a wave joins one query head at a time
+    for (uint32_t q = t >> 6; q < p.group; q += kThreads / 64) {
+        float m, l;
+        join_ml((uint64_t)b * p.q_heads + h * p.group + q, count, t & 63u, 64, m, l);
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const float m2 = __shfl_xor(m, off), l2 = __shfl_xor(l, off);
+            const float big = fmaxf(m, m2);
+            l = l * kv_exp2(m - big) + l2 * kv_exp2(m2 - big);
+            m = big;
+        }
+        if ((t & 63u) == 0u) {
+            sh_m[q] = m;
+            sh_l[q] = l == 0.0f ? 0.0f : 1.0f / l;
+        }
+    }
+    __syncthreads();
+    const uint32_t i = part * kThreads + t;
+    if (i >= vis.count) return;
+    const int32_t *list = p.listed ? p.listed + ((uint64_t)b * c.heads + h) * p.listed_count : nullptr;
+    const int32_t row = visible_row(vis, i, list);
+    if (row < 0) return;
+    const float *x = p.logits + (((uint64_t)b * c.heads + h) * p.max_visible + i) * p.group;
+    float sum = 0.0f;
+    for (uint32_t q = 0; q < p.group; ++q) {
+        // a row without a page has logits of -inf: no weight, also where the sum is 0
+        const float w = kv_exp2(x[q] - sh_m[q]) * sh_l[q];
+        sum += w;
+    }
+    float *at = p.weights + (uint64_t)b * p.weight_batch + (uint64_t)h * p.weight_head + (uint32_t)row;
+    if (i < vis.before_list)
+        *at += sum;
+    else
+        unsafeAtomicAdd(at, sum);  // a row that the list names twice counts twice
+}
+
+template <typename T, bool kSq8, int DP>
+int launch(const KvAttendParams &p, hipStream_t stream) {
+    const uint32_t blocks = (p.group + 15u) / 16u;
+    const dim3 grid(p.chunks, p.c.heads * blocks, p.c.batch);
+    const size_t lds = (size_t)kWaves * (p.group < 16u ? p.group : 16u) * DP * sizeof(float);
+    kv_token_kernel<T, kSq8, DP><<<grid, kThreads, lds, stream>>>(p);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+template <typename T, bool kSq8>
+int launch_dim(const KvAttendParams &p, hipStream_t stream) {
+    switch (kv_padded_dim(p.c.dim)) {
+        case 64: return launch<T, kSq8, 64>(p, stream);
+        case 128: return launch<T, kSq8, 128>(p, stream);
+        default: return launch<T, kSq8, 256>(p, stream);
+    }
+}
+
+}  // namespace
+
+uint32_t kv_padded_dim(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+// Chunks of at least 128 rows (a tile for each wave), as many as it takes to
+// have kPerCu workgroups for each compute unit: with fewer a ragged batch's
+// longest sequence runs alone at the end, with more the partial results and
+// their join cost what the balance gains.
+void kv_token_split(KvAttendParams &p) {
+    constexpr uint32_t kPerCu = 6, kLeast = 128;
+    const uint32_t columns = p.c.heads * ((p.group + 15u) / 16u) * p.c.batch;
+    const uint32_t most = (p.max_visible + kLeast - 1) / kLeast;
+    uint32_t chunks = ((uint32_t)kv_compute_units() * kPerCu + columns - 1) / columns;
+    chunks = chunks < most ? chunks : most;
+    chunks = chunks ? chunks : 1;
+    p.chunk = ((p.max_visible + chunks - 1) / chunks + kLeast - 1) / kLeast * kLeast;
+    if (!p.chunk) p.chunk = kLeast;
+    p.chunks = (p.max_visible + p.chunk - 1) / p.chunk;
+    if (!p.chunks) p.chunks = 1;
+}
+
+int launch_kv_token(const KvAttendParams &p, uint32_t type, bool sq8, hipStream_t stream) {
+    if (type == kKvBf16) return sq8 ? launch_dim<__bf16, true>(p, stream) : launch_dim<__bf16, false>(p, stream);
+    return sq8 ? launch_dim<_Float16, true>(p, stream) : launch_dim<_Float16, false>(p, stream);
+}
+
+int launch_kv_finish(const KvAttendParams &p, uint32_t type, bool prompt, hipStream_t stream) {
+    const uint32_t joins = (uint32_t)(p.tokens * p.q_heads);
+    const uint32_t row_blocks = p.weights && !prompt ? (p.max_visible + kThreads - 1) / kThreads : 0u;
+    const uint32_t blocks = joins + row_blocks * p.c.heads * p.c.batch;
+    const uint32_t dp = kv_padded_dim(p.c.dim);
+    if (type == kKvBf16)
+        kv_finish_kernel<__bf16><<<blocks, kThreads, 0, stream>>>(p, dp, joins, row_blocks, prompt);
+    else
+        kv_finish_kernel<_Float16><<<blocks, kThreads, 0, stream>>>(p, dp, joins, row_blocks, prompt);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+}  // namespace tessa
