@@ -189,10 +189,9 @@ tessa_status attend_of(const tessa_kv_cache *cache, const tessa_kv_sequences *se
         if (!a->offsets) KV_INVALID("kv attend: null offsets");
         p.offsets = a->offsets;
         p.max_new = a->max_new < a->tokens ? a->max_new : (uint32_t)a->tokens;
-        if (p.c.heads > kMaxGrid) KV_UNSUPPORTED("kv attend: %u heads", p.c.heads);
         kv_prompt_split(p);
-        if (((uint64_t)p.max_new * p.group / 128 + 1) * p.chunks > 0x7fffffffull)
-            KV_UNSUPPORTED("kv attend: %u new tokens", p.max_new);
+        if ((double)((uint64_t)p.max_new * p.group / 128 + 1) * p.chunks * p.c.heads * p.c.batch >= 2147483647.0)
+            KV_UNSUPPORTED("kv attend: %u new tokens for each of %u sequences", p.max_new, p.c.batch);
     } else {
         if (a->offsets) KV_INVALID("kv attend: single tokens take no offsets");
         if ((a->listed == nullptr) != (a->listed_count == 0)) KV_INVALID("kv attend: listed and listed_count go together");

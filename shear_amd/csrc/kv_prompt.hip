@@ -32,6 +32,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr uint32_t kQueries = 128;  // of a workgroup
 
+using lds_ptr = __attribute__((address_space(3))) void *;
 typedef short kv_s4 __attribute__((ext_vector_type(4)));
 
 // Piece (16 bytes) of an LDS row in which piece c of row r lies: the K reads
@@ -67,7 +68,13 @@ struct PromptLds {
     uint32_t marks[4][1 + kRows / 32];
 };
 
-template <typename T, bool kSq8, int DP>
+// Zeros that lanes read in the place of rows and dims that are not there.
+__device__ __attribute__((aligned(16))) const uint32_t kv_zeros[4] = {0, 0, 0, 0};
+
+// kWhole: each load of the workgroup lies in one page and rows have DP dims, so
+// that addresses are one scalar and a lane's constant; chosen where page_rows
+// is at least kRowsPer.
+template <typename T, bool kSq8, int DP, bool kWhole>
 __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(KvAttendParams p, uint32_t query_tiles) {
     using E = KvElem<T>;
     using Lds = PromptLds<kSq8, DP>;
@@ -75,17 +82,23 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
     constexpr int kSubs = (int)kRows / 32;       // 32 rows of logits each
     constexpr int kSteps = DP / 16;              // instructions along the dims
     constexpr int kBlocks = DP / 32;             // blocks of 32 dims of the output
-    constexpr int kPieces = kSq8 ? DP / 16 : DP / 8;  // 16-byte pieces of a row in memory
-    constexpr int kLoads = (int)kRows * kPieces / kThreads;  // of a thread, for K and for V each
-    constexpr int kRowsPer = kThreads / kPieces;  // rows of one load of the workgroup
+    constexpr uint32_t kPieces = kSq8 ? DP / 16 : DP / 8;  // 16-byte pieces of a row in memory
+    constexpr int kLoads = (int)(kRows * kPieces) / kThreads;  // of a thread, for K and for V each
+    constexpr uint32_t kRowsPer = kThreads / kPieces;  // rows of one load of the workgroup
     extern __shared__ __align__(16) char smem[];
     Lds &lds = *reinterpret_cast<Lds *>(smem);
 
     const KvCacheParams &c = p.c;
     const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6;
     const uint32_t n = lane & 31u, half = lane >> 5;
-    const uint32_t split = blockIdx.x % p.chunks, query_tile = query_tiles - 1u - blockIdx.x / p.chunks;
-    const uint32_t h = blockIdx.y, b = blockIdx.z;
+    // (sequence, head) pairs by eights, one for each XCD, whose L2 then holds its
+    // rows; within a pair the last queries, which see most rows, come first
+    const uint32_t pairs = c.heads * c.batch, per = query_tiles * p.chunks;
+    const uint32_t together = pairs % 8u == 0u ? 8u : pairs;
+    const uint32_t group = blockIdx.x / (together * per), in_group = blockIdx.x - group * together * per;
+    const uint32_t pair = group * together + in_group % together, item = in_group / together;
+    const uint32_t split = item % p.chunks, query_tile = query_tiles - 1u - item / p.chunks;
+    const uint32_t b = pair / c.heads, h = pair - b * c.heads;
     const uint32_t length = kv_length(c, b);
     const int64_t first_token = p.offsets[b];
     int64_t new64 = (int64_t)p.offsets[b + 1] - first_token;
@@ -103,7 +116,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
     const int32_t pos = row0 + (int32_t)my_token;
     const int32_t pos_first = row0 + (int32_t)(q0 / p.group);
     const int32_t pos_last = row0 + (int32_t)((min(q0 + kQueries, queries) - 1u) / p.group);
-    const int32_t wave_last = row0 + (int32_t)(min(q0 + wave * 32u + 31u, queries - 1u) / p.group);
+    const int32_t wave_last = __builtin_amdgcn_readfirstlane(row0 + (int32_t)(min(q0 + wave * 32u + 31u, queries - 1u) / p.group));
     // rows [0, sinks) and (pos - window, pos]
     const bool windowed = p.window != 0xffffffffu;
     const int32_t window = windowed ? (int32_t)p.window : 0;
@@ -125,8 +138,9 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
     const int32_t *table = c.table + (uint64_t)b * c.table_stride;
     const char *kbase = c.keys.rows + (uint64_t)h * c.keys.head_units * 16u;
     const char *vbase = c.values.rows + (uint64_t)h * c.values.head_units * 16u;
-    const uint32_t piece = t % kPieces, piece_row = t / kPieces;
-    const bool piece_ok = piece * (kSq8 ? 16u : 8u) < c.dim;
+    // the thread's place in a load of the workgroup: row i * kRowsPer + load_row, piece load_piece of the
+    // row in LDS (codes: of the row in memory)
+    const uint32_t load_piece = t % kPieces, load_row = t / kPieces;
 
     kv_u4 qf[kSteps];
     {
@@ -145,30 +159,88 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][e] = 0.0f;
 
+    // bytes of the thread's piece in a load (kWhole); K's order of pieces repeats after 16 rows
+    constexpr int kOffsets = kRowsPer >= 16 ? 1 : 16 / (int)kRowsPer;
+    uint32_t koffset[kOffsets];
+#pragma unroll
+    for (int i = 0; i < kOffsets; ++i)
+        koffset[i] = (load_row * c.keys.row_units + k_piece<DP>((uint32_t)i * kRowsPer + load_row, load_piece)) * 16u;
+    const uint32_t voffset = (load_row * c.values.row_units + v_piece<DP>(load_row, load_piece)) * 16u;
+
     int32_t pages[kLoads];
-    kv_u4 kr[kLoads], vr[kLoads];
+    kv_u4 kr[kSq8 ? kLoads : 1], vr[kSq8 ? kLoads : 1];  // codes on their way to LDS
     float ks = 0.0f, vs = 1.0f;
-    uint32_t missing = 0;  // loads of the thread whose row has no page
-    const kv_u4 zero4 = {0, 0, 0, 0};
+    bool special = false;  // some value was replaced by a zero
 
     auto read_pages = [&](uint32_t it) {
+        const uint32_t r0 = tile_row(it);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const uint32_t row = tile_row(it) + (uint32_t)i * kRowsPer + piece_row;
-            pages[i] = it < last_it && row < length ? table[row >> c.page_shift] : -1;
+            const uint32_t row = r0 + (uint32_t)i * kRowsPer + load_row;
+            if constexpr (kWhole)  // (the load's first row: one page for all threads)
+                pages[i] = it < last_it ? table[min(r0 + (uint32_t)i * kRowsPer, length - 1u) >> c.page_shift] : -1;
+            else
+                pages[i] = it < last_it && row < length ? table[row >> c.page_shift] : -1;
         }
     };
-    auto read_rows = [&](uint32_t it) {
+    // Starts the loads of a tile; 16-bit rows go to LDS without a register.
+    auto read_rows = [&](uint32_t it, uint32_t buf) {
         const uint32_t r0 = tile_row(it);
-        missing = 0;
+        if constexpr (kWhole) {
+            bool all = true;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) all &= (uint32_t)__builtin_amdgcn_readfirstlane(pages[i]) < c.pages;
+            if (all) {  // rows past the length are read too: finish_rows() clears their values
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    const uint32_t page = __builtin_amdgcn_readfirstlane(pages[i]);
+                    const uint32_t slot = (r0 + (uint32_t)i * kRowsPer) & ((1u << c.page_shift) - 1u);
+                    const char *kpage = kbase + (uint64_t)(page * c.keys.page_units + slot * c.keys.row_units) * 16u;
+                    const char *vpage = vbase + (uint64_t)(page * c.values.page_units + slot * c.values.row_units) * 16u;
+                    const uint32_t at = ((uint32_t)i * kThreads + wave * 64u) * 16u;
+                    __builtin_amdgcn_global_load_lds(static_cast<const void *>(kpage + koffset[i & (kOffsets - 1)]),
+                                                     (lds_ptr)(lds.k[buf] + at), 16, 0, 0);
+                    __builtin_amdgcn_global_load_lds(static_cast<const void *>(vpage + voffset), (lds_ptr)(lds.v[buf] + at), 16, 0, 0);
+                }
+                return;
+            }
+        }
+        uint32_t missing = 0;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const uint32_t row = r0 + (uint32_t)i * kRowsPer + piece_row;
-            if (row < length && (uint32_t)pages[i] >= c.pages) missing |= 1u << i;
-            const uint32_t kp = kv_place(c, c.keys, pages[i], row), vp = kv_place(c, c.values, pages[i], row);
-            const bool ok = piece_ok && kp != kKvNoOffset;
-            kr[i] = ok ? *reinterpret_cast<const kv_u4 *>(kbase + ((uint64_t)kp + piece) * 16u) : zero4;
-            vr[i] = ok ? *reinterpret_cast<const kv_u4 *>(vbase + ((uint64_t)vp + piece) * 16u) : zero4;
+            const uint32_t r = (uint32_t)i * kRowsPer + load_row;
+            const uint32_t row = r0 + r;
+            const bool there = (uint32_t)pages[i] < c.pages;
+            missing |= (uint32_t)(!there && row < length) << i;
+            const uint32_t slot = row & ((1u << c.page_shift) - 1u), page = (uint32_t)pages[i];
+            const uint64_t kp = (uint64_t)(page * c.keys.page_units + slot * c.keys.row_units);
+            const uint64_t vp = (uint64_t)(page * c.values.page_units + slot * c.values.row_units);
+            const uint32_t kpiece = kSq8 ? load_piece : k_piece<DP>(r, load_piece);
+            const uint32_t vpiece = kSq8 ? load_piece : v_piece<DP>(r, load_piece);
+            const char *zeros = reinterpret_cast<const char *>(kv_zeros);
+            const uint32_t wide = kSq8 ? 16u : 8u;  // dims of a piece
+            const char *ksrc = there && kpiece * wide < c.dim ? kbase + (kp + kpiece) * 16u : zeros;
+            const char *vsrc = there && vpiece * wide < c.dim ? vbase + (vp + vpiece) * 16u : zeros;
+            if constexpr (kSq8) {
+                kr[i] = *reinterpret_cast<const kv_u4 *>(ksrc);
+                vr[i] = *reinterpret_cast<const kv_u4 *>(vsrc);
+            } else if constexpr (kWhole) {
+                const uint32_t at = ((uint32_t)i * kThreads + t) * 16u;
+                *reinterpret_cast<kv_u4 *>(lds.k[buf] + at) = *reinterpret_cast<const kv_u4 *>(ksrc);
+                *reinterpret_cast<kv_u4 *>(lds.v[buf] + at) = *reinterpret_cast<const kv_u4 *>(vsrc);
+            } else {
+                // the wave's 64 pieces land one after the other
+                const uint32_t at = ((uint32_t)i * kThreads + wave * 64u) * 16u;
+                __builtin_amdgcn_global_load_lds(static_cast<const void *>(ksrc), (lds_ptr)(lds.k[buf] + at), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds(static_cast<const void *>(vsrc), (lds_ptr)(lds.v[buf] + at), 16, 0, 0);
+            }
+        }
+        if (missing) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const uint32_t r = (uint32_t)i * kRowsPer + load_row;
+                if (missing >> i & 1u) atomicOr(&lds.marks[it & 3u][1 + r / 32u], 1u << (r & 31u));
+            }
         }
         if constexpr (kSq8) {
             if (t < kRows) {
@@ -183,36 +255,13 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
             }
         }
     };
-    auto write_rows = [&](uint32_t it, uint32_t buf) {
-        const uint32_t r0 = tile_row(it);
-        const bool watch = masked(r0);
-        uint32_t *marks = lds.marks[it & 3u];
-        if (piece == 0) {
+    // Completes a tile whose loads were started: codes become 16-bit values; in a
+    // tile with a mask infinities and NaN become zeros.
+    auto finish_rows = [&](uint32_t it, uint32_t buf) {
+        if constexpr (kSq8) {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                const uint32_t r = (uint32_t)i * kRowsPer + piece_row;
-                if (missing >> i & 1u) atomicOr(&marks[1 + r / 32u], 1u << (r & 31u));
-            }
-        }
-        if constexpr (!kSq8) {
-            if (watch) {  // infinities and NaN: zeros here, add_special() adds them
-                bool found = false;
-#pragma unroll
-                for (int i = 0; i < kLoads; ++i)
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const bool lo = special_half<T>(vr[i][w]), hi = special_half<T>(vr[i][w] >> 16);
-                        if (lo) vr[i][w] &= 0xffff0000u;
-                        if (hi) vr[i][w] &= 0xffffu;
-                        found |= lo | hi;
-                    }
-                if (found) marks[0] = 1u;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const uint32_t r = (uint32_t)i * kRowsPer + piece_row;
-            if constexpr (kSq8) {
+                const uint32_t r = (uint32_t)i * kRowsPer + load_row;
 #pragma unroll
                 for (int part = 0; part < 2; ++part) {
                     kv_u4 k4, v4;
@@ -222,16 +271,11 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                         k4[e] = E::pack_codes(kv_code(kw, 2 * (e & 1)), kv_code(kw, 2 * (e & 1) + 1));
                         v4[e] = E::pack_codes(kv_code(vw, 2 * (e & 1)), kv_code(vw, 2 * (e & 1) + 1));
                     }
-                    const uint32_t to = 2u * piece + (uint32_t)part;
+                    const uint32_t to = 2u * load_piece + (uint32_t)part;
                     *reinterpret_cast<kv_u4 *>(&lds.k[buf][r * DP * 2 + k_piece<DP>(r, to) * 16u]) = k4;
                     *reinterpret_cast<kv_u4 *>(&lds.v[buf][r * DP * 2 + v_piece<DP>(r, to) * 16u]) = v4;
                 }
-            } else {
-                *reinterpret_cast<kv_u4 *>(&lds.k[buf][r * DP * 2 + k_piece<DP>(r, piece) * 16u]) = kr[i];
-                *reinterpret_cast<kv_u4 *>(&lds.v[buf][r * DP * 2 + v_piece<DP>(r, piece) * 16u]) = vr[i];
             }
-        }
-        if constexpr (kSq8) {
             if (t < kRows) {
                 // a NaN scale: its row is NaN to those that see it, which the logit alone carries
                 const bool bad = vs != vs;
@@ -240,42 +284,37 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                 lds.scale[buf][1][t] = log2f(s);
                 lds.scale[buf][2][t] = 1.0f / s;
             }
-        }
-    };
-    auto sees = [&](int32_t row) { return row <= pos && (!windowed || row < sinks || row > pos - window); };
-    auto add_special = [&](uint32_t r0) {
-        for (uint32_t r = 0; r < kRows; ++r) {
-            const uint32_t row = r0 + r;
-            if (row >= length) break;
-            const int32_t page = table[row >> c.page_shift];
-            const uint32_t place = kv_place(c, c.values, page, row);
-            if (place == kKvNoOffset) continue;
-            const bool seen = sees((int32_t)row);
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (masked(tile_row(it))) {
+                bool found = false;
 #pragma unroll
-            for (int i = 0; i < kBlocks; ++i)
+                for (int i = 0; i < kLoads; ++i) {
+                    kv_u4 *at = reinterpret_cast<kv_u4 *>(lds.v[buf] + ((uint32_t)i * kThreads + t) * 16u);
+                    kv_u4 x = *at;
+                    bool hit = false;
 #pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    const uint32_t d = (uint32_t)i * 32u + 8u * (e / 4) + 4u * half;
-                    if (d < c.dim) {
-                        const kv_u2 x = *reinterpret_cast<const kv_u2 *>(vbase + (uint64_t)place * 16u + 2u * d);
-                        if (seen) {
-                            if (special_half<T>(x[0])) acc[i][e] += E::low(x[0]);
-                            if (special_half<T>(x[0] >> 16)) acc[i][e + 1] += E::high(x[0]);
-                            if (special_half<T>(x[1])) acc[i][e + 2] += E::low(x[1]);
-                            if (special_half<T>(x[1] >> 16)) acc[i][e + 3] += E::high(x[1]);
-                        }
+                    for (int w = 0; w < 4; ++w) {
+                        const bool lo = special_half<T>(x[w]), hi = special_half<T>(x[w] >> 16);
+                        if (lo) x[w] &= 0xffff0000u;
+                        if (hi) x[w] &= 0xffffu;
+                        hit |= lo | hi;
                     }
+                    if (hit) *at = x;
+                    found |= hit && tile_row(it) + (uint32_t)i * kRowsPer + load_row < length;
                 }
+                if (found) lds.marks[it & 3u][0] = 1u;
+            }
         }
     };
 
     if (first_it < last_it) {
         if (t < 4u * (1u + kRows / 32u)) lds.marks[0][t] = 0u;
         read_pages(first_it);
-        read_rows(first_it);
-        read_pages(first_it + 1);
         __syncthreads();  // the marks are cleared
-        write_rows(first_it, 0);
+        read_rows(first_it, 0);
+        read_pages(first_it + 1);
+        finish_rows(first_it, 0);
         __syncthreads();
     }
     for (uint32_t it = first_it; it < last_it; ++it) {
@@ -283,7 +322,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
         const uint32_t r0 = tile_row(it);
         const bool more = it + 1 < last_it;
         if (more) {
-            read_rows(it + 1);
+            read_rows(it + 1, buf ^ 1u);
             read_pages(it + 2);
         }
         const bool mask = masked(r0);
@@ -315,31 +354,48 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                         for (int i = 0; i < 4; ++i) x[u][e + i] = fmaf(x[u][e + i], k4[i], v4[i]);
                     }
             }
-            const float factor = kSq8 ? 1.0f : p.scale_log2;
             if (mask) {
+                // rows relative to the lane's first; opaque, so that the comparisons stay in this branch
+                int32_t last = pos - (int32_t)r0 - 4 * (int32_t)half;  // r is seen if last - width < r <= last,
+                int32_t shown = min(sinks - (int32_t)r0 - 4 * (int32_t)half, last + 1);  // or below this
+                const uint32_t width = windowed ? (uint32_t)window : 0x80000000u;
+                asm volatile("" : "+v"(last), "+v"(shown));
+                if ((int32_t)r0 < sinks) {
 #pragma unroll
-                for (int u = 0; u < kSubs; ++u)
+                    for (int u = 0; u < kSubs; ++u)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int32_t row = (int32_t)r0 + 32 * u + 8 * (e / 4) + 4 * (int32_t)half + e % 4;
-                        if (!sees(row)) x[u][e] = -INFINITY;
-                    }
+                        for (int e = 0; e < 16; ++e) {
+                            const int32_t r = 32 * u + 8 * (e / 4) + e % 4;
+                            if ((uint32_t)(last - r) >= width && r >= shown) x[u][e] = -INFINITY;
+                        }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int32_t r = 32 * u + 8 * (e / 4) + e % 4;
+                            if ((uint32_t)(last - r) >= width) x[u][e] = -INFINITY;
+                        }
+                }
             }
 #pragma unroll
             for (int u = 0; u < kSubs; ++u) {
-                const uint32_t gone = marks[1 + u];
-                if (gone) {
+                uint32_t gone = marks[1 + u];
+                if (__any(gone != 0u)) {
+                    gone >>= 4u * half;
+                    asm volatile("" : "+v"(gone));
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        if (gone >> (8u * (e / 4) + 4u * half + e % 4) & 1u) x[u][e] = -INFINITY;
+                        if (gone >> (8 * (e / 4) + e % 4) & 1u) x[u][e] = -INFINITY;
                 }
             }
-            float top = x[0][0] * factor;
+            const float factor = kSq8 ? 1.0f : p.scale_log2;
+            float top = x[0][0];
 #pragma unroll
             for (int u = 0; u < kSubs; ++u)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) top = fmaxf(top, x[u][e] * factor);
-            top = kv_max32(fmaxf(top, kKvNone));
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, x[u][e]);
+            top = kv_max32(fmaxf(top * factor, kKvNone));
             if (__any(top > m + kKvLag)) {
                 const float higher = fmaxf(m, top);
                 const float f = kv_exp2(m - higher);
@@ -387,14 +443,43 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                 }
             }
             if constexpr (!kSq8)
-                if (mask && marks[0]) add_special(r0);
+                if (mask) special |= marks[0] != 0u;
         }
-        if (more) {
-            write_rows(it + 1, buf ^ 1u);
-            __syncthreads();
-        }
+        if (more) finish_rows(it + 1, buf ^ 1u);
+        __syncthreads();
     }
     l = kv_sum32(l);
+
+    if constexpr (!kSq8) {
+        // values that were replaced by zeros: added to the queries that see their rows
+        if (__any(special)) {
+#pragma unroll 1
+            for (uint32_t it = first_it; it < last_it; ++it) {
+                const uint32_t r0 = tile_row(it);
+                if (!masked(r0)) continue;
+#pragma unroll 1
+                for (uint32_t row = r0; row < min(r0 + kRows, length); ++row) {
+                    const uint32_t place = kv_place(c, c.values, table[row >> c.page_shift], row);
+                    if (place == kKvNoOffset) continue;
+                    const int32_t r = (int32_t)row;
+                    const bool seen = r <= pos && (!windowed || r < sinks || r > pos - window);
+#pragma unroll
+                    for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4) {
+                            const uint32_t d = (uint32_t)i * 32u + 2u * (uint32_t)e + 4u * half;
+                            const kv_u2 x = *reinterpret_cast<const kv_u2 *>(
+                                d < c.dim ? vbase + (uint64_t)place * 16u + 2u * d : reinterpret_cast<const char *>(kv_zeros));
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) {
+                                const float y = w & 1 ? E::high(x[w / 2]) : E::low(x[w / 2]);
+                                acc[i][e + w] += seen && !(fabsf(y) < INFINITY) ? y : 0.0f;
+                            }
+                        }
+                }
+            }
+        }
+    }
 
     if (!query_ok) return;
     const uint64_t token = (uint64_t)first_token + my_token;
@@ -428,22 +513,29 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
     if (half == 0) p.lse[query] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
 }
 
-template <typename T, bool kSq8, int DP>
+template <typename T, bool kSq8, int DP, bool kWhole>
 int launch(const KvAttendParams &p, hipStream_t stream) {
     const uint32_t tiles = (uint32_t)(((uint64_t)p.max_new * p.group + kQueries - 1) / kQueries);
     const int lds = (int)sizeof(PromptLds<kSq8, DP>);
-    auto *kernel = &kv_prompt_kernel<T, kSq8, DP>;
+    auto *kernel = &kv_prompt_kernel<T, kSq8, DP, kWhole>;
     if (ensure_lds_limit(reinterpret_cast<const void *>(kernel), lds) != 0) return -1;
-    kernel<<<dim3(tiles * p.chunks, p.c.heads, p.c.batch), kThreads, lds, stream>>>(p, tiles);
+    kernel<<<tiles * p.chunks * p.c.heads * p.c.batch, kThreads, lds, stream>>>(p, tiles);
     return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+template <typename T, bool kSq8, int DP>
+int launch_pages(const KvAttendParams &p, hipStream_t stream) {
+    if constexpr (!kSq8)
+        if (p.c.dim == DP && (1u << p.c.page_shift) >= kThreads * 8u / DP) return launch<T, kSq8, DP, true>(p, stream);
+    return launch<T, kSq8, DP, false>(p, stream);
 }
 
 template <typename T, bool kSq8>
 int launch_dim(const KvAttendParams &p, hipStream_t stream) {
     switch (kv_padded_dim(p.c.dim)) {
-        case 64: return launch<T, kSq8, 64>(p, stream);
-        case 128: return launch<T, kSq8, 128>(p, stream);
-        default: return launch<T, kSq8, 256>(p, stream);
+        case 64: return launch_pages<T, kSq8, 64>(p, stream);
+        case 128: return launch_pages<T, kSq8, 128>(p, stream);
+        default: return launch_pages<T, kSq8, 256>(p, stream);
     }
 }
 
