@@ -46,6 +46,19 @@ __device__ __forceinline__ uint32_t v_piece(uint32_t r, uint32_t c) {
     return DP == 64 ? c ^ (((r >> 1) & 1u) << 2) : c ^ ((r & 3u) << 2);
 }
 
+// Reads of LDS.  Their pointers are `restrict`, which tells the compiler that no
+// load to LDS in flight writes there; through plain pointers it would wait for
+// the next tile's loads before the first read of this one.  The kernel itself waits
+// for a tile's loads before the barrier after which the tile is read.
+template <typename V>
+__device__ __forceinline__ V lds_read(const V *__restrict__ at) {
+    return *at;
+}
+__device__ __forceinline__ kv_u2 lds_read_transposed(const char *__restrict__ at) {
+    const kv_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) kv_s4 *)const_cast<char *>(at));
+    return __builtin_bit_cast(kv_u2, x);
+}
+
 template <typename T>
 __device__ __forceinline__ bool special_half(uint32_t x) {
     return (x & KvElem<T>::kExponent) == KvElem<T>::kExponent;
@@ -172,16 +185,12 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
     float ks = 0.0f, vs = 1.0f;
     bool special = false;  // some value was replaced by a zero
 
+    // Page ids for a tile (past the end: those of the last row), read a tile before they are used.
     auto read_pages = [&](uint32_t it) {
-        const uint32_t r0 = tile_row(it);
+        const uint32_t r0 = tile_row(min(it, last_it - 1u));
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const uint32_t row = r0 + (uint32_t)i * kRowsPer + load_row;
-            if constexpr (kWhole)  // (the load's first row: one page for all threads)
-                pages[i] = it < last_it ? table[min(r0 + (uint32_t)i * kRowsPer, length - 1u) >> c.page_shift] : -1;
-            else
-                pages[i] = it < last_it && row < length ? table[row >> c.page_shift] : -1;
-        }
+        for (int i = 0; i < kLoads; ++i)  // kWhole: one page for all threads
+            pages[i] = table[min(r0 + (uint32_t)i * kRowsPer + (kWhole ? 0u : load_row), length - 1u) >> c.page_shift];
     };
     // Starts the loads of a tile; 16-bit rows go to LDS without a register.
     auto read_rows = [&](uint32_t it, uint32_t buf) {
@@ -210,7 +219,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
         for (int i = 0; i < kLoads; ++i) {
             const uint32_t r = (uint32_t)i * kRowsPer + load_row;
             const uint32_t row = r0 + r;
-            const bool there = (uint32_t)pages[i] < c.pages;
+            const bool there = row < length && (uint32_t)pages[i] < c.pages;
             missing |= (uint32_t)(!there && row < length) << i;
             const uint32_t slot = row & ((1u << c.page_shift) - 1u), page = (uint32_t)pages[i];
             const uint64_t kp = (uint64_t)(page * c.keys.page_units + slot * c.keys.row_units);
@@ -316,12 +325,16 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
         read_pages(first_it + 1);
         finish_rows(first_it, 0);
         __syncthreads();
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(qf[s]));  // has arrived: no wait for it in the loop
     }
     for (uint32_t it = first_it; it < last_it; ++it) {
         const uint32_t buf = (it - first_it) & 1u;
         const uint32_t r0 = tile_row(it);
         const bool more = it + 1 < last_it;
         if (more) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) asm volatile("" : "+v"(pages[i]));  // their reads had a tile's time
             read_rows(it + 1, buf ^ 1u);
             read_pages(it + 2);
         }
@@ -338,7 +351,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                 const uint32_t r = 32u * u + n;
 #pragma unroll
                 for (int s = 0; s < kSteps; ++s) {
-                    const kv_u4 a = *reinterpret_cast<const kv_u4 *>(&lds.k[buf][r * DP * 2 + k_piece<DP>(r, 2u * s + half) * 16u]);
+                    const kv_u4 a = lds_read(reinterpret_cast<const kv_u4 *>(&lds.k[buf][r * DP * 2 + k_piece<DP>(r, 2u * s + half) * 16u]));
                     x[u] = E::mma32(a, qf[s], x[u]);
                 }
             }
@@ -348,8 +361,8 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
 #pragma unroll
                     for (int e = 0; e < 16; e += 4) {
                         const uint32_t r = 32u * u + 2u * e + 4u * half;
-                        const kv_f4 k4 = *reinterpret_cast<const kv_f4 *>(&lds.scale[buf][0][r]);
-                        const kv_f4 v4 = *reinterpret_cast<const kv_f4 *>(&lds.scale[buf][1][r]);
+                        const kv_f4 k4 = lds_read(reinterpret_cast<const kv_f4 *>(&lds.scale[buf][0][r]));
+                        const kv_f4 v4 = lds_read(reinterpret_cast<const kv_f4 *>(&lds.scale[buf][1][r]));
 #pragma unroll
                         for (int i = 0; i < 4; ++i) x[u][e + i] = fmaf(x[u][e + i], k4[i], v4[i]);
                     }
@@ -380,8 +393,8 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
             }
 #pragma unroll
             for (int u = 0; u < kSubs; ++u) {
-                uint32_t gone = marks[1 + u];
-                if (__any(gone != 0u)) {
+                uint32_t gone = lds_read(&marks[1 + u]);
+                if (__builtin_amdgcn_readfirstlane(gone)) {
                     gone >>= 4u * half;
                     asm volatile("" : "+v"(gone));
 #pragma unroll
@@ -413,37 +426,41 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                     const float w0 = kv_exp2(fmaf(x[u][e], factor, -m)), w1 = kv_exp2(fmaf(x[u][e + 1], factor, -m));
                     if constexpr (kSq8) {
                         const uint32_t r = 32u * u + 8u * (e / 4) + 4u * half + e % 4;
-                        sum = fmaf(w0, lds.scale[buf][2][r], sum);
-                        sum = fmaf(w1, lds.scale[buf][2][r + 1], sum);
+                        sum = fmaf(w0, lds_read(&lds.scale[buf][2][r]), sum);
+                        sum = fmaf(w1, lds_read(&lds.scale[buf][2][r + 1]), sum);
                     } else {
                         sum += w0 + w1;
                     }
                     pf[2 * u + e / 8][(e % 8) / 2] = E::pack(w0, w1);
                 }
             l += sum;
-            // V^T of dims 32 i + n: rows 16 k + 4 half + {0..3}, + 8
+            // V^T of dims 32 i + n: rows 16 k + 4 half + {0..3}, + 8; read a block ahead
+            {
+                kv_u4 a[kBlocks][2 * kSubs];
+                auto read = [&](int i) {
 #pragma unroll
-            for (int i = 0; i < kBlocks; ++i) {
+                    for (int k = 0; k < 2 * kSubs; ++k)
 #pragma unroll
-                for (int k = 0; k < 2 * kSubs; ++k) {
-                    kv_u4 a;
+                        for (int part = 0; part < 2; ++part) {
+                            // of its 16-lane group, lane 4 j + q reads values 4 q .. of row j
+                            const uint32_t r = 16u * k + 8u * part + 4u * half + ((lane & 15u) >> 2);
+                            const uint32_t d = 32u * i + 16u * ((lane >> 4) & 1u) + 4u * (lane & 3u);
+                            const kv_u2 y = lds_read_transposed(
+                                &lds.v[buf][r * DP * 2 + v_piece<DP>(r, d / 8u) * 16u + (d & 7u) * 2u]);
+                            a[i][k][2 * part] = y[0];
+                            a[i][k][2 * part + 1] = y[1];
+                        }
+                };
+                read(0);
 #pragma unroll
-                    for (int part = 0; part < 2; ++part) {
-                        // of its 16-lane group, lane 4 j + q reads values 4 q .. of row j
-                        const uint32_t r = 16u * k + 8u * part + 4u * half + ((lane & 15u) >> 2);
-                        const uint32_t d = 32u * i + 16u * ((lane >> 4) & 1u) + 4u * (lane & 3u);
-                        const char *src = &lds.v[buf][r * DP * 2 + v_piece<DP>(r, d / 8u) * 16u + (d & 7u) * 2u];
-                        const kv_s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (__attribute__((address_space(3))) kv_s4 *)const_cast<char *>(src));
-                        const kv_u2 y2 = __builtin_bit_cast(kv_u2, y);
-                        a[2 * part] = y2[0];
-                        a[2 * part + 1] = y2[1];
-                    }
-                    acc[i] = E::mma32(a, pf[k], acc[i]);
+                for (int i = 0; i < kBlocks; ++i) {
+                    if (i + 1 < kBlocks) read(i + 1);
+#pragma unroll
+                    for (int k = 0; k < 2 * kSubs; ++k) acc[i] = E::mma32(a[i][k], pf[k], acc[i]);
                 }
             }
             if constexpr (!kSq8)
-                if (mask) special |= marks[0] != 0u;
+                if (mask) special |= lds_read(&marks[0]) != 0u;
         }
         if (more) finish_rows(it + 1, buf ^ 1u);
         __syncthreads();
