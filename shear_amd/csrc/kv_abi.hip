@@ -13,15 +13,15 @@ using namespace tessa;
 
 namespace tessa {
 
-// Compute units of the current device (256 where it cannot be asked).
+// Compute units of the first device (256 where it cannot be asked): what splits are planned for.
 int kv_compute_units() {
-    int dev = 0, n = 0;
-    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
-        n <= 0) {
+    static const int units = [] {
+        int n = 0;
+        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, 0) == hipSuccess && n > 0) return n;
         (void)hipGetLastError();
         return 256;
-    }
-    return n;
+    }();
+    return units;
 }
 
 }  // namespace tessa
@@ -207,7 +207,7 @@ tessa_status attend_of(const tessa_kv_cache *cache, const tessa_kv_sequences *se
         p.max_visible = (uint32_t)visible;
         if ((uint64_t)p.c.heads * ((p.group + 15u) / 16u) > kMaxGrid) KV_UNSUPPORTED("kv attend: %u query heads", a->q_heads);
         kv_token_split(p);
-        const uint64_t blocks = (visible + 255) / 256 * p.c.heads * p.c.batch + a->tokens * a->q_heads;
+        const uint64_t blocks = (visible + 255) / 256 * p.c.heads * p.c.batch + a->tokens * a->q_heads * 4u;
         if (blocks > 0x7fffffffull) KV_UNSUPPORTED("kv attend: batch %u of %llu rows", p.c.batch, (unsigned long long)visible);
         if (p.weights) logits = round_up(visible * p.c.heads * p.c.batch * p.group * sizeof(float));
     }

@@ -338,66 +338,77 @@ __global__ __launch_bounds__(kThreads) void kv_token_kernel(KvAttendParams p) {
     }
 }
 
-// Joins the partial results of a query: blocks below `joins` one (query) each,
-// out = sum_c exp2(m_c - m) O_c / sum_c exp2(m_c - m) l_c.  With weights the
-// other blocks turn the logits of 256 visible rows into weights and add them,
-// summed over the group's heads, to the caller's.
-constexpr int kJoinGroups = 8;  // partial results read side by side
+// Joins the partial results of a query, out = sum_c exp2(m_c - m) O_c / sum_c
+// exp2(m_c - m) l_c: blocks below `joins`, one for kJoinDims dims of a query, so
+// that few queries with many parts use many compute units, and the parts of a
+// query are read kJoinGroups side by side.  With weights the other blocks turn the
+// logits of 256 visible rows into weights and add them, summed over the group's
+// heads, to the caller's.
+constexpr uint32_t kJoinDims = 64;
+constexpr uint32_t kJoinGroups = kThreads / (kJoinDims / 4);  // 16
+
+// Largest maximum and sum of a query's parts, in all lanes of a wave.
+__device__ __forceinline__ void join_parts(const KvAttendParams &p, uint64_t query, uint32_t count, float &m, float &l) {
+    m = kKvNone;
+    l = 0.0f;
+    for (uint32_t i = threadIdx.x & 63u; i < count; i += 64) {
+        const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + (query * p.chunks + i) * 2);
+        const float big = fmaxf(m, ml.x);
+        l = l * kv_exp2(m - big) + ml.y * kv_exp2(ml.x - big);
+        m = big;
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const float m2 = __shfl_xor(m, off), l2 = __shfl_xor(l, off);
+        const float big = fmaxf(m, m2);
+        l = l * kv_exp2(m - big) + l2 * kv_exp2(m2 - big);
+        m = big;
+    }
+}
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, uint32_t dp, uint32_t joins, uint32_t row_blocks,
                                                              bool prompt) {
     using E = KvElem<T>;
     const KvCacheParams &c = p.c;
-    __shared__ float sh[kJoinGroups][256];
+    __shared__ __align__(16) float sh[kJoinGroups][kJoinDims];
     __shared__ float sh_m[kThreads], sh_l[kThreads];
     const uint32_t t = threadIdx.x;
-    auto join_ml = [&](uint64_t query, uint32_t count, uint32_t first, uint32_t step, float &m, float &l) {
-        m = kKvNone;
-        for (uint32_t i = first; i < count; i += step) m = fmaxf(m, p.part_ml[(query * p.chunks + i) * 2]);
-        l = 0.0f;
-        for (uint32_t i = first; i < count; i += step) {
-            const float *ml = p.part_ml + (query * p.chunks + i) * 2;
-            l += ml[1] * kv_exp2(ml[0] - m);
-        }
-    };
     if (blockIdx.x < joins) {
-        const uint64_t query = blockIdx.x;
+        const uint32_t slices = (c.dim + kJoinDims - 1) / kJoinDims;
+        const uint64_t query = blockIdx.x / slices;
+        const uint32_t slice = blockIdx.x - (uint32_t)query * slices;
         const uint32_t token = (uint32_t)(query / p.q_heads), head = (uint32_t)(query - (uint64_t)token * p.q_heads);
         uint32_t count = p.chunks;
-        if (!prompt) {
-            const uint32_t visible = kv_visible(p, kv_length(c, token)).count;
-            count = (visible + p.chunk - 1) / p.chunk;
-            if (p.chunks == 1) count = 1;
-        }
+        if (!prompt && p.chunks > 1) count = (kv_visible(p, kv_length(c, token)).count + p.chunk - 1) / p.chunk;
         float m, l;
-        join_ml(query, count, t & 63u, 64, m, l);
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const float m2 = __shfl_xor(m, off), l2 = __shfl_xor(l, off);
-            const float big = fmaxf(m, m2);
-            l = l * kv_exp2(m - big) + l2 * kv_exp2(m2 - big);
-            m = big;
-        }
-        const uint32_t lanes = dp / 4, groups = min((uint32_t)kJoinGroups, (uint32_t)kThreads / lanes);
-        const uint32_t grp = t / lanes, d = (t % lanes) * 4;
+        join_parts(p, query, count, m, l);
+        const uint32_t grp = t / (kJoinDims / 4), d4 = (t % (kJoinDims / 4)) * 4, d = slice * kJoinDims + d4;
         kv_f4 o = {0, 0, 0, 0};
-        if (grp < groups) {
-            for (uint32_t i = grp; i < count; i += groups) {
-                const uint64_t at = query * p.chunks + i;
-                const float f = kv_exp2(p.part_ml[at * 2] - m);
-                o += *reinterpret_cast<const kv_f4 *>(p.part_o + at * dp + d) * f;
+        constexpr int kFlight = 4;
+        for (uint32_t i0 = grp; i0 < count; i0 += kFlight * kJoinGroups) {
+            kv_f4 x[kFlight];
+            float f[kFlight];
+#pragma unroll
+            for (int j = 0; j < kFlight; ++j) {
+                const uint32_t i = i0 + (uint32_t)j * kJoinGroups;
+                const uint64_t at = query * p.chunks + (i < count ? i : i0);
+                x[j] = *reinterpret_cast<const kv_f4 *>(p.part_o + at * dp + d);
+                f[j] = i < count ? kv_exp2(p.part_ml[at * 2] - m) : 0.0f;
             }
-            *reinterpret_cast<kv_f4 *>(&sh[grp][d]) = o;
+#pragma unroll
+            for (int j = 0; j < kFlight; ++j)
+                if (i0 + (uint32_t)j * kJoinGroups < count) o += x[j] * f[j];
         }
+        *reinterpret_cast<kv_f4 *>(&sh[grp][d4]) = o;
         __syncthreads();
-        if (t < lanes && d < c.dim) {
-            for (uint32_t i = 1; i < groups; ++i) o += *reinterpret_cast<const kv_f4 *>(&sh[i][d]);
+        if (grp == 0 && d < c.dim) {
+            for (uint32_t i = 1; i < min(kJoinGroups, count); ++i) o += *reinterpret_cast<const kv_f4 *>(&sh[i][d4]);
             const float r = l == 0.0f ? 0.0f : 1.0f / l;
             const kv_u2 y = {E::pack(o[0] * r, o[1] * r), E::pack(o[2] * r, o[3] * r)};
             *reinterpret_cast<kv_u2 *>(p.out + (uint64_t)token * p.out_token + (uint64_t)head * p.out_head + 2u * d) = y;
         }
-        if (t == 0) p.lse[query] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
+        if (t == 0 && slice == 0) p.lse[query] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
         return;
     }
     // weights of 256 visible rows of one (sequence, head)
@@ -407,34 +418,34 @@ __global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, u
     const KvVisible vis = kv_visible(p, kv_length(c, b));
     if (part * kThreads >= vis.count) return;
     const uint32_t count = p.chunks == 1 ? 1u : (vis.count + p.chunk - 1) / p.chunk;
+    const uint32_t i = part * kThreads + t;
+    const float *x = p.logits + (((uint64_t)b * c.heads + h) * p.max_visible + i) * p.group;
+    kv_f4 first = {0, 0, 0, 0};  // the first four logits travel while the parts are joined
+    const bool fours = p.group % 4u == 0u;
+    if (fours && i < vis.count) first = *reinterpret_cast<const kv_f4 *>(x);
     // a wave joins one query head at a time
     for (uint32_t q = t >> 6; q < p.group; q += kThreads / 64) {
         float m, l;
-        join_ml((uint64_t)b * p.q_heads + h * p.group + q, count, t & 63u, 64, m, l);
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const float m2 = __shfl_xor(m, off), l2 = __shfl_xor(l, off);
-            const float big = fmaxf(m, m2);
-            l = l * kv_exp2(m - big) + l2 * kv_exp2(m2 - big);
-            m = big;
-        }
+        join_parts(p, (uint64_t)b * p.q_heads + h * p.group + q, count, m, l);
         if ((t & 63u) == 0u) {
             sh_m[q] = m;
             sh_l[q] = l == 0.0f ? 0.0f : 1.0f / l;
         }
     }
     __syncthreads();
-    const uint32_t i = part * kThreads + t;
     if (i >= vis.count) return;
     const int32_t *list = p.listed ? p.listed + ((uint64_t)b * c.heads + h) * p.listed_count : nullptr;
     const int32_t row = visible_row(vis, i, list);
     if (row < 0) return;
-    const float *x = p.logits + (((uint64_t)b * c.heads + h) * p.max_visible + i) * p.group;
-    float sum = 0.0f;
-    for (uint32_t q = 0; q < p.group; ++q) {
-        // a row without a page has logits of -inf: no weight, also where the sum is 0
-        const float w = kv_exp2(x[q] - sh_m[q]) * sh_l[q];
-        sum += w;
+    float sum = 0.0f;  // (a row without a page has logits of -inf: no weight)
+    if (fours) {
+        for (uint32_t q = 0; q < p.group; q += 4) {
+            const kv_f4 y = q ? *reinterpret_cast<const kv_f4 *>(x + q) : first;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum += kv_exp2(y[j] - sh_m[q + j]) * sh_l[q + j];
+        }
+    } else {
+        for (uint32_t q = 0; q < p.group; ++q) sum += kv_exp2(x[q] - sh_m[q]) * sh_l[q];
     }
     float *at = p.weights + (uint64_t)b * p.weight_batch + (uint64_t)h * p.weight_head + (uint32_t)row;
     if (i < vis.before_list)
@@ -468,18 +479,20 @@ uint32_t kv_padded_dim(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 
 // Chunks of at least 128 rows (a tile for each wave), as many as it takes to
 // have kPerCu workgroups for each compute unit: with fewer a ragged batch's
 // longest sequence runs alone at the end, with more the partial results and
-// their join cost what the balance gains.
+// their join cost what the balance gains.  Up to 512 rows are one chunk: the
+// join's launch costs more than the rows do.
 void kv_token_split(KvAttendParams &p) {
-    constexpr uint32_t kPerCu = 6, kLeast = 128;
+    constexpr uint32_t kPerCu = 6, kLeast = 128, kWhole = 512;
+    p.chunk = kWhole;
+    p.chunks = 1;
+    if (p.max_visible <= kWhole) return;
     const uint32_t columns = p.c.heads * ((p.group + 15u) / 16u) * p.c.batch;
     const uint32_t most = (p.max_visible + kLeast - 1) / kLeast;
     uint32_t chunks = ((uint32_t)kv_compute_units() * kPerCu + columns - 1) / columns;
     chunks = chunks < most ? chunks : most;
     chunks = chunks ? chunks : 1;
     p.chunk = ((p.max_visible + chunks - 1) / chunks + kLeast - 1) / kLeast * kLeast;
-    if (!p.chunk) p.chunk = kLeast;
     p.chunks = (p.max_visible + p.chunk - 1) / p.chunk;
-    if (!p.chunks) p.chunks = 1;
 }
 
 int launch_kv_token(const KvAttendParams &p, uint32_t type, bool sq8, hipStream_t stream) {
@@ -488,7 +501,7 @@ int launch_kv_token(const KvAttendParams &p, uint32_t type, bool sq8, hipStream_
 }
 
 int launch_kv_finish(const KvAttendParams &p, uint32_t type, bool prompt, hipStream_t stream) {
-    const uint32_t joins = (uint32_t)(p.tokens * p.q_heads);
+    const uint32_t joins = (uint32_t)(p.tokens * p.q_heads) * ((p.c.dim + kJoinDims - 1) / kJoinDims);
     const uint32_t row_blocks = p.weights && !prompt ? (p.max_visible + kThreads - 1) / kThreads : 0u;
     const uint32_t blocks = joins + row_blocks * p.c.heads * p.c.batch;
     const uint32_t dp = kv_padded_dim(p.c.dim);

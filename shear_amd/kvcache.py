@@ -29,6 +29,7 @@ import torch
 
 from . import _native as N
 
+_QUERY_TYPES = {torch.bfloat16: N.KV_BF16, torch.float16: N.KV_F16}
 _TYPES = {torch.bfloat16: N.KV_BF16, torch.float16: N.KV_F16, torch.int8: N.KV_SQ8}
 
 
@@ -95,14 +96,15 @@ class KvCache:
         return self.keys, self.values, self.key_scales, self.value_scales
 
 
-def _check(t: torch.Tensor | None, name: str, dtype: torch.dtype, shape: tuple, device) -> None:
+def _check(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device) -> None:
     """A device tensor of the type and shape (None: any size), its last dimension contiguous."""
-    if t.dtype != dtype or t.dim() != len(shape) or any(w is not None and w != g for w, g in zip(shape, t.shape)):
+    got = t.shape
+    if t.dtype is not dtype or len(got) != len(shape) or any(w is not None and w != g for w, g in zip(shape, got)):
         want = ", ".join("*" if w is None else str(w) for w in shape)
-        raise ValueError(f"{name} must be {dtype} [{want}], got {t.dtype} {list(t.shape)}")
+        raise ValueError(f"{name} must be {dtype} [{want}], got {t.dtype} {list(got)}")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}, not {t.device}")
-    if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
+    if got[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"the last dimension of {name} must be contiguous")
 
 
@@ -119,7 +121,7 @@ def _sequences(cache: KvCache, table: torch.Tensor, lengths: torch.Tensor, max_l
     _check(table, "page_table", torch.int32, (None, None), dev)
     batch, columns = table.shape
     _check(lengths, "lengths", torch.int32, (batch,), dev)
-    covers = columns * cache.page_rows
+    covers = columns * cache._native.page_rows
     if max_length is None:
         max_length = covers
     elif not 0 <= max_length <= covers:
@@ -128,12 +130,14 @@ def _sequences(cache: KvCache, table: torch.Tensor, lengths: torch.Tensor, max_l
                          columns, max_length)
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(stream: torch.cuda.Stream | None, device: torch.device, tensors):
     """The call's stream: (context in which it is current, its handle)."""
     if stream is None:
-        if device.index == torch.cuda.current_device():
-            return contextlib.nullcontext(), torch.cuda.current_stream(device).cuda_stream or None
-        return torch.cuda.device(device), torch.cuda.current_stream(device).cuda_stream or None
+        handle = torch._C._cuda_getCurrentRawStream(device.index) or None
+        return (_HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)), handle
     if stream.device != device:
         raise ValueError(f"stream is on {stream.device}, the cache on {device}")
     for t in tensors:
@@ -180,16 +184,17 @@ def append(cache: KvCache, page_table: torch.Tensor, starts: torch.Tensor, k: to
 def _attend(cache, q, page_table, lengths, max_length, scale, sinks, window, stream, *, listed=None, weights=None,
             offsets=None, max_new=0):
     dev, lib = cache.keys.device, N.load()
-    if q.dim() != 3 or q.dtype not in (torch.bfloat16, torch.float16) or q.device != dev:
+    kind = _QUERY_TYPES.get(q.dtype)
+    if q.dim() != 3 or kind is None or q.device != dev:
         raise ValueError(f"q must be bf16 or fp16 [tokens, q_heads, head_dim] on {dev}")
-    if q.dtype != cache.keys.dtype and cache.keys.dtype != torch.int8:
+    if kind != cache._native.type != N.KV_SQ8:
         raise ValueError(f"q is {q.dtype}, the cache {cache.keys.dtype}")
-    if q.shape[2] != cache.head_dim or q.shape[1] == 0 or q.shape[1] % cache.heads:
+    if q.shape[2] != cache._native.head_dim or q.shape[1] == 0 or q.shape[1] % cache._native.heads:
         raise ValueError(f"q of {q.shape[1]} heads x {q.shape[2]} over a cache of {cache.heads} heads x {cache.head_dim}")
     if sinks < 0 or (window is not None and window < 0):
         raise ValueError(f"sinks {sinks} and window {window} must not be negative")
-    seq = _sequences(cache, page_table, lengths, max_length)
     tokens, heads, dim = q.shape
+    seq = _sequences(cache, page_table, lengths, max_length)
     prompt = offsets is not None
     if not prompt and tokens != seq.batch:
         raise ValueError(f"{tokens} queries for {seq.batch} sequences")
@@ -207,8 +212,9 @@ def _attend(cache, q, page_table, lengths, max_length, scale, sinks, window, str
         q = _rows(q)
         out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=dev)
         lse = torch.empty((tokens, heads), dtype=torch.float32, device=dev)
-        a = N.KvAttend(q.data_ptr(), out.data_ptr(), lse.data_ptr(), _strides(q, 2), (heads * dim, dim),
-                       _TYPES[q.dtype], heads, 1.0 / math.sqrt(dim) if scale is None else scale, min(sinks, seq.max_length),
+        strides = q.stride()
+        a = N.KvAttend(q.data_ptr(), out.data_ptr(), lse.data_ptr(), strides[:2], (heads * dim, dim),
+                       kind, heads, 1.0 / math.sqrt(dim) if scale is None else scale, min(sinks, seq.max_length),
                        N.KV_ALL if window is None else min(window, N.KV_ALL - 1), 0, None, None, (0, 0), None, tokens,
                        max_new, 0)
         if listed is not None:
