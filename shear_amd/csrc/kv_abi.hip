@@ -205,15 +205,17 @@ tessa_status attend_of(const tessa_kv_cache *cache, const tessa_kv_sequences *se
         const uint64_t visible = (shown < p.c.max_length ? shown : p.c.max_length) + p.listed_count;
         if (visible > 0x7fffffffull) KV_UNSUPPORTED("kv attend: %llu visible rows", (unsigned long long)visible);
         p.max_visible = (uint32_t)visible;
-        if ((uint64_t)p.c.heads * ((p.group + 15u) / 16u) > kMaxGrid) KV_UNSUPPORTED("kv attend: %u query heads", a->q_heads);
         kv_token_split(p);
         const uint64_t blocks = (visible + 255) / 256 * p.c.heads * p.c.batch + a->tokens * a->q_heads * 4u;
         if (blocks > 0x7fffffffull) KV_UNSUPPORTED("kv attend: batch %u of %llu rows", p.c.batch, (unsigned long long)visible);
         if (p.weights) logits = round_up(visible * p.c.heads * p.c.batch * p.group * sizeof(float));
     }
-    if (p.chunks > 1 || p.weights) {
-        part_o = round_up(a->tokens * a->q_heads * p.chunks * dp * sizeof(float));
-        part_ml = round_up(a->tokens * a->q_heads * p.chunks * 2 * sizeof(float));
+    uint64_t parts = prompt && p.chunks > 1 ? a->tokens * a->q_heads * p.chunks : 0;
+    if (!prompt && p.workers)
+        parts = ((uint64_t)p.columns * p.c.batch + p.workers) * (p.group < 16u ? p.group : 16u);
+    if (parts) {
+        part_o = round_up(parts * dp * sizeof(float));
+        part_ml = round_up(parts * 2 * sizeof(float));
     }
     return fine();
 }

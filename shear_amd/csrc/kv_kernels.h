@@ -56,11 +56,13 @@ struct KvAttendParams {
     uint32_t max_new;
     uint64_t tokens;
     // the split over the rows
-    uint32_t chunk;            // token: virtual rows of a workgroup; prompt: unused
-    uint32_t chunks;           // partial results of a query
+    uint32_t workers;          // token: workgroups that share all rows out evenly (0: one for each column of rows)
+    uint32_t columns;          // token: (head, block of 16 query heads) pairs
+    uint32_t chunks;           // prompt: partial results of a query
     uint32_t max_visible;      // token: most visible rows of a sequence
-    float *part_o;             // [query][chunks][padded dim]
-    float *part_ml;            // [query][chunks][2]: running maximum (base 2), sum
+    float *part_o;             // [part][padded dim]; prompt: part = query * chunks + chunk,
+                               // token: (column + worker) * query heads of a block + head
+    float *part_ml;            // [part][2]: running maximum (base 2), sum
     float *logits;             // token with weights: [batch][heads][max_visible][group], base 2
 };
 

@@ -570,7 +570,6 @@ void kv_prompt_split(KvAttendParams &p) {
     const uint32_t most = visible / 256u;
     chunks = chunks < most ? chunks : most;
     p.chunks = chunks ? (uint32_t)chunks : 1u;
-    p.chunk = 0;
 }
 
 int launch_kv_prompt(const KvAttendParams &p, uint32_t type, bool sq8, hipStream_t stream) {

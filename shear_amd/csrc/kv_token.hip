@@ -8,6 +8,13 @@
 // workgroup are joined through LDS, workgroups of one (sequence, head) by
 // kv_finish_kernel.
 //
+// The rows of all sequences and heads, in units of 128, are one line that as many
+// workgroups as the card holds at once share out evenly, whatever the sequences'
+// lengths: each takes a contiguous range, often the end of one column of rows
+// (a sequence's rows of one head) and the beginning of the next.  Part (column g,
+// worker i) has place g + i, which no other part has, since along the line
+// every next part is of a later column or a later worker.
+//
 // Every visible row is read once for up to 16 query heads, so the cache's
 // bytes bound it; nothing is staged in LDS but row places.
 //  * S^T = K Q^T on 16x16x32 instructions: the K operand is 16 bytes of a row
@@ -66,7 +73,94 @@ __device__ __forceinline__ int32_t visible_row(const KvVisible &v, uint32_t i, c
     return r >= (int32_t)v.first && r < (int32_t)v.last_begin ? r : -1;
 }
 
-template <typename T, bool kSq8, int DP>
+constexpr uint32_t kUnit = 128;  // rows: a tile for each wave
+
+__device__ __forceinline__ uint32_t units_of(const KvAttendParams &p, uint32_t b) {
+    return (kv_visible(p, kv_length(p.c, b)).count + kUnit - 1) / kUnit;
+}
+
+// The workers of a line: no more than it has units, so that all of them have some.
+__device__ __forceinline__ uint32_t workers_of(const KvAttendParams &p, uint64_t total) {
+    return (uint32_t)min((uint64_t)p.workers, total * p.columns);
+}
+
+// Where unit u lies on the line of `total` units: the worker that has it.
+__device__ __forceinline__ uint32_t worker_of(uint64_t u, uint64_t total, uint32_t workers) {
+    return (uint32_t)(((u + 1) * workers - 1) / total);
+}
+__device__ __forceinline__ uint64_t first_unit(uint32_t worker, uint64_t total, uint32_t workers) {
+    return total * worker / workers;
+}
+
+// Sums over the batch by a workgroup: units of all sequences, and of those
+// before `until`.
+__device__ __forceinline__ void sum_units(const KvAttendParams &p, uint32_t until, uint64_t *sh, uint64_t &total, uint64_t &before) {
+    uint64_t a = 0, c = 0;
+    for (uint32_t b = threadIdx.x; b < p.c.batch; b += kThreads) {
+        const uint32_t n = units_of(p, b);
+        a += n;
+        c += b < until ? n : 0u;
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        a += __shfl_xor(a, off);
+        c += __shfl_xor(c, off);
+    }
+    if ((threadIdx.x & 63u) == 0u) {
+        sh[threadIdx.x >> 6] = a;
+        sh[kWaves + (threadIdx.x >> 6)] = c;
+    }
+    __syncthreads();
+    total = sh[0] + sh[1] + sh[2] + sh[3];
+    before = sh[4] + sh[5] + sh[6] + sh[7];
+    static_assert(kWaves == 4, "");
+}
+
+// The sequence that has unit `u` of the columns' lines (u < total units of the
+// batch, not times columns) and the units before it.
+__device__ __forceinline__ void find_sequence(const KvAttendParams &p, uint64_t u, uint64_t *sh, uint32_t &b, uint64_t &before) {
+    uint64_t base = 0;
+    for (uint32_t b0 = 0;; b0 += kThreads) {
+        const uint32_t mine = b0 + threadIdx.x;
+        const uint64_t n = mine < p.c.batch ? units_of(p, mine) : 0u;
+        uint64_t x = n;  // inclusive sum over the wave, then over the waves
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint64_t y = __shfl_up(x, off);
+            if ((threadIdx.x & 63u) >= (uint32_t)off) x += y;
+        }
+        __syncthreads();  // sh has been read
+        if ((threadIdx.x & 63u) == 63u) sh[threadIdx.x >> 6] = x;
+        if (threadIdx.x == 0) sh[kWaves] = ~0ull;
+        __syncthreads();
+        uint64_t all = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            if ((uint32_t)w < threadIdx.x >> 6) x += sh[w];
+            all += sh[w];
+        }
+        if (u >= base + x - n && u < base + x) {
+            sh[kWaves] = mine;
+            sh[kWaves + 1] = base + x - n;
+        }
+        __syncthreads();
+        if (sh[kWaves] != ~0ull) {
+            b = (uint32_t)sh[kWaves];
+            before = sh[kWaves + 1];
+            return;
+        }
+        base += all;
+        if (b0 + kThreads >= p.c.batch) {  // (u is not on the line: no sequence)
+            b = p.c.batch;
+            before = base;
+            return;
+        }
+    }
+}
+
+// kDirect: one workgroup for each column of rows, which writes the result; else
+// workers and parts.
+template <typename T, bool kSq8, int DP, bool kDirect>
 __global__ __launch_bounds__(kThreads) void kv_token_kernel(KvAttendParams p) {
     using E = KvElem<T>;
     constexpr int kSteps = DP / 32;                 // matrix instructions of 16 logits
@@ -82,16 +176,39 @@ __global__ __launch_bounds__(kThreads) void kv_token_kernel(KvAttendParams p) {
     const KvCacheParams &c = p.c;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t n = lane & 15u, g = lane >> 4;
-    const uint32_t blocks = (p.group + 15u) / 16u;
-    const uint32_t h = blockIdx.y / blocks, first_q = (blockIdx.y - h * blocks) * 16u, b = blockIdx.z;
+    const uint32_t blocks = (p.group + 15u) / 16u, block_heads = min(16u, p.group);
+    // the workgroup's range of units; lines lie sequence by sequence, column by column
+    uint32_t b = blockIdx.y, column = blockIdx.x;
+    uint64_t unit = 0, unit_end = 1, line = 0;  // line: first unit of the column at hand
+    if constexpr (!kDirect) {
+        __shared__ uint64_t sh_sum[2 * kWaves];
+        uint64_t total, before;
+        sum_units(p, 0, sh_sum, total, before);
+        const uint32_t workers = workers_of(p, total);
+        if (blockIdx.x >= workers) return;
+        unit = first_unit(blockIdx.x, total * p.columns, workers);
+        unit_end = first_unit(blockIdx.x + 1, total * p.columns, workers);
+        find_sequence(p, unit / p.columns, sh_sum, b, before);
+        // a sequence's columns follow each other, each of its units
+        line = before * p.columns;
+        const uint32_t n = units_of(p, b);
+        column = (uint32_t)((unit - line) / n);
+        line += (uint64_t)column * n;
+    }
+    bool again = false;
+    while (unit < unit_end) {
+    const uint32_t h = column / blocks, first_q = (column - h * blocks) * 16u;
     const uint32_t heads = min(16u, p.group - first_q);
     const KvVisible vis = kv_visible(p, kv_length(c, b));
-    const uint32_t begin = blockIdx.x * p.chunk, end = min(begin + p.chunk, vis.count);
-    if (begin >= vis.count && p.chunks > 1) return;  // the join counts the chunks by itself
+    const uint32_t units = (vis.count + kUnit - 1) / kUnit;
+    const uint32_t begin = kDirect ? 0u : (uint32_t)(unit - line) * kUnit;
+    const uint32_t end = kDirect ? vis.count : min(vis.count, begin + (uint32_t)min(unit_end - unit, (uint64_t)units) * kUnit);
     const uint32_t rows = end > begin ? end - begin : 0u;
     const uint32_t tiles = (rows + kTile - 1) / kTile;
     const int32_t *list = p.listed ? p.listed + ((uint64_t)b * c.heads + h) * p.listed_count : nullptr;
     const int32_t *table = c.table + (uint64_t)b * c.table_stride;
+    if (again) __syncthreads();  // the last part's sums have been read
+    again = true;
 
     // Q operand: heads are columns; dims of step s as K's lanes hold them
     const bool head_ok = n < heads;
@@ -320,11 +437,12 @@ __global__ __launch_bounds__(kThreads) void kv_token_kernel(KvAttendParams p) {
         }
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) sum += sh_ml[w][1][head] * kv_exp2(sh_ml[w][0][head] - big);
-        if (p.chunks > 1 || p.part_o) {
-            *reinterpret_cast<kv_f4 *>(p.part_o + ((q0 + head) * p.chunks + blockIdx.x) * DP + d) = o;
+        if constexpr (!kDirect) {
+            const uint64_t part = ((uint64_t)b * p.columns + column + blockIdx.x) * block_heads + head;
+            *reinterpret_cast<kv_f4 *>(p.part_o + part * DP + d) = o;
             if (d == 0) {
-                p.part_ml[((q0 + head) * p.chunks + blockIdx.x) * 2] = big;
-                p.part_ml[((q0 + head) * p.chunks + blockIdx.x) * 2 + 1] = sum;
+                p.part_ml[part * 2] = big;
+                p.part_ml[part * 2 + 1] = sum;
             }
         } else {
             const float r = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -335,6 +453,16 @@ __global__ __launch_bounds__(kThreads) void kv_token_kernel(KvAttendParams p) {
             }
             if (d == 0) p.lse[q0 + head] = sum == 0.0f ? -INFINITY : (big + log2f(sum)) * 0.69314718056f;
         }
+    }
+    if constexpr (kDirect) break;
+    // the next column, of this sequence or of the next that has rows
+    unit = line + units;
+    line = unit;
+    if (++column == p.columns) {
+        column = 0;
+        do ++b;
+        while (b < c.batch && unit < unit_end && units_of(p, b) == 0u);
+    }
     }
 }
 
@@ -348,11 +476,11 @@ constexpr uint32_t kJoinDims = 64;
 constexpr uint32_t kJoinGroups = kThreads / (kJoinDims / 4);  // 16
 
 // Largest maximum and sum of a query's parts, in all lanes of a wave.
-__device__ __forceinline__ void join_parts(const KvAttendParams &p, uint64_t query, uint32_t count, float &m, float &l) {
+__device__ __forceinline__ void join_parts(const KvAttendParams &p, uint64_t first, uint32_t step, uint32_t count, float &m, float &l) {
     m = kKvNone;
     l = 0.0f;
     for (uint32_t i = threadIdx.x & 63u; i < count; i += 64) {
-        const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + (query * p.chunks + i) * 2);
+        const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + (first + (uint64_t)i * step) * 2);
         const float big = fmaxf(m, ml.x);
         l = l * kv_exp2(m - big) + ml.y * kv_exp2(ml.x - big);
         m = big;
@@ -366,6 +494,22 @@ __device__ __forceinline__ void join_parts(const KvAttendParams &p, uint64_t que
     }
 }
 
+// The parts of a column of rows: those of the workers that have units of it.
+__device__ __forceinline__ void column_parts(const KvAttendParams &p, uint32_t b, uint32_t column, uint64_t *sh, uint64_t &first,
+                                             uint32_t &count) {
+    uint64_t total, before;
+    sum_units(p, b, sh, total, before);
+    const uint32_t n = units_of(p, b);
+    const uint64_t line = before * p.columns + (uint64_t)column * n;
+    first = (uint64_t)b * p.columns + column;
+    count = 0;
+    if (n) {
+        const uint32_t workers = workers_of(p, total), w0 = worker_of(line, total * p.columns, workers);
+        first += w0;
+        count = worker_of(line + n - 1, total * p.columns, workers) - w0 + 1;
+    }
+}
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, uint32_t dp, uint32_t joins, uint32_t row_blocks,
                                                              bool prompt) {
@@ -373,16 +517,23 @@ __global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, u
     const KvCacheParams &c = p.c;
     __shared__ __align__(16) float sh[kJoinGroups][kJoinDims];
     __shared__ float sh_m[kThreads], sh_l[kThreads];
+    __shared__ uint64_t sh_sum[2 * kWaves];
     const uint32_t t = threadIdx.x;
     if (blockIdx.x < joins) {
         const uint32_t slices = (c.dim + kJoinDims - 1) / kJoinDims;
         const uint64_t query = blockIdx.x / slices;
         const uint32_t slice = blockIdx.x - (uint32_t)query * slices;
         const uint32_t token = (uint32_t)(query / p.q_heads), head = (uint32_t)(query - (uint64_t)token * p.q_heads);
-        uint32_t count = p.chunks;
-        if (!prompt && p.chunks > 1) count = (kv_visible(p, kv_length(c, token)).count + p.chunk - 1) / p.chunk;
+        uint64_t first = query * p.chunks;
+        uint32_t count = p.chunks, step = 1;
+        if (!prompt) {
+            const uint32_t h = head / p.group, q = head - h * p.group;
+            step = min(16u, p.group);
+            column_parts(p, token, h * ((p.group + 15u) / 16u) + q / 16u, sh_sum, first, count);
+            first = first * step + (q & 15u);
+        }
         float m, l;
-        join_parts(p, query, count, m, l);
+        join_parts(p, first, step, count, m, l);
         const uint32_t grp = t / (kJoinDims / 4), d4 = (t % (kJoinDims / 4)) * 4, d = slice * kJoinDims + d4;
         kv_f4 o = {0, 0, 0, 0};
         constexpr int kFlight = 4;
@@ -392,7 +543,7 @@ __global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, u
 #pragma unroll
             for (int j = 0; j < kFlight; ++j) {
                 const uint32_t i = i0 + (uint32_t)j * kJoinGroups;
-                const uint64_t at = query * p.chunks + (i < count ? i : i0);
+                const uint64_t at = first + (uint64_t)(i < count ? i : i0) * step;
                 x[j] = *reinterpret_cast<const kv_f4 *>(p.part_o + at * dp + d);
                 f[j] = i < count ? kv_exp2(p.part_ml[at * 2] - m) : 0.0f;
             }
@@ -417,19 +568,25 @@ __global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, u
     const uint32_t b = bh / c.heads, h = bh - b * c.heads;
     const KvVisible vis = kv_visible(p, kv_length(c, b));
     if (part * kThreads >= vis.count) return;
-    const uint32_t count = p.chunks == 1 ? 1u : (vis.count + p.chunk - 1) / p.chunk;
     const uint32_t i = part * kThreads + t;
     const float *x = p.logits + (((uint64_t)b * c.heads + h) * p.max_visible + i) * p.group;
     kv_f4 first = {0, 0, 0, 0};  // the first four logits travel while the parts are joined
     const bool fours = p.group % 4u == 0u;
     if (fours && i < vis.count) first = *reinterpret_cast<const kv_f4 *>(x);
     // a wave joins one query head at a time
-    for (uint32_t q = t >> 6; q < p.group; q += kThreads / 64) {
-        float m, l;
-        join_parts(p, (uint64_t)b * p.q_heads + h * p.group + q, count, m, l);
-        if ((t & 63u) == 0u) {
-            sh_m[q] = m;
-            sh_l[q] = l == 0.0f ? 0.0f : 1.0f / l;
+    const uint32_t step = min(16u, p.group);
+    for (uint32_t q0 = 0; q0 < p.group; q0 += 16u) {
+        uint64_t first;
+        uint32_t count;
+        if (q0) __syncthreads();
+        column_parts(p, b, h * ((p.group + 15u) / 16u) + q0 / 16u, sh_sum, first, count);
+        for (uint32_t q = q0 + (t >> 6); q < min(q0 + 16u, p.group); q += kWaves) {
+            float m, l;
+            join_parts(p, first * step + (q - q0), step, count, m, l);
+            if ((t & 63u) == 0u) {
+                sh_m[q] = m;
+                sh_l[q] = l == 0.0f ? 0.0f : 1.0f / l;
+            }
         }
     }
     __syncthreads();
@@ -456,10 +613,11 @@ __global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, u
 
 template <typename T, bool kSq8, int DP>
 int launch(const KvAttendParams &p, hipStream_t stream) {
-    const uint32_t blocks = (p.group + 15u) / 16u;
-    const dim3 grid(p.chunks, p.c.heads * blocks, p.c.batch);
     const size_t lds = (size_t)kWaves * (p.group < 16u ? p.group : 16u) * DP * sizeof(float);
-    kv_token_kernel<T, kSq8, DP><<<grid, kThreads, lds, stream>>>(p);
+    if (p.workers)
+        kv_token_kernel<T, kSq8, DP, false><<<p.workers, kThreads, lds, stream>>>(p);
+    else
+        kv_token_kernel<T, kSq8, DP, true><<<dim3(p.columns, p.c.batch), kThreads, lds, stream>>>(p);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
@@ -476,23 +634,19 @@ int launch_dim(const KvAttendParams &p, hipStream_t stream) {
 
 uint32_t kv_padded_dim(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
-// Chunks of at least 128 rows (a tile for each wave), as many as it takes to
-// have kPerCu workgroups for each compute unit: with fewer a ragged batch's
-// longest sequence runs alone at the end, with more the partial results and
-// their join cost what the balance gains.  Up to 512 rows are one chunk: the
-// join's launch costs more than the rows do.
+// Up to 512 rows one workgroup takes a column of rows and writes the result: a
+// join's launch costs more than the rows do.  Otherwise, and where weights are
+// wanted, as many workgroups as the registers of the compute units hold share the rows
+// out, or fewer where there are fewer units.
 void kv_token_split(KvAttendParams &p) {
-    constexpr uint32_t kPerCu = 6, kLeast = 128, kWhole = 512;
-    p.chunk = kWhole;
-    p.chunks = 1;
-    if (p.max_visible <= kWhole) return;
-    const uint32_t columns = p.c.heads * ((p.group + 15u) / 16u) * p.c.batch;
-    const uint32_t most = (p.max_visible + kLeast - 1) / kLeast;
-    uint32_t chunks = ((uint32_t)kv_compute_units() * kPerCu + columns - 1) / columns;
-    chunks = chunks < most ? chunks : most;
-    chunks = chunks ? chunks : 1;
-    p.chunk = ((p.max_visible + chunks - 1) / chunks + kLeast - 1) / kLeast * kLeast;
-    p.chunks = (p.max_visible + p.chunk - 1) / p.chunk;
+    constexpr uint32_t kWhole = 512;
+    p.columns = p.c.heads * ((p.group + 15u) / 16u);
+    p.workers = 0;
+    if (p.max_visible <= kWhole && !p.weights) return;
+    const uint64_t units = (uint64_t)(p.max_visible + kUnit - 1) / kUnit * p.columns * p.c.batch;
+    const uint64_t most = (uint64_t)kv_compute_units() * (kv_padded_dim(p.c.dim) == 256 ? 1u : 2u);
+    p.workers = (uint32_t)(units < most ? units : most);
+    if (!p.workers) p.workers = 1;
 }
 
 int launch_kv_token(const KvAttendParams &p, uint32_t type, bool sq8, hipStream_t stream) {
