@@ -470,8 +470,10 @@ __global__ __launch_bounds__(kThreads) void kv_token_kernel(KvAttendParams p) {
 // exp2(m_c - m) l_c: blocks below `joins`, one for kJoinDims dims of a query, so
 // that few queries with many parts use many compute units, and the parts of a
 // query are read kJoinGroups side by side.  With weights the other blocks turn the
-// logits of 256 visible rows into weights and add them, summed over the group's
+// logits of 1,024 visible rows into weights and add them, summed over the group's
 // heads, to the caller's.
+constexpr int kWeightPer = 4;  // rows of a thread
+constexpr uint32_t kWeightRows = kThreads * kWeightPer;
 constexpr uint32_t kJoinDims = 64;
 constexpr uint32_t kJoinGroups = kThreads / (kJoinDims / 4);  // 16
 
@@ -562,17 +564,29 @@ __global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, u
         if (t == 0 && slice == 0) p.lse[query] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
         return;
     }
-    // weights of 256 visible rows of one (sequence, head)
+    // weights of kWeightRows visible rows of one (sequence, head)
     const uint32_t item = blockIdx.x - joins;
     const uint32_t part = item % row_blocks, bh = item / row_blocks;
     const uint32_t b = bh / c.heads, h = bh - b * c.heads;
     const KvVisible vis = kv_visible(p, kv_length(c, b));
-    if (part * kThreads >= vis.count) return;
-    const uint32_t i = part * kThreads + t;
-    const float *x = p.logits + (((uint64_t)b * c.heads + h) * p.max_visible + i) * p.group;
-    kv_f4 first = {0, 0, 0, 0};  // the first four logits travel while the parts are joined
+    const uint32_t i0 = part * kWeightRows + t;
+    if (part * kWeightRows >= vis.count) return;
+    const float *x = p.logits + ((uint64_t)b * c.heads + h) * p.max_visible * p.group;
     const bool fours = p.group % 4u == 0u;
-    if (fours && i < vis.count) first = *reinterpret_cast<const kv_f4 *>(x);
+    // the first logits and the weights travel while the parts are joined
+    kv_f4 first4[kWeightPer];
+    int32_t row[kWeightPer];
+    float old[kWeightPer];
+    const int32_t *list = p.listed ? p.listed + ((uint64_t)b * c.heads + h) * p.listed_count : nullptr;
+    float *weights = p.weights + (uint64_t)b * p.weight_batch + (uint64_t)h * p.weight_head;
+#pragma unroll
+    for (int j = 0; j < kWeightPer; ++j) {
+        const uint32_t i = i0 + (uint32_t)j * kThreads;
+        row[j] = i < vis.count ? visible_row(vis, i, list) : -1;
+        first4[j] = kv_f4{0, 0, 0, 0};
+        if (fours && i < vis.count) first4[j] = *reinterpret_cast<const kv_f4 *>(x + (uint64_t)i * p.group);
+        old[j] = row[j] >= 0 && i < vis.before_list ? weights[row[j]] : 0.0f;
+    }
     // a wave joins one query head at a time
     const uint32_t step = min(16u, p.group);
     for (uint32_t q0 = 0; q0 < p.group; q0 += 16u) {
@@ -590,25 +604,26 @@ __global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, u
         }
     }
     __syncthreads();
-    if (i >= vis.count) return;
-    const int32_t *list = p.listed ? p.listed + ((uint64_t)b * c.heads + h) * p.listed_count : nullptr;
-    const int32_t row = visible_row(vis, i, list);
-    if (row < 0) return;
-    float sum = 0.0f;  // (a row without a page has logits of -inf: no weight)
-    if (fours) {
-        for (uint32_t q = 0; q < p.group; q += 4) {
-            const kv_f4 y = q ? *reinterpret_cast<const kv_f4 *>(x + q) : first;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sum += kv_exp2(y[j] - sh_m[q + j]) * sh_l[q + j];
+    for (int j = 0; j < kWeightPer; ++j) {
+        const uint32_t i = i0 + (uint32_t)j * kThreads;
+        if (row[j] < 0) continue;
+        const float *y = x + (uint64_t)i * p.group;
+        float sum = 0.0f;  // (a row without a page has logits of -inf: no weight)
+        if (fours) {
+            for (uint32_t q = 0; q < p.group; q += 4) {
+                const kv_f4 z = q ? *reinterpret_cast<const kv_f4 *>(y + q) : first4[j];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum += kv_exp2(z[e] - sh_m[q + e]) * sh_l[q + e];
+            }
+        } else {
+            for (uint32_t q = 0; q < p.group; ++q) sum += kv_exp2(y[q] - sh_m[q]) * sh_l[q];
         }
-    } else {
-        for (uint32_t q = 0; q < p.group; ++q) sum += kv_exp2(x[q] - sh_m[q]) * sh_l[q];
+        if (i < vis.before_list)
+            weights[row[j]] = old[j] + sum;
+        else
+            unsafeAtomicAdd(weights + row[j], sum);  // a row that the list names twice counts twice
     }
-    float *at = p.weights + (uint64_t)b * p.weight_batch + (uint64_t)h * p.weight_head + (uint32_t)row;
-    if (i < vis.before_list)
-        *at += sum;
-    else
-        unsafeAtomicAdd(at, sum);  // a row that the list names twice counts twice
 }
 
 template <typename T, bool kSq8, int DP>
@@ -656,7 +671,7 @@ int launch_kv_token(const KvAttendParams &p, uint32_t type, bool sq8, hipStream_
 
 int launch_kv_finish(const KvAttendParams &p, uint32_t type, bool prompt, hipStream_t stream) {
     const uint32_t joins = (uint32_t)(p.tokens * p.q_heads) * ((p.c.dim + kJoinDims - 1) / kJoinDims);
-    const uint32_t row_blocks = p.weights && !prompt ? (p.max_visible + kThreads - 1) / kThreads : 0u;
+    const uint32_t row_blocks = p.weights && !prompt ? (p.max_visible + kWeightRows - 1) / kWeightRows : 0u;
     const uint32_t blocks = joins + row_blocks * p.c.heads * p.c.batch;
     const uint32_t dp = kv_padded_dim(p.c.dim);
     if (type == kKvBf16)
