@@ -41,25 +41,37 @@ __device__ __forceinline__ uint32_t order_of(float w) {
     return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
+// Sum of sh[i] over i < wave.
+__device__ __forceinline__ uint32_t before_wave(const uint32_t *sh, uint32_t wave) {
+    uint32_t sum = 0;
+#pragma unroll
+    for (int i = 0; i < kSelWaves - 1; ++i) sum += (uint32_t)i < wave ? sh[i] : 0u;
+    return sum;
+}
+
+// The middle rows [sinks, n - recent) by weight: places sinks.. of `kept` and `out`.
+// Lanes past a wave's last candidate hold the lowest value.  They can at most
+// add to the lowest bin and to the ties of the lowest value, after every real
+// candidate of theirs, where no row is left to place.
 template <bool kHeld>
 __device__ __forceinline__ void select_rows(const KvEvictParams &p, const float *w, uint32_t n, int32_t *kept, float *out,
                                             uint32_t *hist, uint32_t (*sh_wave)[kSelWaves], uint32_t *sh_pick) {
     const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6;
     const uint32_t candidates = n - p.sinks - p.recent;
     const uint32_t need = p.keep - p.sinks - p.recent;
+    if (need == 0) return;
     // contiguous rows of a wave, whole groups of 64
     const uint32_t span = ((candidates + kSelWaves - 1) / kSelWaves + 63u) / 64u * 64u;
     const uint32_t lo = wave * span, hi = min(lo + span, candidates);
-    const uint32_t steps = lo < hi ? (hi - lo + 63u) / 64u : 0u;
+    const uint32_t steps = __builtin_amdgcn_readfirstlane(lo < hi ? (hi - lo + 63u) / 64u : 0u);
     const float *mine = w + p.sinks + lo + lane;
-    auto load = [&](uint32_t s) { return lo + s * 64u + lane < hi ? mine[s * 64u] : 0.0f; };
-    auto inside = [&](uint32_t s) { return lo + s * 64u + lane < hi; };
-    float held[kHeld ? kSelPer : 1];
+    auto load = [&](uint32_t s) { return lo + s * 64u + lane < hi ? order_of(mine[s * 64u]) : 0u; };
+    uint32_t held[kHeld ? kSelPer : 1];
     if constexpr (kHeld) {
 #pragma unroll
         for (int s = 0; s < kSelPer; ++s) held[s] = load(s);
     }
-    // f(step, weight) for each of the lane's candidates
+    // f(step, value) for each of the lane's candidates
     auto each = [&](auto &&f) {
         if constexpr (kHeld) {
 #pragma unroll
@@ -67,9 +79,9 @@ __device__ __forceinline__ void select_rows(const KvEvictParams &p, const float 
                 if ((uint32_t)s < steps) f((uint32_t)s, held[s]);
         } else {
             for (uint32_t s0 = 0; s0 < steps; s0 += kSelGroup) {
-                float x[kSelGroup];
+                uint32_t x[kSelGroup];
 #pragma unroll
-                for (int s = 0; s < kSelGroup; ++s) x[s] = s0 + s < steps ? load(s0 + s) : 0.0f;
+                for (int s = 0; s < kSelGroup; ++s) x[s] = load(s0 + s);
 #pragma unroll
                 for (int s = 0; s < kSelGroup; ++s)
                     if (s0 + s < steps) f(s0 + s, x[s]);
@@ -78,88 +90,79 @@ __device__ __forceinline__ void select_rows(const KvEvictParams &p, const float 
     };
 
     // the need-th largest value: three digits from the top
-    uint32_t prefix = 0, known = 0, left = need;  // bits known so far, kept rows still to place among them
-    if (need) {
-#pragma unroll 1
-        for (int pass = 0; pass < 3; ++pass) {
-            const int bits = pass == 2 ? 10 : 11, shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-            for (uint32_t i = t; i < kBins; i += kSelThreads) hist[i] = 0u;
-            __syncthreads();
-            each([&](uint32_t s, float x) {
-                const uint32_t u = order_of(x);
-                if (inside(s) && (known == 0 || (u >> (32 - known)) == prefix)) atomicAdd(&hist[(u >> shift) & ((1u << bits) - 1u)], 1u);
-            });
-            __syncthreads();
-            // bins from the top: thread t has bins 2047 - 2t and 2046 - 2t
-            const uint32_t a = hist[kBins - 1 - 2 * t], c = hist[kBins - 2 - 2 * t];
-            uint32_t sum = a + c;
+    uint32_t least = 0, left = need;  // digits known so far, kept rows still to place among them
+    auto pick = [&](int bits) {       // the digit of the left-th largest value in `hist`
+        // bins from the top: thread t has bins 2047 - 2t and 2046 - 2t
+        const uint32_t a = hist[kBins - 1 - 2 * t], c = hist[kBins - 2 - 2 * t];
+        uint32_t sum = a + c;
 #pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const uint32_t y = __shfl_up(sum, off);
-                if (lane >= (uint32_t)off) sum += y;
-            }
-            if (lane == 63u) sh_wave[0][wave] = sum;
-            __syncthreads();
-            uint32_t before = sum - a - c;
-            for (uint32_t i = 0; i < wave; ++i) before += sh_wave[0][i];
-            if (before < left && left <= before + a + c) {
-                const bool first = left <= before + a;
-                sh_pick[0] = kBins - 1 - 2 * t - (first ? 0u : 1u);
-                sh_pick[1] = left - before - (first ? 0u : a);
-            }
-            __syncthreads();
-            prefix = (prefix << bits) | sh_pick[0];
-            left = sh_pick[1];
-            known += bits;
-            __syncthreads();
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint32_t y = __shfl_up(sum, off);
+            if (lane >= (uint32_t)off) sum += y;
         }
-    }
-    const uint32_t least = need ? prefix : 0xffffffffu;  // nothing is as large as this
-    // rows above it, and equal to it, before each wave's
-    uint32_t above = 0, equal = 0;
-    if (need) {
-        each([&](uint32_t s, float x) {
-            const uint32_t u = order_of(x);
-            above += __popcll(__ballot(inside(s) && u > least));
-            equal += __popcll(__ballot(inside(s) && u == least));
-        });
-        if (lane == 0) {
-            sh_wave[0][wave] = above;
-            sh_wave[1][wave] = equal;
+        if (lane == 63u) sh_wave[0][wave] = sum;
+        __syncthreads();
+        hist[kBins - 1 - 2 * t] = hist[kBins - 2 - 2 * t] = 0u;  // for the next digit
+        const uint32_t before = sum - a - c + before_wave(sh_wave[0], wave);
+        if (before < left && left <= before + a + c) {
+            const bool first = left <= before + a;
+            sh_pick[0] = kBins - 1 - 2 * t - (first ? 0u : 1u);
+            sh_pick[1] = left - before - (first ? 0u : a);
         }
         __syncthreads();
-        uint32_t place = p.sinks, equal_before = 0;
-        for (uint32_t i = 0; i < wave; ++i) {
-            const uint32_t e = sh_wave[1][i], room = left > equal_before ? left - equal_before : 0u;
-            place += sh_wave[0][i] + min(e, room);
-            equal_before += e;
-        }
-        uint32_t room = left > equal_before ? left - equal_before : 0u;
-        const uint64_t below = (1ull << lane) - 1ull;
-        each([&](uint32_t s, float x) {
-            const uint32_t u = order_of(x);
-            const uint64_t ties = __ballot(inside(s) && u == least);
-            const bool tie = inside(s) && u == least && (uint32_t)__popcll(ties & below) < room;
-            const bool keep = tie || (inside(s) && u > least);
-            const uint64_t all = __ballot(keep);
-            if (keep) {
-                const uint32_t at = place + (uint32_t)__popcll(all & below);
-                kept[at] = (int32_t)(p.sinks + lo + s * 64u + lane);
-                out[at] = x;
+        least = (least << bits) | sh_pick[0];
+        left = sh_pick[1];
+    };
+    for (uint32_t i = t; i < kBins; i += kSelThreads) hist[i] = 0u;
+    __syncthreads();
+    each([&](uint32_t, uint32_t u) { atomicAdd(&hist[u >> 21], 1u); });
+    __syncthreads();
+    pick(11);
+    each([&](uint32_t, uint32_t u) {
+        if (u >> 21 == least) atomicAdd(&hist[u >> 10 & 2047u], 1u);
+    });
+    __syncthreads();
+    pick(11);
+    each([&](uint32_t, uint32_t u) {
+        if (u >> 10 == least) atomicAdd(&hist[u & 1023u], 1u);
+    });
+    __syncthreads();
+    pick(10);
+
+    // rows above it, and equal to it, before each wave's
+    uint32_t above = 0, equal = 0;
+    each([&](uint32_t, uint32_t u) {
+        above += __popcll(__ballot(u > least));
+        equal += __popcll(__ballot(u == least));
+    });
+    if (lane == 0) {
+        sh_wave[0][wave] = above;
+        sh_wave[1][wave] = equal;
+    }
+    __syncthreads();
+    const uint32_t equal_before = before_wave(sh_wave[1], wave);
+    uint32_t place = p.sinks + before_wave(sh_wave[0], wave) + min(equal_before, left);
+    uint32_t room = left > equal_before ? left - equal_before : 0u;  // ties of this wave that stay
+    const float *weight = w + p.sinks;
+    each([&](uint32_t s, uint32_t u) {
+        uint64_t keep = __ballot(u > least);
+        if (room) {
+            const uint64_t ties = __ballot(u == least);
+            if (ties) {
+                const uint32_t mine_th = __builtin_amdgcn_mbcnt_hi((uint32_t)(ties >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)ties, 0u));
+                keep |= __ballot(u == least && mine_th < room);
+                const uint32_t used = (uint32_t)__popcll(ties);
+                room = room > used ? room - used : 0u;
             }
-            place += (uint32_t)__popcll(all);
-            const uint32_t used = (uint32_t)__popcll(ties);
-            room = room > used ? room - used : 0u;
-        });
-    }
-    for (uint32_t i = t; i < p.sinks; i += kSelThreads) {
-        kept[i] = (int32_t)i;
-        out[i] = w[i];
-    }
-    for (uint32_t i = t; i < p.recent; i += kSelThreads) {
-        kept[p.keep - p.recent + i] = (int32_t)(n - p.recent + i);
-        out[p.keep - p.recent + i] = w[n - p.recent + i];
-    }
+        }
+        if (keep >> lane & 1u) {
+            const uint32_t at = place + __builtin_amdgcn_mbcnt_hi((uint32_t)(keep >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)keep, 0u));
+            const uint32_t i = lo + s * 64u + lane;
+            kept[at] = (int32_t)(p.sinks + i);
+            out[at] = weight[i];
+        }
+        place += (uint32_t)__popcll(keep);
+    });
 }
 
 __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(KvEvictParams p) {
@@ -182,6 +185,14 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(KvEvictParams p)
             out[i] = w[i];
         }
         return;
+    }
+    for (uint32_t i = t; i < p.sinks; i += kSelThreads) {
+        kept[i] = (int32_t)i;
+        out[i] = w[i];
+    }
+    for (uint32_t i = t; i < p.recent; i += kSelThreads) {
+        kept[p.keep - p.recent + i] = (int32_t)(n - p.recent + i);
+        out[p.keep - p.recent + i] = w[n - p.recent + i];
     }
     if (n - p.sinks - p.recent <= (uint32_t)(kSelThreads * kSelPer))
         select_rows<true>(p, w, n, kept, out, hist, sh_wave, sh_pick);

@@ -161,7 +161,7 @@ __device__ __forceinline__ void find_sequence(const KvAttendParams &p, uint64_t 
 // kDirect: one workgroup for each column of rows, which writes the result; else
 // workers and parts.
 template <typename T, bool kSq8, int DP, bool kDirect>
-__global__ __launch_bounds__(kThreads) void kv_token_kernel(KvAttendParams p) {
+__global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(KvAttendParams p) {
     using E = KvElem<T>;
     constexpr int kSteps = DP / 32;                 // matrix instructions of 16 logits
     constexpr int kPer = DP / 16;                   // values of a row that a lane holds
@@ -248,18 +248,11 @@ __global__ __launch_bounds__(kThreads) void kv_token_kernel(KvAttendParams p) {
         const uint32_t vplace = kv_place(c, c.values, page, (uint32_t)row);
         const bool mine = kplace != kKvNoOffset;
         const uint32_t valid = (uint32_t)__ballot(mine);  // lanes 32..63 repeat 0..31
+        // a row's scales, by lanes 0..31 of the key, by lanes 32..63 of the value (its place: used after the rows' loads are out)
+        float scale = lane < kTile ? 0.0f : 1.0f;
         if constexpr (kSq8) {
-            if (lane < kTile) {
-                float ks = 0.0f, vs = 1.0f;
-                if (mine) {
-                    ks = c.keys.scales[kv_scale_place(c, c.keys, page, (uint32_t)row, h)];
-                    vs = c.values.scales[kv_scale_place(c, c.values, page, (uint32_t)row, h)];
-                }
-                sh_scale[wave][0][lane] = ks * p.scale_log2;
-                vs = vs < kKvLeastScale ? kKvLeastScale : vs;  // a NaN stays
-                sh_scale[wave][1][lane] = log2f(vs);
-                sh_scale[wave][2][lane] = 1.0f / vs;
-            }
+            const KvArray &array = lane < kTile ? c.keys : c.values;
+            if (mine) scale = array.scales[kv_scale_place(c, array, page, (uint32_t)row, h)];
         }
         sh_place[wave][lane >> 5][l32] = mine ? (lane < kTile ? kplace : vplace) : 0u;  // row 0 of page 0 is there to read
         kv_wave_sync();
@@ -286,6 +279,16 @@ __global__ __launch_bounds__(kThreads) void kv_token_kernel(KvAttendParams p) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 vw[4 * t + j] = *reinterpret_cast<const KvWords<kVWords> *>(vbase + (uint64_t)place[j] * 16u + vbyte);
+        }
+        if constexpr (kSq8) {
+            if (lane < kTile) {
+                sh_scale[wave][0][l32] = scale * p.scale_log2;
+            } else {
+                scale = scale < kKvLeastScale ? kKvLeastScale : scale;  // a NaN stays
+                sh_scale[wave][1][l32] = log2f(scale);
+                sh_scale[wave][2][l32] = 1.0f / scale;
+            }
+            kv_wave_sync();
         }
         if (DP != c.dim) {  // dims past the row meet zeros of Q and must be finite
 #pragma unroll
