@@ -10,8 +10,8 @@
 // bits from the top); the last leaves the exact value of the last kept row and
 // how many rows of that value are kept.  A wave owns a contiguous range of rows, so
 // ballots and one sum over the waves give each kept row its place, in order
-// and without a sort.  Up to 32,768 candidates stay in registers from one read
-// (a chain of passes over few bytes: latency-bound).
+// and without a sort.  Up to 32,768 candidates stay in LDS from one read (a chain
+// of passes over few bytes: latency-bound).
 //
 // kv_move_kernel: copy-bound.  Into other pages, workgroups share the kept rows
 // out; in place, the destination of a row is never after its source, so one
@@ -19,6 +19,7 @@
 // reading a batch of rows into registers, waiting for all of it, and writing:
 // what a batch writes lies before every source of the later ones.  Columns
 // are independent, which is where the parallelism comes from.
+#include "kernel_attr.h"
 #include "kv_device.h"
 
 namespace tessa {
@@ -27,8 +28,8 @@ namespace {
 
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / 64;
-constexpr int kSelPer = 32;       // candidates of a lane held in registers
-constexpr int kSelGroup = 8;      // loads in flight where they are not held
+constexpr uint32_t kSelHeld = 32768;  // candidates held in LDS
+constexpr int kSelGroup = 8;      // loads in flight
 constexpr int kBins = 2048;
 constexpr int kMoveThreads = 256;
 constexpr int kMovePer = 8;       // rows of a thread in flight
@@ -49,13 +50,18 @@ __device__ __forceinline__ uint32_t before_wave(const uint32_t *sh, uint32_t wav
     return sum;
 }
 
+// The weight of a key (-0 as 0).
+__device__ __forceinline__ float weight_of(uint32_t u) {
+    return __uint_as_float(u == 0u ? 0x7fc00000u : u >> 31 ? u ^ 0x80000000u : ~u);
+}
+
 // The middle rows [sinks, n - recent) by weight: places sinks.. of `kept` and `out`.
 // Lanes past a wave's last candidate hold the lowest value.  They can at most
 // add to the lowest bin and to the ties of the lowest value, after every real
 // candidate of theirs, where no row is left to place.
 template <bool kHeld>
 __device__ __forceinline__ void select_rows(const KvEvictParams &p, const float *w, uint32_t n, int32_t *kept, float *out,
-                                            uint32_t *hist, uint32_t (*sh_wave)[kSelWaves], uint32_t *sh_pick) {
+                                            uint32_t *held, uint32_t *hist, uint32_t (*sh_wave)[kSelWaves], uint32_t *sh_pick) {
     const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6;
     const uint32_t candidates = n - p.sinks - p.recent;
     const uint32_t need = p.keep - p.sinks - p.recent;
@@ -66,29 +72,21 @@ __device__ __forceinline__ void select_rows(const KvEvictParams &p, const float 
     const uint32_t steps = __builtin_amdgcn_readfirstlane(lo < hi ? (hi - lo + 63u) / 64u : 0u);
     const float *mine = w + p.sinks + lo + lane;
     auto load = [&](uint32_t s) { return lo + s * 64u + lane < hi ? order_of(mine[s * 64u]) : 0u; };
-    uint32_t held[kHeld ? kSelPer : 1];
-    if constexpr (kHeld) {
+    // f(step, value) for each of the lane's candidates.  The loops stay loops: unrolled
+    // over the 32 steps of 32,768 candidates, each instruction runs once a wave and fetching them takes
+    // longer than the work.
+    auto each = [&](auto &&value, auto &&f) {
+#pragma unroll 1
+        for (uint32_t s0 = 0; s0 < steps; s0 += kSelGroup) {
+            uint32_t x[kSelGroup];
 #pragma unroll
-        for (int s = 0; s < kSelPer; ++s) held[s] = load(s);
-    }
-    // f(step, value) for each of the lane's candidates
-    auto each = [&](auto &&f) {
-        if constexpr (kHeld) {
+            for (int s = 0; s < kSelGroup; ++s) x[s] = value(s0 + s);
 #pragma unroll
-            for (int s = 0; s < kSelPer; ++s)
-                if ((uint32_t)s < steps) f((uint32_t)s, held[s]);
-        } else {
-            for (uint32_t s0 = 0; s0 < steps; s0 += kSelGroup) {
-                uint32_t x[kSelGroup];
-#pragma unroll
-                for (int s = 0; s < kSelGroup; ++s) x[s] = load(s0 + s);
-#pragma unroll
-                for (int s = 0; s < kSelGroup; ++s)
-                    if (s0 + s < steps) f(s0 + s, x[s]);
-            }
+            for (int s = 0; s < kSelGroup; ++s) f(s0 + s, x[s]);
         }
     };
-
+    uint32_t *own = held + lo + lane;  // (whole groups of 64 of each wave: span * waves <= kSelHeld)
+    auto again = [&](uint32_t s) { return kHeld ? (s < steps ? own[s * 64u] : 0u) : load(s); };
     // the need-th largest value: three digits from the top
     uint32_t least = 0, left = need;  // digits known so far, kept rows still to place among them
     auto pick = [&](int bits) {       // the digit of the left-th largest value in `hist`
@@ -115,25 +113,30 @@ __device__ __forceinline__ void select_rows(const KvEvictParams &p, const float 
     };
     for (uint32_t i = t; i < kBins; i += kSelThreads) hist[i] = 0u;
     __syncthreads();
-    each([&](uint32_t, uint32_t u) { atomicAdd(&hist[u >> 21], 1u); });
-    __syncthreads();
-    pick(11);
-    each([&](uint32_t, uint32_t u) {
-        if (u >> 21 == least) atomicAdd(&hist[u >> 10 & 2047u], 1u);
+    each(load, [&](uint32_t s, uint32_t u) {
+        if (s < steps) {
+            if constexpr (kHeld) own[s * 64u] = u;
+            atomicAdd(&hist[u >> 21], 1u);
+        }
     });
     __syncthreads();
     pick(11);
-    each([&](uint32_t, uint32_t u) {
-        if (u >> 10 == least) atomicAdd(&hist[u & 1023u], 1u);
+    each(again, [&](uint32_t s, uint32_t u) {
+        if (s < steps && u >> 21 == least) atomicAdd(&hist[u >> 10 & 2047u], 1u);
+    });
+    __syncthreads();
+    pick(11);
+    each(again, [&](uint32_t s, uint32_t u) {
+        if (s < steps && u >> 10 == least) atomicAdd(&hist[u & 1023u], 1u);
     });
     __syncthreads();
     pick(10);
 
     // rows above it, and equal to it, before each wave's
     uint32_t above = 0, equal = 0;
-    each([&](uint32_t, uint32_t u) {
+    each(again, [&](uint32_t s, uint32_t u) {
         above += __popcll(__ballot(u > least));
-        equal += __popcll(__ballot(u == least));
+        equal += __popcll(__ballot(s < steps && u == least));
     });
     if (lane == 0) {
         sh_wave[0][wave] = above;
@@ -143,10 +146,9 @@ __device__ __forceinline__ void select_rows(const KvEvictParams &p, const float 
     const uint32_t equal_before = before_wave(sh_wave[1], wave);
     uint32_t place = p.sinks + before_wave(sh_wave[0], wave) + min(equal_before, left);
     uint32_t room = left > equal_before ? left - equal_before : 0u;  // ties of this wave that stay
-    const float *weight = w + p.sinks;
-    each([&](uint32_t s, uint32_t u) {
+    each(again, [&](uint32_t s, uint32_t u) {
         uint64_t keep = __ballot(u > least);
-        if (room) {
+        if (room && s < steps) {
             const uint64_t ties = __ballot(u == least);
             if (ties) {
                 const uint32_t mine_th = __builtin_amdgcn_mbcnt_hi((uint32_t)(ties >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)ties, 0u));
@@ -159,13 +161,14 @@ __device__ __forceinline__ void select_rows(const KvEvictParams &p, const float 
             const uint32_t at = place + __builtin_amdgcn_mbcnt_hi((uint32_t)(keep >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)keep, 0u));
             const uint32_t i = lo + s * 64u + lane;
             kept[at] = (int32_t)(p.sinks + i);
-            out[at] = weight[i];
+            out[at] = weight_of(u);
         }
         place += (uint32_t)__popcll(keep);
     });
 }
 
 __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(KvEvictParams p) {
+    extern __shared__ uint32_t sh_held[];
     __shared__ uint32_t hist[kBins];
     __shared__ uint32_t sh_wave[2][kSelWaves];
     __shared__ uint32_t sh_pick[2];
@@ -176,28 +179,23 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(KvEvictParams p)
     int32_t *kept = p.kept + bh * p.keep;
     float *out = p.new_weights + bh * p.weight_rows;
     const uint32_t count = min(n, p.keep);
+    if (n > p.keep) {
+        if (n - p.sinks - p.recent <= kSelHeld)
+            select_rows<true>(p, w, n, kept, out, sh_held, hist, sh_wave, sh_pick);
+        else
+            select_rows<false>(p, w, n, kept, out, sh_held, hist, sh_wave, sh_pick);
+    }
+    // the rows that stay without being asked, and what follows the kept ones (after the
+    // selection, whose loads would wait for these stores)
     if (h == 0 && t == 0) p.new_lengths[b] = (int32_t)count;
+    const uint32_t first = n > p.keep ? p.sinks : n, last = n > p.keep ? p.recent : 0u;
+    for (uint32_t i = t; i < first + last; i += kSelThreads) {
+        const uint32_t from = i < first ? i : n - last + (i - first), to = i < first ? i : count - last + (i - first);
+        kept[to] = (int32_t)from;
+        out[to] = w[from];
+    }
     for (uint32_t i = count + t; i < p.keep; i += kSelThreads) kept[i] = -1;
     for (uint32_t i = count + t; i < p.weight_rows; i += kSelThreads) out[i] = 0.0f;
-    if (n <= p.keep) {
-        for (uint32_t i = t; i < n; i += kSelThreads) {
-            kept[i] = (int32_t)i;
-            out[i] = w[i];
-        }
-        return;
-    }
-    for (uint32_t i = t; i < p.sinks; i += kSelThreads) {
-        kept[i] = (int32_t)i;
-        out[i] = w[i];
-    }
-    for (uint32_t i = t; i < p.recent; i += kSelThreads) {
-        kept[p.keep - p.recent + i] = (int32_t)(n - p.recent + i);
-        out[p.keep - p.recent + i] = w[n - p.recent + i];
-    }
-    if (n - p.sinks - p.recent <= (uint32_t)(kSelThreads * kSelPer))
-        select_rows<true>(p, w, n, kept, out, hist, sh_wave, sh_pick);
-    else
-        select_rows<false>(p, w, n, kept, out, hist, sh_wave, sh_pick);
 }
 
 // units: 16-byte pieces of a row that the workgroup moves, from piece `column *
@@ -268,7 +266,11 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(KvEvictParams p, 
 
 int launch_kv_evict(const KvEvictParams &p, uint32_t type, hipStream_t stream) {
     if (p.c.batch == 0) return 0;
-    kv_select_kernel<<<dim3(p.c.heads, p.c.batch), kSelThreads, 0, stream>>>(p);
+    // candidates of the longest sequence that lets them be held, in whole groups of 64 a wave
+    const uint32_t most = p.c.max_length > p.keep ? p.c.max_length - p.sinks - p.recent : 0u;
+    const uint32_t held = most < kSelHeld ? (most + kSelThreads - 1) / kSelThreads * kSelThreads : kSelHeld;
+    if (ensure_lds_limit(reinterpret_cast<const void *>(&kv_select_kernel), (int)(kSelHeld * sizeof(uint32_t))) != 0) return -1;
+    kv_select_kernel<<<dim3(p.c.heads, p.c.batch), kSelThreads, held * sizeof(uint32_t), stream>>>(p);
     if (hipGetLastError() != hipSuccess) return -1;
     const bool in_place = p.into == p.c.table;
     const uint32_t row_units = p.c.dim * (type == kKvSq8 ? 1u : 2u) / 16u;
