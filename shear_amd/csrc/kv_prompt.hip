@@ -13,8 +13,9 @@
 //    half, so the running maximum and sum cost one exchange a tile.
 //  * O^T = V^T P^T: the logits' registers are the P^T operand as they
 //    stand; V^T comes from LDS by transposing reads of 4 rows x 16 values.
-//  * The maximum follows only a logit 2^8 times as large (kKvLag), and tiles that
-//    every query of the workgroup sees in full carry no mask.
+//  * The maximum follows only where a tile's weights would sum to 2^15 (SQ8: a logit
+//    2^8 times as large), and tiles that every query of the workgroup sees in full
+//    carry no mask.
 //  * P is rounded to the queries' type once (an error of the size of the
 //    result's own rounding); sums are in f32.
 //  * SQ8 rows become 16-bit whole numbers on the way into LDS, exactly; scales
@@ -44,6 +45,17 @@ __device__ __forceinline__ uint32_t k_piece(uint32_t r, uint32_t c) {
 template <int DP>
 __device__ __forceinline__ uint32_t v_piece(uint32_t r, uint32_t c) {
     return DP == 64 ? c ^ (((r >> 1) & 1u) << 2) : c ^ ((r & 3u) << 2);
+}
+
+// 16 bytes a lane from base + offset to LDS, lane after lane from `to` on.  The base is a scalar
+// resource and the offset a register of the lane, so no vector instruction forms an
+// address.
+__device__ __forceinline__ void lds_load(const char *base, uint32_t offset, uint32_t scalar_offset, char *to) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int kReach = 0x7fffffff, kRaw = 0x00027000;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, kReach, kRaw),
+                                             (lds_ptr)to, 16, offset, scalar_offset, 0, 0);
+#endif
 }
 
 // Reads of LDS.  Their pointers are `restrict`, which tells the compiler that no
@@ -196,10 +208,23 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
     auto read_rows = [&](uint32_t it, uint32_t buf) {
         const uint32_t r0 = tile_row(it);
         if constexpr (kWhole) {
+            const uint32_t page0 = __builtin_amdgcn_readfirstlane(pages[0]);
+            if ((1u << c.page_shift) >= kRows && page0 < c.pages) {  // the whole tile lies in one page
+                const uint32_t slot = r0 & ((1u << c.page_shift) - 1u);
+                const char *kpage = kbase + (uint64_t)(page0 * c.keys.page_units + slot * c.keys.row_units) * 16u;
+                const char *vpage = vbase + (uint64_t)(page0 * c.values.page_units + slot * c.values.row_units) * 16u;
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    const uint32_t at = ((uint32_t)i * kThreads + wave * 64u) * 16u, rows = (uint32_t)i * kRowsPer * 16u;
+                    lds_load(kpage, koffset[i & (kOffsets - 1)], rows * c.keys.row_units, lds.k[buf] + at);
+                    lds_load(vpage, voffset, rows * c.values.row_units, lds.v[buf] + at);
+                }
+                return;
+            }
             bool all = true;
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) all &= (uint32_t)__builtin_amdgcn_readfirstlane(pages[i]) < c.pages;
-            if (all) {  // rows past the length are read too: finish_rows() clears their values
+            if (all) {  // a page for each load; rows past the length are read too: finish_rows() clears their values
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
                     const uint32_t page = __builtin_amdgcn_readfirstlane(pages[i]);
@@ -207,9 +232,8 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                     const char *kpage = kbase + (uint64_t)(page * c.keys.page_units + slot * c.keys.row_units) * 16u;
                     const char *vpage = vbase + (uint64_t)(page * c.values.page_units + slot * c.values.row_units) * 16u;
                     const uint32_t at = ((uint32_t)i * kThreads + wave * 64u) * 16u;
-                    __builtin_amdgcn_global_load_lds(static_cast<const void *>(kpage + koffset[i & (kOffsets - 1)]),
-                                                     (lds_ptr)(lds.k[buf] + at), 16, 0, 0);
-                    __builtin_amdgcn_global_load_lds(static_cast<const void *>(vpage + voffset), (lds_ptr)(lds.v[buf] + at), 16, 0, 0);
+                    lds_load(kpage, koffset[i & (kOffsets - 1)], 0, lds.k[buf] + at);
+                    lds_load(vpage, voffset, 0, lds.v[buf] + at);
                 }
                 return;
             }
@@ -403,36 +427,52 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                 }
             }
             const float factor = kSq8 ? 1.0f : p.scale_log2;
-            float top = x[0][0];
+            // The running maximum follows the largest logit.
+            auto follow = [&] {
+                float top = x[0][0];
 #pragma unroll
-            for (int u = 0; u < kSubs; ++u)
+                for (int u = 0; u < kSubs; ++u)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) top = fmaxf(top, x[u][e]);
-            top = kv_max32(fmaxf(top * factor, kKvNone));
-            if (__any(top > m + kKvLag)) {
-                const float higher = fmaxf(m, top);
+                    for (int e = 0; e < 16; ++e) top = fmaxf(top, x[u][e]);
+                const float higher = fmaxf(m, kv_max32(fmaxf(top * factor, kKvNone)));
                 const float f = kv_exp2(m - higher);
                 m = higher;
                 l *= f;
 #pragma unroll
                 for (int i = 0; i < kBlocks; ++i) acc[i] *= f;
-            }
+            };
             kv_u4 pf[2 * kSubs];  // P^T operands of 16 rows each
-            float sum = 0.0f;
+            float sum;
+            if constexpr (kSq8) {
+                float top = x[0][0];
 #pragma unroll
-            for (int u = 0; u < kSubs; ++u)
+                for (int u = 0; u < kSubs; ++u)
 #pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                    const float w0 = kv_exp2(fmaf(x[u][e], factor, -m)), w1 = kv_exp2(fmaf(x[u][e + 1], factor, -m));
-                    if constexpr (kSq8) {
-                        const uint32_t r = 32u * u + 8u * (e / 4) + 4u * half + e % 4;
-                        sum = fmaf(w0, lds_read(&lds.scale[buf][2][r]), sum);
-                        sum = fmaf(w1, lds_read(&lds.scale[buf][2][r + 1]), sum);
-                    } else {
-                        sum += w0 + w1;
+                    for (int e = 0; e < 16; ++e) top = fmaxf(top, x[u][e]);
+                if (__any(kv_max32(top) > m + kKvLag)) follow();
+            }
+            // 16-bit rows: the weights are formed with the old maximum, and their sum tells
+            // whether it still served (it does but for a sequence's first tiles): a search for
+            // the largest logit of every tile would stand between the products and the weights
+            for (bool again = false;; again = true) {
+                sum = 0.0f;
+#pragma unroll
+                for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const float w0 = kv_exp2(fmaf(x[u][e], factor, -m)), w1 = kv_exp2(fmaf(x[u][e + 1], factor, -m));
+                        if constexpr (kSq8) {
+                            const uint32_t r = 32u * u + 8u * (e / 4) + 4u * half + e % 4;
+                            sum = fmaf(w0, lds_read(&lds.scale[buf][2][r]), sum);
+                            sum = fmaf(w1, lds_read(&lds.scale[buf][2][r + 1]), sum);
+                        } else {
+                            sum += w0 + w1;
+                        }
+                        pf[2 * u + e / 8][(e % 8) / 2] = E::pack(w0, w1);
                     }
-                    pf[2 * u + e / 8][(e % 8) / 2] = E::pack(w0, w1);
-                }
+                if (kSq8 || again || !__any(!(sum < kKvMost))) break;
+                follow();
+            }
             l += sum;
             // V^T of dims 32 i + n: rows 16 k + 4 half + {0..3}, + 8; read a block ahead
             {
@@ -543,7 +583,10 @@ int launch(const KvAttendParams &p, hipStream_t stream) {
 template <typename T, bool kSq8, int DP>
 int launch_pages(const KvAttendParams &p, hipStream_t stream) {
     if constexpr (!kSq8)
-        if (p.c.dim == DP && (1u << p.c.page_shift) >= kThreads * 8u / DP) return launch<T, kSq8, DP, true>(p, stream);
+        // (a tile's rows within 2^30 bytes: their offsets are 32-bit)
+        if (p.c.dim == DP && (1u << p.c.page_shift) >= kThreads * 8u / DP && p.c.keys.row_units <= 1u << 20 &&
+            p.c.values.row_units <= 1u << 20)
+            return launch<T, kSq8, DP, true>(p, stream);
     return launch<T, kSq8, DP, false>(p, stream);
 }
 
