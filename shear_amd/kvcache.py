@@ -99,10 +99,10 @@ class KvCache:
 def _check(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device) -> None:
     """A device tensor of the type and shape (None: any size), its last dimension contiguous."""
     got = t.shape
-    if t.dtype is not dtype or len(got) != len(shape) or any(w is not None and w != g for w, g in zip(shape, got)):
+    if t.dtype is not dtype or len(got) != len(shape) or not all(w is None or w == g for w, g in zip(shape, got)):
         want = ", ".join("*" if w is None else str(w) for w in shape)
         raise ValueError(f"{name} must be {dtype} [{want}], got {t.dtype} {list(got)}")
-    if t.device != device:
+    if t.get_device() != device.index:
         raise ValueError(f"{name} must be on {device}, not {t.device}")
     if got[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"the last dimension of {name} must be contiguous")
@@ -210,7 +210,7 @@ def _attend(cache, q, page_table, lengths, max_length, scale, sinks, window, str
     on, handle = _on(stream, dev, (*cache._tensors(), q, page_table, lengths, listed, weights, offsets))
     with on:
         q = _rows(q)
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=dev)
+        out = q.new_empty(q.shape)
         lse = torch.empty((tokens, heads), dtype=torch.float32, device=dev)
         strides = q.stride()
         a = N.KvAttend(q.data_ptr(), out.data_ptr(), lse.data_ptr(), strides[:2], (heads * dim, dim),
