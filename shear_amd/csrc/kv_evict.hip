@@ -33,6 +33,7 @@ constexpr int kSelGroup = 8;      // loads in flight
 constexpr int kBins = 2048;
 constexpr int kMoveThreads = 256;
 constexpr int kMovePer = 8;       // rows of a thread in flight
+constexpr uint64_t kMoveHere = 65536;
 
 // An integer that orders as the weight does; NaN is 0.
 __device__ __forceinline__ uint32_t order_of(float w) {
@@ -167,53 +168,17 @@ __device__ __forceinline__ void select_rows(const KvEvictParams &p, const float 
     });
 }
 
-__global__ __launch_bounds__(kSelThreads) void kv_select_kernel(KvEvictParams p) {
-    extern __shared__ uint32_t sh_held[];
-    __shared__ uint32_t hist[kBins];
-    __shared__ uint32_t sh_wave[2][kSelWaves];
-    __shared__ uint32_t sh_pick[2];
-    const uint32_t h = blockIdx.x, b = blockIdx.y, t = threadIdx.x;
-    const uint32_t n = kv_length(p.c, b);
-    const uint64_t bh = (uint64_t)b * p.c.heads + h;
-    const float *w = p.weights + (uint64_t)b * p.weight_batch + (uint64_t)h * p.weight_head;
-    int32_t *kept = p.kept + bh * p.keep;
-    float *out = p.new_weights + bh * p.weight_rows;
-    const uint32_t count = min(n, p.keep);
-    if (n > p.keep) {
-        if (n - p.sinks - p.recent <= kSelHeld)
-            select_rows<true>(p, w, n, kept, out, sh_held, hist, sh_wave, sh_pick);
-        else
-            select_rows<false>(p, w, n, kept, out, sh_held, hist, sh_wave, sh_pick);
-    }
-    // the rows that stay without being asked, and what follows the kept ones (after the
-    // selection, whose loads would wait for these stores)
-    if (h == 0 && t == 0) p.new_lengths[b] = (int32_t)count;
-    const uint32_t first = n > p.keep ? p.sinks : n, last = n > p.keep ? p.recent : 0u;
-    for (uint32_t i = t; i < first + last; i += kSelThreads) {
-        const uint32_t from = i < first ? i : n - last + (i - first), to = i < first ? i : count - last + (i - first);
-        kept[to] = (int32_t)from;
-        out[to] = w[from];
-    }
-    for (uint32_t i = count + t; i < p.keep; i += kSelThreads) kept[i] = -1;
-    for (uint32_t i = count + t; i < p.weight_rows; i += kSelThreads) out[i] = 0.0f;
-}
-
-// units: 16-byte pieces of a row that the workgroup moves, from piece `column *
-// units` on, by 2^lanes_log2 lanes; span: rows of a workgroup (in place: all).
-__global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(KvEvictParams p, uint32_t row_units, uint32_t columns, uint32_t units,
-                                                               uint32_t lanes_log2, uint32_t span, bool in_place) {
+// Moves rows [first, last) of the kept ones of one (sequence, head): of the keys or the
+// values, pieces of 16 bytes from `unit0` on, `units` of them by 2^lanes_log2 lanes of a row.
+template <int kThreads>
+__device__ __forceinline__ void move_rows(const KvEvictParams &p, const KvArray &a, uint32_t b, uint32_t h, uint32_t first, uint32_t last,
+                                          uint32_t row_units, uint32_t unit0, uint32_t units, uint32_t lanes_log2, bool in_place) {
     const KvCacheParams &c = p.c;
-    const uint32_t h = blockIdx.y / (2 * columns), rest = blockIdx.y - h * 2 * columns;
-    const uint32_t b = blockIdx.z, t = threadIdx.x;
-    const uint32_t column = rest >> 1;
-    const KvArray &a = (rest & 1u) ? c.values : c.keys;
-    const uint32_t n = kv_length(c, b), count = min(n, p.keep);
-    const uint32_t first = blockIdx.x * span, last = min(first + span, count);
-    if (first >= last || (in_place && n <= p.keep)) return;
+    const uint32_t t = threadIdx.x;
     const int32_t *kept = p.kept + ((uint64_t)b * c.heads + h) * p.keep;
     const int32_t *from = c.table + (uint64_t)b * c.table_stride, *to = p.into + (uint64_t)b * p.into_stride;
-    const uint32_t lane = t & ((1u << lanes_log2) - 1u), per = kMoveThreads >> lanes_log2;
-    const uint32_t unit = column * units + lane;
+    const uint32_t lane = t & ((1u << lanes_log2) - 1u), per = kThreads >> lanes_log2;
+    const uint32_t unit = unit0 + lane;
     const bool mine = lane < units && unit < row_units;
     const bool scales = a.scales != nullptr && unit == 0;
     char *base = a.rows + ((uint64_t)h * a.head_units + unit) * 16u;
@@ -262,6 +227,55 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(KvEvictParams p, 
     }
 }
 
+__global__ __launch_bounds__(kSelThreads) void kv_select_kernel(KvEvictParams p, uint32_t row_units, uint32_t lanes_log2, bool move) {
+    extern __shared__ uint32_t sh_held[];
+    __shared__ uint32_t hist[kBins];
+    __shared__ uint32_t sh_wave[2][kSelWaves];
+    __shared__ uint32_t sh_pick[2];
+    const uint32_t h = blockIdx.x, b = blockIdx.y, t = threadIdx.x;
+    const uint32_t n = kv_length(p.c, b);
+    const uint64_t bh = (uint64_t)b * p.c.heads + h;
+    const float *w = p.weights + (uint64_t)b * p.weight_batch + (uint64_t)h * p.weight_head;
+    int32_t *kept = p.kept + bh * p.keep;
+    float *out = p.new_weights + bh * p.weight_rows;
+    const uint32_t count = min(n, p.keep);
+    if (n > p.keep) {
+        if (n - p.sinks - p.recent <= kSelHeld)
+            select_rows<true>(p, w, n, kept, out, sh_held, hist, sh_wave, sh_pick);
+        else
+            select_rows<false>(p, w, n, kept, out, sh_held, hist, sh_wave, sh_pick);
+    }
+    // the rows that stay without being asked, and what follows the kept ones (after the
+    // selection, whose loads would wait for these stores)
+    if (h == 0 && t == 0) p.new_lengths[b] = (int32_t)count;
+    const uint32_t first = n > p.keep ? p.sinks : n, last = n > p.keep ? p.recent : 0u;
+    for (uint32_t i = t; i < first + last; i += kSelThreads) {
+        const uint32_t from = i < first ? i : n - last + (i - first), to = i < first ? i : count - last + (i - first);
+        kept[to] = (int32_t)from;
+        out[to] = w[from];
+    }
+    for (uint32_t i = count + t; i < p.keep; i += kSelThreads) kept[i] = -1;
+    for (uint32_t i = count + t; i < p.weight_rows; i += kSelThreads) out[i] = 0.0f;
+    if (move) {  // few rows: here, without another launch
+        const bool in_place = p.into == p.c.table;
+        if (in_place && n <= p.keep) return;
+        __syncthreads();  // the kept rows are listed
+        move_rows<kSelThreads>(p, p.c.keys, b, h, 0, count, row_units, 0, row_units, lanes_log2, in_place);
+        move_rows<kSelThreads>(p, p.c.values, b, h, 0, count, row_units, 0, row_units, lanes_log2, in_place);
+    }
+}
+
+// span: rows of a workgroup (in place: all); `columns` workgroups share a row out.
+__global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(KvEvictParams p, uint32_t row_units, uint32_t columns, uint32_t units,
+                                                               uint32_t lanes_log2, uint32_t span, bool in_place) {
+    const uint32_t h = blockIdx.y / (2 * columns), rest = blockIdx.y - h * 2 * columns, b = blockIdx.z;
+    const uint32_t n = kv_length(p.c, b), count = min(n, p.keep);
+    const uint32_t first = blockIdx.x * span, last = min(first + span, count);
+    if (first >= last || (in_place && n <= p.keep)) return;
+    move_rows<kMoveThreads>(p, (rest & 1u) ? p.c.values : p.c.keys, b, h, first, last, row_units, (rest >> 1) * units, units, lanes_log2,
+                            in_place);
+}
+
 }  // namespace
 
 int launch_kv_evict(const KvEvictParams &p, uint32_t type, hipStream_t stream) {
@@ -270,10 +284,16 @@ int launch_kv_evict(const KvEvictParams &p, uint32_t type, hipStream_t stream) {
     const uint32_t most = p.c.max_length > p.keep ? p.c.max_length - p.sinks - p.recent : 0u;
     const uint32_t held = most < kSelHeld ? (most + kSelThreads - 1) / kSelThreads * kSelThreads : kSelHeld;
     if (ensure_lds_limit(reinterpret_cast<const void *>(&kv_select_kernel), (int)(kSelHeld * sizeof(uint32_t))) != 0) return -1;
-    kv_select_kernel<<<dim3(p.c.heads, p.c.batch), kSelThreads, held * sizeof(uint32_t), stream>>>(p);
-    if (hipGetLastError() != hipSuccess) return -1;
     const bool in_place = p.into == p.c.table;
     const uint32_t row_units = p.c.dim * (type == kKvSq8 ? 1u : 2u) / 16u;
+    uint32_t row_lanes_log2 = 0;
+    while ((1u << row_lanes_log2) < row_units) ++row_lanes_log2;
+    // up to kMoveHere bytes of keys the workgroup that selected the rows moves them too: 256 rows of
+    // 128 bytes, two kernels 7.7 + 7.5 us, one 11.0
+    const bool here = (uint64_t)p.keep * row_units * 16u <= kMoveHere;
+    kv_select_kernel<<<dim3(p.c.heads, p.c.batch), kSelThreads, held * sizeof(uint32_t), stream>>>(p, row_units, row_lanes_log2, here);
+    if (hipGetLastError() != hipSuccess) return -1;
+    if (here) return 0;
     const uint32_t units = in_place ? 4u : row_units;  // 64-byte columns in place, else whole rows
     const uint32_t columns = (row_units + units - 1) / units;
     uint32_t lanes_log2 = 0;
