@@ -71,8 +71,10 @@ __device__ __forceinline__ void select_rows(const KvEvictParams &p, const float 
     const uint32_t span = ((candidates + kSelWaves - 1) / kSelWaves + 63u) / 64u * 64u;
     const uint32_t lo = wave * span, hi = min(lo + span, candidates);
     const uint32_t steps = __builtin_amdgcn_readfirstlane(lo < hi ? (hi - lo + 63u) / 64u : 0u);
-    const float *mine = w + p.sinks + lo + lane;
-    auto load = [&](uint32_t s) { return lo + s * 64u + lane < hi ? order_of(mine[s * 64u]) : 0u; };
+    // (loads without a branch, so that a group of them is out at once)
+    const float *middle = w + p.sinks;
+    auto load = [&](uint32_t s) { return __float_as_uint(middle[min(lo + s * 64u + lane, candidates - 1u)]); };
+    auto order = [&](uint32_t s, uint32_t x) { return lo + s * 64u + lane < hi ? order_of(__uint_as_float(x)) : 0u; };
     // f(step, value) for each of the lane's candidates.  The loops stay loops: unrolled
     // over the 32 steps of 32,768 candidates, each instruction runs once a wave and fetching them takes
     // longer than the work.
@@ -87,7 +89,8 @@ __device__ __forceinline__ void select_rows(const KvEvictParams &p, const float 
         }
     };
     uint32_t *own = held + lo + lane;  // (whole groups of 64 of each wave: span * waves <= kSelHeld)
-    auto again = [&](uint32_t s) { return kHeld ? (s < steps ? own[s * 64u] : 0u) : load(s); };
+    auto again = [&](uint32_t s) { return kHeld ? own[min(s, steps - 1u) * 64u] : load(s); };
+    auto known = [&](uint32_t s, uint32_t x) { return s >= steps ? 0u : kHeld ? x : order(s, x); };
     // the need-th largest value: three digits from the top
     uint32_t least = 0, left = need;  // digits known so far, kept rows still to place among them
     auto pick = [&](int bits) {       // the digit of the left-th largest value in `hist`
@@ -114,7 +117,8 @@ __device__ __forceinline__ void select_rows(const KvEvictParams &p, const float 
     };
     for (uint32_t i = t; i < kBins; i += kSelThreads) hist[i] = 0u;
     __syncthreads();
-    each(load, [&](uint32_t s, uint32_t u) {
+    each(load, [&](uint32_t s, uint32_t x) {
+        const uint32_t u = order(s, x);
         if (s < steps) {
             if constexpr (kHeld) own[s * 64u] = u;
             atomicAdd(&hist[u >> 21], 1u);
@@ -122,12 +126,14 @@ __device__ __forceinline__ void select_rows(const KvEvictParams &p, const float 
     });
     __syncthreads();
     pick(11);
-    each(again, [&](uint32_t s, uint32_t u) {
+    each(again, [&](uint32_t s, uint32_t x) {
+        const uint32_t u = known(s, x);
         if (s < steps && u >> 21 == least) atomicAdd(&hist[u >> 10 & 2047u], 1u);
     });
     __syncthreads();
     pick(11);
-    each(again, [&](uint32_t s, uint32_t u) {
+    each(again, [&](uint32_t s, uint32_t x) {
+        const uint32_t u = known(s, x);
         if (s < steps && u >> 10 == least) atomicAdd(&hist[u & 1023u], 1u);
     });
     __syncthreads();
@@ -135,7 +141,8 @@ __device__ __forceinline__ void select_rows(const KvEvictParams &p, const float 
 
     // rows above it, and equal to it, before each wave's
     uint32_t above = 0, equal = 0;
-    each(again, [&](uint32_t s, uint32_t u) {
+    each(again, [&](uint32_t s, uint32_t x) {
+        const uint32_t u = known(s, x);
         above += __popcll(__ballot(u > least));
         equal += __popcll(__ballot(s < steps && u == least));
     });
@@ -147,7 +154,8 @@ __device__ __forceinline__ void select_rows(const KvEvictParams &p, const float 
     const uint32_t equal_before = before_wave(sh_wave[1], wave);
     uint32_t place = p.sinks + before_wave(sh_wave[0], wave) + min(equal_before, left);
     uint32_t room = left > equal_before ? left - equal_before : 0u;  // ties of this wave that stay
-    each(again, [&](uint32_t s, uint32_t u) {
+    each(again, [&](uint32_t s, uint32_t x) {
+        const uint32_t u = known(s, x);
         uint64_t keep = __ballot(u > least);
         if (room && s < steps) {
             const uint64_t ties = __ballot(u == least);
