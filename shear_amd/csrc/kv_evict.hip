@@ -189,35 +189,30 @@ __device__ __forceinline__ void move_rows(const KvEvictParams &p, const KvArray 
     const uint32_t unit = unit0 + lane;
     const bool mine = lane < units && unit < row_units;
     const bool scales = a.scales != nullptr && unit == 0;
-    char *base = a.rows + ((uint64_t)h * a.head_units + unit) * 16u;
+    char *base = a.rows + ((uint64_t)h * a.head_units + (mine ? unit : 0u)) * 16u;
     const uint32_t into_rows = p.into_columns << c.page_shift;
+    last = min(last, into_rows);
     for (uint32_t j0 = first; j0 < last; j0 += per * kMovePer) {
+        // one load after the other for all rows of the batch, without a branch between: what
+        // is not moved reads the last row's entries and row 0 of page 0
+        uint32_t row[kMovePer], dst[kMovePer];
+        int32_t src_page[kMovePer], dst_page[kMovePer];
         kv_u4 x[kMovePer];
         float sx[kMovePer];
-        uint32_t dst[kMovePer];
-        uint64_t sdst[kMovePer];
+#pragma unroll
+        for (int i = 0; i < kMovePer; ++i) row[i] = (uint32_t)kept[min(j0 + i * per + (t >> lanes_log2), last - 1u)];
 #pragma unroll
         for (int i = 0; i < kMovePer; ++i) {
-            const uint32_t j = j0 + i * per + (t >> lanes_log2);
-            dst[i] = kKvNoOffset;
-            sdst[i] = 0;
+            src_page[i] = from[row[i] >> c.page_shift];
+            dst_page[i] = to[min(j0 + i * per + (t >> lanes_log2), last - 1u) >> c.page_shift];
+        }
+#pragma unroll
+        for (int i = 0; i < kMovePer; ++i) {
+            const uint32_t j = j0 + i * per + (t >> lanes_log2), src = kv_place(c, a, src_page[i], row[i]);
+            dst[i] = j < last && !(in_place && row[i] == j) && src != kKvNoOffset ? kv_place(c, a, dst_page[i], j) : kKvNoOffset;
+            x[i] = *reinterpret_cast<const kv_u4 *>(base + (uint64_t)(dst[i] != kKvNoOffset ? src : 0u) * 16u);
             sx[i] = 0.0f;
-            x[i] = kv_u4{0, 0, 0, 0};
-            if (j < last && j < into_rows) {
-                const uint32_t row = (uint32_t)kept[j];
-                if (!(in_place && row == j)) {
-                    const int32_t src_page = from[row >> c.page_shift], dst_page = to[j >> c.page_shift];
-                    const uint32_t src = kv_place(c, a, src_page, row);
-                    dst[i] = src == kKvNoOffset ? kKvNoOffset : kv_place(c, a, dst_page, j);
-                    if (dst[i] != kKvNoOffset) {
-                        if (mine) x[i] = *reinterpret_cast<const kv_u4 *>(base + (uint64_t)src * 16u);
-                        if (scales) {
-                            sx[i] = a.scales[kv_scale_place(c, a, src_page, row, h)];
-                            sdst[i] = kv_scale_place(c, a, dst_page, j, h);
-                        }
-                    }
-                }
-            }
+            if (scales && dst[i] != kKvNoOffset) sx[i] = a.scales[kv_scale_place(c, a, src_page[i], row[i], h)];
         }
         if (in_place) {
             // every row of the batch has arrived before any is written
@@ -229,7 +224,7 @@ __device__ __forceinline__ void move_rows(const KvEvictParams &p, const KvArray 
         for (int i = 0; i < kMovePer; ++i) {
             if (dst[i] != kKvNoOffset) {
                 if (mine) *reinterpret_cast<kv_u4 *>(base + (uint64_t)dst[i] * 16u) = x[i];
-                if (scales) a.scales[sdst[i]] = sx[i];
+                if (scales) a.scales[kv_scale_place(c, a, dst_page[i], j0 + i * per + (t >> lanes_log2), h)] = sx[i];
             }
         }
     }
