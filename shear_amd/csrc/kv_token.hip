@@ -183,15 +183,48 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
     if constexpr (!kDirect) {
         __shared__ uint64_t sh_sum[2 * kWaves];
         uint64_t total, before;
-        sum_units(p, 0, sh_sum, total, before);
-        const uint32_t workers = workers_of(p, total);
-        if (blockIdx.x >= workers) return;
-        unit = first_unit(blockIdx.x, total * p.columns, workers);
-        unit_end = first_unit(blockIdx.x + 1, total * p.columns, workers);
-        find_sequence(p, unit / p.columns, sh_sum, b, before);
+        uint32_t n;
+        if (c.batch <= kThreads) {  // the lengths are read once: a thread has one sequence's
+            const uint32_t mine = threadIdx.x < c.batch ? units_of(p, threadIdx.x) : 0u;
+            uint32_t upto = mine;  // (at most 256 * 2^23 units)
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const uint32_t y = __shfl_up(upto, off);
+                if (lane >= (uint32_t)off) upto += y;
+            }
+            if (lane == 63u) sh_sum[wave] = upto;
+            __syncthreads();
+            total = 0;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                if ((uint32_t)w < wave) upto += (uint32_t)sh_sum[w];
+                total += sh_sum[w];
+            }
+            const uint32_t workers = workers_of(p, total);
+            if (blockIdx.x >= workers) return;
+            unit = first_unit(blockIdx.x, total * p.columns, workers);
+            unit_end = first_unit(blockIdx.x + 1, total * p.columns, workers);
+            const uint64_t u = unit / p.columns;
+            if (u >= upto - mine && u < upto) {
+                sh_sum[kWaves] = threadIdx.x;
+                sh_sum[kWaves + 1] = upto - mine;
+                sh_sum[kWaves + 2] = mine;
+            }
+            __syncthreads();
+            b = (uint32_t)sh_sum[kWaves];
+            before = sh_sum[kWaves + 1];
+            n = (uint32_t)sh_sum[kWaves + 2];
+        } else {
+            sum_units(p, 0, sh_sum, total, before);
+            const uint32_t workers = workers_of(p, total);
+            if (blockIdx.x >= workers) return;
+            unit = first_unit(blockIdx.x, total * p.columns, workers);
+            unit_end = first_unit(blockIdx.x + 1, total * p.columns, workers);
+            find_sequence(p, unit / p.columns, sh_sum, b, before);
+            n = units_of(p, b);
+        }
         // a sequence's columns follow each other, each of its units
         line = before * p.columns;
-        const uint32_t n = units_of(p, b);
         column = (uint32_t)((unit - line) / n);
         line += (uint64_t)column * n;
     }
