@@ -186,7 +186,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
         uint32_t n;
         if (c.batch <= kThreads) {  // the lengths are read once: a thread has one sequence's
             const uint32_t mine = threadIdx.x < c.batch ? units_of(p, threadIdx.x) : 0u;
-            uint32_t upto = mine;  // (at most 256 * 2^23 units)
+            uint32_t upto = mine;  // (the host keeps a batch under 2^32 units)
 #pragma unroll
             for (int off = 1; off < 64; off <<= 1) {
                 const uint32_t y = __shfl_up(upto, off);

@@ -390,6 +390,87 @@ def test_prompt_values_that_only_later_queries_see(gpu, dim, q_type, cache_type)
     assert torch.isfinite(out[80:90]).all() and torch.isfinite(out[130:]).all()
 
 
+@pytest.mark.parametrize("cache_type", [BF16, SQ8])
+@pytest.mark.parametrize("dim,page", [(128, 64), (128, 16), (64, 32), (256, 128), (64, 128)])
+def test_prompt_missing_pages_of_every_size(gpu, cache_type, dim, page):
+    # a tile in one page, of several pages, and smaller than one
+    new, lengths = [200, 40, 3], [700, 650, 500]
+    pool, g = pool_with(lengths, 2, page, dim, cache_type, BF16, dim + page)
+    pool.table_host[0, 1] = -1
+    pool.table_host[0, 4] = 2**30
+    pool.table_host[1, 0] = -(2**31)
+    pool.table_host[2, :] = -1
+    pool.table = torch.from_numpy(pool.table_host).cuda()
+    q = normal(g, sum(new), 4, dim, scale=2)
+    out, lse = prompt(pool, lengths, new, q)
+    check_prompt(pool, lengths, new, q, out, lse, None, 0)
+    assert (out[240:] == 0).all() and (lse[240:] == -math.inf).all()
+    out, lse = prompt(pool, lengths, new, q, sinks=3, window=90)
+    check_prompt(pool, lengths, new, q, out, lse, 90, 3)
+
+
+@pytest.mark.parametrize("dim,page", [(64, 128), (128, 64), (256, 32)])
+@pytest.mark.parametrize("q_type", [BF16, F16])
+def test_prompt_values_not_finite_in_pages_of_whole_tiles(gpu, dim, page, q_type):
+    """As above where a tile lies in one page: a column with such a value is infinite or NaN
+    from the query on that sees the row, and the others are the results without it."""
+    n = 400
+    g = np.random.default_rng(dim + page)
+    k, v = normal(g, n, 1, dim, dtype=q_type), normal(g, n, 1, dim, dtype=q_type)
+    q = normal(g, n, 2, dim, dtype=q_type)
+    plain = Pool(1, 16, 1, page, dim, q_type, 6)
+    plain.fill([n], k, v)
+    want, want_lse = prompt(plain, [n], [n], q)
+    check_prompt(plain, [n], [n], q, want, want_lse, None, 0)
+    v[75, 0, 0], v[140, 0, dim - 1], v[300, 0, 9] = math.inf, -math.inf, math.nan
+    pool = Pool(1, 16, 1, page, dim, q_type, 6)
+    pool.fill([n], k, v)
+    out, lse = prompt(pool, [n], [n], q)
+    rest = [d for d in range(dim) if d not in (0, 9, dim - 1)]
+    assert torch.equal(out[:, :, rest], want[:, :, rest]) and torch.equal(lse, want_lse)
+    for row, col, of in ((75, 0, torch.isposinf), (140, dim - 1, torch.isneginf), (300, 9, torch.isnan)):
+        assert torch.equal(out[:row, :, col], want[:row, :, col]) and of(out[row:, :, col]).all(), (row, col)
+
+
+@pytest.mark.parametrize("cache_type,q_type", [(BF16, BF16), (F16, F16), (SQ8, BF16), (SQ8, F16)])
+@pytest.mark.parametrize("dim,page", [(128, 64), (64, 16)])
+@pytest.mark.parametrize("how", ["grow", "fall", "jump", "low"])
+def test_prompt_maxima_that_move(gpu, cache_type, q_type, dim, page, how):
+    """Logits that grow along the rows, that fall, that jump by hundreds within a
+    tile, and that are all far below zero."""
+    n, new = 640, 640
+    g = np.random.default_rng(dim)
+    j = np.arange(n)
+    size = {"grow": j / 40, "fall": (n - j) / 40, "jump": np.where(j % 200 == 170, 60.0, 1.0), "low": np.ones(n)}[how]
+    q = normal(g, new, 2, dim, dtype=q_type)
+    k = normal(g, n, 1, dim)
+    if how in ("jump", "low"):  # keys along the queries' common part
+        q[:, :, 0], k[:, :, 0] = 4, (-100 if how == "low" else 4)
+    k = (k.float() * torch.from_numpy(size.astype(np.float32)).cuda()[:, None, None]).to(q_type)
+    v = normal(g, n, 1, dim, dtype=q_type)
+    pool = Pool(1, -(-n // page), 1, page, dim, cache_type, 9)
+    pool.fill([n], k, v)
+    out, lse = prompt(pool, [n], [new], q)
+    check_prompt(pool, [n], [new], q, out, lse, None, 0)
+    out, lse = KV.attend_token(q[-1:].contiguous(), pool.cache, pool.table, lens([n]))
+    check_token(pool, [n], q[-1:], out, lse, None, 0)
+
+
+@pytest.mark.parametrize("window,sinks", [(None, 0), (200, 2)])
+def test_token_many_sequences(gpu, window, sinks):
+    # more sequences than a workgroup has threads, most of them short, some empty
+    g = np.random.default_rng(3)
+    lengths = g.integers(0, 60, 700).tolist()
+    lengths[5], lengths[300], lengths[699] = 1500, 900, 513
+    pool, g = pool_with(lengths, 1, 64, 32, BF16, BF16, 12)
+    q = normal(g, 700, 3, 32, scale=2)
+    weights = torch.zeros((700, 1, 1600), device="cuda")
+    out, lse = KV.attend_token(q, pool.cache, pool.table, lens(lengths), sinks=sinks, window=window, weights=weights)
+    check_token(pool, lengths, q, out, lse, window, sinks, gained=weights)
+    bare, bare_lse = KV.attend_token(q, pool.cache, pool.table, lens(lengths), sinks=sinks, window=window)
+    check_token(pool, lengths, q, bare, bare_lse, window, sinks)
+
+
 def test_prompt_agrees_with_single_tokens(gpu):
     lengths = [257, 64]
     pool, g = pool_with(lengths, 2, 32, 128, BF16, BF16, 41)
