@@ -201,6 +201,15 @@ tessa_status attend_of(const tessa_kv_cache *cache, const tessa_kv_sequences *se
         p.weights = a->weights;
         p.weight_batch = a->weight_strides[0];
         p.weight_head = a->weight_strides[1];
+        if (a->weights) {  // sums are read and written back: no two rows may be one place
+            const uint64_t n[2] = {p.c.batch, p.c.heads}, rows = p.c.max_length;
+            const int inner = n[1] <= 1 || (n[0] > 1 && a->weight_strides[0] < a->weight_strides[1]) ? 0 : 1;
+            const uint64_t near = a->weight_strides[inner], far = a->weight_strides[1 - inner];
+            if (near >= (1ull << 40) || far >= (1ull << 40) || (n[inner] > 1 && near < rows) ||
+                (n[1 - inner] > 1 && far < near * (n[inner] - 1) + rows))
+                KV_INVALID("kv attend: weight strides %llu and %llu for %u rows", (unsigned long long)a->weight_strides[0],
+                           (unsigned long long)a->weight_strides[1], p.c.max_length);
+        }
         const uint64_t shown = p.window == TESSA_KV_ALL ? p.c.max_length : (uint64_t)p.sinks + p.window;
         const uint64_t visible = (shown < p.c.max_length ? shown : p.c.max_length) + p.listed_count;
         if (visible > 0x7fffffffull) KV_UNSUPPORTED("kv attend: %llu visible rows", (unsigned long long)visible);

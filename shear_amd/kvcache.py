@@ -37,11 +37,12 @@ def _strides(t: torch.Tensor, count: int):
     return (C.c_uint64 * count)(*t.stride()[:count])
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class KvCache:
     """Pages of keys and values: [pages, heads, page_rows, head_dim] each, in
     any order of the first three dimensions (rows contiguous, 16-byte aligned);
-    SQ8 caches carry f32 scales [pages, heads, page_rows]."""
+    SQ8 caches carry f32 scales [pages, heads, page_rows].  A cache keeps the
+    tensors that it was made of."""
 
     keys: torch.Tensor
     values: torch.Tensor
@@ -69,7 +70,7 @@ class KvCache:
             n.key_scale_strides, n.value_scale_strides = _strides(self.key_scales, 3), _strides(self.value_scales, 3)
         elif self.key_scales is not None or self.value_scales is not None:
             raise ValueError("only an SQ8 cache has scales")
-        self._native = n
+        object.__setattr__(self, "_native", n)
 
     @classmethod
     def allocate(cls, pages: int, heads: int, page_rows: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
@@ -99,7 +100,10 @@ class KvCache:
 def _check(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device) -> None:
     """A device tensor of the type and shape (None: any size), its last dimension contiguous."""
     got = t.shape
-    if t.dtype is not dtype or len(got) != len(shape) or not all(w is None or w == g for w, g in zip(shape, got)):
+    alike = t.dtype is dtype and len(got) == len(shape)
+    for w, g in zip(shape, got):
+        alike = alike and (w is None or w == g)
+    if not alike:
         want = ", ".join("*" if w is None else str(w) for w in shape)
         raise ValueError(f"{name} must be {dtype} [{want}], got {t.dtype} {list(got)}")
     if t.get_device() != device.index:
@@ -157,14 +161,16 @@ def append(cache: KvCache, page_table: torch.Tensor, starts: torch.Tensor, k: to
     1]`` of ``k`` and ``v`` ([tokens, heads, head_dim]); without ``offsets`` one token
     for each sequence.  ``max_new``: no sequence has more new tokens (default:
     all of them).  Rows past the page table are not written."""
-    dev = cache.keys.device
+    dev, native = cache.keys.device, cache._native
     seq = _sequences(cache, page_table, starts, None)
-    dtype = k.dtype if cache.keys.dtype == torch.int8 and k.dtype in (torch.bfloat16, torch.float16) else (
-        torch.bfloat16 if cache.keys.dtype == torch.int8 else cache.keys.dtype)
-    tokens = k.shape[0]
+    dtype = cache.keys.dtype
+    if dtype == torch.int8:
+        dtype = k.dtype if k.dtype in _QUERY_TYPES else torch.bfloat16
+    tokens = k.shape[0] if k.dim() else 0
+    shape = (tokens, native.heads, native.head_dim)
     for t, name in ((k, "k"), (v, "v")):
-        if t.dtype != dtype or t.dim() != 3 or t.shape != (tokens, cache.heads, cache.head_dim) or t.device != dev:
-            raise ValueError(f"{name} must be {dtype} [{tokens}, {cache.heads}, {cache.head_dim}] on {dev}")
+        if t.dtype != dtype or t.shape != shape or t.device != dev:
+            raise ValueError(f"{name} must be {dtype} {list(shape)} on {dev}")
     if offsets is not None:
         _offsets(offsets, seq.batch, dev)
     elif tokens != seq.batch:
@@ -176,7 +182,7 @@ def append(cache: KvCache, page_table: torch.Tensor, starts: torch.Tensor, k: to
     on, handle = _on(stream, dev, (*cache._tensors(), page_table, starts, k, v, offsets))
     with on:
         k, v = _rows(k), _rows(v)
-        new = N.KvTokens(k.data_ptr(), v.data_ptr(), _strides(k, 2), _strides(v, 2),
+        new = N.KvTokens(k.data_ptr(), v.data_ptr(), k.stride()[:2], v.stride()[:2],
                          None if offsets is None else offsets.data_ptr(), tokens, min(max_new, tokens), _TYPES[dtype])
         N.check(N.load().tessa_kv_append(C.byref(cache._native), C.byref(seq), C.byref(new), handle), "kv append")
 
@@ -221,7 +227,7 @@ def _attend(cache, q, page_table, lengths, max_length, scale, sinks, window, str
             listed = listed.contiguous()
             a.listed, a.listed_count = listed.data_ptr(), listed.shape[2]
         if weights is not None:
-            a.weights, a.weight_strides = weights.data_ptr(), _strides(weights, 2)
+            a.weights, a.weight_strides = weights.data_ptr(), weights.stride()[:2]
         if prompt:
             a.offsets = offsets.data_ptr()
         sizes = (prompt, seq.batch, seq.columns, seq.max_length, tokens, heads, max_new, a.sinks, a.window,
@@ -304,7 +310,7 @@ def evict(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tensor, weigh
         new_weights = torch.empty((seq.batch, cache.heads, rows), dtype=torch.float32, device=dev)
         kept = torch.empty((seq.batch, cache.heads, keep), dtype=torch.int32, device=dev)
         new_lengths = torch.empty(seq.batch, dtype=torch.int32, device=dev)
-        e = N.KvEviction(weights.data_ptr(), _strides(weights, 2), new_weights.data_ptr(), kept.data_ptr(),
+        e = N.KvEviction(weights.data_ptr(), weights.stride()[:2], new_weights.data_ptr(), kept.data_ptr(),
                          new_lengths.data_ptr(), None if into is None else into.data_ptr(),
                          0 if into is None else into.stride(0) if seq.batch > 1 else into.shape[1],
                          0 if into is None else into.shape[1], rows, keep, sinks, recent, 0)

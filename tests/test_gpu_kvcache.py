@@ -8,6 +8,7 @@ import torch
 
 from gpu_helpers import require_gpu
 from kv_reference import Pool, attend, close
+from shear_amd import _native as N
 from shear_amd import kvcache as KV
 from shear_amd import tessa as T
 
@@ -680,3 +681,14 @@ def test_refusals(gpu):
     assert out.shape == (0, 4, 64)
     kept, new, _ = KV.evict(c, none, n[:0], torch.zeros((0, 2, 48), device="cuda"), 8)
     assert kept.shape == (0, 2, 8) and new.shape == (0,)
+
+
+def test_a_cache_keeps_its_tensors(gpu):
+    pool, g = pool_with([20], 2, 16, 64, BF16, BF16, 1)
+    for name in ("keys", "values", "key_scales"):
+        with pytest.raises(AttributeError):
+            setattr(pool.cache, name, torch.zeros_like(pool.cache.keys))
+    q = normal(g, 1, 4, 64)
+    shared = torch.zeros((1, 1, 32), device="cuda").expand(1, 2, 32)  # one sum for both heads
+    with pytest.raises(N.TessaError, match="weight strides"):
+        KV.attend_token(q, pool.cache, pool.table, lens([20]), weights=shared)

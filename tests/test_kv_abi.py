@@ -150,3 +150,25 @@ def test_prompt_append_and_evict_refuse():
     a["tokens"].tokens = 0
     assert lib.tessa_kv_append(C.byref(a["cache"]), C.byref(a["seq"]), C.byref(a["tokens"]), None).code == 0
     assert lib.tessa_kv_evict(C.byref(a["cache"]), C.byref(a["seq"]), C.byref(a["evict"]), None).code == 0
+
+
+@pytest.mark.parametrize("strides,right", [
+    ((128, 64), True), ((64, 128), True), ((200, 70), True), ((0, 64), False), ((128, 0), False), ((64, 64), False),
+    ((127, 64), False), ((64, 127), False), ((63, 256), False), ((0, 0), False), ((2**40, 64), False)])
+def test_weights_that_share_a_place_are_refused(strides, right):
+    # 2 sequences x 2 heads x 64 rows, each of them read, added to and written
+    a = good()
+    a["attend"].weights, a["attend"].weight_strides = 0xB000, strides
+    st, _ = token_scratch(a)
+    assert (st.code == 0) == right
+    if not right:
+        assert st.code == 1 and "weight strides" in st.msg.decode()
+
+
+def test_weight_strides_of_a_single_sequence_or_head():
+    a = good()
+    a["attend"].weights, a["attend"].weight_strides = 0xB000, (0, 64)
+    a["seq"].batch = a["attend"].tokens = 1
+    assert token_scratch(a)[0].code == 0
+    a["attend"].weight_strides = (0, 63)
+    assert token_scratch(a)[0].code == 1
