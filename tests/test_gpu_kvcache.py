@@ -526,6 +526,36 @@ def test_append(gpu, dtype, dim):
         assert rest[~written].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("mixed", [False, True])
+def test_append_codes_of_every_magnitude(gpu, dtype, mixed):
+    """The rule bit for bit: maxima of every significand and of exponents over the type's
+    range, subnormal ones among them, alone or next to others in a wave."""
+    g = np.random.default_rng(8)
+    n, heads, dim = 4096, 2, 64
+    x = torch.from_numpy(g.integers(0, 65536, (n, heads, dim)).astype(np.uint16).view(np.int16)).view(dtype).float()
+    x = torch.where(torch.isfinite(x), x, torch.zeros(()))
+    low, high = (-133, 126) if dtype == BF16 else (-24, 14)
+    size = g.integers(low, high, (n, heads, 1)) if mixed else np.repeat(np.sort(g.integers(low, high, (n, 1, 1)), 0), 2, 1)
+    # significands in 1..2, at most eight powers of two below the row's maximum
+    frac = torch.frexp(x)[0].double() * 2 * torch.from_numpy(2.0 ** -g.integers(0, 9, (n, heads, dim)))
+    k = (frac * torch.from_numpy(2.0 ** size.astype(np.float64))).to(dtype)
+    assert torch.isfinite(k).all()
+    pool = Pool(1, n // 64, heads, 64, dim, SQ8, 2)
+    k = k.cuda()
+    pool.fill([n], k, -k)
+    y = k.float().cpu().numpy()
+    top = np.abs(y).max(-1)
+    scale = (top * (np.float32(1) / np.float32(127))).astype(np.float32)
+    scale = np.where(scale > 0, scale, np.float32(1))
+    q = (y / scale[..., None]).astype(np.float32).astype(np.float64)
+    codes = np.clip(np.sign(q) * np.floor(np.abs(q) + 0.5), -127, 127)
+    page, slot = pool.table_host[0, np.arange(n) // 64].astype(np.int64), np.arange(n) % 64
+    for rows, scales, sign in ((pool.cache.keys, pool.cache.key_scales, 1), (pool.cache.values, pool.cache.value_scales, -1)):
+        assert (scales.cpu().numpy()[page, :, slot] == scale).all()
+        assert (rows.cpu().numpy()[page, :, slot] == sign * codes).all()
+
+
 def test_append_single_tokens_rows_past_the_table_and_not_finite(gpu):
     g = np.random.default_rng(3)
     pool = Pool(3, 2, 2, 8, 32, BF16, 2)
