@@ -360,7 +360,9 @@ tessa_status tessa_kv_evict(const tessa_kv_cache *cache, const tessa_kv_sequence
         }
         p.into = e->into ? e->into : seq->table;
         p.into_stride = e->into ? e->into_stride : seq->table_stride;
-        p.into_columns = e->into ? e->into_columns : seq->columns;
+        // (pages past the kept rows' are not used; their rows need not fit 32 bits)
+        const uint32_t used = (e->keep - 1u) / cache->page_rows + 1u, given = e->into ? e->into_columns : seq->columns;
+        p.into_columns = used < given ? used : given;
         p.keep = e->keep;
         p.sinks = e->sinks;
         p.recent = e->recent;

@@ -31,6 +31,7 @@ from . import _native as N
 
 _QUERY_TYPES = {torch.bfloat16: N.KV_BF16, torch.float16: N.KV_F16}
 _TYPES = {torch.bfloat16: N.KV_BF16, torch.float16: N.KV_F16, torch.int8: N.KV_SQ8}
+_MOST_ROWS = 2**30 - 1  # of a sequence, whatever its table covers
 
 
 def _strides(t: torch.Tensor, count: int):
@@ -125,7 +126,7 @@ def _sequences(cache: KvCache, table: torch.Tensor, lengths: torch.Tensor, max_l
     _check(table, "page_table", torch.int32, (None, None), dev)
     batch, columns = table.shape
     _check(lengths, "lengths", torch.int32, (batch,), dev)
-    covers = columns * cache._native.page_rows
+    covers = min(columns * cache._native.page_rows, _MOST_ROWS)
     if max_length is None:
         max_length = covers
     elif not 0 <= max_length <= covers:
@@ -257,7 +258,8 @@ def attend_token(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, leng
     (int32 [batch, heads, n], negative: none) names for each head of the cache,
     each once.  ``weights`` (f32 [batch, heads, >= max_length]) gets each row's
     weight added, summed over the head's queries.  ``max_length``: no sequence is
-    longer (default: what the page table covers); ``scale`` 1/sqrt(head_dim)."""
+    longer (default: what the page table covers, at most 2^30 - 1); ``scale``
+    1/sqrt(head_dim)."""
     return _attend(cache, q, page_table, lengths, max_length, scale, sinks, window, stream, listed=listed,
                    weights=weights)
 

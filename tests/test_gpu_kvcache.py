@@ -631,6 +631,27 @@ def test_evict(gpu, in_place, cache_type, dim, page, keep, sinks, recent):
             assert np.array_equal(got[0], old[b][h][0][want]) and np.array_equal(got[1], old[b][h][1][want]), (b, h)
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+def test_evict_over_tables_of_more_rows_than_32_bits_count(gpu, in_place):
+    # 65,536 columns of 65,536 rows, of which the sequence uses the first
+    g = np.random.default_rng(2)
+    cache = KV.KvCache.allocate(2, 1, 65536, 16)
+    table, into = (torch.full((1, 65536), -1, dtype=torch.int32, device="cuda") for _ in range(2))
+    table[0, 0], into[0, 0] = 0, 1
+    k, v = normal(g, 900, 1, 16), normal(g, 900, 1, 16)
+    KV.append(cache, table, lens([0]), k, v, offsets=lens([0, 900]))
+    w = torch.from_numpy(g.random((1, 1, 1000)).astype(np.float32)).cuda()
+    kept, n, _ = KV.evict(cache, table, lens([900]), w, 300, sinks=2, recent=10, max_length=900,
+                          into=None if in_place else into)
+    want = kept_rows(w[0, 0].cpu().numpy(), 900, 300, 2, 10)
+    out, lse = KV.attend_token(k[:1].contiguous(), cache, table, lens([1]), window=4)  # (with the default max_length)
+    assert torch.equal(out, cache.values[0, :, :1].transpose(0, 1))
+    assert n.tolist() == [300] and kept[0, 0].tolist() == want
+    page = 0 if in_place else 1
+    assert torch.equal(cache.keys[page, 0, :300], k[kept[0, 0].long(), 0])
+    assert torch.equal(cache.values[page, 0, :300], v[kept[0, 0].long(), 0])
+
+
 @pytest.mark.parametrize("n,keep", [(32768 + 40, 9000), (40000, 39999), (100001, 20000), (33000, 200)])
 def test_evict_long(gpu, n, keep):
     """Around and above the number of candidates held in registers; in place over many steps."""
