@@ -503,15 +503,17 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
 }
 
 // Joins the partial results of a query, out = sum_c exp2(m_c - m) O_c / sum_c
-// exp2(m_c - m) l_c: blocks below `joins`, one for kJoinDims dims of a query, so
-// that few queries with many parts use many compute units, and the parts of a
-// query are read kJoinGroups side by side.  With weights the other blocks turn the
+// exp2(m_c - m) l_c: blocks below `joins`, one for join_dims dims of a query, whose
+// parts it reads 1,024 / join_dims side by side.  Where there are fewer than
+// kJoinBlocks queries a block has fewer dims, 64 at the least, so that few queries with
+// many parts use many compute units (32 queries of 128 dims over 131,071 rows: 59.6 us, with
+// whole queries 62.4; 1,536 queries over 4,100 rows: 131.5, with whole queries 128).  With weights the other blocks turn the
 // logits of 1,024 visible rows into weights and add them, summed over the group's
 // heads, to the caller's.
 constexpr int kWeightPer = 4;  // rows of a thread
 constexpr uint32_t kWeightRows = kThreads * kWeightPer;
 constexpr uint32_t kJoinDims = 64;
-constexpr uint32_t kJoinGroups = kThreads / (kJoinDims / 4);  // 16
+constexpr uint64_t kJoinBlocks = 1024;
 
 // Largest maximum and sum of a query's parts, in all lanes of a wave.
 __device__ __forceinline__ void join_parts(const KvAttendParams &p, uint64_t first, uint32_t step, uint32_t count, float &m, float &l) {
@@ -549,16 +551,16 @@ __device__ __forceinline__ void column_parts(const KvAttendParams &p, uint32_t b
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, uint32_t dp, uint32_t joins, uint32_t row_blocks,
-                                                             bool prompt) {
+__global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, uint32_t dp, uint32_t join_dims, uint32_t joins,
+                                                             uint32_t row_blocks, bool prompt) {
     using E = KvElem<T>;
     const KvCacheParams &c = p.c;
-    __shared__ __align__(16) float sh[kJoinGroups][kJoinDims];
+    __shared__ __align__(16) float sh[kThreads * 4];  // [groups][dims of the block]
     __shared__ float sh_m[kThreads], sh_l[kThreads];
     __shared__ uint64_t sh_sum[2 * kWaves];
     const uint32_t t = threadIdx.x;
     if (blockIdx.x < joins) {
-        const uint32_t slices = (c.dim + kJoinDims - 1) / kJoinDims;
+        const uint32_t slices = (c.dim + join_dims - 1) / join_dims, groups = kThreads * 4 / join_dims;
         const uint64_t query = blockIdx.x / slices;
         const uint32_t slice = blockIdx.x - (uint32_t)query * slices;
         const uint32_t token = (uint32_t)(query / p.q_heads), head = (uint32_t)(query - (uint64_t)token * p.q_heads);
@@ -572,27 +574,27 @@ __global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, u
         }
         float m, l;
         join_parts(p, first, step, count, m, l);
-        const uint32_t grp = t / (kJoinDims / 4), d4 = (t % (kJoinDims / 4)) * 4, d = slice * kJoinDims + d4;
+        const uint32_t grp = t * 4 / join_dims, d4 = t * 4 % join_dims, d = slice * join_dims + d4;
         kv_f4 o = {0, 0, 0, 0};
         constexpr int kFlight = 4;
-        for (uint32_t i0 = grp; i0 < count; i0 += kFlight * kJoinGroups) {
+        for (uint32_t i0 = grp; i0 < count; i0 += kFlight * groups) {
             kv_f4 x[kFlight];
             float f[kFlight];
 #pragma unroll
             for (int j = 0; j < kFlight; ++j) {
-                const uint32_t i = i0 + (uint32_t)j * kJoinGroups;
+                const uint32_t i = i0 + (uint32_t)j * groups;
                 const uint64_t at = first + (uint64_t)(i < count ? i : i0) * step;
                 x[j] = *reinterpret_cast<const kv_f4 *>(p.part_o + at * dp + d);
                 f[j] = i < count ? kv_exp2(p.part_ml[at * 2] - m) : 0.0f;
             }
 #pragma unroll
             for (int j = 0; j < kFlight; ++j)
-                if (i0 + (uint32_t)j * kJoinGroups < count) o += x[j] * f[j];
+                if (i0 + (uint32_t)j * groups < count) o += x[j] * f[j];
         }
-        *reinterpret_cast<kv_f4 *>(&sh[grp][d4]) = o;
+        *reinterpret_cast<kv_f4 *>(&sh[t * 4]) = o;
         __syncthreads();
         if (grp == 0 && d < c.dim) {
-            for (uint32_t i = 1; i < min(kJoinGroups, count); ++i) o += *reinterpret_cast<const kv_f4 *>(&sh[i][d4]);
+            for (uint32_t i = 1; i < min(groups, count); ++i) o += *reinterpret_cast<const kv_f4 *>(&sh[i * join_dims + d4]);
             const float r = l == 0.0f ? 0.0f : 1.0f / l;
             const kv_u2 y = {E::pack(o[0] * r, o[1] * r), E::pack(o[2] * r, o[3] * r)};
             *reinterpret_cast<kv_u2 *>(p.out + (uint64_t)token * p.out_token + (uint64_t)head * p.out_head + 2u * d) = y;
@@ -706,14 +708,17 @@ int launch_kv_token(const KvAttendParams &p, uint32_t type, bool sq8, hipStream_
 }
 
 int launch_kv_finish(const KvAttendParams &p, uint32_t type, bool prompt, hipStream_t stream) {
-    const uint32_t joins = (uint32_t)(p.tokens * p.q_heads) * ((p.c.dim + kJoinDims - 1) / kJoinDims);
+    const uint64_t queries = p.tokens * p.q_heads;
+    const uint32_t dp = kv_padded_dim(p.c.dim);
+    uint32_t dims = dp;
+    while (dims > kJoinDims && queries * (dp / dims) < kJoinBlocks) dims /= 2;
+    const uint32_t joins = (uint32_t)queries * ((p.c.dim + dims - 1) / dims);
     const uint32_t row_blocks = p.weights && !prompt ? (p.max_visible + kWeightRows - 1) / kWeightRows : 0u;
     const uint32_t blocks = joins + row_blocks * p.c.heads * p.c.batch;
-    const uint32_t dp = kv_padded_dim(p.c.dim);
     if (type == kKvBf16)
-        kv_finish_kernel<__bf16><<<blocks, kThreads, 0, stream>>>(p, dp, joins, row_blocks, prompt);
+        kv_finish_kernel<__bf16><<<blocks, kThreads, 0, stream>>>(p, dp, dims, joins, row_blocks, prompt);
     else
-        kv_finish_kernel<_Float16><<<blocks, kThreads, 0, stream>>>(p, dp, joins, row_blocks, prompt);
+        kv_finish_kernel<_Float16><<<blocks, kThreads, 0, stream>>>(p, dp, dims, joins, row_blocks, prompt);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
