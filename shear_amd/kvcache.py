@@ -190,17 +190,17 @@ def append(cache: KvCache, page_table: torch.Tensor, starts: torch.Tensor, k: to
 
 def _attend(cache, q, page_table, lengths, max_length, scale, sinks, window, stream, *, listed=None, weights=None,
             offsets=None, max_new=0):
-    dev, lib = cache.keys.device, N.load()
+    dev, lib, native = cache.keys.device, N.load(), cache._native
     kind = _QUERY_TYPES.get(q.dtype)
     if q.dim() != 3 or kind is None or q.device != dev:
         raise ValueError(f"q must be bf16 or fp16 [tokens, q_heads, head_dim] on {dev}")
-    if kind != cache._native.type != N.KV_SQ8:
+    if kind != native.type != N.KV_SQ8:
         raise ValueError(f"q is {q.dtype}, the cache {cache.keys.dtype}")
-    if q.shape[2] != cache._native.head_dim or q.shape[1] == 0 or q.shape[1] % cache._native.heads:
-        raise ValueError(f"q of {q.shape[1]} heads x {q.shape[2]} over a cache of {cache.heads} heads x {cache.head_dim}")
+    tokens, heads, dim = q.shape
+    if dim != native.head_dim or heads == 0 or heads % native.heads:
+        raise ValueError(f"q of {heads} heads x {dim} over a cache of {cache.heads} heads x {cache.head_dim}")
     if sinks < 0 or (window is not None and window < 0):
         raise ValueError(f"sinks {sinks} and window {window} must not be negative")
-    tokens, heads, dim = q.shape
     seq = _sequences(cache, page_table, lengths, max_length)
     prompt = offsets is not None
     if not prompt and tokens != seq.batch:
@@ -217,10 +217,9 @@ def _attend(cache, q, page_table, lengths, max_length, scale, sinks, window, str
     on, handle = _on(stream, dev, (*cache._tensors(), q, page_table, lengths, listed, weights, offsets))
     with on:
         q = _rows(q)
-        out = q.new_empty(q.shape)
-        lse = torch.empty((tokens, heads), dtype=torch.float32, device=dev)
-        strides = q.stride()
-        a = N.KvAttend(q.data_ptr(), out.data_ptr(), lse.data_ptr(), strides[:2], (heads * dim, dim),
+        out = torch.empty(tokens, heads, dim, dtype=q.dtype, device=dev)
+        lse = torch.empty(tokens, heads, dtype=torch.float32, device=dev)
+        a = N.KvAttend(q.data_ptr(), out.data_ptr(), lse.data_ptr(), q.stride()[:2], (heads * dim, dim),
                        kind, heads, 1.0 / math.sqrt(dim) if scale is None else scale, min(sinks, seq.max_length),
                        N.KV_ALL if window is None else min(window, N.KV_ALL - 1), 0, None, None, (0, 0), None, tokens,
                        max_new, 0)
@@ -237,13 +236,13 @@ def _attend(cache, q, page_table, lengths, max_length, scale, sinks, window, str
         if need is None:
             size = C.c_uint64(0)
             fn = lib.tessa_kv_attend_prompt_scratch if prompt else lib.tessa_kv_attend_token_scratch
-            N.check(fn(C.byref(cache._native), C.byref(seq), C.byref(a), C.byref(size)), "kv attend")
+            N.check(fn(C.byref(native), C.byref(seq), C.byref(a), C.byref(size)), "kv attend")
             if len(cache._scratch) >= 1024:
                 cache._scratch.clear()
             need = cache._scratch[sizes] = size.value
         scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         fn = lib.tessa_kv_attend_prompt if prompt else lib.tessa_kv_attend_token
-        N.check(fn(C.byref(cache._native), C.byref(seq), C.byref(a), scratch.data_ptr() if need else None, need, handle),
+        N.check(fn(C.byref(native), C.byref(seq), C.byref(a), scratch.data_ptr() if need else None, need, handle),
                 "kv attend")
     return out, lse
 
@@ -309,8 +308,8 @@ def evict(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tensor, weigh
             raise ValueError(f"into covers {into.shape[1] * cache.page_rows} rows, {min(keep, seq.max_length)} stay")
     on, handle = _on(stream, dev, (*cache._tensors(), page_table, lengths, weights, into))
     with on:
-        new_weights = torch.empty((seq.batch, cache.heads, rows), dtype=torch.float32, device=dev)
-        kept = torch.empty((seq.batch, cache.heads, keep), dtype=torch.int32, device=dev)
+        new_weights = torch.empty(seq.batch, cache.heads, rows, dtype=torch.float32, device=dev)
+        kept = torch.empty(seq.batch, cache.heads, keep, dtype=torch.int32, device=dev)
         new_lengths = torch.empty(seq.batch, dtype=torch.int32, device=dev)
         e = N.KvEviction(weights.data_ptr(), weights.stride()[:2], new_weights.data_ptr(), kept.data_ptr(),
                          new_lengths.data_ptr(), None if into is None else into.data_ptr(),
