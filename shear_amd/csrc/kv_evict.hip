@@ -10,10 +10,12 @@
 // bits from the top); the last leaves the exact value of the last kept row and
 // how many rows of that value are kept.  A wave owns a contiguous range of rows, so
 // ballots and one sum over the waves give each kept row its place, in order
-// and without a sort.  Up to 32,768 candidates stay in LDS from one read (a chain
-// of passes over few bytes: latency-bound).
+// and without a sort.  Up to 32,768 candidates stay in LDS from one read.  A chain
+// of passes over few bytes, latency-bound: 8 sequences of up to 32,768 rows, 8 heads,
+// 27 us.
 //
-// kv_move_kernel: copy-bound.  Into other pages, workgroups share the kept rows
+// kv_move_kernel: copy-bound (8 x 8,000 rows kept of 8 heads, 128 dims, 16 bits: 524 MB
+// read and written in 109 us, 4.8 TB/s).  Into other pages, workgroups share the kept rows
 // out; in place, the destination of a row is never after its source, so one
 // workgroup walks the rows of one 64-byte column of a (sequence, head) in order,
 // reading a batch of rows into registers, waiting for all of it, and writing:
@@ -291,8 +293,10 @@ int launch_kv_evict(const KvEvictParams &p, uint32_t type, hipStream_t stream) {
     const uint32_t row_units = p.c.dim * (type == kKvSq8 ? 1u : 2u) / 16u;
     uint32_t row_lanes_log2 = 0;
     while ((1u << row_lanes_log2) < row_units) ++row_lanes_log2;
-    // up to kMoveHere bytes of keys the workgroup that selected the rows moves them too: 256 rows of
-    // 128 bytes, two kernels 7.7 + 7.5 us, one 11.0
+    // up to kMoveHere bytes of keys the workgroup that selected the rows moves them too, which saves the
+    // host a launch: 256 of 700 rows of 128 bytes, two kernels 7.7 + 7.5 us, one 11.0.  Of 4,096 rows, 8 heads,
+    // replayed from a graph, two kernels and one: 2 sequences 512 rows of 128 bytes 14.1, 15.3 us, 16 sequences 18.7,
+    // 17.0; at four times the bytes 17.5, 37.0 and 50.5, 80.8
     const bool here = (uint64_t)p.keep * row_units * 16u <= kMoveHere;
     kv_select_kernel<<<dim3(p.c.heads, p.c.batch), kSelThreads, held * sizeof(uint32_t), stream>>>(p, row_units, row_lanes_log2, here);
     if (hipGetLastError() != hipSuccess) return -1;

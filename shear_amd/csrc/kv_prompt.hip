@@ -6,8 +6,15 @@
 // heads), token-major, 128 to a workgroup and 32 to a wave, so that the heads
 // of a group share every K and V tile and a short prompt still fills the
 // instructions' columns.  Tiles of 64 rows (32 at 256 dims) are staged in LDS twice over: while
-// one is worked on, the next comes from memory into registers (its page ids
-// were read a tile earlier) and goes to the other half afterwards.
+// one is worked on, the next comes from memory (its page ids were read a tile
+// earlier): 16-bit rows go to the other half without a register, codes through registers.
+//
+// Bound by the issue of instructions: beside 32 matrix instructions of a wave and
+// tile (128 dims) stand some 260 of the vector units, most of them the weights.  Two
+// prompts of 4,096 tokens, 16 heads over 4 of 128 dims, causal: 153 us,
+// 899 TFLOP/s of 1,207 that a product of 8,192^3 reaches; 12,001 tokens with a
+// window of 1,024 and 4 first rows: 145 us, 667 TFLOP/s (a workgroup's 32
+// tokens see 1,060 rows, its tiles have 1,216).
 //  * S^T = K Q^T on 32x32x16 instructions (rows are the tile's, columns the
 //    queries): a lane has half of the logits of one query, its partner lane (+- 32) the other
 //    half, so the running maximum and sum cost one exchange a tile.
@@ -22,7 +29,9 @@
 //    enter as in kv_token.hip.
 //  * A row that only some queries see may hold infinities or NaN, which would
 //    reach the others as 0 * inf.  In tiles with a mask such values go to LDS as zeros,
-//    and add_special() adds them to the queries that see them.
+//    and are added at the end to the queries that see them.
+#include <cmath>
+
 #include "kernel_attr.h"
 #include "kv_device.h"
 
@@ -98,7 +107,8 @@ __device__ __attribute__((aligned(16))) const uint32_t kv_zeros[4] = {0, 0, 0, 0
 
 // kWhole: each load of the workgroup lies in one page and rows have DP dims, so
 // that addresses are one scalar and a lane's constant; chosen where page_rows
-// is at least kRowsPer.
+// is at least kRowsPer.  (The prompts above: 208 us, with an address of each lane's own 233, before
+// the later steps.)
 template <typename T, bool kSq8, int DP, bool kWhole>
 __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(KvAttendParams p, uint32_t query_tiles) {
     using E = KvElem<T>;
@@ -601,18 +611,27 @@ int launch_dim(const KvAttendParams &p, hipStream_t stream) {
 
 }  // namespace
 
-// One workgroup for all rows of its queries where the queries fill the card;
-// else the rows are split until there are two workgroups a compute unit, with
-// at least 256 rows (4 tiles) each, and the partial results joined.
+// One workgroup for all rows of its queries where the queries fill the card or the
+// rows are few; else the rows are split, into as many parts as keep the card in one
+// round and at least 256 rows (4 tiles) each, and the partial results joined.
+// Where that saves most: a workgroup alone takes 18.5, 26.5 and 53 ns a row
+// at 64, 128 and 256 dims, a join 4 us and 3 ps for each dim of a query's part.
+// Measured, 32 heads of 128 dims over 8, us without and with it:
+//   1 token over 512 rows 17.7, 13.6; over 4,096 106, 14.6; over 32,768 915, 32.6
+//   2 x 256 tokens over 512 rows 20.8, 26.0 (not split); over 2,048 58.8, 49.8; over 4,096 121, 62
 void kv_prompt_split(KvAttendParams &p) {
+    constexpr float kPartCost = 3e-6f, kJoinCost = 4.0f;  // us
     const uint64_t tiles = ((uint64_t)p.max_new * p.group + kQueries - 1) / kQueries * p.c.heads * p.c.batch;
     const uint32_t visible = p.window == 0xffffffffu
                                  ? p.c.max_length
                                  : (uint32_t)min((uint64_t)p.c.max_length, (uint64_t)p.sinks + p.window + kQueries / p.group);
-    uint64_t chunks = tiles ? ((uint64_t)kv_compute_units() * 2 + tiles - 1) / tiles : 1;
-    const uint32_t most = visible / 256u;
-    chunks = chunks < most ? chunks : most;
-    p.chunks = chunks ? (uint32_t)chunks : 1u;
+    const uint32_t dp = kv_padded_dim(p.c.dim);
+    const uint64_t fill = tiles ? (uint64_t)kv_compute_units() * (dp == 256 ? 1u : 2u) / tiles : 1;
+    const uint64_t most = fill < visible / 256u ? fill : visible / 256u;
+    const float rows = (dp == 64 ? 0.0185f : dp == 128 ? 0.0265f : 0.053f) * (float)visible;
+    const float part = (float)(p.tokens * p.q_heads) * (float)dp * kPartCost, best = std::sqrt(rows / part);
+    const uint64_t chunks = best < (float)most ? (uint64_t)best : most;
+    p.chunks = chunks > 1 && rows / (float)chunks + (float)chunks * part + kJoinCost < rows ? (uint32_t)chunks : 1u;
 }
 
 int launch_kv_prompt(const KvAttendParams &p, uint32_t type, bool sq8, hipStream_t stream) {

@@ -16,7 +16,14 @@
 // every next part is of a later column or a later worker.
 //
 // Every visible row is read once for up to 16 query heads, so the cache's
-// bytes bound it; nothing is staged in LDS but row places.
+// bytes bound it; nothing is staged in LDS but row places.  Measured, 32 heads over 8
+// of 128 dims (4 for the third), kernel and join:
+//   48 sequences of up to 4,100 rows, with weights   533 MB   115 + 14 us   4.1 TB/s
+//   8 of up to 40,000 SQ8 rows, with weights         522 MB   122 + 15 us   3.8 TB/s
+//   one of 131,071 rows                              268 MB    52 +  7 us   4.5 TB/s
+//   16, 2,016 rows each of which 1,500 are listed     49 MB    16 +  5 us   2.3 TB/s
+// (a copy reaches 4.9 to 5.5 TB/s here).  The last is a chain of dependent
+// reads, length, list, page, row, and then only two units a workgroup.
 //  * S^T = K Q^T on 16x16x32 instructions: the K operand is 16 bytes of a row
 //    per lane, straight from memory.  Query heads are the columns, so a lane
 //    holds logits of one head and the maximum, sum and rescaling are its own.
@@ -515,6 +522,9 @@ constexpr uint32_t kWeightRows = kThreads * kWeightPer;
 constexpr uint32_t kJoinDims = 64;
 constexpr uint64_t kJoinBlocks = 1024;
 
+// With join_dims 0 (prompts of at least kJoinBlocks queries) a wave takes a query: 16,384 queries
+// of 128 dims over 512 rows in two parts each, the whole call 26 us, and 44 with a block a query.
+
 // Largest maximum and sum of a query's parts, in all lanes of a wave.
 __device__ __forceinline__ void join_parts(const KvAttendParams &p, uint64_t first, uint32_t step, uint32_t count, float &m, float &l) {
     m = kKvNone;
@@ -559,6 +569,44 @@ __global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, u
     __shared__ float sh_m[kThreads], sh_l[kThreads];
     __shared__ uint64_t sh_sum[2 * kWaves];
     const uint32_t t = threadIdx.x;
+    if (join_dims == 0) {  // a wave for a query, a lane for each 64th dim
+        const uint64_t query = (uint64_t)blockIdx.x * kWaves + (t >> 6);
+        if (query >= p.tokens * p.q_heads) return;
+        const uint64_t first = query * p.chunks;
+        const uint32_t lane = t & 63u;
+        float m, l;
+        join_parts(p, first, 1, p.chunks, m, l);
+        constexpr int kMost = 4;  // 256 dims
+        kv_f4 o = {0, 0, 0, 0};
+        const uint32_t per = dp / 64, d = lane * per;
+#pragma unroll 4
+        for (uint32_t i = 0; i < p.chunks; ++i) {
+            const float f = kv_exp2(p.part_ml[(first + i) * 2] - m);
+            const float *x = p.part_o + (first + i) * dp + d;
+            if (per == kMost) {
+                o += *reinterpret_cast<const kv_f4 *>(x) * f;
+            } else if (per == 2) {
+                const float2 y = *reinterpret_cast<const float2 *>(x);
+                o[0] = fmaf(y.x, f, o[0]);
+                o[1] = fmaf(y.y, f, o[1]);
+            } else {
+                o[0] = fmaf(x[0], f, o[0]);
+            }
+        }
+        const uint32_t token = (uint32_t)(query / p.q_heads), head = (uint32_t)(query - (uint64_t)token * p.q_heads);
+        const float r = l == 0.0f ? 0.0f : 1.0f / l;
+        char *to = p.out + (uint64_t)token * p.out_token + (uint64_t)head * p.out_head + 2u * d;
+        if (d < c.dim) {
+            if (per == kMost)
+                *reinterpret_cast<kv_u2 *>(to) = kv_u2{E::pack(o[0] * r, o[1] * r), E::pack(o[2] * r, o[3] * r)};
+            else if (per == 2)
+                *reinterpret_cast<uint32_t *>(to) = E::pack(o[0] * r, o[1] * r);
+            else
+                *reinterpret_cast<uint16_t *>(to) = (uint16_t)E::pack(o[0] * r, 0.0f);
+        }
+        if (lane == 0) p.lse[query] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
+        return;
+    }
     if (blockIdx.x < joins) {
         const uint32_t slices = (c.dim + join_dims - 1) / join_dims, groups = kThreads * 4 / join_dims;
         const uint64_t query = blockIdx.x / slices;
@@ -687,17 +735,25 @@ int launch_dim(const KvAttendParams &p, hipStream_t stream) {
 
 uint32_t kv_padded_dim(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
-// Up to 512 rows one workgroup takes a column of rows and writes the result: a
-// join's launch costs more than the rows do.  Otherwise, and where weights are
-// wanted, as many workgroups as the registers of the compute units hold share the rows
-// out, or fewer where there are fewer units.
+// Up to 512 rows, or 8 for each column of rows of the batch and up to 2,048, one
+// workgroup takes a column and writes the result: a join's launch costs more than
+// the rows do, and many columns fill the card by themselves.  Otherwise, and
+// where weights are wanted, as many workgroups as the registers of the compute units
+// hold share the rows out, or fewer where there are fewer units.
+// Measured, groups of 4 heads of 128 dims, whole columns against shared rows, us:
+//   64 columns of 512 rows    9.8, 11.7    of 1,024   16.9, 14.4
+//   256 columns of 512 rows  15.2, 21.1    of 1,024   24.2, 29.9    of 2,048   43.3, 49.8
+//   512 columns of 1,024     42.7, 52.6    of 2,048   98.9, 109     of 4,096   190, 199
+// and with lengths far apart (the squares of even ones) 256 columns of up to 2,048
+// rows 26.2, 25.3, 512 of up to 4,096 117, 101.
 void kv_token_split(KvAttendParams &p) {
-    constexpr uint32_t kWhole = 512;
+    constexpr uint64_t kWhole = 512, kMostWhole = 2048, kWholeOfColumn = 8;
     p.columns = p.c.heads * ((p.group + 15u) / 16u);
     p.workers = 0;
-    if (p.max_visible <= kWhole && !p.weights) return;
-    const uint64_t units = (uint64_t)(p.max_visible + kUnit - 1) / kUnit * p.columns * p.c.batch;
     const uint64_t most = (uint64_t)kv_compute_units() * (kv_padded_dim(p.c.dim) == 256 ? 1u : 2u);
+    const uint64_t whole = kWholeOfColumn * p.columns * p.c.batch;
+    if (p.max_visible <= (whole < kWhole ? kWhole : whole < kMostWhole ? whole : kMostWhole) && !p.weights) return;
+    const uint64_t units = (uint64_t)(p.max_visible + kUnit - 1) / kUnit * p.columns * p.c.batch;
     p.workers = (uint32_t)(units < most ? units : most);
     if (!p.workers) p.workers = 1;
 }
@@ -712,7 +768,11 @@ int launch_kv_finish(const KvAttendParams &p, uint32_t type, bool prompt, hipStr
     const uint32_t dp = kv_padded_dim(p.c.dim);
     uint32_t dims = dp;
     while (dims > kJoinDims && queries * (dp / dims) < kJoinBlocks) dims /= 2;
-    const uint32_t joins = (uint32_t)queries * ((p.c.dim + dims - 1) / dims);
+    uint32_t joins = (uint32_t)queries * ((p.c.dim + dims - 1) / dims);
+    if (prompt && queries >= kJoinBlocks) {
+        dims = 0;
+        joins = (uint32_t)((queries + kWaves - 1) / kWaves);
+    }
     const uint32_t row_blocks = p.weights && !prompt ? (p.max_visible + kWeightRows - 1) / kWeightRows : 0u;
     const uint32_t blocks = joins + row_blocks * p.c.heads * p.c.batch;
     if (type == kKvBf16)
