@@ -345,6 +345,28 @@ def test_prompt_few_tokens_over_a_long_cache(gpu, cache_type, window, sinks):
     check_prompt(pool, lengths, new, q, out, lse, window, sinks)
 
 
+@pytest.mark.parametrize("q_type,cache_type", [(BF16, BF16), (F16, SQ8)])
+@pytest.mark.parametrize("dim", [16, 64, 80, 128, 144, 256])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (700, 5)])
+def test_prompt_many_queries_over_a_longer_cache(gpu, q_type, cache_type, dim, window, sinks):
+    # split over the rows, and 1,760 queries to join
+    new, lengths = [150, 70], [1100, 900]
+    pool, g = pool_with(lengths, 2, 32, dim, cache_type, q_type, dim)
+    q = normal(g, 220, 8, dim, dtype=q_type, scale=2)
+    out, lse = prompt(pool, lengths, new, q, max_new=150, sinks=sinks, window=window)
+    check_prompt(pool, lengths, new, q, out, lse, window, sinks)
+
+
+@pytest.mark.parametrize("columns,rows", [(60, 512), (60, 513), (72, 576), (72, 577), (256, 2048), (256, 2049)])
+def test_token_on_both_sides_of_whole_columns(gpu, columns, rows):
+    g = np.random.default_rng(columns)
+    lengths = [rows, 0, 1, rows - 1] + g.integers(0, 90, columns // 4 - 4).tolist()
+    pool, g = pool_with(lengths, 4, 64, 32, BF16, BF16, rows)
+    q = normal(g, columns // 4, 8, 32, scale=2)
+    out, lse = KV.attend_token(q, pool.cache, pool.table, lens(lengths), max_length=rows)
+    check_token(pool, lengths, q, out, lse, None, 0)
+
+
 def test_prompt_more_tokens_than_rows_and_missing_pages(gpu):
     new, lengths = [10, 150, 40], [4, 150, 40]
     pool, g = pool_with(lengths, 1, 16, 64, BF16, BF16, 23)
