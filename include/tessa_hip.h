@@ -966,7 +966,7 @@ typedef struct tessa_kv_sequences {
     uint64_t table_stride;
     uint32_t batch;
     uint32_t columns;        /* page ids of a sequence */
-    uint32_t max_length;     /* no length is larger; at most columns * page_rows */
+    uint32_t max_length;     /* no length is larger; at most columns * page_rows and 2^30 - 1 */
     uint32_t reserved;
 } tessa_kv_sequences;
 
@@ -1013,7 +1013,7 @@ typedef struct tessa_kv_attend {
     uint32_t listed_count;
     const int32_t *listed;
     float *weights;
-    uint64_t weight_strides[2];            /* floats: sequence, head; rows contiguous */
+    uint64_t weight_strides[2];            /* floats: sequence, head; max_length each, none shared */
     const int32_t *offsets;
     uint64_t tokens;
     uint32_t max_new;
