@@ -31,6 +31,7 @@ from . import _native as N
 
 _QUERY_TYPES = {torch.bfloat16: N.KV_BF16, torch.float16: N.KV_F16}
 _TYPES = {torch.bfloat16: N.KV_BF16, torch.float16: N.KV_F16, torch.int8: N.KV_SQ8}
+_INT = torch.int32
 _MOST_ROWS = 2**30 - 1  # of a sequence, whatever its table covers
 
 
@@ -123,9 +124,12 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 def _sequences(cache: KvCache, table: torch.Tensor, lengths: torch.Tensor, max_length: int | None) -> N.KvSequences:
     dev = cache.keys.device
-    _check(table, "page_table", torch.int32, (None, None), dev)
+    if not (table.dtype is _INT and table.dim() == 2 and table.get_device() == dev.index and table.is_contiguous()):
+        _check(table, "page_table", _INT, (None, None), dev)
     batch, columns = table.shape
-    _check(lengths, "lengths", torch.int32, (batch,), dev)
+    if not (lengths.dtype is _INT and lengths.shape == (batch,) and lengths.get_device() == dev.index
+            and lengths.is_contiguous()):
+        _check(lengths, "lengths", _INT, (batch,), dev)
     covers = min(columns * cache._native.page_rows, _MOST_ROWS)
     if max_length is None:
         max_length = covers
@@ -142,7 +146,7 @@ def _on(stream: torch.cuda.Stream | None, device: torch.device, tensors):
     """The call's stream: (context in which it is current, its handle)."""
     if stream is None:
         handle = torch._C._cuda_getCurrentRawStream(device.index) or None
-        return (_HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)), handle
+        return (_HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)), handle
     if stream.device != device:
         raise ValueError(f"stream is on {stream.device}, the cache on {device}")
     for t in tensors:
@@ -180,7 +184,8 @@ def append(cache: KvCache, page_table: torch.Tensor, starts: torch.Tensor, k: to
         max_new = tokens
     if max_new < 0:
         raise ValueError(f"max_new {max_new} is negative")
-    on, handle = _on(stream, dev, (*cache._tensors(), page_table, starts, k, v, offsets))
+    on, handle = _on(stream, dev, (cache.keys, cache.values, cache.key_scales, cache.value_scales, page_table, starts, k, v,
+                                   offsets))
     with on:
         k, v = _rows(k), _rows(v)
         new = N.KvTokens(k.data_ptr(), v.data_ptr(), k.stride()[:2], v.stride()[:2],
