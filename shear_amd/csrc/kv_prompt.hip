@@ -5,7 +5,7 @@
 // Per head h of the cache the queries are the pairs (token, one of the G query
 // heads), token-major, 128 to a workgroup and 32 to a wave, so that the heads
 // of a group share every K and V tile and a short prompt still fills the
-// instructions' columns.  Tiles of 64 rows (32 at 256 dims) are staged in LDS twice over: while
+// instructions' columns.  Tiles of 64 rows (32 at 256 dims of 16 bits) are staged in LDS twice over: while
 // one is worked on, the next comes from memory (its page ids were read a tile
 // earlier): 16-bit rows go to the other half without a register, codes through registers.
 //
@@ -86,15 +86,17 @@ __device__ __forceinline__ bool special_half(uint32_t x) {
     return (x & KvElem<T>::kExponent) == KvElem<T>::kExponent;
 }
 
-// Rows of a tile: at 256 dims half as many, for the registers' sake.
-template <int DP>
+// Rows of a tile: at 256 dims of 16-bit rows half as many, for the registers' sake.  (Two
+// prompts of 4,096 tokens, 16 heads over 4 of 256: 516 us, with 64 rows and spills 1,390;
+// SQ8 602 with 64 rows, 742 with 32.)
+template <bool kSq8, int DP>
 constexpr uint32_t prompt_rows() {
-    return DP == 256 ? 32u : 64u;
+    return DP == 256 && !kSq8 ? 32u : 64u;
 }
 
 template <bool kSq8, int DP>
 struct PromptLds {
-    static constexpr uint32_t kRows = prompt_rows<DP>();
+    static constexpr uint32_t kRows = prompt_rows<kSq8, DP>();
     alignas(16) char k[2][kRows * DP * 2];
     alignas(16) char v[2][kRows * DP * 2];
     alignas(16) float scale[kSq8 ? 2 : 1][3][kSq8 ? kRows : 4];
