@@ -19,12 +19,12 @@ constexpr float kKvNone = -3.0e38f;
 // 2^kKvLag times as large: the weights stay below 2^kKvLag (far from either
 // type's largest value), and almost no tile pays for rescaling the output.
 constexpr float kKvLag = 8.0f;
+// The same for SQ8 rows, whose weights are multiplied by the values' scales: these are at
+// most 2^121.1 (the largest bf16 number over 127), so the products stay finite.
+constexpr float kKvLagScaled = 6.0f;
 // A tile's weights, formed with a maximum that may be too small, serve while their sum is
 // below this: each then is a finite number of either type.
 constexpr float kKvMost = 32768.0f;
-// The smallest scale of SQ8 values: below it (values under 1.3e-28) the sum of
-// w_j / v_j could leave f32's range, and such values count as if they had it.
-constexpr float kKvLeastScale = 1.0e-30f;
 
 template <typename T>
 struct KvElem;

@@ -21,17 +21,19 @@
 //    half, so the running maximum and sum cost one exchange a tile.
 //  * O^T = V^T P^T: the logits' registers are the P^T operand as they
 //    stand; V^T comes from LDS by transposing reads of 4 rows x 16 values.
-//  * The maximum follows only where a tile's weights would sum to 2^15 (SQ8: a logit
-//    2^8 times as large), and tiles that every query of the workgroup sees in full
+//  * The maximum follows only where a tile's weights would sum to 2^15 (SQ8: a weight
+//    would be 2^6), and tiles that every query of the workgroup sees in full
 //    carry no mask.
 //  * P is rounded to the queries' type once (an error of the size of the
 //    result's own rounding); sums are in f32.
 //  * SQ8 rows become 16-bit whole numbers on the way into LDS, exactly; scales
-//    enter as in kv_token.hip.
+//    enter as in kv_token.hip, the weights in bf16, for fp16 queries as the sum of
+//    two parts (one alone would be rounded to 8 bits, the result to 11).
 //  * A row that only some queries see may hold infinities or NaN, which would
 //    reach the others as 0 * inf.  In tiles with a mask such values go to LDS as zeros,
 //    and are added at the end to the queries that see them.
 #include <cmath>
+#include <type_traits>
 
 #include "kernel_attr.h"
 #include "kv_device.h"
@@ -99,7 +101,7 @@ struct PromptLds {
     static constexpr uint32_t kRows = prompt_rows<kSq8, DP>();
     alignas(16) char k[2][kRows * DP * 2];
     alignas(16) char v[2][kRows * DP * 2];
-    alignas(16) float scale[kSq8 ? 2 : 1][3][kSq8 ? kRows : 4];
+    alignas(16) float scale[kSq8 ? 2 : 1][2][kSq8 ? kRows : 4];  // of keys (a logit's factor) and values
     // of tile i at i % 4: whether a value was replaced, and the rows without a page.
     // Cleared two tiles ahead, when nothing reads or sets them.
     uint32_t marks[4][1 + kRows / 32];
@@ -115,6 +117,8 @@ __device__ __attribute__((aligned(16))) const uint32_t kv_zeros[4] = {0, 0, 0, 0
 template <typename T, bool kSq8, int DP, bool kWhole>
 __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(KvAttendParams p, uint32_t query_tiles) {
     using E = KvElem<T>;
+    using P = KvElem<std::conditional_t<kSq8, __bf16, T>>;  // of the weights and the values
+    constexpr bool kTwoParts = kSq8 && !std::is_same_v<T, __bf16>;
     using Lds = PromptLds<kSq8, DP>;
     constexpr uint32_t kRows = Lds::kRows;
     constexpr int kSubs = (int)kRows / 32;       // 32 rows of logits each
@@ -208,7 +212,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
     int32_t pages[kLoads];
     kv_u4 kr[kSq8 ? kLoads : 1], vr[kSq8 ? kLoads : 1];  // codes on their way to LDS
     float ks = 0.0f, vs = 1.0f;
-    bool special = false;  // some value was replaced by a zero
+    bool special = false;  // some value or scale was replaced
 
     // Page ids for a tile (past the end: those of the last row), read a tile before they are used.
     auto read_pages = [&](uint32_t it) {
@@ -315,7 +319,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                     for (int e = 0; e < 4; ++e) {
                         const uint32_t kw = kr[i][2 * part + e / 2], vw = vr[i][2 * part + e / 2];
                         k4[e] = E::pack_codes(kv_code(kw, 2 * (e & 1)), kv_code(kw, 2 * (e & 1) + 1));
-                        v4[e] = E::pack_codes(kv_code(vw, 2 * (e & 1)), kv_code(vw, 2 * (e & 1) + 1));
+                        v4[e] = P::pack_codes(kv_code(vw, 2 * (e & 1)), kv_code(vw, 2 * (e & 1) + 1));
                     }
                     const uint32_t to = 2u * load_piece + (uint32_t)part;
                     *reinterpret_cast<kv_u4 *>(&lds.k[buf][r * DP * 2 + k_piece<DP>(r, to) * 16u]) = k4;
@@ -323,12 +327,11 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                 }
             }
             if (t < kRows) {
-                // a NaN scale: its row is NaN to those that see it, which the logit alone carries
-                const bool bad = vs != vs;
-                const float s = bad ? 1.0f : vs < kKvLeastScale ? kKvLeastScale : vs;
-                lds.scale[buf][0][t] = bad ? vs : ks * p.scale_log2;
-                lds.scale[buf][1][t] = log2f(s);
-                lds.scale[buf][2][t] = 1.0f / s;
+                // a value's NaN scale would reach those that do not see the row as 0 * NaN
+                const bool bad = vs != vs && masked(tile_row(it));
+                lds.scale[buf][0][t] = ks * p.scale_log2;
+                lds.scale[buf][1][t] = bad ? 1.0f : vs;
+                if (bad) lds.marks[it & 3u][0] = 1u;
             }
         } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -399,9 +402,8 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                     for (int e = 0; e < 16; e += 4) {
                         const uint32_t r = 32u * u + 2u * e + 4u * half;
                         const kv_f4 k4 = lds_read(reinterpret_cast<const kv_f4 *>(&lds.scale[buf][0][r]));
-                        const kv_f4 v4 = lds_read(reinterpret_cast<const kv_f4 *>(&lds.scale[buf][1][r]));
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) x[u][e + i] = fmaf(x[u][e + i], k4[i], v4[i]);
+                        for (int i = 0; i < 4; ++i) x[u][e + i] *= k4[i];
                     }
             }
             if (mask) {
@@ -454,7 +456,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
 #pragma unroll
                 for (int i = 0; i < kBlocks; ++i) acc[i] *= f;
             };
-            kv_u4 pf[2 * kSubs];  // P^T operands of 16 rows each
+            kv_u4 pf[2 * kSubs], rest[kTwoParts ? 2 * kSubs : 1];  // P^T operands of 16 rows each
             float sum;
             if constexpr (kSq8) {
                 float top = x[0][0];
@@ -462,7 +464,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                 for (int u = 0; u < kSubs; ++u)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) top = fmaxf(top, x[u][e]);
-                if (__any(kv_max32(top) > m + kKvLag)) follow();
+                if (__any(kv_max32(top) > m + kKvLagScaled)) follow();
             }
             // 16-bit rows: the weights are formed with the old maximum, and their sum tells
             // whether it still served (it does but for a sequence's first tiles): a search for
@@ -473,15 +475,16 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                 for (int u = 0; u < kSubs; ++u)
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
-                        const float w0 = kv_exp2(fmaf(x[u][e], factor, -m)), w1 = kv_exp2(fmaf(x[u][e + 1], factor, -m));
+                        float w0 = kv_exp2(fmaf(x[u][e], factor, -m)), w1 = kv_exp2(fmaf(x[u][e + 1], factor, -m));
+                        sum += w0 + w1;
                         if constexpr (kSq8) {
                             const uint32_t r = 32u * u + 8u * (e / 4) + 4u * half + e % 4;
-                            sum = fmaf(w0, lds_read(&lds.scale[buf][2][r]), sum);
-                            sum = fmaf(w1, lds_read(&lds.scale[buf][2][r + 1]), sum);
-                        } else {
-                            sum += w0 + w1;
+                            w0 *= lds_read(&lds.scale[buf][1][r]);
+                            w1 *= lds_read(&lds.scale[buf][1][r + 1]);
                         }
-                        pf[2 * u + e / 8][(e % 8) / 2] = E::pack(w0, w1);
+                        const uint32_t both = P::pack(w0, w1);
+                        pf[2 * u + e / 8][(e % 8) / 2] = both;
+                        if constexpr (kTwoParts) rest[2 * u + e / 8][(e % 8) / 2] = P::pack(w0 - P::low(both), w1 - P::high(both));
                     }
                 if (kSq8 || again || !__any(!(sum < kKvMost))) break;
                 follow();
@@ -509,30 +512,38 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                 for (int i = 0; i < kBlocks; ++i) {
                     if (i + 1 < kBlocks) read(i + 1);
 #pragma unroll
-                    for (int k = 0; k < 2 * kSubs; ++k) acc[i] = E::mma32(a[i][k], pf[k], acc[i]);
+                    for (int k = 0; k < 2 * kSubs; ++k) {
+                        acc[i] = P::mma32(a[i][k], pf[k], acc[i]);
+                        if constexpr (kTwoParts) acc[i] = P::mma32(a[i][k], rest[k], acc[i]);
+                    }
                 }
             }
-            if constexpr (!kSq8)
-                if (mask) special |= lds_read(&marks[0]) != 0u;
+            if (mask) special |= lds_read(&marks[0]) != 0u;
         }
         if (more) finish_rows(it + 1, buf ^ 1u);
         __syncthreads();
     }
     l = kv_sum32(l);
 
-    if constexpr (!kSq8) {
-        // values that were replaced by zeros: added to the queries that see their rows
-        if (__any(special)) {
+    // values (SQ8: scales) that were replaced: added to the queries that see their rows
+    if (__any(special)) {
 #pragma unroll 1
-            for (uint32_t it = first_it; it < last_it; ++it) {
-                const uint32_t r0 = tile_row(it);
-                if (!masked(r0)) continue;
+        for (uint32_t it = first_it; it < last_it; ++it) {
+            const uint32_t r0 = tile_row(it);
+            if (!masked(r0)) continue;
 #pragma unroll 1
-                for (uint32_t row = r0; row < min(r0 + kRows, length); ++row) {
-                    const uint32_t place = kv_place(c, c.values, table[row >> c.page_shift], row);
-                    if (place == kKvNoOffset) continue;
-                    const int32_t r = (int32_t)row;
-                    const bool seen = r <= pos && (!windowed || r < sinks || r > pos - window);
+            for (uint32_t row = r0; row < min(r0 + kRows, length); ++row) {
+                const int32_t page = table[row >> c.page_shift];
+                const uint32_t place = kv_place(c, c.values, page, row);
+                if (place == kKvNoOffset) continue;
+                const int32_t r = (int32_t)row;
+                const bool seen = r <= pos && (!windowed || r < sinks || r > pos - window);
+                if constexpr (kSq8) {
+                    const float scale = c.values.scales[kv_scale_place(c, c.values, page, row, h)];
+                    if (seen && scale != scale)
+#pragma unroll
+                        for (int i = 0; i < kBlocks; ++i) acc[i] += scale;
+                } else {
 #pragma unroll
                     for (int i = 0; i < kBlocks; ++i)
 #pragma unroll

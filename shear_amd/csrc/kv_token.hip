@@ -37,12 +37,14 @@
 //    add an error as large as that of rounding the result; the instructions
 //    it costs are idle otherwise.
 //  * SQ8 rows: codes are whole numbers that both 16-bit types hold exactly.
-//    The key's scale multiplies the logit.  The value's scale v_j enters as
-//    w_j = exp2(s_j + log2 v_j - m), with m the running maximum of that sum, so w_j stays
-//    in range whatever the scales are; l sums w_j / v_j.
+//    The key's scale multiplies the logit, the value's the weight, after l has
+//    summed it; O is formed in bf16 whatever q's type is, because the scales of
+//    a cache can lie further apart than fp16 reaches (a row of zeros has scale 1).
 //  * A row that the table leaves without a page, and a place of the list that
 //    names no further visible row, weighs nothing; its values are replaced by zeros
 //    (0 * NaN would be NaN).
+#include <type_traits>
+
 #include "kv_device.h"
 
 namespace tessa {
@@ -170,13 +172,15 @@ __device__ __forceinline__ void find_sequence(const KvAttendParams &p, uint64_t 
 template <typename T, bool kSq8, int DP, bool kDirect>
 __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(KvAttendParams p) {
     using E = KvElem<T>;
+    using P = KvElem<std::conditional_t<kSq8, __bf16, T>>;  // of the weights and the values
+    constexpr float kLag = kSq8 ? kKvLagScaled : kKvLag;
     constexpr int kSteps = DP / 32;                 // matrix instructions of 16 logits
     constexpr int kPer = DP / 16;                   // values of a row that a lane holds
     constexpr int kKWords = kSq8 ? DP / 16 : DP / 8;  // words of a K row that a lane holds
     constexpr int kVWords = kSq8 ? kPer / 4 : kPer / 2;
     constexpr int kKLoads = kKWords / 4;
     __shared__ uint32_t sh_place[kWaves][2][kTile];
-    __shared__ float sh_scale[kSq8 ? kWaves : 1][3][kTile];
+    __shared__ float sh_scale[kSq8 ? kWaves : 1][2][kTile];
     __shared__ float sh_ml[kWaves][2][16];
     extern __shared__ __align__(16) float sh_out[];  // [waves][heads of the block][DP]
 
@@ -321,13 +325,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
                 vw[4 * t + j] = *reinterpret_cast<const KvWords<kVWords> *>(vbase + (uint64_t)place[j] * 16u + vbyte);
         }
         if constexpr (kSq8) {
-            if (lane < kTile) {
-                sh_scale[wave][0][l32] = scale * p.scale_log2;
-            } else {
-                scale = scale < kKvLeastScale ? kKvLeastScale : scale;  // a NaN stays
-                sh_scale[wave][1][l32] = log2f(scale);
-                sh_scale[wave][2][l32] = 1.0f / scale;
-            }
+            sh_scale[wave][lane >> 5][l32] = lane < kTile ? scale * p.scale_log2 : scale;
             kv_wave_sync();
         }
         if (DP != c.dim) {  // dims past the row meet zeros of Q and must be finite
@@ -390,26 +388,13 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
                     if (head_ok && tile * kTile + r < rows) at[(uint64_t)r * p.group] = x[t][i];
                 }
         }
-        float inv[2][4];
-        if constexpr (kSq8) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const kv_f4 lv = *reinterpret_cast<const kv_f4 *>(&sh_scale[wave][1][16 * t + 4 * g]);
-                const kv_f4 iv = *reinterpret_cast<const kv_f4 *>(&sh_scale[wave][2][16 * t + 4 * g]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[t][i] += lv[i];
-                    inv[t][i] = iv[i];
-                }
-            }
-        }
         float top = kKvNone;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, x[t][i]);
         top = kv_max16(top);
-        if (__any(top > m + kKvLag)) {
+        if (__any(top > m + kLag)) {
             const float higher = fmaxf(m, top);
             const float f = kv_exp2(m - higher);
             m = higher;
@@ -419,30 +404,34 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
         }
         kv_u4 hi, lo;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t) {
+            kv_f4 vs = {1, 1, 1, 1};
+            if constexpr (kSq8) vs = *reinterpret_cast<const kv_f4 *>(&sh_scale[wave][1][16 * t + 4 * g]);
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
-                const float w0 = kv_exp2(x[t][i] - m), w1 = kv_exp2(x[t][i + 1] - m);
-                if constexpr (kSq8)
-                    l = fmaf(w1, inv[t][i + 1], fmaf(w0, inv[t][i], l));
-                else
-                    l += w0 + w1;
-                const uint32_t r = E::pack(w0, w1);
+                float w0 = kv_exp2(x[t][i] - m), w1 = kv_exp2(x[t][i + 1] - m);
+                l += w0 + w1;
+                if constexpr (kSq8) {
+                    w0 *= vs[i];
+                    w1 *= vs[i + 1];
+                }
+                const uint32_t r = P::pack(w0, w1);
                 hi[2 * t + i / 2] = r;
-                lo[2 * t + i / 2] = E::pack(w0 - E::low(r), w1 - E::high(r));
+                lo[2 * t + i / 2] = P::pack(w0 - P::low(r), w1 - P::high(r));
             }
+        }
 #pragma unroll
         for (int e = 0; e < kPer; ++e) {
             kv_u4 a;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if constexpr (kSq8)
-                    a[j] = E::pack_codes(kv_code(vw[2 * j].w[e / 4], e & 3), kv_code(vw[2 * j + 1].w[e / 4], e & 3));
+                    a[j] = P::pack_codes(kv_code(vw[2 * j].w[e / 4], e & 3), kv_code(vw[2 * j + 1].w[e / 4], e & 3));
                 else
                     a[j] = __builtin_amdgcn_perm(vw[2 * j + 1].w[e / 2], vw[2 * j].w[e / 2], e & 1 ? 0x07060302u : 0x05040100u);
             }
-            acc[e] = E::mma16(a, hi, acc[e]);
-            acc[e] = E::mma16(a, lo, acc[e]);
+            acc[e] = P::mma16(a, hi, acc[e]);
+            acc[e] = P::mma16(a, lo, acc[e]);
         }
     }
     l = kv_sum16(l);
