@@ -25,7 +25,9 @@
 //    would be 2^6), and tiles that every query of the workgroup sees in full
 //    carry no mask.
 //  * P is rounded to the queries' type once (an error of the size of the
-//    result's own rounding); sums are in f32.
+//    result's own rounding); sums are in f32.  fp16 has nothing between 0 and 2^-24: there
+//    the largest weight lies between 2^9 and 2^15, so a weight is right to 11 bits
+//    or to 2^-34 of the largest, and many small ones beside a large one add up.
 //  * SQ8 rows become 16-bit whole numbers on the way into LDS, exactly; scales
 //    enter as in kv_token.hip, the weights in bf16, for fp16 queries as the sum of
 //    two parts (one alone would be rounded to 8 bits, the result to 11).
@@ -119,6 +121,8 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
     using E = KvElem<T>;
     using P = KvElem<std::conditional_t<kSq8, __bf16, T>>;  // of the weights and the values
     constexpr bool kTwoParts = kSq8 && !std::is_same_v<T, __bf16>;
+    // what the largest weight is brought to, as a power of two: 32 rows' of it stay below kKvMost
+    constexpr float kLift = !kSq8 && std::is_same_v<T, _Float16> ? 9.0f : 0.0f;
     using Lds = PromptLds<kSq8, DP>;
     constexpr uint32_t kRows = Lds::kRows;
     constexpr int kSubs = (int)kRows / 32;       // 32 rows of logits each
@@ -449,7 +453,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                 for (int u = 0; u < kSubs; ++u)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) top = fmaxf(top, x[u][e]);
-                const float higher = fmaxf(m, kv_max32(fmaxf(top * factor, kKvNone)));
+                const float higher = fmaxf(m, kv_max32(fmaxf(top * factor - kLift, kKvNone)));
                 const float f = kv_exp2(m - higher);
                 m = higher;
                 l *= f;

@@ -35,7 +35,10 @@
 //  * P is given to the matrix instructions as the sum of two 16-bit parts (the
 //    rounded value and the rounded rest), because a single rounding of P would
 //    add an error as large as that of rounding the result; the instructions
-//    it costs are idle otherwise.
+//    it costs are idle otherwise.  fp16 has nothing between 0 and 2^-24: there the
+//    largest weight lies between 2^7 and 2^15, and the rest is multiplied by
+//    2^12 and summed by itself, so that a weight is right to 2^-44 of the largest and
+//    many small ones beside a large one (a first row that takes the attention) add up.
 //  * SQ8 rows: codes are whole numbers that both 16-bit types hold exactly.
 //    The key's scale multiplies the logit, the value's the weight, after l has
 //    summed it; O is formed in bf16 whatever q's type is, because the scales of
@@ -173,7 +176,8 @@ template <typename T, bool kSq8, int DP, bool kDirect>
 __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(KvAttendParams p) {
     using E = KvElem<T>;
     using P = KvElem<std::conditional_t<kSq8, __bf16, T>>;  // of the weights and the values
-    constexpr float kLag = kSq8 ? kKvLagScaled : kKvLag;
+    constexpr bool kHalf = !kSq8 && std::is_same_v<T, _Float16>;  // fp16 weights
+    constexpr float kLag = kSq8 ? kKvLagScaled : kKvLag, kLift = kHalf ? 7.0f : 0.0f, kRest = kHalf ? 4096.0f : 1.0f;
     constexpr int kSteps = DP / 32;                 // matrix instructions of 16 logits
     constexpr int kPer = DP / 16;                   // values of a row that a lane holds
     constexpr int kKWords = kSq8 ? DP / 16 : DP / 8;  // words of a K row that a lane holds
@@ -256,15 +260,24 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
 
     // Q operand: heads are columns; dims of step s as K's lanes hold them
     const bool head_ok = n < heads;
-    kv_u4 qf[kSteps];
+    // beside the second sum of 256 dims the queries would not fit the registers (48 sequences of up to 4,100 rows,
+    // 32 heads over 2 of 256 dims: 71 us, in registers with spills 77, bf16 64)
+    constexpr bool kQueryInLds = kHalf && DP == 256;
+    __shared__ kv_u4 sh_q[kQueryInLds ? kSteps : 1][64];
+    kv_u4 qf[kQueryInLds ? 1 : kSteps];
     {
         const char *q = p.q + (uint64_t)b * p.q_token + (uint64_t)(h * p.group + first_q + (head_ok ? n : 0u)) * p.q_head;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             const uint32_t d = kSq8 ? (uint32_t)(s / 2) * 64u + g * 16u + (uint32_t)(s & 1) * 8u : (uint32_t)s * 32u + g * 8u;
             const kv_u4 zero = {0, 0, 0, 0};
-            qf[s] = head_ok && d < c.dim ? *reinterpret_cast<const kv_u4 *>(q + 2u * d) : zero;
+            const kv_u4 x = head_ok && d < c.dim ? *reinterpret_cast<const kv_u4 *>(q + 2u * d) : zero;
+            if constexpr (!kQueryInLds)
+                qf[s] = x;
+            else if (wave == 0)
+                sh_q[s][lane] = x;
         }
+        if constexpr (kQueryInLds) __syncthreads();
     }
     const char *kbase = c.keys.rows + (uint64_t)h * c.keys.head_units * 16u;
     const char *vbase = c.values.rows + (uint64_t)h * c.values.head_units * 16u;
@@ -272,9 +285,12 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
     const uint32_t vbyte = (n * kPer < c.dim ? n * kPer : 0u) * (kSq8 ? 1u : 2u);
 
     float m = kKvNone, l = 0.0f;
-    kv_f4 acc[kPer];
+    kv_f4 acc[kPer], rest[kHalf ? kPer : 1];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) acc[i] = kv_f4{0, 0, 0, 0};
+    for (int i = 0; i < kPer; ++i) {
+        acc[i] = kv_f4{0, 0, 0, 0};
+        if constexpr (kHalf) rest[i] = acc[i];
+    }
 
     // row of the tile after next, page of the next tile: each load waits a whole step
     const uint32_t l32 = lane & 31u;
@@ -356,7 +372,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
 #pragma unroll
                     for (int e = 0; e < 4; ++e) a[e] = kw[t][s].w[e];
                 }
-                sacc = E::mma16(a, qf[s], sacc);
+                sacc = E::mma16(a, kQueryInLds ? sh_q[kQueryInLds ? s : 0][lane] : qf[kQueryInLds ? 0 : s], sacc);
             }
             if constexpr (kSq8) {
                 const kv_f4 ks = *reinterpret_cast<const kv_f4 *>(&sh_scale[wave][0][16 * t + 4 * g]);
@@ -394,13 +410,16 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, x[t][i]);
         top = kv_max16(top);
-        if (__any(top > m + kLag)) {
-            const float higher = fmaxf(m, top);
+        if (__any(top > m + (kLag + kLift))) {
+            const float higher = fmaxf(m, top - kLift);
             const float f = kv_exp2(m - higher);
             m = higher;
             l *= f;
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) acc[i] *= f;
+            for (int i = 0; i < kPer; ++i) {
+                acc[i] *= f;
+                if constexpr (kHalf) rest[i] *= f;
+            }
         }
         kv_u4 hi, lo;
 #pragma unroll
@@ -417,7 +436,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
                 }
                 const uint32_t r = P::pack(w0, w1);
                 hi[2 * t + i / 2] = r;
-                lo[2 * t + i / 2] = P::pack(w0 - P::low(r), w1 - P::high(r));
+                lo[2 * t + i / 2] = P::pack((w0 - P::low(r)) * kRest, (w1 - P::high(r)) * kRest);
             }
         }
 #pragma unroll
@@ -431,10 +450,17 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
                     a[j] = __builtin_amdgcn_perm(vw[2 * j + 1].w[e / 2], vw[2 * j].w[e / 2], e & 1 ? 0x07060302u : 0x05040100u);
             }
             acc[e] = P::mma16(a, hi, acc[e]);
-            acc[e] = P::mma16(a, lo, acc[e]);
+            if constexpr (kHalf)
+                rest[e] = P::mma16(a, lo, rest[e]);
+            else
+                acc[e] = P::mma16(a, lo, acc[e]);
         }
     }
     l = kv_sum16(l);
+    if constexpr (kHalf) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) acc[i] += rest[i] * (1.0f / kRest);
+    }
 
     // join the waves: sums relative to the largest maximum
     if (g == 0) {

@@ -78,3 +78,38 @@ def test_sq8_value_row_that_is_nan_leaves_the_logits_alone(gpu, q_type, dim):
     seen = ((rows >= bad[0]) & (rows < bad[0] + 60)) | ((rows >= bad[1]) & (rows < bad[1] + 60))
     assert broken[2][seen].isnan().all() and torch.equal(broken[2][~seen], clean[2][~seen])
     assert torch.equal(broken[4][0], clean[4][0]) and broken[4][1].isnan().all()
+
+
+@pytest.mark.parametrize("q_type", [BF16, F16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("gap,size", [(12.0, 1.0), (16.0, 1.0), (18.0, 1.0), (22.0, 1.0), (16.0, 30.0)])
+def test_rows_under_one_that_takes_the_weight(gpu, q_type, dim, gap, size):
+    """A first row without a value takes almost all of the weight; the others' sum is the result."""
+    n = 2000
+    g = np.random.default_rng(dim)
+    q, k = dominated(g, n, 1, dim, q_type, gap, 0)
+    v = (normal(g, n, 1, dim).float() * size).to(q_type)
+    v[0] = 0.0
+    pool = Pool(1, 32, 1, 64, dim, q_type, 3)
+    pool.fill([n], k, v)
+    out, lse = prompt(pool, [n], [n], q)
+    check_prompt(pool, [n], [n], q, out, lse, None, 0)
+
+
+@pytest.mark.parametrize("q_type", [BF16, F16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("gap,size", [(16.0, 1.0), (20.0, 30.0), (24.0, 30.0)])
+@pytest.mark.parametrize("n", [500, 20000])
+def test_token_rows_under_one_that_takes_the_weight(gpu, q_type, dim, gap, size, n):
+    g = np.random.default_rng(dim)
+    q, k = dominated(g, n, 1, dim, q_type, gap, n // 3)
+    v = (normal(g, n, 1, dim).float() * size).to(q_type)
+    v[n // 3] = 0.0
+    pool = Pool(1, -(-n // 64), 1, 64, dim, q_type, 3)
+    pool.fill([n], k, v)
+    q = q[-1:].contiguous()
+    weights = torch.zeros((1, 1, n), device="cuda")
+    out, lse = KV.attend_token(q, pool.cache, pool.table, lens([n]), max_length=n, weights=weights)
+    check_token(pool, [n], q, out, lse, None, 0, gained=weights)
+    out, lse = KV.attend_token(q, pool.cache, pool.table, lens([n]), max_length=n)
+    check_token(pool, [n], q, out, lse, None, 0)
