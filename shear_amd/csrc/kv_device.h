@@ -95,6 +95,20 @@ __device__ __forceinline__ float kv_sum16(float x) {
     return kv_sum32(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
+// Infinities and NaN among the values: p * inf is an infinity, but a weight too small for its type
+// gives 0 * inf and parts of different sign inf - inf.  A sum that has become NaN
+// under weights that are numbers is formed again from such values alone, whose sum s the
+// finite ones cannot change; 0 says that there was none.
+__device__ __forceinline__ float kv_not_finite(float x) { return fabsf(x) < INFINITY ? 0.0f : x; }
+__device__ __forceinline__ float kv_settled(float sum, float s) { return s == 0.0f ? sum : s; }
+__device__ __forceinline__ kv_f4 kv_not_finite(kv_f4 x) {
+    return kv_f4{kv_not_finite(x[0]), kv_not_finite(x[1]), kv_not_finite(x[2]), kv_not_finite(x[3])};
+}
+__device__ __forceinline__ kv_f4 kv_settled(kv_f4 x, kv_f4 s) {
+    return kv_f4{kv_settled(x[0], s[0]), kv_settled(x[1], s[1]), kv_settled(x[2], s[2]), kv_settled(x[3], s[3])};
+}
+__device__ __forceinline__ bool kv_nan(kv_f4 x) { return !(x[0] == x[0] && x[1] == x[1] && x[2] == x[2] && x[3] == x[3]); }
+
 // Orders a wave's LDS writes before its own later reads by other lanes.
 __device__ __forceinline__ void kv_wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

@@ -33,7 +33,7 @@
 //    two parts (one alone would be rounded to 8 bits, the result to 11).
 //  * A row that only some queries see may hold infinities or NaN, which would
 //    reach the others as 0 * inf.  In tiles with a mask such values go to LDS as zeros,
-//    and are added at the end to the queries that see them.
+//    and come back at the end for the queries that see them.
 #include <cmath>
 #include <type_traits>
 
@@ -91,8 +91,8 @@ __device__ __forceinline__ bool special_half(uint32_t x) {
 }
 
 // Rows of a tile: at 256 dims of 16-bit rows half as many, for the registers' sake.  (Two
-// prompts of 4,096 tokens, 16 heads over 4 of 256: 516 us, with 64 rows and spills 1,390;
-// SQ8 602 with 64 rows, 742 with 32.)
+// prompts of 4,096 tokens, 16 heads over 4 of 256: 545 us, with 64 rows and spills 1,390;
+// SQ8 617 with 64 rows, 742 with 32.)
 template <bool kSq8, int DP>
 constexpr uint32_t prompt_rows() {
     return DP == 256 && !kSq8 ? 32u : 64u;
@@ -529,39 +529,76 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
     }
     l = kv_sum32(l);
 
-    // values (SQ8: scales) that were replaced: added to the queries that see their rows
-    if (__any(special)) {
-#pragma unroll 1
-        for (uint32_t it = first_it; it < last_it; ++it) {
-            const uint32_t r0 = tile_row(it);
-            if (!masked(r0)) continue;
-#pragma unroll 1
-            for (uint32_t row = r0; row < min(r0 + kRows, length); ++row) {
-                const int32_t page = table[row >> c.page_shift];
-                const uint32_t place = kv_place(c, c.values, page, row);
-                if (place == kKvNoOffset) continue;
-                const int32_t r = (int32_t)row;
-                const bool seen = r <= pos && (!windowed || r < sinks || r > pos - window);
-                if constexpr (kSq8) {
-                    const float scale = c.values.scales[kv_scale_place(c, c.values, page, row, h)];
-                    if (seen && scale != scale)
+    // values (SQ8: scales) that were replaced in tiles with a mask, for the queries that see their
+    // rows; all tiles' where a sum became NaN under weights that are numbers
+    bool lost = false;
+    if constexpr (!kSq8) {
 #pragma unroll
-                        for (int i = 0; i < kBlocks; ++i) acc[i] += scale;
-                } else {
+        for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-                    for (int i = 0; i < kBlocks; ++i)
+            for (int e = 0; e < 16; ++e) lost |= acc[i][e] != acc[i][e];
+        lost = __any(lost && l == l);
+    }
+    if (lost || __any(special)) {
+        auto seen = [&](uint32_t row) {
+            const int32_t r = (int32_t)row;
+            return r <= pos && (!windowed || r < sinks || r > pos - window);
+        };
+#pragma unroll
+        for (int i = 0; i < (kSq8 ? 1 : kBlocks); ++i) {
+            float s[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+#pragma unroll 1
+            for (uint32_t it = first_it; it < last_it; ++it) {
+                const uint32_t r0 = tile_row(it);
+                if (!lost && !masked(r0)) continue;
+                // the rows that have such values in these dims, a lane for a row
+                const uint32_t mine = r0 + lane;
+                bool odd = false;
+                if (lane < kRows && mine < length) {
+                    const int32_t page = table[mine >> c.page_shift];
+                    const uint32_t place = kv_place(c, c.values, page, mine);
+                    if constexpr (kSq8) {
+                        if (place != kKvNoOffset) {
+                            const float scale = c.values.scales[kv_scale_place(c, c.values, page, mine, h)];
+                            odd = scale != scale;
+                        }
+                    } else {
+#pragma unroll 1
+                        for (uint32_t d = 32u * i; d < min(32u * i + 32u, c.dim) && place != kKvNoOffset; d += 8) {
+                            const kv_u4 x = *reinterpret_cast<const kv_u4 *>(vbase + (uint64_t)place * 16u + 2u * d);
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) odd |= special_half<T>(x[w]) || special_half<T>(x[w] >> 16);
+                        }
+                    }
+                }
+                for (uint64_t rows = __ballot(odd); rows; rows &= rows - 1) {
+                    const uint32_t row = r0 + (uint32_t)__builtin_ctzll(rows);
+                    if constexpr (kSq8) {
+                        s[0] = seen(row) ? NAN : s[0];
+                    } else {
+                        const uint64_t place = kv_place(c, c.values, table[row >> c.page_shift], row);
 #pragma unroll
                         for (int e = 0; e < 16; e += 4) {
-                            const uint32_t d = (uint32_t)i * 32u + 2u * (uint32_t)e + 4u * half;
-                            const kv_u2 x = *reinterpret_cast<const kv_u2 *>(
-                                d < c.dim ? vbase + (uint64_t)place * 16u + 2u * d : reinterpret_cast<const char *>(kv_zeros));
+                            const uint32_t d = 32u * i + 2u * (uint32_t)e + 4u * half;
+                            const kv_u2 x = *reinterpret_cast<const kv_u2 *>(d < c.dim ? vbase + place * 16u + 2u * d
+                                                                                        : reinterpret_cast<const char *>(kv_zeros));
 #pragma unroll
                             for (int w = 0; w < 4; ++w) {
-                                const float y = w & 1 ? E::high(x[w / 2]) : E::low(x[w / 2]);
-                                acc[i][e + w] += seen && !(fabsf(y) < INFINITY) ? y : 0.0f;
+                                const float y = kv_not_finite(w & 1 ? E::high(x[w / 2]) : E::low(x[w / 2]));
+                                s[e + w] += seen(row) ? y : 0.0f;
                             }
                         }
+                    }
                 }
+            }
+            if constexpr (kSq8) {
+#pragma unroll
+                for (int j = 0; j < kBlocks; ++j) acc[j] += s[0];
+            } else if (l == l) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][e] = kv_settled(acc[i][e], s[e]);
             }
         }
     }

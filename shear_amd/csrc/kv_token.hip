@@ -495,6 +495,19 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
         }
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) sum += sh_ml[w][1][head] * kv_exp2(sh_ml[w][0][head] - big);
+        if constexpr (!kSq8) {
+            if (kv_nan(o) && sum == sum && d < c.dim) {  // values that are not finite, under weights that are
+                kv_f4 s = {0, 0, 0, 0};
+                for (uint32_t i = begin; i < end; ++i) {
+                    const int32_t r = visible_row(vis, i, list);
+                    const uint32_t place = kv_place(c, c.values, page_of(r), (uint32_t)r);
+                    if (place == kKvNoOffset) continue;
+                    const kv_u2 y = *reinterpret_cast<const kv_u2 *>(vbase + (uint64_t)place * 16u + 2u * d);
+                    s += kv_not_finite(kv_f4{E::low(y[0]), E::high(y[0]), E::low(y[1]), E::high(y[1])});
+                }
+                o = kv_settled(o, s);
+            }
+        }
         if constexpr (!kDirect) {
             const uint64_t part = ((uint64_t)b * p.columns + column + blockIdx.x) * block_heads + head;
             *reinterpret_cast<kv_f4 *>(p.part_o + part * DP + d) = o;
@@ -608,6 +621,14 @@ __global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, u
                 o[0] = fmaf(x[0], f, o[0]);
             }
         }
+        if (kv_nan(o) && l == l) {
+            kv_f4 s = {0, 0, 0, 0};
+            for (uint32_t i = 0; i < p.chunks; ++i)
+#pragma unroll
+                for (int e = 0; e < kMost; ++e)
+                    if ((uint32_t)e < per) s[e] += kv_not_finite(p.part_o[(first + i) * dp + d + e]);
+            o = kv_settled(o, s);
+        }
         const uint32_t token = (uint32_t)(query / p.q_heads), head = (uint32_t)(query - (uint64_t)token * p.q_heads);
         const float r = l == 0.0f ? 0.0f : 1.0f / l;
         char *to = p.out + (uint64_t)token * p.out_token + (uint64_t)head * p.out_head + 2u * d;
@@ -658,6 +679,12 @@ __global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, u
         __syncthreads();
         if (grp == 0 && d < c.dim) {
             for (uint32_t i = 1; i < min(groups, count); ++i) o += *reinterpret_cast<const kv_f4 *>(&sh[i * join_dims + d4]);
+            if (kv_nan(o) && l == l) {
+                kv_f4 s = {0, 0, 0, 0};
+                for (uint32_t i = 0; i < count; ++i)
+                    s += kv_not_finite(*reinterpret_cast<const kv_f4 *>(p.part_o + (first + (uint64_t)i * step) * dp + d));
+                o = kv_settled(o, s);
+            }
             const float r = l == 0.0f ? 0.0f : 1.0f / l;
             const kv_u2 y = {E::pack(o[0] * r, o[1] * r), E::pack(o[2] * r, o[3] * r)};
             *reinterpret_cast<kv_u2 *>(p.out + (uint64_t)token * p.out_token + (uint64_t)head * p.out_head + 2u * d) = y;

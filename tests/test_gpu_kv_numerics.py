@@ -113,3 +113,85 @@ def test_token_rows_under_one_that_takes_the_weight(gpu, q_type, dim, gap, size,
     check_token(pool, [n], q, out, lse, None, 0, gained=weights)
     out, lse = KV.attend_token(q, pool.cache, pool.table, lens([n]), max_length=n)
     check_token(pool, [n], q, out, lse, None, 0)
+
+
+def with_values(v, rows):
+    """Copy of v [n, 1, dim] whose values (row, dim) -> x of ``rows`` are x, and the columns that have any."""
+    v = v.clone()
+    for (row, d), x in rows.items():
+        v[row, 0, d] = x
+    return v, sorted({d for _, d in rows})
+
+
+def settled(rows, seen, d):
+    """What the values of column d that are not finite make of a sum over the rows that ``seen`` marks, 0: nothing."""
+    return sum((x for (row, col), x in rows.items() if col == d and seen[row]), 0.0)
+
+
+def check_special(out, clean, rows, seen):
+    """One query: columns are infinite or NaN as the seen values make them, and else as without them."""
+    for d in range(out.shape[-1]):
+        want = settled(rows, seen, d)
+        if want == 0.0:
+            assert (out[..., d] == clean[..., d]).all(), d
+        elif math.isnan(want):
+            assert out[..., d].isnan().all(), d
+        else:
+            assert (out[..., d] == want).all(), d
+
+
+@pytest.mark.parametrize("q_type", [BF16, F16])
+@pytest.mark.parametrize("dim", [64, 80, 128, 256])
+@pytest.mark.parametrize("n,gap", [(500, 0.0), (500, 40.0), (500, 80.0), (9000, 0.0), (9000, 40.0)])
+def test_token_values_that_are_infinite(gpu, q_type, dim, n, gap):
+    """An infinity reaches the result as it is, however small its row's weight, and NaN or both signs as NaN."""
+    g = np.random.default_rng(dim)
+    q, k = dominated(g, n, 1, dim, q_type, gap, n - 30)
+    rows = {(5, 0): math.inf, (n - 1, 1): -math.inf, (n // 2, dim - 1): math.nan, (9, 7): math.inf, (n - 2, 7): math.inf,
+            (n - 30, 20): -math.inf, (11, 33): math.inf, (n - 40, 33): -math.inf, (200, 50): -math.inf}
+    plain = normal(g, n, 1, dim, dtype=q_type)
+    v, cols = with_values(plain, rows)
+    plain[:, :, cols] = torch.where(torch.isfinite(v[:, :, cols]), plain[:, :, cols], 0)
+    q = q[-1:].contiguous()
+    listed = torch.tensor([[[5, 200, 17]]], dtype=torch.int32, device="cuda")
+    got = []
+    for values in (plain, v):
+        pool = Pool(1, -(-n // 64), 1, 64, dim, q_type, 3)
+        pool.fill([n], k, values)
+        weights = torch.zeros((1, 1, n), device="cuda")
+        got.append((KV.attend_token(q, pool.cache, pool.table, lens([n]), max_length=n),
+                    KV.attend_token(q, pool.cache, pool.table, lens([n]), max_length=n, weights=weights),
+                    KV.attend_token(q, pool.cache, pool.table, lens([n]), max_length=n, window=60, sinks=4, listed=listed)))
+    j = np.arange(n)
+    near = (j < 4) | (j >= n - 60) | (j == 5) | (j == 200) | (j == 17)
+    for i, seen in ((0, j >= 0), (1, j >= 0), (2, near)):
+        assert torch.equal(got[0][i][1], got[1][i][1])
+        check_special(got[1][i][0], got[0][i][0], rows, seen)
+
+
+@pytest.mark.parametrize("q_type", [BF16, F16])
+@pytest.mark.parametrize("dim,page", [(64, 16), (80, 64), (128, 64), (256, 32)])
+@pytest.mark.parametrize("n,new,gap", [(400, 400, 0.0), (400, 400, 40.0), (400, 400, 80.0), (5000, 3, 0.0), (5000, 3, 40.0),
+                                       (900, 300, 40.0)])
+def test_prompt_values_that_are_infinite(gpu, q_type, dim, page, n, new, gap):
+    g = np.random.default_rng(dim)
+    q, k = dominated(g, n, 1, dim, q_type, gap, 60)
+    rows = {(5, 0): math.inf, (n - 1, 1): -math.inf, (n // 2, dim - 1): math.nan, (9, 7): math.inf, (n - 2, 7): math.inf,
+            (60, 20): -math.inf, (11, 33): math.inf, (n - 40, 33): -math.inf, (200, 50): -math.inf}
+    plain = normal(g, n, 1, dim, dtype=q_type)
+    v, cols = with_values(plain, rows)
+    plain[:, :, cols] = torch.where(torch.isfinite(v[:, :, cols]), plain[:, :, cols], 0)
+    q = q[n - new:].contiguous()
+    got = []
+    for values in (plain, v):
+        pool = Pool(1, -(-n // page), 1, page, dim, q_type, 3)
+        pool.fill([n], k, values)
+        got.append((prompt(pool, [n], [new], q), prompt(pool, [n], [new], q, window=150, sinks=7)))
+    j = np.arange(n)
+    for i, window in ((0, None), (1, 150)):
+        (out, lse), (clean, clean_lse) = got[1][i], got[0][i]
+        assert torch.equal(lse, clean_lse)
+        for t in sorted({0, 1, 2, new - 1, new - 2, new // 2, *range(3, new, max(1, new // 40))} & set(range(new))):
+            pos = n - new + t
+            seen = (j <= pos) if window is None else (j <= pos) & ((j < 7) | (j > pos - window))
+            check_special(out[t].cpu(), clean[t].cpu(), rows, seen)
