@@ -48,6 +48,7 @@
 //    (0 * NaN would be NaN).
 #include <type_traits>
 
+#include "kernel_attr.h"
 #include "kv_device.h"
 
 namespace tessa {
@@ -757,10 +758,10 @@ __global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, u
 template <typename T, bool kSq8, int DP>
 int launch(const KvAttendParams &p, hipStream_t stream) {
     const size_t lds = (size_t)kWaves * (p.group < 16u ? p.group : 16u) * DP * sizeof(float);
-    if (p.workers)
-        kv_token_kernel<T, kSq8, DP, false><<<p.workers, kThreads, lds, stream>>>(p);
-    else
-        kv_token_kernel<T, kSq8, DP, true><<<dim3(p.columns, p.c.batch), kThreads, lds, stream>>>(p);
+    auto *kernel = p.workers ? &kv_token_kernel<T, kSq8, DP, false> : &kv_token_kernel<T, kSq8, DP, true>;
+    // 16 heads of 256 dims are 64 KiB, beside up to 10 KiB that the kernel has anyway: above the default limit
+    if (lds > 32768 && ensure_lds_limit(reinterpret_cast<const void *>(kernel), (int)lds) != 0) return -1;
+    kernel<<<p.workers ? dim3(p.workers) : dim3(p.columns, p.c.batch), kThreads, lds, stream>>>(p);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 

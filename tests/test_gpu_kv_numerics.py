@@ -9,7 +9,7 @@ import torch
 from gpu_helpers import require_gpu
 from kv_reference import Pool
 from shear_amd import kvcache as KV
-from test_gpu_kvcache import BF16, F16, SQ8, check_prompt, check_token, lens, normal, prompt
+from test_gpu_kvcache import BF16, F16, SQ8, check_prompt, check_token, lens, normal, pool_with, prompt
 
 pytestmark = pytest.mark.gpu
 
@@ -195,3 +195,18 @@ def test_prompt_values_that_are_infinite(gpu, q_type, dim, page, n, new, gap):
             pos = n - new + t
             seen = (j <= pos) if window is None else (j <= pos) & ((j < 7) | (j > pos - window))
             check_special(out[t].cpu(), clean[t].cpu(), rows, seen)
+
+
+@pytest.mark.parametrize("cache_type,q_type", [(BF16, BF16), (F16, F16), (SQ8, BF16), (SQ8, F16)])
+@pytest.mark.parametrize("dim", [144, 256])
+@pytest.mark.parametrize("group", [14, 16, 17, 40])
+def test_token_whole_blocks_of_heads_of_wide_rows(gpu, cache_type, q_type, dim, group):
+    """16 heads of 256 dims take more LDS than a kernel has by default; whole columns and shared rows."""
+    lengths = [300, 1, 0, 129]
+    pool, g = pool_with(lengths, 2, 16, dim, cache_type, q_type, dim + group)
+    q = normal(g, len(lengths), 2 * group, dim, dtype=q_type, scale=2)
+    out, lse = KV.attend_token(q, pool.cache, pool.table, lens(lengths))
+    check_token(pool, lengths, q, out, lse, None, 0)
+    weights = torch.zeros((len(lengths), 2, 304), device="cuda")
+    out, lse = KV.attend_token(q, pool.cache, pool.table, lens(lengths), weights=weights)
+    check_token(pool, lengths, q, out, lse, None, 0, gained=weights)
