@@ -184,8 +184,8 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
     constexpr int kKWords = kSq8 ? DP / 16 : DP / 8;  // words of a K row that a lane holds
     constexpr int kVWords = kSq8 ? kPer / 4 : kPer / 2;
     constexpr int kKLoads = kKWords / 4;
-    __shared__ uint32_t sh_place[kWaves][2][kTile];
-    __shared__ float sh_scale[kSq8 ? kWaves : 1][2][kTile];
+    __shared__ __align__(16) uint32_t sh_place[kWaves][2][kTile];  // (read four at a time)
+    __shared__ __align__(16) float sh_scale[kSq8 ? kWaves : 1][2][kTile];
     __shared__ float sh_ml[kWaves][2][16];
     extern __shared__ __align__(16) float sh_out[];  // [waves][heads of the block][DP]
 
