@@ -992,7 +992,8 @@ tessa_status tessa_kv_append(const tessa_kv_cache *cache, const tessa_kv_sequenc
  *   out = sum_j p_j v_j,  p = softmax(scale * q . k_j),  lse = log sum_j exp(scale * q . k_j).
  * A query at row p sees rows j <= p with j < sinks or j > p - window (all with
  * TESSA_KV_ALL).  A query that sees nothing has out 0 and lse -inf; a row whose
- * logit is -inf weighs nothing.
+ * logit is -inf weighs nothing (its values must be finite).  Logits are formed in
+ * base 2: beyond +-2.3e38 they are infinite.
  *   tessa_kv_attend_token: one query for each sequence, at its last row; `tokens`
  *     = batch, no offsets.  listed: rows visible besides the window, listed_count
  *     for each (sequence, head), e.g. a search's results; entries that are

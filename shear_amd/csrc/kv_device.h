@@ -12,9 +12,9 @@ using kv_f16 = float __attribute__((ext_vector_type(16)));
 using kv_u4 = uint32_t __attribute__((ext_vector_type(4)));
 using kv_u2 = uint32_t __attribute__((ext_vector_type(2)));
 
-// A running maximum before any visible row: below every finite logit, and
+// A running maximum before any visible row: above no finite logit, and
 // exp2(-inf - kKvNone) is 0 where exp2(-inf - -inf) would be NaN.
-constexpr float kKvNone = -3.0e38f;
+constexpr float kKvNone = -3.402823466e38f;
 // The running maximum follows a larger logit only when that is more than
 // 2^kKvLag times as large: the weights stay below 2^kKvLag (far from either
 // type's largest value), and almost no tile pays for rescaling the output.

@@ -217,6 +217,10 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
     kv_u4 kr[kSq8 ? kLoads : 1], vr[kSq8 ? kLoads : 1];  // codes on their way to LDS
     float ks = 0.0f, vs = 1.0f;
     bool special = false;  // some value or scale was replaced
+    // some maximum is so large that its rounding is felt (from 2^23 on it would be binades of a
+    // weight): logits are then rounded as it was, before it is taken from them
+    bool huge = false;
+    constexpr float kHuge = 4194304.0f;  // 2^22, rounded to a quarter
 
     // Page ids for a tile (past the end: those of the last row), read a tile before they are used.
     auto read_pages = [&](uint32_t it) {
@@ -445,7 +449,15 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                         if (gone >> (8 * (e / 4) + e % 4) & 1u) x[u][e] = -INFINITY;
                 }
             }
-            const float factor = kSq8 ? 1.0f : p.scale_log2;
+            float factor = kSq8 ? 1.0f : p.scale_log2;
+            auto scale_first = [&] {
+#pragma unroll
+                for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[u][e] *= factor;
+                factor = 1.0f;
+            };
+            if (!kSq8 && huge) scale_first();
             // The running maximum follows the largest logit.
             auto follow = [&] {
                 float top = x[0][0];
@@ -492,6 +504,10 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                     }
                 if (kSq8 || again || !__any(!(sum < kKvMost))) break;
                 follow();
+                if (!huge && __any(fabsf(m) >= kHuge && m > kKvNone)) {
+                    huge = true;
+                    scale_first();
+                }
             }
             l += sum;
             // V^T of dims 32 i + n: rows 16 k + 4 half + {0..3}, + 8; read a block ahead

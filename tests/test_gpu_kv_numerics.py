@@ -210,3 +210,33 @@ def test_token_whole_blocks_of_heads_of_wide_rows(gpu, cache_type, q_type, dim, 
     weights = torch.zeros((len(lengths), 2, 304), device="cuda")
     out, lse = KV.attend_token(q, pool.cache, pool.table, lens(lengths), weights=weights)
     check_token(pool, lengths, q, out, lse, None, 0, gained=weights)
+
+
+@pytest.mark.parametrize("cache_type,q_type,size,sign", [
+    (BF16, BF16, 2.2e38, -1.0), (SQ8, BF16, 2.2e38, -1.0), (BF16, BF16, 2.2e38, 1.0), (BF16, BF16, 3.1e7, 1.0),
+    (F16, F16, 60000.0, -20000.0), (F16, F16, 60000.0, 20000.0), (F16, F16, 50001.0, 99.0), (SQ8, F16, 60000.0, 20000.0)])
+def test_logits_of_any_size(gpu, cache_type, q_type, size, sign):
+    """Rows whose logits are alike weigh as much as each other, to the ends of f32 (2.2e38 is 3.2e38 in base 2)."""
+    n, dim = 130, 64
+    g = np.random.default_rng(5)
+    k = torch.zeros((n, 1, dim), dtype=q_type, device="cuda")
+    k[..., 0] = size
+    q = torch.zeros((n, 2, dim), dtype=q_type, device="cuda")
+    q[..., 0] = sign
+    v = normal(g, n, 1, dim, dtype=q_type)
+    pool = Pool(1, 3, 1, 64, dim, cache_type, 3)
+    pool.fill([n], k, v)
+    values = torch.from_numpy(pool.rows(0, n, 0)[1]).cuda()
+    want = values.cumsum(0) / torch.arange(1, n + 1, device="cuda")[:, None]
+    out, lse = KV.attend_prompt(q, lens([0, n]), pool.cache, pool.table, lens([n]), scale=1.0)
+    logit = float(q[0, 0, 0]) * pool.rows(0, 1, 0)[0][0, 0]
+    # a rounding of the result and one of the weights, which are all alike
+    assert ((out[:, 0].double() - want).abs() <= 2**-8 * want.abs() + (2**-8 + 2**-19) * values.abs().mean() + 1e-6).all()
+    rows = torch.arange(1, n + 1, device="cuda").double()[:, None]
+    assert ((lse.double() - logit - rows.log()).abs() <= 2**-21 * abs(logit)).all()
+    weights = torch.zeros((1, 1, 192), device="cuda")
+    for kw in ({}, {"weights": weights}):
+        out, lse = KV.attend_token(q[:1], pool.cache, pool.table, lens([n]), scale=1.0, **kw)
+        assert ((out[0].double() - want[-1]).abs() <= 2**-8 * want[-1].abs() + 2**-17).all()
+        assert ((lse.double() - logit - math.log(n)).abs() <= 2**-21 * abs(logit)).all()
+    assert torch.allclose(weights[0, 0, :n], torch.full((n,), 2.0 / n, device="cuda"), rtol=2**-20, atol=0)
