@@ -748,6 +748,10 @@ __global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, u
         } else {
             for (uint32_t q = 0; q < p.group; ++q) sum += kv_exp2(y[q] - sh_m[q]) * sh_l[q];
         }
+        if (sum != sum) {  // a query's sum is NaN: its weights are, but that of a logit of -inf is none
+            sum = 0.0f;
+            for (uint32_t q = 0; q < p.group; ++q) sum += y[q] == -INFINITY ? 0.0f : kv_exp2(y[q] - sh_m[q]) * sh_l[q];
+        }
         if (i < vis.before_list)
             weights[row[j]] = old[j] + sum;
         else

@@ -240,3 +240,24 @@ def test_logits_of_any_size(gpu, cache_type, q_type, size, sign):
         assert ((out[0].double() - want[-1]).abs() <= 2**-8 * want[-1].abs() + 2**-17).all()
         assert ((lse.double() - logit - math.log(n)).abs() <= 2**-21 * abs(logit)).all()
     assert torch.allclose(weights[0, 0, :n], torch.full((n,), 2.0 / n, device="cuda"), rtol=2**-20, atol=0)
+
+
+@pytest.mark.parametrize("group", [3, 4])
+def test_weights_of_rows_without_a_page_beside_nan(gpu, group):
+    """A key that is NaN makes the weights NaN, but not those of rows that are not there or not seen."""
+    n = 300
+    pool, g = pool_with([n], 1, 16, 64, BF16, BF16, group)
+    k = normal(g, 1, 1, 64)
+    k[0, 0, 3] = math.nan
+    KV.append(pool.cache, pool.table, lens([150]), k, k)
+    pool.table_host[0, 4:6] = -1
+    pool.table = torch.from_numpy(pool.table_host).cuda()
+    q = normal(g, 1, group, 64)
+    weights = torch.ones((1, 1, 304), device="cuda")
+    out, _ = KV.attend_token(q, pool.cache, pool.table, lens([n]), weights=weights)
+    w = weights[0, 0]
+    assert out.isnan().all() and (w[64:96] == 1).all() and (w[n:] == 1).all()
+    assert w[:64].isnan().all() and w[96:n].isnan().all()
+    weights.fill_(1)
+    KV.attend_token(q, pool.cache, pool.table, lens([n]), window=200, sinks=70, weights=weights)
+    assert (w[64:100] == 1).all() and w[:64].isnan().all() and w[100:n].isnan().all()
