@@ -15,8 +15,9 @@ max|x| * (1/127), symmetric by row like ``tessa.quantize_sq_int8_matrix``).
 * ``evict``          keeps the first, the last and the most attended rows
 
 Every computation happens in libtessa_hip.so, queued on the given or the current
-stream; nothing waits for the device.  Tensors that live on another stream
-than the call's are marked as used there.
+stream; nothing waits for the device.  With ``stream`` the call's tensors are
+marked as used there.  There are no gradients: tensors that require one are
+refused while gradients are recorded.
 """
 from __future__ import annotations
 
@@ -114,6 +115,12 @@ def _check(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device)
         raise ValueError(f"the last dimension of {name} must be contiguous")
 
 
+def _no_gradient(*tensors) -> None:
+    """There are no backward forms: a graph that would end here without a word is refused."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError("the key-value cache has no gradients: detach the tensors or call under torch.no_grad()")
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t itself where its rows lie on 16-byte boundaries, else a copy of it."""
     s = t.stride()
@@ -167,6 +174,7 @@ def append(cache: KvCache, page_table: torch.Tensor, starts: torch.Tensor, k: to
     for each sequence.  ``max_new``: no sequence has more new tokens (default:
     all of them).  Rows past the page table are not written."""
     dev, native = cache.keys.device, cache._native
+    _no_gradient(k, v, *cache._tensors())
     seq = _sequences(cache, page_table, starts, None)
     dtype = cache.keys.dtype
     if dtype == torch.int8:
@@ -196,6 +204,7 @@ def append(cache: KvCache, page_table: torch.Tensor, starts: torch.Tensor, k: to
 def _attend(cache, q, page_table, lengths, max_length, scale, sinks, window, stream, *, listed=None, weights=None,
             offsets=None, max_new=0):
     dev, lib, native = cache.keys.device, N.load(), cache._native
+    _no_gradient(q, weights, *cache._tensors())
     kind = _QUERY_TYPES.get(q.dtype)
     if q.dim() != 3 or kind is None or q.device != dev:
         raise ValueError(f"q must be bf16 or fp16 [tokens, q_heads, head_dim] on {dev}")
@@ -300,6 +309,7 @@ def evict(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tensor, weigh
     move to, its pages not among those read (default: in place; no page may then
     belong to two sequences).  ``weights`` is left as it is."""
     dev = cache.keys.device
+    _no_gradient(weights, *cache._tensors())
     seq = _sequences(cache, page_table, lengths, max_length)
     _check(weights, "weights", torch.float32, (seq.batch, cache.heads, None), dev)
     rows = weights.shape[2]
