@@ -202,7 +202,7 @@ def append(cache: KvCache, page_table: torch.Tensor, starts: torch.Tensor, k: to
 
 
 def _attend(cache, q, page_table, lengths, max_length, scale, sinks, window, stream, *, listed=None, weights=None,
-            offsets=None, max_new=0):
+            offsets=None, max_new=0, prompt=False):
     dev, lib, native = cache.keys.device, N.load(), cache._native
     _no_gradient(q, weights, *cache._tensors())
     kind = _QUERY_TYPES.get(q.dtype)
@@ -216,8 +216,13 @@ def _attend(cache, q, page_table, lengths, max_length, scale, sinks, window, str
     if sinks < 0 or (window is not None and window < 0):
         raise ValueError(f"sinks {sinks} and window {window} must not be negative")
     seq = _sequences(cache, page_table, lengths, max_length)
-    prompt = offsets is not None
-    if not prompt and tokens != seq.batch:
+    if prompt:
+        _offsets(offsets, seq.batch, dev)
+        max_new = tokens if max_new is None else max_new
+        if max_new < 0:
+            raise ValueError(f"max_new {max_new} is negative")
+        max_new = min(max_new, tokens)
+    elif tokens != seq.batch:
         raise ValueError(f"{tokens} queries for {seq.batch} sequences")
     if listed is not None:
         _check(listed, "listed", torch.int32, (seq.batch, cache.heads, None), dev)
@@ -287,15 +292,8 @@ def attend_prompt(q: torch.Tensor, offsets: torch.Tensor, cache: KvCache, page_t
     ``sinks`` and its last ``window``).  Their keys and values are in the cache
     already; ``offsets`` cover all tokens.  ``max_new``: no sequence has more new
     tokens (default: all of them)."""
-    dev = cache.keys.device
-    _offsets(offsets, page_table.shape[0], dev)
-    tokens = q.shape[0]
-    if max_new is None:
-        max_new = tokens
-    if max_new < 0:
-        raise ValueError(f"max_new {max_new} is negative")
     return _attend(cache, q, page_table, lengths, max_length, scale, sinks, window, stream, offsets=offsets,
-                   max_new=min(max_new, tokens))
+                   max_new=max_new, prompt=True)
 
 
 def evict(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tensor, weights: torch.Tensor, keep: int,
