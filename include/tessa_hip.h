@@ -1034,10 +1034,13 @@ tessa_status tessa_kv_attend_prompt(const tessa_kv_cache *cache, const tessa_kv_
  * the largest weights stay (equal weights: the lower row; NaN below everything),
  * in ascending order as rows 0.. of `into` (page ids as in the sequences' table;
  * null: in place).  In place, no page may belong to two sequences; other pages
- * must not be among those read.  new_weights (batch x heads x weight_rows,
+ * must not be among those read.  A row whose page id names no page is not there: it
+ * does not stay, whichever it is, and of a sequence with at most `keep` rows
+ * that are there all of those do.  Rows that move to such a page id are lost and
+ * weigh nothing.  new_weights (batch x heads x weight_rows,
  * contiguous, not the weights themselves) gets the kept rows' weights and zeros
  * after them, kept (batch x heads x keep) the kept rows and -1 after them,
- * new_lengths min(length, keep). */
+ * new_lengths how many they are. */
 typedef struct tessa_kv_eviction {
     const float *weights;
     uint64_t weight_strides[2];  /* floats: sequence, head */

@@ -3,7 +3,9 @@
 // Of the n rows of a (sequence, head) with n > keep, the first `sinks` and the
 // last `recent` stay, and of the others the keep - sinks - recent with the
 // largest weights, equal weights by the lower row, NaN below everything.  The
-// kept rows, in ascending order, become rows 0.. of the destination pages.
+// kept rows, in ascending order, become rows 0.. of the destination pages.  A row
+// whose page id names no page is not there: it is never kept, so that no row of the
+// destination is counted without having been written.
 //
 // kv_select_kernel: one workgroup per (sequence, head).  The weights, as
 // integers of the same order, go through three histograms in LDS (11, 11 and 10
@@ -58,25 +60,38 @@ __device__ __forceinline__ float weight_of(uint32_t u) {
     return __uint_as_float(u == 0u ? 0x7fc00000u : u >> 31 ? u ^ 0x80000000u : ~u);
 }
 
-// The middle rows [sinks, n - recent) by weight: places sinks.. of `kept` and `out`.
+// The `need` candidates of the largest weights, fewer than there are: places `place`.. of `kept`
+// and `out`.  Candidates are the middle rows [sinks, n - recent); with kHoles (a page is
+// missing) all rows, of which the first and the last are above every weight and
+// those that are not there below NaN.
 // Lanes past a wave's last candidate hold the lowest value.  They can at most
 // add to the lowest bin and to the ties of the lowest value, after every real
 // candidate of theirs, where no row is left to place.
-template <bool kHeld>
-__device__ __forceinline__ void select_rows(const KvEvictParams &p, const float *w, uint32_t n, int32_t *kept, float *out,
-                                            uint32_t *held, uint32_t *hist, uint32_t (*sh_wave)[kSelWaves], uint32_t *sh_pick) {
+template <bool kHeld, bool kHoles>
+__device__ __forceinline__ void select_rows(const KvEvictParams &p, const float *w, const int32_t *table, uint32_t n, uint32_t need,
+                                            uint32_t place, int32_t *kept, float *out, uint32_t *held, uint32_t *hist,
+                                            uint32_t (*sh_wave)[kSelWaves], uint32_t *sh_pick) {
     const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6;
-    const uint32_t candidates = n - p.sinks - p.recent;
-    const uint32_t need = p.keep - p.sinks - p.recent;
+    const uint32_t skipped = kHoles ? 0u : p.sinks;
+    const uint32_t candidates = kHoles ? n : n - p.sinks - p.recent;
     if (need == 0) return;
     // contiguous rows of a wave, whole groups of 64
     const uint32_t span = ((candidates + kSelWaves - 1) / kSelWaves + 63u) / 64u * 64u;
     const uint32_t lo = wave * span, hi = min(lo + span, candidates);
     const uint32_t steps = __builtin_amdgcn_readfirstlane(lo < hi ? (hi - lo + 63u) / 64u : 0u);
     // (loads without a branch, so that a group of them is out at once)
-    const float *middle = w + p.sinks;
+    const float *middle = w + skipped;
     auto load = [&](uint32_t s) { return __float_as_uint(middle[min(lo + s * 64u + lane, candidates - 1u)]); };
-    auto order = [&](uint32_t s, uint32_t x) { return lo + s * 64u + lane < hi ? order_of(__uint_as_float(x)) : 0u; };
+    auto order = [&](uint32_t s, uint32_t x) {
+        const uint32_t i = lo + s * 64u + lane;
+        if (i >= hi) return 0u;
+        const uint32_t u = order_of(__uint_as_float(x));
+        if constexpr (kHoles) {
+            if ((uint32_t)table[i >> p.c.page_shift] >= p.c.pages) return 0u;
+            return i < p.sinks || i >= n - p.recent ? 0xffffffffu : max(u, 1u);
+        }
+        return u;
+    };
     // f(step, value) for each of the lane's candidates.  The loops stay loops: unrolled
     // over the 32 steps of 32,768 candidates, each instruction runs once a wave and fetching them takes
     // longer than the work.
@@ -154,7 +169,7 @@ __device__ __forceinline__ void select_rows(const KvEvictParams &p, const float 
     }
     __syncthreads();
     const uint32_t equal_before = before_wave(sh_wave[1], wave);
-    uint32_t place = p.sinks + before_wave(sh_wave[0], wave) + min(equal_before, left);
+    place += before_wave(sh_wave[0], wave) + min(equal_before, left);
     uint32_t room = left > equal_before ? left - equal_before : 0u;  // ties of this wave that stay
     each(again, [&](uint32_t s, uint32_t x) {
         const uint32_t u = known(s, x);
@@ -171,8 +186,8 @@ __device__ __forceinline__ void select_rows(const KvEvictParams &p, const float 
         if (keep >> lane & 1u) {
             const uint32_t at = place + __builtin_amdgcn_mbcnt_hi((uint32_t)(keep >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)keep, 0u));
             const uint32_t i = lo + s * 64u + lane;
-            kept[at] = (int32_t)(p.sinks + i);
-            out[at] = weight_of(u);
+            kept[at] = (int32_t)(skipped + i);
+            out[at] = kHoles ? w[i] : weight_of(u);
         }
         place += (uint32_t)__popcll(keep);
     });
@@ -237,23 +252,39 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(KvEvictParams p,
     __shared__ uint32_t hist[kBins];
     __shared__ uint32_t sh_wave[2][kSelWaves];
     __shared__ uint32_t sh_pick[2];
+    __shared__ uint32_t sh_missing;
     const uint32_t h = blockIdx.x, b = blockIdx.y, t = threadIdx.x;
     const uint32_t n = kv_length(p.c, b);
     const uint64_t bh = (uint64_t)b * p.c.heads + h;
     const float *w = p.weights + (uint64_t)b * p.weight_batch + (uint64_t)h * p.weight_head;
     int32_t *kept = p.kept + bh * p.keep;
     float *out = p.new_weights + bh * p.weight_rows;
-    const uint32_t count = min(n, p.keep);
-    if (n > p.keep) {
+    // rows whose page is none
+    const int32_t *table = p.c.table + (uint64_t)b * p.c.table_stride;
+    const uint32_t table_pages = n ? ((n - 1u) >> p.c.page_shift) + 1u : 0u, page_rows = 1u << p.c.page_shift;
+    uint32_t missing = 0;
+    for (uint32_t i = t; i < table_pages; i += kSelThreads)
+        if ((uint32_t)table[i] >= p.c.pages) missing += min(page_rows, n - i * page_rows);
+    const bool holes = __syncthreads_or(missing != 0);
+    uint32_t count = min(n, p.keep);
+    if (holes) {
+        if (t == 0) sh_missing = 0u;
+        __syncthreads();
+        if (missing) atomicAdd(&sh_missing, missing);
+        __syncthreads();
+        count = min(n - sh_missing, p.keep);
+        select_rows<false, true>(p, w, table, n, count, 0u, kept, out, sh_held, hist, sh_wave, sh_pick);
+    } else if (n > p.keep) {
+        const uint32_t need = p.keep - p.sinks - p.recent;
         if (n - p.sinks - p.recent <= kSelHeld)
-            select_rows<true>(p, w, n, kept, out, sh_held, hist, sh_wave, sh_pick);
+            select_rows<true, false>(p, w, table, n, need, p.sinks, kept, out, sh_held, hist, sh_wave, sh_pick);
         else
-            select_rows<false>(p, w, n, kept, out, sh_held, hist, sh_wave, sh_pick);
+            select_rows<false, false>(p, w, table, n, need, p.sinks, kept, out, sh_held, hist, sh_wave, sh_pick);
     }
     // the rows that stay without being asked, and what follows the kept ones (after the
     // selection, whose loads would wait for these stores)
     if (h == 0 && t == 0) p.new_lengths[b] = (int32_t)count;
-    const uint32_t first = n > p.keep ? p.sinks : n, last = n > p.keep ? p.recent : 0u;
+    const uint32_t first = holes ? 0u : n > p.keep ? p.sinks : n, last = holes || n <= p.keep ? 0u : p.recent;
     for (uint32_t i = t; i < first + last; i += kSelThreads) {
         const uint32_t from = i < first ? i : n - last + (i - first), to = i < first ? i : count - last + (i - first);
         kept[to] = (int32_t)from;
@@ -263,7 +294,7 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(KvEvictParams p,
     for (uint32_t i = count + t; i < p.weight_rows; i += kSelThreads) out[i] = 0.0f;
     if (move) {  // few rows: here, without another launch
         const bool in_place = p.into == p.c.table;
-        if (in_place && n <= p.keep) return;
+        if (in_place && count == n) return;
         __syncthreads();  // the kept rows are listed
         move_rows<kSelThreads>(p, p.c.keys, b, h, 0, count, row_units, 0, row_units, lanes_log2, in_place);
         move_rows<kSelThreads>(p, p.c.values, b, h, 0, count, row_units, 0, row_units, lanes_log2, in_place);
@@ -274,9 +305,9 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(KvEvictParams p,
 __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(KvEvictParams p, uint32_t row_units, uint32_t columns, uint32_t units,
                                                                uint32_t lanes_log2, uint32_t span, bool in_place) {
     const uint32_t h = blockIdx.y / (2 * columns), rest = blockIdx.y - h * 2 * columns, b = blockIdx.z;
-    const uint32_t n = kv_length(p.c, b), count = min(n, p.keep);
+    const uint32_t n = kv_length(p.c, b), count = (uint32_t)p.new_lengths[b];
     const uint32_t first = blockIdx.x * span, last = min(first + span, count);
-    if (first >= last || (in_place && n <= p.keep)) return;
+    if (first >= last || (in_place && count == n)) return;
     move_rows<kMoveThreads>(p, (rest & 1u) ? p.c.values : p.c.keys, b, h, first, last, row_units, (rest >> 1) * units, units, lanes_log2,
                             in_place);
 }

@@ -305,7 +305,8 @@ def evict(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tensor, weigh
     ascending order; ``kept`` names the rows they were (-1 past the new length), the
     new weights are theirs and zeros after them.  ``into``: the page table that they
     move to, its pages not among those read (default: in place; no page may then
-    belong to two sequences).  ``weights`` is left as it is."""
+    belong to two sequences).  Rows whose page id names no page do not stay, and
+    rows that move to such an id are lost.  ``weights`` is left as it is."""
     dev = cache.keys.device
     _no_gradient(weights, *cache._tensors())
     seq = _sequences(cache, page_table, lengths, max_length)
