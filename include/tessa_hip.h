@@ -1040,7 +1040,7 @@ tessa_status tessa_kv_attend_prompt(const tessa_kv_cache *cache, const tessa_kv_
  * weigh nothing.  new_weights (batch x heads x weight_rows,
  * contiguous, not the weights themselves) gets the kept rows' weights and zeros
  * after them, kept (batch x heads x keep) the kept rows and -1 after them,
- * new_lengths how many they are. */
+ * new_lengths how many they are (not the lengths themselves, which every head reads). */
 typedef struct tessa_kv_eviction {
     const float *weights;
     uint64_t weight_strides[2];  /* floats: sequence, head */

@@ -349,6 +349,7 @@ tessa_status tessa_kv_evict(const tessa_kv_cache *cache, const tessa_kv_sequence
         if (!seq->batch) return fine();
         if (!e->weights || !e->new_weights || !e->kept || !e->new_lengths) KV_INVALID("kv evict: null pointer");
         if (e->weights == e->new_weights) KV_INVALID("kv evict: new_weights are the weights");
+        if (e->new_lengths == seq->lengths) KV_INVALID("kv evict: new_lengths are the lengths");
         if (e->weight_rows < e->keep) KV_INVALID("kv evict: %u weight rows below keep %u", e->weight_rows, e->keep);
         if (e->into) {
             if (seq->batch > 1 && e->into_stride < e->into_columns)
