@@ -59,7 +59,11 @@ def distinct(rows: torch.Tensor) -> torch.Tensor:
 
 @dataclass
 class LongContext:
-    """Conversations over one layer's cache: ``heads`` key heads shared by the query heads."""
+    """Conversations over one layer's cache: ``heads`` key heads shared by the query heads.
+
+    ``lengths`` is kept by the methods, as are the rows' counts on the
+    host; a call that would pass ``max_rows`` is refused and changes nothing.  ``weights`` gathers what
+    single tokens attend to (a prompt's own attention is not in it)."""
 
     batch: int
     heads: int
@@ -72,8 +76,10 @@ class LongContext:
     found: int = 64                     # rows that each query head's search adds
     list_size: int = 128                # of the search
     indexes: list = field(init=False, default_factory=list)
+    _rows: list = field(init=False, repr=False)     # of each sequence
 
     def __post_init__(self):
+        self._rows = [0] * self.batch
         columns = -(-self.max_rows // self.page_rows)
         pages = self.batch * columns
         self.cache = KV.KvCache.allocate(pages, self.heads, self.page_rows, self.head_dim, self.dtype)
@@ -81,17 +87,30 @@ class LongContext:
         self.lengths = torch.zeros(self.batch, dtype=torch.int32, device="cuda")
         self.weights = torch.zeros((self.batch, self.heads, columns * self.page_rows), device="cuda")
 
+    def _grown(self, new: list[int]) -> list[int]:
+        """Rows of each sequence with ``new`` more."""
+        if len(new) != self.batch or min(new, default=0) < 0:
+            raise ValueError(f"new rows {new} for {self.batch} sequences")
+        rows = [n + more for n, more in zip(self._rows, new)]
+        if max(rows, default=0) > self.max_rows:
+            raise ValueError(f"{max(rows)} rows of a sequence, room for {self.max_rows}")
+        return rows
+
     def prompt(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, new: list[int]) -> torch.Tensor:
         """Appends ``new[b]`` tokens of each sequence and returns their causal attention over all rows."""
+        rows = self._grown(new)
+        if sum(new) != k.shape[0]:
+            raise ValueError(f"{k.shape[0]} tokens, {sum(new)} new rows")
         offsets = torch.tensor([sum(new[:b]) for b in range(len(new) + 1)], dtype=torch.int32, device="cuda")
         KV.append(self.cache, self.table, self.lengths, k, v, offsets=offsets, max_new=max(new))
         self.lengths = self.lengths + (offsets[1:] - offsets[:-1])
+        self._rows = rows
         return KV.attend_prompt(q, offsets, self.cache, self.table, self.lengths, max_new=max(new))[0]
 
     def build(self) -> None:
         """Graphs over the rows that are cached now."""
         self.indexes = []
-        for b, n in enumerate(self.lengths.tolist()):
+        for b, n in enumerate(self._rows):
             rows = torch.arange(n, device="cuda")
             pages, slots = self.table[b, rows // self.page_rows].long(), rows % self.page_rows
             keys = self.cache.keys[pages, :, slots].float()
@@ -111,8 +130,10 @@ class LongContext:
     def token(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
         """Appends one token to each sequence and returns its attention over the first, the last and the
         found rows (over all rows while there are no graphs)."""
+        rows = self._grown([1] * self.batch)
         KV.append(self.cache, self.table, self.lengths, k, v)
         self.lengths = self.lengths + 1
+        self._rows = rows
         listed = self.find(q)
         return KV.attend_token(q, self.cache, self.table, self.lengths, sinks=self.sinks,
                                window=None if listed is None else self.window, listed=listed, weights=self.weights)[0]
@@ -122,6 +143,7 @@ class LongContext:
         graphs' rows are gone, so attention is over all that is left until ``build`` is called."""
         kept, self.lengths, self.weights = KV.evict(self.cache, self.table, self.lengths, self.weights, keep,
                                                     sinks=self.sinks, recent=min(self.window, keep - self.sinks))
+        self._rows = [min(n, keep) for n in self._rows]
         self.indexes = []
         return kept
 
