@@ -61,7 +61,8 @@ def distinct(rows: torch.Tensor) -> torch.Tensor:
 class LongContext:
     """Conversations over one layer's cache: ``heads`` key heads shared by the query heads.
 
-    ``lengths`` is kept by the methods, as are the rows' counts on the
+    The graphs cover the rows that were cached when ``build`` was called; rows added since stay
+    visible until it is called again.  ``lengths`` is kept by the methods, as are the rows' counts on the
     host; a call that would pass ``max_rows`` is refused and changes nothing.  ``weights`` gathers what
     single tokens attend to (a prompt's own attention is not in it)."""
 
@@ -77,9 +78,11 @@ class LongContext:
     list_size: int = 128                # of the search
     indexes: list = field(init=False, default_factory=list)
     _rows: list = field(init=False, repr=False)     # of each sequence
+    _indexed: list = field(init=False, repr=False)  # of them, in the graphs
 
     def __post_init__(self):
         self._rows = [0] * self.batch
+        self._indexed = [0] * self.batch
         columns = -(-self.max_rows // self.page_rows)
         pages = self.batch * columns
         self.cache = KV.KvCache.allocate(pages, self.heads, self.page_rows, self.head_dim, self.dtype)
@@ -96,6 +99,13 @@ class LongContext:
             raise ValueError(f"{max(rows)} rows of a sequence, room for {self.max_rows}")
         return rows
 
+    def shown(self) -> int | None:
+        """Last rows that a token sees besides the first and the found ones: ``window``, and all
+        that are in no graph yet.  None: there are no graphs, every row is visible."""
+        if not self.indexes:
+            return None
+        return max(self.window, *(n - indexed for n, indexed in zip(self._rows, self._indexed)))
+
     def prompt(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, new: list[int]) -> torch.Tensor:
         """Appends ``new[b]`` tokens of each sequence and returns their causal attention over all rows."""
         rows = self._grown(new)
@@ -110,6 +120,7 @@ class LongContext:
     def build(self) -> None:
         """Graphs over the rows that are cached now."""
         self.indexes = []
+        self._indexed = list(self._rows)
         for b, n in enumerate(self._rows):
             rows = torch.arange(n, device="cuda")
             pages, slots = self.table[b, rows // self.page_rows].long(), rows % self.page_rows
@@ -128,15 +139,15 @@ class LongContext:
         return distinct(torch.stack([torch.stack(r) for r in rows]))
 
     def token(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
-        """Appends one token to each sequence and returns its attention over the first, the last and the
-        found rows (over all rows while there are no graphs)."""
+        """Appends one token to each sequence and returns its attention over the first, the last (``shown``)
+        and the found rows (over all rows while there are no graphs)."""
         rows = self._grown([1] * self.batch)
         KV.append(self.cache, self.table, self.lengths, k, v)
         self.lengths = self.lengths + 1
         self._rows = rows
         listed = self.find(q)
         return KV.attend_token(q, self.cache, self.table, self.lengths, sinks=self.sinks,
-                               window=None if listed is None else self.window, listed=listed, weights=self.weights)[0]
+                               window=self.shown(), listed=listed, weights=self.weights)[0]
 
     def evict(self, keep: int) -> torch.Tensor:
         """Keeps the first, the last and the most attended rows, ``keep`` of each head, in place; the
@@ -176,7 +187,7 @@ def run(rows: int = 6000, batch: int = 2, heads: int = 2, group: int = 4, dim: i
         q = queries(batch)
         out = c.token(q, normal(batch, heads, dim).bfloat16(), normal(batch, heads, dim).bfloat16())
         full, lse = KV.attend_token(q, c.cache, c.table, c.lengths)
-        _, seen = KV.attend_token(q, c.cache, c.table, c.lengths, sinks=c.sinks, window=c.window, listed=c.find(q))
+        _, seen = KV.attend_token(q, c.cache, c.table, c.lengths, sinks=c.sinks, window=c.shown(), listed=c.find(q))
         carried += float(torch.exp(seen - lse).mean()) / tokens
         error += float((out.float() - full.float()).norm() / full.float().norm()) / tokens
     kept = c.evict(keep)

@@ -1,4 +1,4 @@
-"""A long context at the end of its room."""
+"""A long context after its graphs were built, and at the end of its room."""
 import pytest
 import torch
 
@@ -37,7 +37,7 @@ class Conversation:
         self.keep(k, v, new)
 
     def token(self):
-        """One step, checked against the attention over all rows."""
+        """One step, checked against the attention over the first, the last, the found and the new rows."""
         c = self.c
         q, k, v = self.normal(self.batch, 4), self.normal(self.batch, 2), self.normal(self.batch, 2)
         before = c.weights.clone()
@@ -48,6 +48,11 @@ class Conversation:
             assert int(c.lengths[b]) == n
             for h in range(2):
                 rows = torch.arange(n, device="cuda")
+                if c.indexes:
+                    found = c.indexes[b][h].search(q[b, 2 * h: 2 * h + 2], c.found, c.list_size).flatten().long()
+                    since = n - c.shown()
+                    assert since <= self.built[b]
+                    rows = torch.cat([found[found >= 0], rows[: c.sinks], rows[since:]]).unique()
                 p = torch.softmax(q[b, 2 * h: 2 * h + 2].double() @ self.k[b][rows, h].t() / 8, -1)
                 want = p @ self.v[b][rows, h]
                 # one rounding of the result and f32 arithmetic
@@ -55,6 +60,34 @@ class Conversation:
                 grown = (c.weights[b, h] != before[b, h]).nonzero().squeeze(-1)
                 assert set(grown.tolist()) <= set(rows.tolist()) and n - 1 in grown
         return out
+
+    def build(self):
+        self.c.build()
+        self.built = [x.shape[0] for x in self.k]
+
+
+def test_a_second_prompt_is_seen(gpu):
+    t = Conversation(1, batch=2, max_rows=1500, sinks=3, window=50, found=20, list_size=40)
+    t.prompt([700, 640])
+    t.build()
+    t.token()
+    t.prompt([300, 10])  # far more than the window
+    weights = t.c.weights.clone()
+    t.token()
+    gained = t.c.weights - weights
+    assert (gained[0, :, 700:1002] > 0).all()  # every row that is in no graph
+    t.build()
+    t.token()
+
+
+def test_more_tokens_than_the_window(gpu):
+    t = Conversation(2, max_rows=800, sinks=2, window=8, found=10, list_size=20)
+    t.prompt([600])
+    t.build()
+    for _ in range(20):
+        t.token()
+    t.build()
+    t.token()
 
 
 @pytest.mark.parametrize("page_rows", [64, 16])
