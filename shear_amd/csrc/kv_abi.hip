@@ -182,6 +182,7 @@ tessa_status attend_of(const tessa_kv_cache *cache, const tessa_kv_sequences *se
     const uint64_t dp = kv_padded_dim(p.c.dim);
     if (!prompt && a->tokens != p.c.batch)
         KV_INVALID("kv attend: %llu tokens for %u sequences", (unsigned long long)a->tokens, p.c.batch);
+    if (a->tokens && !p.c.batch) KV_INVALID("kv attend: %llu tokens of no sequence", (unsigned long long)a->tokens);
     p.chunks = 1;
     if (!a->tokens || !p.c.batch) return fine();
     if (prompt) {
