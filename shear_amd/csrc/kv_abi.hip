@@ -262,7 +262,7 @@ tessa_status attend(const tessa_kv_cache *cache, const tessa_kv_sequences *seq, 
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const bool sq8 = cache->type == TESSA_KV_SQ8;
     int rc = prompt ? launch_kv_prompt(p, a->type, sq8, s) : launch_kv_token(p, a->type, sq8, s);
-    if (rc == 0 && o) rc = launch_kv_finish(p, a->type, prompt, s);
+    if (rc == 0 && o) rc = launch_kv_finish(p, a->type, sq8, prompt, s);
     if (rc) return status(TESSA_ERR_HIP, "kv attend: launch failed");
     return fine();
 }

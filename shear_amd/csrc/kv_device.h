@@ -15,16 +15,13 @@ using kv_u2 = uint32_t __attribute__((ext_vector_type(2)));
 // A running maximum before any visible row: above no finite logit, and
 // exp2(-inf - kKvNone) is 0 where exp2(-inf - -inf) would be NaN.
 constexpr float kKvNone = -3.402823466e38f;
-// The running maximum follows a larger logit only when that is more than
-// 2^kKvLag times as large: the weights stay below 2^kKvLag (far from either
-// type's largest value), and almost no tile pays for rescaling the output.
-constexpr float kKvLag = 8.0f;
-// The same for SQ8 rows, whose weights are multiplied by the values' scales: these are at
-// most 2^121.1 (the largest bf16 number over 127), so the products stay finite.
-constexpr float kKvLagScaled = 6.0f;
-// A tile's weights, formed with a maximum that may be too small, serve while their sum is
-// below this: each then is a finite number of either type.
-constexpr float kKvMost = 32768.0f;
+// Weights are exp2(logit - m) with m near the running maximum, which m follows only now and
+// then, so that almost no tile pays for rescaling the output: it is set 2^kv_lift below
+// the largest weight and stays until one (prompts of 16-bit rows: a tile's sum of them) passes
+// 2^kv_top.  bf16 has f32's range and weights of at most 1 keep the sums of the largest
+// values finite; fp16 has its range above 1 as well as below it, and uses all of it.
+constexpr float kv_lift(bool half, bool prompt) { return half ? (prompt ? 9.0f : 7.0f) : (prompt ? -15.0f : -8.0f); }
+constexpr float kv_top(bool half) { return half ? 15.0f : 0.0f; }
 
 template <typename T>
 struct KvElem;
@@ -76,6 +73,11 @@ struct KvElem<_Float16> {
 __device__ __forceinline__ float kv_code(uint32_t x, int e) { return (float)(int8_t)(x >> (8 * e)); }
 
 __device__ __forceinline__ float kv_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// log of the sum of exp from m and the sum of weights, which is near 2^lift: two numbers of the result's size are added
+__device__ __forceinline__ float kv_lse(float m, float sum, float lift) {
+    return sum == 0.0f ? -INFINITY : ((m + lift) + log2f(sum * kv_exp2(-lift))) * 0.69314718056f;
+}
 
 // max / sum of x over the lanes that differ in bit 5, in bits 4 and 5
 __device__ __forceinline__ float kv_max32(float x) {

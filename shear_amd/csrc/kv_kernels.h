@@ -46,6 +46,7 @@ struct KvAttendParams {
     uint64_t q_token, q_head, out_token, out_head;  // bytes
     uint32_t q_heads, group;   // group: query heads of a key head
     float scale_log2;          // scale * log2(e)
+    float lift;                // of the partial sums: kv_lift()
     uint32_t sinks, window;    // window 0xffffffff: none
     const int32_t *listed;     // batch x heads x listed_count, or null
     uint32_t listed_count;
@@ -88,7 +89,7 @@ int kv_compute_units();
 int launch_kv_append(const KvAppendParams &p, uint32_t source, bool sq8, hipStream_t stream);
 void kv_token_split(KvAttendParams &p);
 int launch_kv_token(const KvAttendParams &p, uint32_t type, bool sq8, hipStream_t stream);
-int launch_kv_finish(const KvAttendParams &p, uint32_t type, bool prompt, hipStream_t stream);
+int launch_kv_finish(const KvAttendParams &params, uint32_t type, bool sq8, bool prompt, hipStream_t stream);
 void kv_prompt_split(KvAttendParams &p);
 int launch_kv_prompt(const KvAttendParams &p, uint32_t type, bool sq8, hipStream_t stream);
 int launch_kv_evict(const KvEvictParams &p, uint32_t type, hipStream_t stream);

@@ -21,8 +21,8 @@
 //    half, so the running maximum and sum cost one exchange a tile.
 //  * O^T = V^T P^T: the logits' registers are the P^T operand as they
 //    stand; V^T comes from LDS by transposing reads of 4 rows x 16 values.
-//  * The maximum follows only where a tile's weights would sum to 2^15 (SQ8: a weight
-//    would be 2^6), and tiles that every query of the workgroup sees in full
+//  * The maximum follows only where a tile's weights would sum to 2^15 times the largest that it
+//    was set for, or more (SQ8: a weight would be that), and tiles that every query of the workgroup sees in full
 //    carry no mask.
 //  * P is rounded to the queries' type once (an error of the size of the
 //    result's own rounding); sums are in f32.  fp16 has nothing between 0 and 2^-24: there
@@ -121,8 +121,9 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
     using E = KvElem<T>;
     using P = KvElem<std::conditional_t<kSq8, __bf16, T>>;  // of the weights and the values
     constexpr bool kTwoParts = kSq8 && !std::is_same_v<T, __bf16>;
-    // what the largest weight is brought to, as a power of two: 32 rows' of it stay below kKvMost
-    constexpr float kLift = !kSq8 && std::is_same_v<T, _Float16> ? 9.0f : 0.0f;
+    constexpr bool kHalf = !kSq8 && std::is_same_v<T, _Float16>;  // fp16 weights
+    // (32 alike rows at the lift sum to 2^5 times it, below the top)
+    constexpr float kLift = kv_lift(kHalf, true), kTop = kv_top(kHalf), kMost = kHalf ? 32768.0f : 1.0f;  // kMost = 2^kTop
     using Lds = PromptLds<kSq8, DP>;
     constexpr uint32_t kRows = Lds::kRows;
     constexpr int kSubs = (int)kRows / 32;       // 32 rows of logits each
@@ -480,7 +481,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                 for (int u = 0; u < kSubs; ++u)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) top = fmaxf(top, x[u][e]);
-                if (__any(kv_max32(top) > m + kKvLagScaled)) follow();
+                if (__any(kv_max32(top) > m + kTop)) follow();
             }
             // 16-bit rows: the weights are formed with the old maximum, and their sum tells
             // whether it still served (it does but for a sequence's first tiles): a search for
@@ -502,7 +503,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                         pf[2 * u + e / 8][(e % 8) / 2] = both;
                         if constexpr (kTwoParts) rest[2 * u + e / 8][(e % 8) / 2] = P::pack(w0 - P::low(both), w1 - P::high(both));
                     }
-                if (kSq8 || again || !__any(!(sum < kKvMost))) break;
+                if (kSq8 || again || !__any(!(sum < kMost))) break;
                 follow();
                 if (!huge && __any(fabsf(m) >= kHuge && m > kKvNone)) {
                     huge = true;
@@ -648,7 +649,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                 *reinterpret_cast<kv_u2 *>(o + 2u * d) = y;
             }
         }
-    if (half == 0) p.lse[query] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
+    if (half == 0) p.lse[query] = kv_lse(m, l, kLift);
 }
 
 template <typename T, bool kSq8, int DP, bool kWhole>

@@ -178,7 +178,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
     using E = KvElem<T>;
     using P = KvElem<std::conditional_t<kSq8, __bf16, T>>;  // of the weights and the values
     constexpr bool kHalf = !kSq8 && std::is_same_v<T, _Float16>;  // fp16 weights
-    constexpr float kLag = kSq8 ? kKvLagScaled : kKvLag, kLift = kHalf ? 7.0f : 0.0f, kRest = kHalf ? 4096.0f : 1.0f;
+    constexpr float kLift = kv_lift(kHalf, false), kTop = kv_top(kHalf), kRest = kHalf ? 4096.0f : 1.0f;
     constexpr int kSteps = DP / 32;                 // matrix instructions of 16 logits
     constexpr int kPer = DP / 16;                   // values of a row that a lane holds
     constexpr int kKWords = kSq8 ? DP / 16 : DP / 8;  // words of a K row that a lane holds
@@ -411,7 +411,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, x[t][i]);
         top = kv_max16(top);
-        if (__any(top > m + (kLag + kLift))) {
+        if (__any(top > m + kTop)) {
             const float higher = fmaxf(m, top - kLift);
             const float f = kv_exp2(m - higher);
             m = higher;
@@ -523,7 +523,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
                 *reinterpret_cast<kv_u2 *>(p.out + (uint64_t)b * p.out_token + (uint64_t)(h * p.group + first_q + head) * p.out_head +
                                            2u * d) = y;
             }
-            if (d == 0) p.lse[q0 + head] = sum == 0.0f ? -INFINITY : (big + log2f(sum)) * 0.69314718056f;
+            if (d == 0) p.lse[q0 + head] = kv_lse(big, sum, kLift);
         }
     }
     if constexpr (kDirect) break;
@@ -641,7 +641,7 @@ __global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, u
             else
                 *reinterpret_cast<uint16_t *>(to) = (uint16_t)E::pack(o[0] * r, 0.0f);
         }
-        if (lane == 0) p.lse[query] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
+        if (lane == 0) p.lse[query] = kv_lse(m, l, p.lift);
         return;
     }
     if (blockIdx.x < joins) {
@@ -690,7 +690,7 @@ __global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, u
             const kv_u2 y = {E::pack(o[0] * r, o[1] * r), E::pack(o[2] * r, o[3] * r)};
             *reinterpret_cast<kv_u2 *>(p.out + (uint64_t)token * p.out_token + (uint64_t)head * p.out_head + 2u * d) = y;
         }
-        if (t == 0 && slice == 0) p.lse[query] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
+        if (t == 0 && slice == 0) p.lse[query] = kv_lse(m, l, p.lift);
         return;
     }
     // weights of kWeightRows visible rows of one (sequence, head)
@@ -810,7 +810,9 @@ int launch_kv_token(const KvAttendParams &p, uint32_t type, bool sq8, hipStream_
     return sq8 ? launch_dim<_Float16, true>(p, stream) : launch_dim<_Float16, false>(p, stream);
 }
 
-int launch_kv_finish(const KvAttendParams &p, uint32_t type, bool prompt, hipStream_t stream) {
+int launch_kv_finish(const KvAttendParams &params, uint32_t type, bool sq8, bool prompt, hipStream_t stream) {
+    KvAttendParams p = params;
+    p.lift = kv_lift(!sq8 && type == kKvF16, prompt);
     const uint64_t queries = p.tokens * p.q_heads;
     const uint32_t dp = kv_padded_dim(p.c.dim);
     uint32_t dims = dp;

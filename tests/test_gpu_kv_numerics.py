@@ -261,3 +261,25 @@ def test_weights_of_rows_without_a_page_beside_nan(gpu, group):
     weights.fill_(1)
     KV.attend_token(q, pool.cache, pool.table, lens([n]), window=200, sinks=70, weights=weights)
     assert (w[64:100] == 1).all() and w[:64].isnan().all() and w[100:n].isnan().all()
+
+
+@pytest.mark.parametrize("cache_type", [BF16, SQ8])
+@pytest.mark.parametrize("size", [3e38, 1e-22])
+@pytest.mark.parametrize("how", ["level", "grow", "same"])
+def test_values_near_the_ends_of_bf16(gpu, cache_type, size, how):
+    """Values as large as bf16 has them stay finite sums while the maximum of the logits moves; small ones keep their bits."""
+    n, dim = 640, 64
+    g = np.random.default_rng(7)
+    q, k = normal(g, n, 2, dim), normal(g, n, 1, dim)
+    if how == "grow":
+        k = (k.float() * torch.linspace(0, 12, n, device="cuda")[:, None, None]).bfloat16()
+    v = (torch.from_numpy(g.uniform(0.5, 1.0, (n, 1, dim)).astype(np.float32)).cuda() * size).bfloat16()
+    if how != "same":
+        v = v * torch.from_numpy(g.choice([-1.0, 1.0], (n, 1, dim))).cuda().bfloat16()
+    pool = Pool(1, 10, 1, 64, dim, cache_type, 3)
+    pool.fill([n], k, v)
+    out, lse = prompt(pool, [n], [n], q)
+    check_prompt(pool, [n], [n], q, out, lse, None, 0)
+    for kw in ({}, {"weights": torch.zeros((1, 1, n), device="cuda")}):
+        out, lse = KV.attend_token(q[-1:].contiguous(), pool.cache, pool.table, lens([n]), **kw)
+        check_token(pool, [n], q[-1:], out, lse, None, 0)
