@@ -115,10 +115,12 @@ def _check(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device)
         raise ValueError(f"the last dimension of {name} must be contiguous")
 
 
-def _no_gradient(*tensors) -> None:
+def _no_gradient(cache: KvCache, a: torch.Tensor, b: torch.Tensor | None = None) -> None:
     """There are no backward forms: a graph that would end here without a word is refused."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError("the key-value cache has no gradients: detach the tensors or call under torch.no_grad()")
+    if (a.requires_grad or (b is not None and b.requires_grad) or cache.keys.requires_grad or cache.values.requires_grad
+            or (cache.key_scales is not None and (cache.key_scales.requires_grad or cache.value_scales.requires_grad))):
+        if torch.is_grad_enabled():
+            raise ValueError("the key-value cache has no gradients: detach the tensors or call under torch.no_grad()")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -174,7 +176,7 @@ def append(cache: KvCache, page_table: torch.Tensor, starts: torch.Tensor, k: to
     for each sequence.  ``max_new``: no sequence has more new tokens (default:
     all of them).  Rows past the page table are not written."""
     dev, native = cache.keys.device, cache._native
-    _no_gradient(k, v, *cache._tensors())
+    _no_gradient(cache, k, v)
     seq = _sequences(cache, page_table, starts, None)
     dtype = cache.keys.dtype
     if dtype == torch.int8:
@@ -204,7 +206,7 @@ def append(cache: KvCache, page_table: torch.Tensor, starts: torch.Tensor, k: to
 def _attend(cache, q, page_table, lengths, max_length, scale, sinks, window, stream, *, listed=None, weights=None,
             offsets=None, max_new=0, prompt=False):
     dev, lib, native = cache.keys.device, N.load(), cache._native
-    _no_gradient(q, weights, *cache._tensors())
+    _no_gradient(cache, q, weights)
     kind = _QUERY_TYPES.get(q.dtype)
     if q.dim() != 3 or kind is None or q.device != dev:
         raise ValueError(f"q must be bf16 or fp16 [tokens, q_heads, head_dim] on {dev}")
@@ -308,7 +310,7 @@ def evict(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tensor, weigh
     belong to two sequences).  Rows whose page id names no page do not stay, and
     rows that move to such an id are lost.  ``weights`` is left as it is."""
     dev = cache.keys.device
-    _no_gradient(weights, *cache._tensors())
+    _no_gradient(cache, weights)
     seq = _sequences(cache, page_table, lengths, max_length)
     _check(weights, "weights", torch.float32, (seq.batch, cache.heads, None), dev)
     rows = weights.shape[2]
