@@ -14,7 +14,7 @@
 // ballots and one sum over the waves give each kept row its place, in order
 // and without a sort.  Up to 32,768 candidates stay in LDS from one read.  A chain
 // of passes over few bytes, latency-bound: 8 sequences of up to 32,768 rows, 8 heads,
-// 27 us.
+// 28 us.  (Weights that are all equal meet in one bin: 68 us more.)
 //
 // kv_move_kernel: copy-bound (8 x 8,000 rows kept of 8 heads, 128 dims, 16 bits: 524 MB
 // read and written in 109 us, 4.8 TB/s).  Into other pages, workgroups share the kept rows

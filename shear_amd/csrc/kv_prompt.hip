@@ -10,10 +10,10 @@
 // earlier): 16-bit rows go to the other half without a register, codes through registers.
 //
 // Bound by the issue of instructions: beside 32 matrix instructions of a wave and
-// tile (128 dims) stand some 180 vector ones, most of them the weights', and 130 scalar
-// ones (with a window 230 and 150: masks).  No LDS bank conflict was counted.  Two
-// prompts of 4,096 tokens, 16 heads over 4 of 128 dims, causal: 153 us,
-// 899 TFLOP/s of 1,207 that a product of 8,192^3 reaches; 12,001 tokens with a
+// tile (128 dims) stand some 185 vector ones, most of them the weights', and 130 scalar
+// ones (with a window 235 and 155: masks).  No LDS bank conflict was counted.  Two
+// prompts of 4,096 tokens, 16 heads over 4 of 128 dims, causal: 154 us,
+// 893 TFLOP/s of 1,207 that a product of 8,192^3 reaches; 12,001 tokens with a
 // window of 1,024 and 4 first rows: 145 us, 667 TFLOP/s (a workgroup's 32
 // tokens see 1,060 rows, its tiles have 1,216).
 //  * S^T = K Q^T on 32x32x16 instructions (rows are the tile's, columns the
@@ -21,9 +21,9 @@
 //    half, so the running maximum and sum cost one exchange a tile.
 //  * O^T = V^T P^T: the logits' registers are the P^T operand as they
 //    stand; V^T comes from LDS by transposing reads of 4 rows x 16 values.
-//  * The maximum follows only where a tile's weights would sum to 2^15 times the largest that it
-//    was set for, or more (SQ8: a weight would be that), and tiles that every query of the workgroup sees in full
-//    carry no mask.
+//  * The maximum follows only where a tile's weights would sum to 2^15 times the
+//    largest that it was set for (fp16 2^6 times; SQ8: a weight would be that),
+//    and tiles that every query of the workgroup sees in full carry no mask.
 //  * P is rounded to the queries' type once (an error of the size of the
 //    result's own rounding); sums are in f32.  fp16 has nothing between 0 and 2^-24: there
 //    the largest weight lies between 2^9 and 2^15, so a weight is right to 11 bits
@@ -91,8 +91,8 @@ __device__ __forceinline__ bool special_half(uint32_t x) {
 }
 
 // Rows of a tile: at 256 dims of 16-bit rows half as many, for the registers' sake.  (Two
-// prompts of 4,096 tokens, 16 heads over 4 of 256: 545 us, with 64 rows and spills 1,390;
-// SQ8 617 with 64 rows, 742 with 32.)
+// prompts of 4,096 tokens, 16 heads over 4 of 256: 549 us, with 64 rows and spills 1,390;
+// SQ8 609 with 64 rows, 742 with 32.)
 template <bool kSq8, int DP>
 constexpr uint32_t prompt_rows() {
     return DP == 256 && !kSq8 ? 32u : 64u;

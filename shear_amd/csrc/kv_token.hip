@@ -21,7 +21,7 @@
 //   48 sequences of up to 4,100 rows, with weights   533 MB   115 + 14 us   4.1 TB/s
 //   8 of up to 40,000 SQ8 rows, with weights         522 MB   122 + 15 us   3.8 TB/s
 //   one of 131,071 rows                              268 MB    52 +  7 us   4.5 TB/s
-//   16, 2,016 rows each of which 1,500 are listed     49 MB    16 +  5 us   2.3 TB/s
+//   16, 2,016 rows each of which 1,500 are listed     49 MB    17 +  5 us   2.3 TB/s
 // (a copy reaches 4.9 to 5.5 TB/s here).  The last is a chain of dependent
 // reads, length, list, page, row, and then only two units a workgroup.
 //  * S^T = K Q^T on 16x16x32 instructions: the K operand is 16 bytes of a row
@@ -262,7 +262,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
     // Q operand: heads are columns; dims of step s as K's lanes hold them
     const bool head_ok = n < heads;
     // beside the second sum of 256 dims the queries would not fit the registers (48 sequences of up to 4,100 rows,
-    // 32 heads over 2 of 256 dims: 71 us, in registers with spills 77, bf16 64)
+    // 32 heads over 2 of 256 dims: 72 us, in registers with spills 77, bf16 65)
     constexpr bool kQueryInLds = kHalf && DP == 256;
     __shared__ kv_u4 sh_q[kQueryInLds ? kSteps : 1][64];
     kv_u4 qf[kQueryInLds ? 1 : kSteps];
