@@ -32,10 +32,12 @@
 //    stand.  V comes as whole rows (16 lanes a row, head_dim / 16 values each,
 //    eight rows a lane); the operand of instruction c is value c of each of
 //    the eight, one byte permute per two values.
-//  * P is given to the matrix instructions as the sum of two 16-bit parts (the
-//    rounded value and the rounded rest), because a single rounding of P would
-//    add an error as large as that of rounding the result; the instructions
-//    it costs are idle otherwise.  fp16 has nothing between 0 and 2^-24: there the
+//  * P is given to the matrix instructions as the sum of three bf16 parts (the
+//    rounded value, the rounded rest and the rest of that: f32's 24 bits) or two of
+//    fp16, because a single rounding of P would add an error as large as that of
+//    rounding the result, and two bf16 parts 2^-18 of the sum of |p v|, which shows
+//    where that cancels.  The instructions they cost are idle otherwise (the second
+//    SQ8 case above 137.4 us with two parts, 138.3 with three).  fp16 has nothing between 0 and 2^-24: there the
 //    largest weight lies between 2^7 and 2^15, and the rest is multiplied by
 //    2^12 and summed by itself, so that a weight is right to 2^-44 of the largest and
 //    many small ones beside a large one (a first row that takes the attention) add up.
@@ -422,7 +424,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
                 if constexpr (kHalf) rest[i] *= f;
             }
         }
-        kv_u4 hi, lo;
+        kv_u4 hi, lo, least;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             kv_f4 vs = {1, 1, 1, 1};
@@ -437,7 +439,10 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
                 }
                 const uint32_t r = P::pack(w0, w1);
                 hi[2 * t + i / 2] = r;
-                lo[2 * t + i / 2] = P::pack((w0 - P::low(r)) * kRest, (w1 - P::high(r)) * kRest);
+                const float r0 = (w0 - P::low(r)) * kRest, r1 = (w1 - P::high(r)) * kRest;
+                const uint32_t y = P::pack(r0, r1);
+                lo[2 * t + i / 2] = y;
+                if constexpr (!kHalf) least[2 * t + i / 2] = P::pack(r0 - P::low(y), r1 - P::high(y));
             }
         }
 #pragma unroll
@@ -454,7 +459,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
             if constexpr (kHalf)
                 rest[e] = P::mma16(a, lo, rest[e]);
             else
-                acc[e] = P::mma16(a, lo, acc[e]);
+                acc[e] = P::mma16(a, least, P::mma16(a, lo, acc[e]));
         }
     }
     l = kv_sum16(l);

@@ -283,3 +283,15 @@ def test_values_near_the_ends_of_bf16(gpu, cache_type, size, how):
     for kw in ({}, {"weights": torch.zeros((1, 1, n), device="cuda")}):
         out, lse = KV.attend_token(q[-1:].contiguous(), pool.cache, pool.table, lens([n]), **kw)
         check_token(pool, [n], q[-1:], out, lse, None, 0)
+
+
+@pytest.mark.parametrize("cache_type,q_type", [(BF16, BF16), (F16, F16), (SQ8, BF16), (SQ8, F16)])
+@pytest.mark.parametrize("n", [2, 6])
+def test_token_sums_that_cancel(gpu, cache_type, q_type, n):
+    """Many short sequences of nearly equal weights: some results are small beside their terms."""
+    b = 200
+    lengths = [n] * b
+    pool, g = pool_with(lengths, 1, 16, 48, cache_type, q_type, n)
+    q = normal(g, b, 17, 48, dtype=q_type, scale=0.01)
+    out, lse = KV.attend_token(q, pool.cache, pool.table, lens(lengths))
+    check_token(pool, lengths, q, out, lse, None, 0)
