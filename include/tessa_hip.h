@@ -935,24 +935,29 @@ uint32_t tessa_abi_version(void);
  * A cache holds keys and values in pages of page_rows rows (a power of two);
  * row j of sequence b lies in page table[b][j / page_rows], slot j % page_rows.
  * A row is head_dim values (a multiple of 16, at most 256) for each of `heads`
- * heads: bf16, fp16, or SQ8 codes with one f32 scale (value = scale * code, scale
- * = max|x| * (1/127), code = x / scale rounded half away from zero).  Strides are between pages, heads and rows, in
- * elements; rows are contiguous and 16-byte aligned.  Nothing here allocates,
+ * heads: bf16, fp16, SQ8 codes with one f32 scale (value = scale * code, scale
+ * = max|x| * (1/127), code = x / scale rounded half away from zero), or MX4: 4-bit
+ * codes, two to a byte (the even dim in the low bits), of a sign bit, two bits of exponent and one
+ * of fraction (0, 0.5, 1, 1.5, 2, 3, 4, 6), and for each 32 dims a byte e, value = 2^(e - 127) * code
+ * (head_dim a multiple of 32).  e makes max|x| round to 6 at most: with max|x| = m 2^k, 1 <= m < 2, e is
+ * 127 + k - 2, or one more from m = 1.75 on, held in 2..252; codes are the nearest, ties to the even code.  32 dims of which one is not
+ * finite have e = 255 and are NaN.  Strides are between pages, heads and rows, in
+ * elements (of 4 bits for MX4); rows are contiguous and 16-byte aligned.  Nothing here allocates,
  * waits for the device or keeps anything between calls: results are queued on
  * `stream`, scratch is the caller's, and the calls may be captured in a graph.
  *
  * No counterpart in the reference: its search ends with the ids
  * (tessa_graph_search); these operators attend over the rows that they name. */
-enum tessa_kv_type { TESSA_KV_BF16 = 1, TESSA_KV_F16 = 2, TESSA_KV_SQ8 = 3 };
+enum tessa_kv_type { TESSA_KV_BF16 = 1, TESSA_KV_F16 = 2, TESSA_KV_SQ8 = 3, TESSA_KV_MX4 = 5, TESSA_KV_F32 = 6 /* of tessa_kv_read, weights */ };
 #define TESSA_KV_ALL 0xffffffffu /* tessa_kv_attend.window: every row is visible */
 
 typedef struct tessa_kv_cache {
     void *keys;
     void *values;
-    float *key_scales;   /* SQ8 only */
-    float *value_scales;
+    void *key_scales;    /* SQ8: floats, one a row; MX4: bytes, head_dim / 32 a row, contiguous */
+    void *value_scales;
     uint64_t key_strides[3], value_strides[3];             /* elements: page, head, row */
-    uint64_t key_scale_strides[3], value_scale_strides[3]; /* floats */
+    uint64_t key_scale_strides[3], value_scale_strides[3]; /* floats, MX4: bytes */
     uint32_t type;       /* enum tessa_kv_type */
     uint32_t pages, heads, page_rows, head_dim;
     uint32_t reserved;
@@ -973,7 +978,7 @@ typedef struct tessa_kv_sequences {
 /* New rows.  Token t of sequence b (offsets[b] <= t < offsets[b + 1]; without
  * offsets one token for each sequence) becomes row lengths[b] + t - offsets[b]:
  * here `lengths` are the rows before the call.  k and v: tokens x heads rows of
- * bf16 or fp16 (`type`; the cache's own type unless that is SQ8), strides in
+ * bf16 or fp16 (`type`; the cache's own type unless it holds codes), strides in
  * elements, 16-byte aligned.  An SQ8 row with a value that is not finite gets the
  * scale NaN. */
 typedef struct tessa_kv_tokens {
@@ -1007,7 +1012,7 @@ typedef struct tessa_kv_attend {
     void *out;
     float *lse;                            /* tokens x q_heads */
     uint64_t q_strides[2], out_strides[2]; /* elements: token, head; 16-byte aligned rows */
-    uint32_t type;                         /* of q and out; the cache's own unless that is SQ8 */
+    uint32_t type;                         /* of q and out; the cache's own unless it holds codes */
     uint32_t q_heads;
     float scale;
     uint32_t sinks, window;
@@ -1056,6 +1061,83 @@ typedef struct tessa_kv_eviction {
 } tessa_kv_eviction;
 tessa_status tessa_kv_evict(const tessa_kv_cache *cache, const tessa_kv_sequences *seq, const tessa_kv_eviction *e,
                             void *stream);
+
+/* New rows by place, normalized and rotated on their way: for each token and head
+ *   y = x * rsqrt(mean x^2 + eps) * weight      of q and of k (null weight: y = x)
+ *   (a, b) -> (a cos t - b sin t, a sin t + b cos t),  t = position * frequencies[i]
+ * for the pairs i < rotated / 2 of dims (i, i + rotated / 2), or (2 i, 2 i + 1) with `interleaved`;
+ * dims from `rotated` on stay.  t is formed in 64 bits, the rest in f32, rounded once to `type`.  q's rows go to `out`
+ * (it may be q), k's and v's (v as it is) to row slots[token] % page_rows of page slots[token] / page_rows, as
+ * tessa_kv_append writes them.  A slot outside the cache is not written; a token whose position is
+ * negative is of no sequence: nothing of it is written and its rows of `out` are zeros.  No two tokens may have the
+ * same slot. */
+typedef struct tessa_kv_rotated {
+    const void *q;
+    const void *k;
+    const void *v;
+    void *out;
+    uint64_t q_strides[2], k_strides[2], v_strides[2], out_strides[2]; /* elements: token, head; 16-byte aligned rows */
+    const int32_t *positions;   /* tokens */
+    const int64_t *slots;       /* tokens */
+    const double *frequencies;  /* rotated / 2: radians for each position */
+    const void *q_weight;       /* head_dim values each, 16-byte aligned, or null */
+    const void *k_weight;
+    uint64_t tokens;
+    uint32_t type;              /* of q, k, v and out; the cache's own unless it holds codes */
+    uint32_t weight_type;       /* `type` or TESSA_KV_F32 */
+    uint32_t q_heads;
+    uint32_t rotated;           /* a multiple of 16 up to head_dim, or 0 */
+    uint32_t interleaved;
+    float eps;
+} tessa_kv_rotated;
+tessa_status tessa_kv_append_rotated(const tessa_kv_cache *cache, const tessa_kv_rotated *tokens, void *stream);
+
+/* Rows by place, as values of `type` (bf16, fp16 or f32): k and v (null: keys
+ * only) get count x heads x head_dim values, contiguous, of row slots[i] % page_rows of page slots[i] /
+ * page_rows; zeros where the slot is outside the cache. */
+typedef struct tessa_kv_rows {
+    const int64_t *slots;
+    void *k;
+    void *v;
+    uint64_t count;
+    uint32_t type;
+    uint32_t reserved;
+} tessa_kv_rows;
+tessa_status tessa_kv_read(const tessa_kv_cache *cache, const tessa_kv_rows *rows, void *stream);
+
+/* The pages and places of a step.  Sequence b has lengths[b] rows in the first
+ * held[b] pages of its table row, and fresh[b] new tokens, or ends (negative: it keeps no rows and gives its pages
+ * back).  Tokens lie sequence by sequence: offsets (batch + 1) are the sums of the counts before.
+ * `free` is a stack of count[0] ids of free pages, with room for `pages`.
+ *  - A sequence whose rows would pass its table (columns * page_rows, at most 2^30 - 1), or whose tokens
+ *    lie past `tokens`, gets no new rows (granted 0).
+ *  - Pages that a sequence holds and needs no more go back to the stack, in the order of the sequences and columns.
+ *  - A sequence that needs more pages gets them from the top, in the same order, if what all sequences up to it
+ *    need is there; else it gets no new rows.  Others that need none are served all the same.
+ * new_lengths, new_held, new_count and granted say how it went; the table's new ids and the stack's are
+ * written in place, and what lies past them is left as it was (ids past new_held are not the sequence's).
+ * For each of `tokens` places: the position (row) of the token, its sequence and its slot (page * page_rows + row of the
+ * page); -1 past the last token, position and slot -1 too where the token was not granted. */
+typedef struct tessa_kv_step {
+    int32_t *table;              /* batch x table_stride */
+    uint64_t table_stride;
+    const int32_t *lengths;
+    const int32_t *held;
+    const int32_t *fresh;
+    int32_t *free;
+    const int32_t *count;
+    int32_t *new_lengths;
+    int32_t *new_held;
+    int32_t *new_count;
+    int32_t *granted;
+    int32_t *offsets;
+    int32_t *positions;
+    int32_t *sequences;
+    int64_t *slots;
+    uint64_t tokens;
+    uint32_t batch, columns, pages, page_rows;
+} tessa_kv_step;
+tessa_status tessa_kv_plan(const tessa_kv_step *step, void *stream);
 
 #ifdef __cplusplus
 }

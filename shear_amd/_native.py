@@ -313,7 +313,7 @@ class TierLiftStats(C.Structure):
         return {f: getattr(self, f) for f, _ in self._fields_}
 
 
-KV_BF16, KV_F16, KV_SQ8 = 1, 2, 3
+KV_BF16, KV_F16, KV_SQ8, KV_MX4, KV_F32 = 1, 2, 3, 5, 6
 KV_ALL = 0xFFFFFFFF
 
 
@@ -348,6 +348,28 @@ class KvEviction(C.Structure):
                 ("kept", C.c_void_p), ("new_lengths", C.c_void_p), ("into", C.c_void_p), ("into_stride", C.c_uint64),
                 ("into_columns", C.c_uint32), ("weight_rows", C.c_uint32), ("keep", C.c_uint32), ("sinks", C.c_uint32),
                 ("recent", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class KvRotated(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p),
+                ("q_strides", C.c_uint64 * 2), ("k_strides", C.c_uint64 * 2), ("v_strides", C.c_uint64 * 2),
+                ("out_strides", C.c_uint64 * 2), ("positions", C.c_void_p), ("slots", C.c_void_p),
+                ("frequencies", C.c_void_p), ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("tokens", C.c_uint64),
+                ("type", C.c_uint32), ("weight_type", C.c_uint32), ("q_heads", C.c_uint32), ("rotated", C.c_uint32),
+                ("interleaved", C.c_uint32), ("eps", C.c_float)]
+
+
+class KvRows(C.Structure):
+    _fields_ = [("slots", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("count", C.c_uint64), ("type", C.c_uint32),
+                ("reserved", C.c_uint32)]
+
+
+class KvStep(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("table_stride", C.c_uint64), ("lengths", C.c_void_p), ("held", C.c_void_p),
+                ("fresh", C.c_void_p), ("free", C.c_void_p), ("count", C.c_void_p), ("new_lengths", C.c_void_p),
+                ("new_held", C.c_void_p), ("new_count", C.c_void_p), ("granted", C.c_void_p), ("offsets", C.c_void_p),
+                ("positions", C.c_void_p), ("sequences", C.c_void_p), ("slots", C.c_void_p), ("tokens", C.c_uint64),
+                ("batch", C.c_uint32), ("columns", C.c_uint32), ("pages", C.c_uint32), ("page_rows", C.c_uint32)]
 
 
 # Every symbol include/tessa_hip.h declares, with its ctypes signature.
@@ -453,6 +475,9 @@ SIGNATURES = {
                                                      C.POINTER(_U64)]),
     "tessa_kv_attend_prompt": (TessaStatus, [C.POINTER(KvCache), C.POINTER(KvSequences), C.POINTER(KvAttend), _P, _U64,
                                              _P]),
+    "tessa_kv_append_rotated": (TessaStatus, [C.POINTER(KvCache), C.POINTER(KvRotated), _P]),
+    "tessa_kv_read": (TessaStatus, [C.POINTER(KvCache), C.POINTER(KvRows), _P]),
+    "tessa_kv_plan": (TessaStatus, [C.POINTER(KvStep), _P]),
     "tessa_kv_evict": (TessaStatus, [C.POINTER(KvCache), C.POINTER(KvSequences), C.POINTER(KvEviction), _P]),
 }
 

@@ -55,22 +55,26 @@ tessa_status fine() {
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+KvRows rows_kind(uint32_t cache) {
+    return cache == TESSA_KV_SQ8 ? kRowsSq8 : cache == TESSA_KV_MX4 ? kRowsMx4 : kRowsPlain;
+}
+
 // One page array in 16-byte units; false where a row is misaligned or its place
 // would not fit 32 bits.
-tessa_status page_array(const tessa_kv_cache &k, const char *what, void *rows, const uint64_t (&strides)[3], float *scales,
+tessa_status page_array(const tessa_kv_cache &k, const char *what, void *rows, const uint64_t (&strides)[3], void *scales,
                         const uint64_t (&scale_strides)[3], KvArray &out) {
-    const uint64_t size = k.type == TESSA_KV_SQ8 ? 1 : 2;
+    const uint64_t unit = k.type == TESSA_KV_MX4 ? 32 : k.type == TESSA_KV_SQ8 ? 16 : 8;  // elements of 16 bytes
     if (!rows) KV_INVALID("kv cache: null %s", what);
     if (!aligned16(rows)) KV_INVALID("kv cache: %s are not 16-byte aligned", what);
     uint64_t units[3];
     for (int i = 0; i < 3; ++i) {
-        if (strides[i] >= (1ull << 40) || (strides[i] * size) % 16 != 0)
+        if (strides[i] >= (1ull << 40) || strides[i] % unit != 0)
             KV_INVALID("kv cache: %s stride %llu is not a multiple of 16 bytes", what, (unsigned long long)strides[i]);
-        units[i] = strides[i] * size / 16;
+        units[i] = strides[i] / unit;
     }
     const uint64_t counts[3] = {k.pages, k.heads, k.page_rows};
     // units are below 2^37 and counts below 2^32: sum them as doubles first
-    double last = (double)k.head_dim * size / 16.0;
+    double last = (double)k.head_dim / (double)unit;
     for (int i = 0; i < 3; ++i) last += (double)units[i] * (double)(counts[i] - 1);
     if (last >= 4294967295.0 || units[0] > 0xffffffffull || units[1] > 0xffffffffull || units[2] > 0xffffffffull)
         KV_UNSUPPORTED("kv cache: %s span more than 64 GiB", what);
@@ -80,8 +84,10 @@ tessa_status page_array(const tessa_kv_cache &k, const char *what, void *rows, c
     out.row_units = (uint32_t)units[2];
     out.scales = nullptr;
     out.scale_page = out.scale_head = out.scale_row = 0;
-    if (k.type == TESSA_KV_SQ8) {
-        if (!scales) KV_INVALID("kv cache: SQ8 %s need scales", what);
+    if (k.type == TESSA_KV_SQ8 || k.type == TESSA_KV_MX4) {
+        if (!scales) KV_INVALID("kv cache: %s %s need scales", k.type == TESSA_KV_SQ8 ? "SQ8" : "MX4", what);
+        for (int i = 0; i < 3 && k.type == TESSA_KV_MX4; ++i)
+            if (scale_strides[i] >= (1ull << 40)) KV_INVALID("kv cache: scale stride of %s", what);
         out.scales = scales;
         out.scale_page = scale_strides[0];
         out.scale_head = scale_strides[1];
@@ -90,18 +96,42 @@ tessa_status page_array(const tessa_kv_cache &k, const char *what, void *rows, c
     return fine();
 }
 
-tessa_status cache_of(const tessa_kv_cache *k, const tessa_kv_sequences *s, KvCacheParams &c) {
-    if (!k || !s) KV_INVALID("kv cache: null pointer");
-    if (k->type < TESSA_KV_BF16 || k->type > TESSA_KV_SQ8) KV_INVALID("kv cache: unknown type %u", k->type);
+// Whether an MX4 row's scales lie together in a word that may be read as one.
+bool word_scales(const tessa_kv_cache &k, const void *scales, const uint64_t (&strides)[3]) {
+    const uint64_t word = k.head_dim / 32;
+    if (word != 2 && word != 4 && word != 8) return false;
+    return ((reinterpret_cast<uintptr_t>(scales) | strides[0] | strides[1] | strides[2]) & (word - 1)) == 0;
+}
+
+tessa_status pages_of(const tessa_kv_cache *k, KvCacheParams &c) {
+    if (!k) KV_INVALID("kv cache: null pointer");
+    if (k->type != TESSA_KV_MX4 && (k->type < TESSA_KV_BF16 || k->type > TESSA_KV_SQ8))
+        KV_INVALID("kv cache: unknown type %u", k->type);
     if (!k->pages || !k->heads) KV_INVALID("kv cache: %u pages, %u heads", k->pages, k->heads);
     if (k->pages > 0x7fffffffu || k->heads > 1024u) KV_UNSUPPORTED("kv cache: %u pages, %u heads", k->pages, k->heads);
     if (!k->page_rows || (k->page_rows & (k->page_rows - 1u)) || k->page_rows > 65536u)
         KV_INVALID("kv cache: page_rows must be a power of two in 1..=65536, got %u", k->page_rows);
     if (!k->head_dim || k->head_dim % 16u || k->head_dim > 256u)
         KV_UNSUPPORTED("kv cache: head_dim must be a multiple of 16 in 16..=256, got %u", k->head_dim);
+    if (k->type == TESSA_KV_MX4 && k->head_dim % 32u)
+        KV_UNSUPPORTED("kv cache: MX4 head_dim must be a multiple of 32, got %u", k->head_dim);
     tessa_status st = page_array(*k, "keys", k->keys, k->key_strides, k->key_scales, k->key_scale_strides, c.keys);
     if (st.code) return st;
     st = page_array(*k, "values", k->values, k->value_strides, k->value_scales, k->value_scale_strides, c.values);
+    if (st.code) return st;
+    c.pages = k->pages;
+    c.heads = k->heads;
+    c.dim = k->head_dim;
+    c.page_shift = (uint32_t)__builtin_ctz(k->page_rows);
+    c.mx4 = k->type == TESSA_KV_MX4;
+    c.scales_together = c.mx4 && word_scales(*k, k->key_scales, k->key_scale_strides) &&
+                        word_scales(*k, k->value_scales, k->value_scale_strides);
+    return fine();
+}
+
+tessa_status cache_of(const tessa_kv_cache *k, const tessa_kv_sequences *s, KvCacheParams &c) {
+    if (!k || !s) KV_INVALID("kv cache: null pointer");
+    const tessa_status st = pages_of(k, c);
     if (st.code) return st;
     if (s->batch > kMaxGrid) KV_UNSUPPORTED("kv cache: batch %u over %u", s->batch, kMaxGrid);
     if (s->batch && (!s->lengths || (s->columns && !s->table))) KV_INVALID("kv cache: null table or lengths");
@@ -116,17 +146,13 @@ tessa_status cache_of(const tessa_kv_cache *k, const tessa_kv_sequences *s, KvCa
     c.lengths = s->lengths;
     c.batch = s->batch;
     c.max_length = s->max_length;
-    c.pages = k->pages;
-    c.heads = k->heads;
-    c.dim = k->head_dim;
-    c.page_shift = (uint32_t)__builtin_ctz(k->page_rows);
     return fine();
 }
 
-// The 16-bit type of q, k, v: the cache's own, or either for an SQ8 cache.
+// The 16-bit type of q, k, v: the cache's own, or either for a cache of codes.
 tessa_status own_type(uint32_t cache, uint32_t type) {
     if (type != TESSA_KV_BF16 && type != TESSA_KV_F16) KV_INVALID("kv: type %u is neither bf16 nor fp16", type);
-    if (cache != TESSA_KV_SQ8 && cache != type) KV_INVALID("kv: type %u over a cache of type %u", type, cache);
+    if (rows_kind(cache) == kRowsPlain && cache != type) KV_INVALID("kv: type %u over a cache of type %u", type, cache);
     return fine();
 }
 
@@ -260,9 +286,9 @@ tessa_status attend(const tessa_kv_cache *cache, const tessa_kv_sequences *seq, 
         if (logits) p.logits = reinterpret_cast<float *>(at + o + ml);
     }
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    const bool sq8 = cache->type == TESSA_KV_SQ8;
-    int rc = prompt ? launch_kv_prompt(p, a->type, sq8, s) : launch_kv_token(p, a->type, sq8, s);
-    if (rc == 0 && o) rc = launch_kv_finish(p, a->type, sq8, prompt, s);
+    const KvRows rows = rows_kind(cache->type);
+    int rc = prompt ? launch_kv_prompt(p, a->type, rows, s) : launch_kv_token(p, a->type, rows, s);
+    if (rc == 0 && o) rc = launch_kv_finish(p, a->type, rows, prompt, s);
     if (rc) return status(TESSA_ERR_HIP, "kv attend: launch failed");
     return fine();
 }
@@ -311,7 +337,7 @@ tessa_status tessa_kv_append(const tessa_kv_cache *cache, const tessa_kv_sequenc
         if (p.max_new > tokens->tokens) p.max_new = (uint32_t)tokens->tokens;
         // 2^5 lanes a row at most, 256 threads a workgroup
         if ((uint64_t)p.max_new * p.c.heads / 8 + 1 > 0x7fffffffull) KV_UNSUPPORTED("kv append: %u new tokens", p.max_new);
-        if (launch_kv_append(p, tokens->type, cache->type == TESSA_KV_SQ8, reinterpret_cast<hipStream_t>(stream)))
+        if (launch_kv_append(p, tokens->type, rows_kind(cache->type), reinterpret_cast<hipStream_t>(stream)))
             return status(TESSA_ERR_HIP, "kv append: launch failed");
         return fine();
     });
@@ -377,6 +403,135 @@ tessa_status tessa_kv_evict(const tessa_kv_cache *cache, const tessa_kv_sequence
         p.new_lengths = e->new_lengths;
         if (launch_kv_evict(p, cache->type, reinterpret_cast<hipStream_t>(stream)))
             return status(TESSA_ERR_HIP, "kv evict: launch failed");
+        return fine();
+    });
+}
+
+tessa_status tessa_kv_append_rotated(const tessa_kv_cache *cache, const tessa_kv_rotated *t, void *stream) {
+    return guarded([&]() -> tessa_status {
+        if (!t) KV_INVALID("kv append rotated: null pointer");
+        KvRotateParams p;
+        std::memset(&p, 0, sizeof(p));
+        tessa_status st = pages_of(cache, p.c);
+        if (st.code) return st;
+        st = own_type(cache->type, t->type);
+        if (st.code) return st;
+        if (!t->q_heads || t->q_heads > kMaxGroup * 1024u) KV_INVALID("kv append rotated: %u query heads", t->q_heads);
+        if (t->rotated % 16u || t->rotated > p.c.dim)
+            KV_INVALID("kv append rotated: rotated dims must be a multiple of 16 up to %u, got %u", p.c.dim, t->rotated);
+        if (t->rotated && !t->frequencies) KV_INVALID("kv append rotated: null frequencies");
+        if ((reinterpret_cast<uintptr_t>(t->frequencies) & 7u) != 0) KV_INVALID("kv append rotated: frequencies are not 8-byte aligned");
+        if (t->weight_type != t->type && t->weight_type != TESSA_KV_F32)
+            KV_INVALID("kv append rotated: weights of type %u for tokens of type %u", t->weight_type, t->type);
+        if (!aligned16(t->q_weight) || !aligned16(t->k_weight)) KV_INVALID("kv append rotated: weights are not 16-byte aligned");
+        if (!(t->eps >= 0.0f) || !std::isfinite(t->eps)) KV_INVALID("kv append rotated: eps must be finite and not negative");
+        if (!t->tokens) return fine();
+        const uint64_t rows = (uint64_t)t->q_heads + 2u * p.c.heads;
+        if (t->tokens > kMaxRows || t->tokens * rows > 0x7fffffffull)
+            KV_UNSUPPORTED("kv append rotated: %llu tokens of %llu rows", (unsigned long long)t->tokens, (unsigned long long)rows);
+        uint64_t b[2];
+        st = rows_of("q", t->q, t->q_strides, b);
+        if (st.code) return st;
+        p.q = static_cast<const char *>(t->q);
+        p.q_token = b[0];
+        p.q_head = b[1];
+        st = rows_of("k", t->k, t->k_strides, b);
+        if (st.code) return st;
+        p.k = static_cast<const char *>(t->k);
+        p.k_token = b[0];
+        p.k_head = b[1];
+        st = rows_of("v", t->v, t->v_strides, b);
+        if (st.code) return st;
+        p.v = static_cast<const char *>(t->v);
+        p.v_token = b[0];
+        p.v_head = b[1];
+        st = rows_of("out", t->out, t->out_strides, b);
+        if (st.code) return st;
+        p.out = static_cast<char *>(t->out);
+        p.out_token = b[0];
+        p.out_head = b[1];
+        if (!t->positions || !t->slots) KV_INVALID("kv append rotated: null positions or slots");
+        p.positions = t->positions;
+        p.slots = t->slots;
+        p.frequencies = t->frequencies;
+        p.q_weight = t->q_weight;
+        p.k_weight = t->k_weight;
+        p.tokens = t->tokens;
+        p.q_heads = t->q_heads;
+        p.half = t->rotated / 2;
+        p.eps = t->eps;
+        p.interleaved = t->interleaved != 0;
+        p.wide_weights = t->weight_type == TESSA_KV_F32;
+        if (launch_kv_rotate(p, t->type, rows_kind(cache->type), reinterpret_cast<hipStream_t>(stream)))
+            return status(TESSA_ERR_HIP, "kv append rotated: launch failed");
+        return fine();
+    });
+}
+
+tessa_status tessa_kv_read(const tessa_kv_cache *cache, const tessa_kv_rows *r, void *stream) {
+    return guarded([&]() -> tessa_status {
+        if (!r) KV_INVALID("kv read: null pointer");
+        KvReadParams p;
+        std::memset(&p, 0, sizeof(p));
+        const tessa_status st = pages_of(cache, p.c);
+        if (st.code) return st;
+        if (r->type != TESSA_KV_BF16 && r->type != TESSA_KV_F16 && r->type != TESSA_KV_F32)
+            KV_INVALID("kv read: type %u is neither bf16, fp16 nor f32", r->type);
+        if (!r->count) return fine();
+        if (r->count > kMaxRows || r->count * p.c.heads > 0x7fffffffull)
+            KV_UNSUPPORTED("kv read: %llu rows of %u heads", (unsigned long long)r->count, p.c.heads);
+        if (!r->slots || !r->k) KV_INVALID("kv read: null pointer");
+        if (!aligned16(r->k) || !aligned16(r->v)) KV_INVALID("kv read: k and v are not 16-byte aligned");
+        p.slots = r->slots;
+        p.k = static_cast<char *>(r->k);
+        p.v = static_cast<char *>(r->v);
+        p.count = r->count;
+        if (launch_kv_read(p, cache->type, r->type, reinterpret_cast<hipStream_t>(stream)))
+            return status(TESSA_ERR_HIP, "kv read: launch failed");
+        return fine();
+    });
+}
+
+tessa_status tessa_kv_plan(const tessa_kv_step *s, void *stream) {
+    return guarded([&]() -> tessa_status {
+        if (!s) KV_INVALID("kv plan: null pointer");
+        if (!s->page_rows || (s->page_rows & (s->page_rows - 1u)) || s->page_rows > 65536u)
+            KV_INVALID("kv plan: page_rows must be a power of two in 1..=65536, got %u", s->page_rows);
+        if (s->batch > kMaxGrid) KV_UNSUPPORTED("kv plan: batch %u over %u", s->batch, kMaxGrid);
+        if (s->pages > 0x7fffffffu || s->columns > 0x7fffffffu) KV_UNSUPPORTED("kv plan: %u pages, %u columns", s->pages, s->columns);
+        if (s->tokens > 0x7fffffffull) KV_UNSUPPORTED("kv plan: %llu tokens", (unsigned long long)s->tokens);
+        if (!s->count || !s->new_count || !s->offsets || (s->pages && !s->free)) KV_INVALID("kv plan: null pointer");
+        if (s->batch && (!s->lengths || !s->held || !s->fresh || !s->new_lengths || !s->new_held || !s->granted ||
+                         (s->columns && !s->table)))
+            KV_INVALID("kv plan: null pointer");
+        if (s->batch > 1 && s->table_stride < s->columns)
+            KV_INVALID("kv plan: table stride %llu below %u columns", (unsigned long long)s->table_stride, s->columns);
+        if (s->tokens && (!s->positions || !s->sequences || !s->slots)) KV_INVALID("kv plan: null pointer");
+        if ((s->batch && (s->new_lengths == s->lengths || s->new_held == s->held)) || s->new_count == s->count)
+            KV_INVALID("kv plan: results may not be the arguments");
+        KvPlanParams p;
+        std::memset(&p, 0, sizeof(p));
+        p.table = s->table;
+        p.table_stride = s->table_stride;
+        p.lengths = s->lengths;
+        p.held = s->held;
+        p.fresh = s->fresh;
+        p.free = s->free;
+        p.count = s->count;
+        p.new_lengths = s->new_lengths;
+        p.new_held = s->new_held;
+        p.new_count = s->new_count;
+        p.granted = s->granted;
+        p.offsets = s->offsets;
+        p.positions = s->positions;
+        p.sequences = s->sequences;
+        p.slots = s->slots;
+        p.tokens = s->tokens;
+        p.batch = s->batch;
+        p.columns = s->columns;
+        p.pages = s->pages;
+        p.page_shift = (uint32_t)__builtin_ctz(s->page_rows);
+        if (launch_kv_plan(p, reinterpret_cast<hipStream_t>(stream))) return status(TESSA_ERR_HIP, "kv plan: launch failed");
         return fine();
     });
 }

@@ -3,6 +3,9 @@
 // between the 16- and 32-lane groups of a wave, the table lookup.
 #pragma once
 
+#include <type_traits>
+#include <utility>
+
 #include "kv_kernels.h"
 
 namespace tessa {
@@ -47,6 +50,16 @@ struct KvElem<__bf16> {
         return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
     }
     static constexpr uint32_t kExponent = 0x7f80u;  // all ones: infinity or NaN
+    // two 4-bit codes (byte kByte of x) times the power of two `scale`: exact unless below 2^-126
+    template <int kByte>
+    static __device__ __forceinline__ uint32_t from_mx4(uint32_t x, float scale) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, scale, kByte));
+    }
+    // byte kByte of old: two values over `scale`, rounded to the nearest codes, ties to the even one, at most 6
+    template <int kByte>
+    static __device__ __forceinline__ uint32_t to_mx4(uint32_t old, uint32_t x, float scale) {
+        return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(old, __builtin_bit_cast(v2, x), scale, kByte);
+    }
 };
 
 template <>
@@ -67,10 +80,32 @@ struct KvElem<_Float16> {
     static __device__ __forceinline__ float high(uint32_t x) { return (float)__builtin_bit_cast(v2, x)[1]; }
     static __device__ __forceinline__ uint32_t pack_codes(float lo, float hi) { return pack(lo, hi); }
     static constexpr uint32_t kExponent = 0x7c00u;
+    template <int kByte>
+    static __device__ __forceinline__ uint32_t from_mx4(uint32_t x, float scale) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, scale, kByte));
+    }
+    template <int kByte>
+    static __device__ __forceinline__ uint32_t to_mx4(uint32_t old, uint32_t x, float scale) {
+        return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(old, __builtin_bit_cast(v2, x), scale, kByte);
+    }
 };
 
 // byte e of x as a signed code
 __device__ __forceinline__ float kv_code(uint32_t x, int e) { return (float)(int8_t)(x >> (8 * e)); }
+
+// 4-bit rows: 32 dims share a scale 2^(byte - 127); 255 says that one of them is not finite.  As
+// the exponent of an f32 the byte is what the conversions want, 255 (an infinity) included: they make it NaN.
+constexpr uint32_t kMxGroup = 32;
+constexpr uint32_t kMxNan = 255;
+__device__ __forceinline__ float kv_mx_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// Eight codes as values.
+template <typename T>
+__device__ __forceinline__ kv_u4 kv_mx_values(uint32_t codes, float scale) {
+    using E = KvElem<T>;
+    return kv_u4{E::template from_mx4<0>(codes, scale), E::template from_mx4<1>(codes, scale), E::template from_mx4<2>(codes, scale),
+                 E::template from_mx4<3>(codes, scale)};
+}
 
 __device__ __forceinline__ float kv_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -134,6 +169,19 @@ __device__ __forceinline__ uint64_t kv_scale_place(const KvCacheParams &c, const
                                                    uint32_t head) {
     return (uint64_t)(uint32_t)page * a.scale_page + (uint64_t)head * a.scale_head +
            (uint64_t)(row & ((1u << c.page_shift) - 1u)) * a.scale_row;
+}
+
+__device__ __forceinline__ float *kv_row_scales(const KvArray &a) { return static_cast<float *>(a.scales); }
+__device__ __forceinline__ uint8_t *kv_group_scales(const KvArray &a) { return static_cast<uint8_t *>(a.scales); }
+
+// f(integral_constant i) for i below kCount, in order: for builtins that want constants.
+template <typename F, int... i>
+__device__ __forceinline__ void kv_each_of(F &&f, std::integer_sequence<int, i...>) {
+    (f(std::integral_constant<int, i>{}), ...);
+}
+template <int kCount, typename F>
+__device__ __forceinline__ void kv_each(F &&f) {
+    kv_each_of(f, std::make_integer_sequence<int, kCount>{});
 }
 
 // The visible rows of a single token: [0, first), [last_begin, length) and the

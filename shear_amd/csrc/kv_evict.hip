@@ -205,7 +205,8 @@ __device__ __forceinline__ void move_rows(const KvEvictParams &p, const KvArray 
     const uint32_t lane = t & ((1u << lanes_log2) - 1u), per = kThreads >> lanes_log2;
     const uint32_t unit = unit0 + lane;
     const bool mine = lane < units && unit < row_units;
-    const bool scales = a.scales != nullptr && unit == 0;
+    // with the row's first piece its SQ8 scale, with each piece the scale of its 32 dims
+    const bool bytes = c.mx4 && mine, scales = a.scales != nullptr && !c.mx4 && unit == 0;
     char *base = a.rows + ((uint64_t)h * a.head_units + (mine ? unit : 0u)) * 16u;
     const uint32_t into_rows = p.into_columns << c.page_shift;
     last = min(last, into_rows);
@@ -216,6 +217,7 @@ __device__ __forceinline__ void move_rows(const KvEvictParams &p, const KvArray 
         int32_t src_page[kMovePer], dst_page[kMovePer];
         kv_u4 x[kMovePer];
         float sx[kMovePer];
+        uint32_t bx[kMovePer];
 #pragma unroll
         for (int i = 0; i < kMovePer; ++i) row[i] = (uint32_t)kept[min(j0 + i * per + (t >> lanes_log2), last - 1u)];
 #pragma unroll
@@ -229,19 +231,23 @@ __device__ __forceinline__ void move_rows(const KvEvictParams &p, const KvArray 
             dst[i] = j < last && !(in_place && row[i] == j) && src != kKvNoOffset ? kv_place(c, a, dst_page[i], j) : kKvNoOffset;
             x[i] = *reinterpret_cast<const kv_u4 *>(base + (uint64_t)(dst[i] != kKvNoOffset ? src : 0u) * 16u);
             sx[i] = 0.0f;
-            if (scales && dst[i] != kKvNoOffset) sx[i] = a.scales[kv_scale_place(c, a, src_page[i], row[i], h)];
+            bx[i] = 0u;
+            if (scales && dst[i] != kKvNoOffset) sx[i] = kv_row_scales(a)[kv_scale_place(c, a, src_page[i], row[i], h)];
+            if (bytes && dst[i] != kKvNoOffset) bx[i] = kv_group_scales(a)[kv_scale_place(c, a, src_page[i], row[i], h) + unit];
         }
         if (in_place) {
             // every row of the batch has arrived before any is written
 #pragma unroll
-            for (int i = 0; i < kMovePer; ++i) asm volatile("" : "+v"(x[i]), "+v"(sx[i]));
+            for (int i = 0; i < kMovePer; ++i) asm volatile("" : "+v"(x[i]), "+v"(sx[i]), "+v"(bx[i]));
             __syncthreads();
         }
 #pragma unroll
         for (int i = 0; i < kMovePer; ++i) {
             if (dst[i] != kKvNoOffset) {
                 if (mine) *reinterpret_cast<kv_u4 *>(base + (uint64_t)dst[i] * 16u) = x[i];
-                if (scales) a.scales[kv_scale_place(c, a, dst_page[i], j0 + i * per + (t >> lanes_log2), h)] = sx[i];
+                const uint32_t j = j0 + i * per + (t >> lanes_log2);
+                if (scales) kv_row_scales(a)[kv_scale_place(c, a, dst_page[i], j, h)] = sx[i];
+                if (bytes) kv_group_scales(a)[kv_scale_place(c, a, dst_page[i], j, h) + unit] = (uint8_t)bx[i];
             }
         }
     }
@@ -321,7 +327,7 @@ int launch_kv_evict(const KvEvictParams &p, uint32_t type, hipStream_t stream) {
     const uint32_t held = most < kSelHeld ? (most + kSelThreads - 1) / kSelThreads * kSelThreads : kSelHeld;
     if (ensure_lds_limit(reinterpret_cast<const void *>(&kv_select_kernel), (int)(kSelHeld * sizeof(uint32_t))) != 0) return -1;
     const bool in_place = p.into == p.c.table;
-    const uint32_t row_units = p.c.dim * (type == kKvSq8 ? 1u : 2u) / 16u;
+    const uint32_t row_units = type == kKvMx4 ? p.c.dim / 32u : p.c.dim * (type == kKvSq8 ? 1u : 2u) / 16u;
     uint32_t row_lanes_log2 = 0;
     while ((1u << row_lanes_log2) < row_units) ++row_lanes_log2;
     // up to kMoveHere bytes of keys the workgroup that selected the rows moves them too, which saves the

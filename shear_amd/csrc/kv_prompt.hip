@@ -93,17 +93,18 @@ __device__ __forceinline__ bool special_half(uint32_t x) {
 // Rows of a tile: at 256 dims of 16-bit rows half as many, for the registers' sake.  (Two
 // prompts of 4,096 tokens, 16 heads over 4 of 256: 549 us, with 64 rows and spills 1,390;
 // SQ8 609 with 64 rows, 742 with 32.)
-template <bool kSq8, int DP>
+template <int kRowsKind, int DP>
 constexpr uint32_t prompt_rows() {
-    return DP == 256 && !kSq8 ? 32u : 64u;
+    return DP == 256 && kRowsKind == kRowsPlain ? 32u : 64u;
 }
 
-template <bool kSq8, int DP>
+template <int kRowsKind, int DP>
 struct PromptLds {
-    static constexpr uint32_t kRows = prompt_rows<kSq8, DP>();
+    static constexpr uint32_t kRows = prompt_rows<kRowsKind, DP>();
+    static constexpr bool kCodes = kRowsKind != kRowsPlain;
     alignas(16) char k[2][kRows * DP * 2];
     alignas(16) char v[2][kRows * DP * 2];
-    alignas(16) float scale[kSq8 ? 2 : 1][2][kSq8 ? kRows : 4];  // of keys (a logit's factor) and values
+    alignas(16) float scale[kCodes ? 2 : 1][2][kCodes ? kRows : 4];  // of keys (a logit's factor) and values
     // of tile i at i % 4: whether a value was replaced, and the rows without a page.
     // Cleared two tiles ahead, when nothing reads or sets them.
     uint32_t marks[4][1 + kRows / 32];
@@ -116,21 +117,27 @@ __device__ __attribute__((aligned(16))) const uint32_t kv_zeros[4] = {0, 0, 0, 0
 // that addresses are one scalar and a lane's constant; chosen where page_rows
 // is at least kRowsPer.  (The prompts above: 208 us, with an address of each lane's own 233, before
 // the later steps.)
-template <typename T, bool kSq8, int DP, bool kWhole>
+template <typename T, int kRowsKind, int DP, bool kWhole>
 __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(KvAttendParams p, uint32_t query_tiles) {
     using E = KvElem<T>;
-    using P = KvElem<std::conditional_t<kSq8, __bf16, T>>;  // of the weights and the values
-    constexpr bool kTwoParts = kSq8 && !std::is_same_v<T, __bf16>;
-    constexpr bool kHalf = !kSq8 && std::is_same_v<T, _Float16>;  // fp16 weights
+    constexpr bool kSq8 = kRowsKind == kRowsSq8, kMx4 = kRowsKind == kRowsMx4, kCodes = kSq8 || kMx4;
+    using V = std::conditional_t<kCodes, __bf16, T>;  // type of the weights and the values
+    using P = KvElem<V>;
+    constexpr bool kTwoParts = kCodes && !std::is_same_v<T, __bf16>;
+    constexpr bool kHalf = !kCodes && std::is_same_v<T, _Float16>;  // fp16 weights
+    // logits get a factor of their row: an SQ8 row's scale, the largest scale of an MX4 row where keys are fp16
+    constexpr bool kRowScale = kSq8 || (kMx4 && !std::is_same_v<T, __bf16>);
     // (32 alike rows at the lift sum to 2^5 times it, below the top)
     constexpr float kLift = kv_lift(kHalf, true), kTop = kv_top(kHalf), kMost = kHalf ? 32768.0f : 1.0f;  // kMost = 2^kTop
-    using Lds = PromptLds<kSq8, DP>;
+    using Lds = PromptLds<kRowsKind, DP>;
     constexpr uint32_t kRows = Lds::kRows;
     constexpr int kSubs = (int)kRows / 32;       // 32 rows of logits each
     constexpr int kSteps = DP / 16;              // instructions along the dims
     constexpr int kBlocks = DP / 32;             // blocks of 32 dims of the output
-    constexpr uint32_t kPieces = kSq8 ? DP / 16 : DP / 8;  // 16-byte pieces of a row in memory
-    constexpr int kLoads = (int)(kRows * kPieces) / kThreads;  // of a thread, for K and for V each
+    constexpr uint32_t kWide = kMx4 ? 32u : kSq8 ? 16u : 8u;  // dims of a 16-byte piece
+    constexpr uint32_t kPieces = DP / kWide;                  // of a row in memory
+    // loads of a thread, for K and for V each (MX4, 64 dims: of half of the threads)
+    constexpr int kLoads = kRows * kPieces < (uint32_t)kThreads ? 1 : (int)(kRows * kPieces) / kThreads;
     constexpr uint32_t kRowsPer = kThreads / kPieces;  // rows of one load of the workgroup
     extern __shared__ __align__(16) char smem[];
     Lds &lds = *reinterpret_cast<Lds *>(smem);
@@ -215,8 +222,9 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
     const uint32_t voffset = (load_row * c.values.row_units + v_piece<DP>(load_row, load_piece)) * 16u;
 
     int32_t pages[kLoads];
-    kv_u4 kr[kSq8 ? kLoads : 1], vr[kSq8 ? kLoads : 1];  // codes on their way to LDS
+    kv_u4 kr[kCodes ? kLoads : 1], vr[kCodes ? kLoads : 1];  // codes on their way to LDS
     float ks = 0.0f, vs = 1.0f;
+    uint32_t kb[kMx4 ? kLoads : 1], vb[kMx4 ? kLoads : 1];  // scale bytes of the pieces
     bool special = false;  // some value or scale was replaced
     // some maximum is so large that its rounding is felt (from 2^23 on it would be binades of a
     // weight): logits are then rounded as it was, before it is taken from them
@@ -269,18 +277,24 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
         for (int i = 0; i < kLoads; ++i) {
             const uint32_t r = (uint32_t)i * kRowsPer + load_row;
             const uint32_t row = r0 + r;
-            const bool there = row < length && (uint32_t)pages[i] < c.pages;
-            missing |= (uint32_t)(!there && row < length) << i;
+            const bool there = row < length && r < kRows && (uint32_t)pages[i] < c.pages;
+            missing |= (uint32_t)(!there && row < length && r < kRows) << i;
             const uint32_t slot = row & ((1u << c.page_shift) - 1u), page = (uint32_t)pages[i];
             const uint64_t kp = (uint64_t)(page * c.keys.page_units + slot * c.keys.row_units);
             const uint64_t vp = (uint64_t)(page * c.values.page_units + slot * c.values.row_units);
-            const uint32_t kpiece = kSq8 ? load_piece : k_piece<DP>(r, load_piece);
-            const uint32_t vpiece = kSq8 ? load_piece : v_piece<DP>(r, load_piece);
+            const uint32_t kpiece = kCodes ? load_piece : k_piece<DP>(r, load_piece);
+            const uint32_t vpiece = kCodes ? load_piece : v_piece<DP>(r, load_piece);
             const char *zeros = reinterpret_cast<const char *>(kv_zeros);
-            const uint32_t wide = kSq8 ? 16u : 8u;  // dims of a piece
-            const char *ksrc = there && kpiece * wide < c.dim ? kbase + (kp + kpiece) * 16u : zeros;
-            const char *vsrc = there && vpiece * wide < c.dim ? vbase + (vp + vpiece) * 16u : zeros;
-            if constexpr (kSq8) {
+            const char *ksrc = there && kpiece * kWide < c.dim ? kbase + (kp + kpiece) * 16u : zeros;
+            const char *vsrc = there && vpiece * kWide < c.dim ? vbase + (vp + vpiece) * 16u : zeros;
+            if constexpr (kMx4) {  // a piece is a group
+                kb[i] = vb[i] = 0u;
+                if (there && load_piece * kWide < c.dim) {
+                    kb[i] = kv_group_scales(c.keys)[kv_scale_place(c, c.keys, pages[i], row, h) + load_piece];
+                    vb[i] = kv_group_scales(c.values)[kv_scale_place(c, c.values, pages[i], row, h) + load_piece];
+                }
+            }
+            if constexpr (kCodes) {
                 kr[i] = *reinterpret_cast<const kv_u4 *>(ksrc);
                 vr[i] = *reinterpret_cast<const kv_u4 *>(vsrc);
             } else if constexpr (kWhole) {
@@ -308,8 +322,8 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                 ks = 0.0f;
                 vs = 1.0f;
                 if ((uint32_t)page < c.pages) {
-                    ks = c.keys.scales[kv_scale_place(c, c.keys, page, row, h)];
-                    vs = c.values.scales[kv_scale_place(c, c.values, page, row, h)];
+                    ks = kv_row_scales(c.keys)[kv_scale_place(c, c.keys, page, row, h)];
+                    vs = kv_row_scales(c.values)[kv_scale_place(c, c.values, page, row, h)];
                 }
             }
         }
@@ -317,7 +331,37 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
     // Completes a tile whose loads were started: codes become 16-bit values; in a
     // tile with a mask infinities and NaN become zeros.
     auto finish_rows = [&](uint32_t it, uint32_t buf) {
-        if constexpr (kSq8) {
+        if constexpr (kMx4) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const uint32_t r = (uint32_t)i * kRowsPer + load_row;
+                float kscale = kv_mx_scale(kb[i]);
+                if constexpr (kRowScale) {
+                    // fp16 holds no scale of any size: the row's largest goes to the logit, keys are
+                    // relative to it (below 2^-24 of it they vanish: 2^-26 of the row's largest value)
+                    uint32_t most = kb[i];
+#pragma unroll
+                    for (uint32_t off = 1; off < kPieces; off <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, (int)off));
+                    const bool nan = most == kMxNan;
+                    kscale = kv_mx_scale(nan ? 0x7fu : (uint32_t)max(127 - (int)(most - kb[i]), 0));
+                    if (load_piece == 0 && r < kRows)
+                        lds.scale[buf][0][r] = nan ? NAN : (most ? kv_mx_scale(most) : __uint_as_float(0x400000u)) * p.scale_log2;
+                }
+                // NaN would reach those that do not see the row as 0 * NaN
+                const bool bad = vb[i] == kMxNan && masked(tile_row(it));
+                if (bad) lds.marks[it & 3u][0] = 1u;
+                const float vscale = kv_mx_scale(bad ? 0x7fu : vb[i]);
+                if (r < kRows) {
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t to = 4u * load_piece + (uint32_t)w;
+                        *reinterpret_cast<kv_u4 *>(&lds.k[buf][r * DP * 2 + k_piece<DP>(r, to) * 16u]) = kv_mx_values<T>(kr[i][w], kscale);
+                        *reinterpret_cast<kv_u4 *>(&lds.v[buf][r * DP * 2 + v_piece<DP>(r, to) * 16u]) =
+                            kv_mx_values<V>(bad ? 0u : vr[i][w], vscale);
+                    }
+                }
+            }
+        } else if constexpr (kSq8) {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
                 const uint32_t r = (uint32_t)i * kRowsPer + load_row;
@@ -404,7 +448,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                     x[u] = E::mma32(a, qf[s], x[u]);
                 }
             }
-            if constexpr (kSq8) {
+            if constexpr (kRowScale) {
 #pragma unroll
                 for (int u = 0; u < kSubs; ++u)
 #pragma unroll
@@ -450,7 +494,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                         if (gone >> (8 * (e / 4) + e % 4) & 1u) x[u][e] = -INFINITY;
                 }
             }
-            float factor = kSq8 ? 1.0f : p.scale_log2;
+            float factor = kRowScale ? 1.0f : p.scale_log2;
             auto scale_first = [&] {
 #pragma unroll
                 for (int u = 0; u < kSubs; ++u)
@@ -458,7 +502,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                     for (int e = 0; e < 16; ++e) x[u][e] *= factor;
                 factor = 1.0f;
             };
-            if (!kSq8 && huge) scale_first();
+            if (!kRowScale && huge) scale_first();
             // The running maximum follows the largest logit.
             auto follow = [&] {
                 float top = x[0][0];
@@ -505,7 +549,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                     }
                 if (kSq8 || again || !__any(!(sum < kMost))) break;
                 follow();
-                if (!huge && __any(fabsf(m) >= kHuge && m > kKvNone)) {
+                if (!kRowScale && !huge && __any(fabsf(m) >= kHuge && m > kKvNone)) {
                     huge = true;
                     scale_first();
                 }
@@ -549,7 +593,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
     // values (SQ8: scales) that were replaced in tiles with a mask, for the queries that see their
     // rows; all tiles' where a sum became NaN under weights that are numbers
     bool lost = false;
-    if constexpr (!kSq8) {
+    if constexpr (!kCodes) {
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
@@ -562,7 +606,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
             return r <= pos && (!windowed || r < sinks || r > pos - window);
         };
 #pragma unroll
-        for (int i = 0; i < (kSq8 ? 1 : kBlocks); ++i) {
+        for (int i = 0; i < (kSq8 ? 1 : kBlocks); ++i) {  // (MX4: a block's dims are a group)
             float s[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = 0.0f;
@@ -578,9 +622,12 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                     const uint32_t place = kv_place(c, c.values, page, mine);
                     if constexpr (kSq8) {
                         if (place != kKvNoOffset) {
-                            const float scale = c.values.scales[kv_scale_place(c, c.values, page, mine, h)];
+                            const float scale = kv_row_scales(c.values)[kv_scale_place(c, c.values, page, mine, h)];
                             odd = scale != scale;
                         }
+                    } else if constexpr (kMx4) {
+                        if (place != kKvNoOffset && 32u * i < c.dim)
+                            odd = kv_group_scales(c.values)[kv_scale_place(c, c.values, page, mine, h) + i] == kMxNan;
                     } else {
 #pragma unroll 1
                         for (uint32_t d = 32u * i; d < min(32u * i + 32u, c.dim) && place != kKvNoOffset; d += 8) {
@@ -592,7 +639,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                 }
                 for (uint64_t rows = __ballot(odd); rows; rows &= rows - 1) {
                     const uint32_t row = r0 + (uint32_t)__builtin_ctzll(rows);
-                    if constexpr (kSq8) {
+                    if constexpr (kCodes) {
                         s[0] = seen(row) ? NAN : s[0];
                     } else {
                         const uint64_t place = kv_place(c, c.values, table[row >> c.page_shift], row);
@@ -613,6 +660,8 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
             if constexpr (kSq8) {
 #pragma unroll
                 for (int j = 0; j < kBlocks; ++j) acc[j] += s[0];
+            } else if constexpr (kMx4) {
+                acc[i] += s[0];
             } else if (l == l) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[i][e] = kv_settled(acc[i][e], s[e]);
@@ -652,32 +701,41 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
     if (half == 0) p.lse[query] = kv_lse(m, l, kLift);
 }
 
-template <typename T, bool kSq8, int DP, bool kWhole>
+template <typename T, int kRowsKind, int DP, bool kWhole>
 int launch(const KvAttendParams &p, hipStream_t stream) {
     const uint32_t tiles = (uint32_t)(((uint64_t)p.max_new * p.group + kQueries - 1) / kQueries);
-    const int lds = (int)sizeof(PromptLds<kSq8, DP>);
-    auto *kernel = &kv_prompt_kernel<T, kSq8, DP, kWhole>;
+    const int lds = (int)sizeof(PromptLds<kRowsKind, DP>);
+    auto *kernel = &kv_prompt_kernel<T, kRowsKind, DP, kWhole>;
     if (ensure_lds_limit(reinterpret_cast<const void *>(kernel), lds) != 0) return -1;
     kernel<<<tiles * p.chunks * p.c.heads * p.c.batch, kThreads, lds, stream>>>(p, tiles);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
-template <typename T, bool kSq8, int DP>
+template <typename T, int kRowsKind, int DP>
 int launch_pages(const KvAttendParams &p, hipStream_t stream) {
-    if constexpr (!kSq8)
+    if constexpr (kRowsKind == kRowsPlain)
         // (a tile's rows within 2^30 bytes: their offsets are 32-bit)
         if (p.c.dim == DP && (1u << p.c.page_shift) >= kThreads * 8u / DP && p.c.keys.row_units <= 1u << 20 &&
             p.c.values.row_units <= 1u << 20)
-            return launch<T, kSq8, DP, true>(p, stream);
-    return launch<T, kSq8, DP, false>(p, stream);
+            return launch<T, kRowsKind, DP, true>(p, stream);
+    return launch<T, kRowsKind, DP, false>(p, stream);
 }
 
-template <typename T, bool kSq8>
+template <typename T, int kRowsKind>
 int launch_dim(const KvAttendParams &p, hipStream_t stream) {
     switch (kv_padded_dim(p.c.dim)) {
-        case 64: return launch_pages<T, kSq8, 64>(p, stream);
-        case 128: return launch_pages<T, kSq8, 128>(p, stream);
-        default: return launch_pages<T, kSq8, 256>(p, stream);
+        case 64: return launch_pages<T, kRowsKind, 64>(p, stream);
+        case 128: return launch_pages<T, kRowsKind, 128>(p, stream);
+        default: return launch_pages<T, kRowsKind, 256>(p, stream);
+    }
+}
+
+template <typename T>
+int launch_rows(const KvAttendParams &p, KvRows rows, hipStream_t stream) {
+    switch (rows) {
+        case kRowsPlain: return launch_dim<T, kRowsPlain>(p, stream);
+        case kRowsSq8: return launch_dim<T, kRowsSq8>(p, stream);
+        default: return launch_dim<T, kRowsMx4>(p, stream);
     }
 }
 
@@ -706,10 +764,9 @@ void kv_prompt_split(KvAttendParams &p) {
     p.chunks = chunks > 1 && rows / (float)chunks + (float)chunks * part + kJoinCost < rows ? (uint32_t)chunks : 1u;
 }
 
-int launch_kv_prompt(const KvAttendParams &p, uint32_t type, bool sq8, hipStream_t stream) {
+int launch_kv_prompt(const KvAttendParams &p, uint32_t type, KvRows rows, hipStream_t stream) {
     if (p.tokens == 0 || p.max_new == 0 || p.c.batch == 0) return 0;
-    if (type == kKvBf16) return sq8 ? launch_dim<__bf16, true>(p, stream) : launch_dim<__bf16, false>(p, stream);
-    return sq8 ? launch_dim<_Float16, true>(p, stream) : launch_dim<_Float16, false>(p, stream);
+    return type == kKvBf16 ? launch_rows<__bf16>(p, rows, stream) : launch_rows<_Float16>(p, rows, stream);
 }
 
 }  // namespace tessa

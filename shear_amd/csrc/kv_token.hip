@@ -175,19 +175,26 @@ __device__ __forceinline__ void find_sequence(const KvAttendParams &p, uint64_t 
 
 // kDirect: one workgroup for each column of rows, which writes the result; else
 // workers and parts.
-template <typename T, bool kSq8, int DP, bool kDirect>
+template <typename T, int kRowsKind, int DP, bool kDirect>
 __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(KvAttendParams p) {
+    constexpr bool kSq8 = kRowsKind == kRowsSq8, kMx4 = kRowsKind == kRowsMx4;
     using E = KvElem<T>;
-    using P = KvElem<std::conditional_t<kSq8, __bf16, T>>;  // of the weights and the values
-    constexpr bool kHalf = !kSq8 && std::is_same_v<T, _Float16>;  // fp16 weights
+    using K = KvElem<std::conditional_t<kMx4, __bf16, T>>;  // of the logits' products
+    using P = KvElem<std::conditional_t<kSq8 || kMx4, __bf16, T>>;  // of the weights and the values
+    constexpr bool kHalf = !kSq8 && !kMx4 && std::is_same_v<T, _Float16>;  // fp16 weights
+    constexpr int kQueryParts = kMx4 && std::is_same_v<T, _Float16> ? 2 : 1;  // bf16 parts of an fp16 query, exactly
     constexpr float kLift = kv_lift(kHalf, false), kTop = kv_top(kHalf), kRest = kHalf ? 4096.0f : 1.0f;
     constexpr int kSteps = DP / 32;                 // matrix instructions of 16 logits
     constexpr int kPer = DP / 16;                   // values of a row that a lane holds
-    constexpr int kKWords = kSq8 ? DP / 16 : DP / 8;  // words of a K row that a lane holds
-    constexpr int kVWords = kSq8 ? kPer / 4 : kPer / 2;
-    constexpr int kKLoads = kKWords / 4;
+    constexpr int kKWords = kMx4 ? DP / 32 : kSq8 ? DP / 16 : DP / 8;  // words of a K row that a lane holds
+    constexpr int kVWords = kMx4 ? (kPer + 7) / 8 : kSq8 ? kPer / 4 : kPer / 2;
+    constexpr int kKLoad = kKWords < 4 ? kKWords : 4;  // words of one load
+    constexpr int kKLoads = kKWords / kKLoad;
+    constexpr uint32_t kKDims = DP / 4 / kKLoads;      // dims of a lane's load, which four lanes share out
+    constexpr int kMxGroups = DP / (int)kMxGroup;
     __shared__ __align__(16) uint32_t sh_place[kWaves][2][kTile];  // (read four at a time)
     __shared__ __align__(16) float sh_scale[kSq8 ? kWaves : 1][2][kTile];
+    __shared__ __align__(16) float sh_group[kMx4 ? kWaves : 1][2][kMx4 ? kMxGroups : 1][kTile];  // scales of 32 dims
     __shared__ float sh_ml[kWaves][2][16];
     extern __shared__ __align__(16) float sh_out[];  // [waves][heads of the block][DP]
 
@@ -267,16 +274,24 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
     // 32 heads over 2 of 256 dims: 72 us, in registers with spills 77, bf16 65)
     constexpr bool kQueryInLds = kHalf && DP == 256;
     __shared__ kv_u4 sh_q[kQueryInLds ? kSteps : 1][64];
-    kv_u4 qf[kQueryInLds ? 1 : kSteps];
+    kv_u4 qf[kQueryParts][kQueryInLds ? 1 : kSteps];
     {
         const char *q = p.q + (uint64_t)b * p.q_token + (uint64_t)(h * p.group + first_q + (head_ok ? n : 0u)) * p.q_head;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            const uint32_t d = kSq8 ? (uint32_t)(s / 2) * 64u + g * 16u + (uint32_t)(s & 1) * 8u : (uint32_t)s * 32u + g * 8u;
+            constexpr int kHere = kMx4 ? kKWords / kKLoads : kSq8 ? 2 : 1;  // steps of a load
+            const uint32_t d = (uint32_t)(s / kHere) * 4u * kKDims + g * kKDims + (uint32_t)(s % kHere) * 8u;
             const kv_u4 zero = {0, 0, 0, 0};
             const kv_u4 x = head_ok && d < c.dim ? *reinterpret_cast<const kv_u4 *>(q + 2u * d) : zero;
-            if constexpr (!kQueryInLds)
-                qf[s] = x;
+            if constexpr (kQueryParts == 2) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float lo = E::low(x[e]), hi = E::high(x[e]);
+                    qf[0][s][e] = K::pack(lo, hi);
+                    qf[1][s][e] = K::pack(lo - K::low(qf[0][s][e]), hi - K::high(qf[0][s][e]));
+                }
+            } else if constexpr (!kQueryInLds)
+                qf[0][s] = x;
             else if (wave == 0)
                 sh_q[s][lane] = x;
         }
@@ -285,7 +300,8 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
     const char *kbase = c.keys.rows + (uint64_t)h * c.keys.head_units * 16u;
     const char *vbase = c.values.rows + (uint64_t)h * c.values.head_units * 16u;
     // byte of the lane's values in a row (lanes past the row repeat its start; their outputs are not stored)
-    const uint32_t vbyte = (n * kPer < c.dim ? n * kPer : 0u) * (kSq8 ? 1u : 2u);
+    const uint32_t vdim = n * kPer < c.dim ? n * kPer : 0u;
+    const uint32_t vbyte = kMx4 ? vdim / 2u : kSq8 ? vdim : 2u * vdim;
 
     float m = kKvNone, l = 0.0f;
     kv_f4 acc[kPer], rest[kHalf ? kPer : 1];
@@ -315,7 +331,36 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
         float scale = lane < kTile ? 0.0f : 1.0f;
         if constexpr (kSq8) {
             const KvArray &array = lane < kTile ? c.keys : c.values;
-            if (mine) scale = array.scales[kv_scale_place(c, array, page, (uint32_t)row, h)];
+            if (mine) scale = kv_row_scales(array)[kv_scale_place(c, array, page, (uint32_t)row, h)];
+        }
+        // MX4: a byte of each group, of the same rows by the same lanes (1 where there is no row: 0 * NaN would be NaN)
+        uint32_t bytes[kMx4 ? (kMxGroups + 3) / 4 : 1];
+        if constexpr (kMx4) {
+            const KvArray &array = lane < kTile ? c.keys : c.values;
+            const uint8_t *at = kv_group_scales(array);
+#pragma unroll
+            for (int w = 0; w < (kMxGroups + 3) / 4; ++w) bytes[w] = 0x7f7f7f7fu;
+            if (mine) {
+                at += kv_scale_place(c, array, page, (uint32_t)row, h);
+                if (c.scales_together) {  // as one word
+                    if constexpr (DP == 64) bytes[0] = *reinterpret_cast<const uint16_t *>(at);
+                    if constexpr (DP == 128) bytes[0] = *reinterpret_cast<const uint32_t *>(at);
+                    if constexpr (DP == 256) {
+                        const kv_u2 both = *reinterpret_cast<const kv_u2 *>(at);
+                        bytes[0] = both[0];
+                        bytes[kMxGroups / 4 - 1] = both[1];
+                    }
+                } else {
+#pragma unroll
+                    for (int w = 0; w < (kMxGroups + 3) / 4; ++w) {
+                        uint32_t x = 0;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (4 * w + i < kMxGroups) x |= (uint32_t)at[kMxGroup * (4 * w + i) < c.dim ? 4 * w + i : 0] << (8 * i);
+                        bytes[w] = x;
+                    }
+                }
+            }
         }
         sh_place[wave][lane >> 5][l32] = mine ? (lane < kTile ? kplace : vplace) : 0u;  // row 0 of page 0 is there to read
         kv_wave_sync();
@@ -324,14 +369,14 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
         next_row = row_of(tile + 2 * kWaves);
 
         // K: rows n and 16 + n
-        KvWords<4> kw[2][kKLoads];
+        KvWords<kKLoad> kw[2][kKLoads];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const char *src = kbase + (uint64_t)sh_place[wave][0][16 * t + n] * 16u;
 #pragma unroll
             for (int s = 0; s < kKLoads; ++s) {
-                const uint32_t d = kSq8 ? (uint32_t)s * 64u + g * 16u : (uint32_t)s * 32u + g * 8u;
-                kw[t][s] = *reinterpret_cast<const KvWords<4> *>(src + (d < c.dim ? d : 0u) * (kSq8 ? 1u : 2u));
+                const uint32_t d = (uint32_t)s * 4u * kKDims + g * kKDims, there = d < c.dim ? d : 0u;
+                kw[t][s] = *reinterpret_cast<const KvWords<kKLoad> *>(src + (kMx4 ? there / 2u : kSq8 ? there : 2u * there));
             }
         }
         // V: rows 16 (j / 4) + 4 g + j % 4
@@ -340,21 +385,32 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
         for (int t = 0; t < 2; ++t) {
             const kv_u4 place = *reinterpret_cast<const kv_u4 *>(&sh_place[wave][1][16 * t + 4 * g]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                vw[4 * t + j] = *reinterpret_cast<const KvWords<kVWords> *>(vbase + (uint64_t)place[j] * 16u + vbyte);
+            for (int j = 0; j < 4; ++j) {
+                const char *src = vbase + (uint64_t)place[j] * 16u + vbyte;
+                if constexpr (kMx4 && kPer == 4)
+                    vw[4 * t + j].w[0] = *reinterpret_cast<const uint16_t *>(src);
+                else
+                    vw[4 * t + j] = *reinterpret_cast<const KvWords<kVWords> *>(src);
+            }
+        }
+        if constexpr (kMx4) {
+#pragma unroll
+            for (int i = 0; i < kMxGroups; ++i)
+                sh_group[wave][lane >> 5][i][l32] = kv_mx_scale(bytes[i / 4] >> (8 * (i & 3)) & 255u);
+            kv_wave_sync();
         }
         if constexpr (kSq8) {
             sh_scale[wave][lane >> 5][l32] = lane < kTile ? scale * p.scale_log2 : scale;
             kv_wave_sync();
         }
-        if (DP != c.dim) {  // dims past the row meet zeros of Q and must be finite
+        if (!kMx4 && DP != c.dim) {  // (codes of 4 bits are) dims past the row meet zeros of Q and must be finite
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int s = 0; s < kKLoads; ++s) {
-                    const uint32_t d = kSq8 ? (uint32_t)s * 64u + g * 16u : (uint32_t)s * 32u + g * 8u;
+                    const uint32_t d = (uint32_t)s * 4u * kKDims + g * kKDims;
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) kw[t][s].w[w] = d < c.dim ? kw[t][s].w[w] : 0u;
+                    for (int w = 0; w < kKLoad; ++w) kw[t][s].w[w] = d < c.dim ? kw[t][s].w[w] : 0u;
                 }
         }
         // logits of rows 16 t + 4 g + i
@@ -365,7 +421,10 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 kv_u4 a;
-                if constexpr (kSq8) {
+                if constexpr (kMx4) {
+                    const uint32_t d = (uint32_t)(s / kKLoad) * 4u * kKDims + g * kKDims;
+                    a = kv_mx_values<__bf16>(kw[t][s / kKLoad].w[s % kKLoad], sh_group[wave][0][d / kMxGroup][16 * t + n]);
+                } else if constexpr (kSq8) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const uint32_t word = kw[t][s / 2].w[2 * (s & 1) + e / 2];
@@ -375,7 +434,8 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
 #pragma unroll
                     for (int e = 0; e < 4; ++e) a[e] = kw[t][s].w[e];
                 }
-                sacc = E::mma16(a, kQueryInLds ? sh_q[kQueryInLds ? s : 0][lane] : qf[kQueryInLds ? 0 : s], sacc);
+                sacc = K::mma16(a, kQueryInLds ? sh_q[kQueryInLds ? s : 0][lane] : qf[0][kQueryInLds ? 0 : s], sacc);
+                if constexpr (kQueryParts == 2) sacc = K::mma16(a, qf[1][s], sacc);
             }
             if constexpr (kSq8) {
                 const kv_f4 ks = *reinterpret_cast<const kv_f4 *>(&sh_scale[wave][0][16 * t + 4 * g]);
@@ -445,8 +505,31 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
                 if constexpr (!kHalf) least[2 * t + i / 2] = P::pack(r0 - P::low(y), r1 - P::high(y));
             }
         }
+        if constexpr (kMx4) {
+            // two dims at a time: each row's pair of codes in one conversion, then rows beside each other
+            float vs[8];
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
+            for (int t = 0; t < 2; ++t) {
+                const kv_f4 s4 = *reinterpret_cast<const kv_f4 *>(&sh_group[wave][1][vdim / kMxGroup][16 * t + 4 * g]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) vs[4 * t + i] = s4[i];
+            }
+            kv_each<kPer / 2>([&](auto at) {
+                constexpr int e = 2 * decltype(at)::value;
+                kv_u4 a0, a1;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t x = P::template from_mx4<(e % 8) / 2>(vw[2 * j].w[e / 8], vs[2 * j]);
+                    const uint32_t y = P::template from_mx4<(e % 8) / 2>(vw[2 * j + 1].w[e / 8], vs[2 * j + 1]);
+                    a0[j] = __builtin_amdgcn_perm(y, x, 0x05040100u);
+                    a1[j] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+                }
+                acc[e] = P::mma16(a0, least, P::mma16(a0, lo, P::mma16(a0, hi, acc[e])));
+                acc[e + 1] = P::mma16(a1, least, P::mma16(a1, lo, P::mma16(a1, hi, acc[e + 1])));
+            });
+        }
+#pragma unroll
+        for (int e = 0; e < (kMx4 ? 0 : kPer); ++e) {
             kv_u4 a;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -501,7 +584,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
         }
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) sum += sh_ml[w][1][head] * kv_exp2(sh_ml[w][0][head] - big);
-        if constexpr (!kSq8) {
+        if constexpr (kRowsKind == kRowsPlain) {
             if (kv_nan(o) && sum == sum && d < c.dim) {  // values that are not finite, under weights that are
                 kv_f4 s = {0, 0, 0, 0};
                 for (uint32_t i = begin; i < end; ++i) {
@@ -764,22 +847,31 @@ __global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, u
     }
 }
 
-template <typename T, bool kSq8, int DP>
+template <typename T, int kRowsKind, int DP>
 int launch(const KvAttendParams &p, hipStream_t stream) {
     const size_t lds = (size_t)kWaves * (p.group < 16u ? p.group : 16u) * DP * sizeof(float);
-    auto *kernel = p.workers ? &kv_token_kernel<T, kSq8, DP, false> : &kv_token_kernel<T, kSq8, DP, true>;
+    auto *kernel = p.workers ? &kv_token_kernel<T, kRowsKind, DP, false> : &kv_token_kernel<T, kRowsKind, DP, true>;
     // 16 heads of 256 dims are 64 KiB, beside up to 10 KiB that the kernel has anyway: above the default limit
     if (lds > 32768 && ensure_lds_limit(reinterpret_cast<const void *>(kernel), (int)lds) != 0) return -1;
     kernel<<<p.workers ? dim3(p.workers) : dim3(p.columns, p.c.batch), kThreads, lds, stream>>>(p);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
-template <typename T, bool kSq8>
+template <typename T, int kRowsKind>
 int launch_dim(const KvAttendParams &p, hipStream_t stream) {
     switch (kv_padded_dim(p.c.dim)) {
-        case 64: return launch<T, kSq8, 64>(p, stream);
-        case 128: return launch<T, kSq8, 128>(p, stream);
-        default: return launch<T, kSq8, 256>(p, stream);
+        case 64: return launch<T, kRowsKind, 64>(p, stream);
+        case 128: return launch<T, kRowsKind, 128>(p, stream);
+        default: return launch<T, kRowsKind, 256>(p, stream);
+    }
+}
+
+template <typename T>
+int launch_rows(const KvAttendParams &p, KvRows rows, hipStream_t stream) {
+    switch (rows) {
+        case kRowsPlain: return launch_dim<T, kRowsPlain>(p, stream);
+        case kRowsSq8: return launch_dim<T, kRowsSq8>(p, stream);
+        default: return launch_dim<T, kRowsMx4>(p, stream);
     }
 }
 
@@ -810,14 +902,13 @@ void kv_token_split(KvAttendParams &p) {
     if (!p.workers) p.workers = 1;
 }
 
-int launch_kv_token(const KvAttendParams &p, uint32_t type, bool sq8, hipStream_t stream) {
-    if (type == kKvBf16) return sq8 ? launch_dim<__bf16, true>(p, stream) : launch_dim<__bf16, false>(p, stream);
-    return sq8 ? launch_dim<_Float16, true>(p, stream) : launch_dim<_Float16, false>(p, stream);
+int launch_kv_token(const KvAttendParams &p, uint32_t type, KvRows rows, hipStream_t stream) {
+    return type == kKvBf16 ? launch_rows<__bf16>(p, rows, stream) : launch_rows<_Float16>(p, rows, stream);
 }
 
-int launch_kv_finish(const KvAttendParams &params, uint32_t type, bool sq8, bool prompt, hipStream_t stream) {
+int launch_kv_finish(const KvAttendParams &params, uint32_t type, KvRows rows, bool prompt, hipStream_t stream) {
     KvAttendParams p = params;
-    p.lift = kv_lift(!sq8 && type == kKvF16, prompt);
+    p.lift = kv_lift(rows == kRowsPlain && type == kKvF16, prompt);
     const uint64_t queries = p.tokens * p.q_heads;
     const uint32_t dp = kv_padded_dim(p.c.dim);
     uint32_t dims = dp;

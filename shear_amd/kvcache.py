@@ -3,10 +3,16 @@ finds, and eviction by attention weight.
 
 A ``KvCache`` holds keys and values in pages of ``page_rows`` rows; a page table
 (int32 [batch, columns]) names the pages of each sequence, ``lengths`` (int32
-[batch]) its rows.  Rows are bf16, fp16, or SQ8 (int8 codes with one f32 scale
-max|x| * (1/127), symmetric by row like ``tessa.quantize_sq_int8_matrix``).
+[batch]) its rows.  Rows are bf16, fp16, SQ8 (int8 codes with one f32 scale
+max|x| * (1/127), symmetric by row like ``tessa.quantize_sq_int8_matrix``), or MX4
+(4-bit floating point codes, two to a byte, with a power of two for each 32 dims).
 
+* ``plan``           which pages a step's new rows go to and which come back; the
+                     position, sequence and place (slot) of each token
 * ``append``         new keys and values into the pages
+* ``append_rotated`` the same by slot, with the norm of queries and keys for each head
+                     and their rotation by position on the way
+* ``read``           rows by slot, as values
 * ``attend_prompt``  causal attention of the new tokens of each sequence, over all
                      rows or the first ``sinks`` and the last ``window``
 * ``attend_token``   attention of one new token for each sequence; ``listed``
@@ -31,21 +37,26 @@ import torch
 from . import _native as N
 
 _QUERY_TYPES = {torch.bfloat16: N.KV_BF16, torch.float16: N.KV_F16}
-_TYPES = {torch.bfloat16: N.KV_BF16, torch.float16: N.KV_F16, torch.int8: N.KV_SQ8}
+MX4 = torch.float4_e2m1fn_x2  # a cache's type: two 4-bit codes in each element
+_SCALE = torch.float8_e8m0fnu  # of 32 dims of an MX4 row: a power of two
+_TYPES = {torch.bfloat16: N.KV_BF16, torch.float16: N.KV_F16, torch.int8: N.KV_SQ8, MX4: N.KV_MX4}
+_VALUE_TYPES = {**_QUERY_TYPES, torch.float32: N.KV_F32}
 _INT = torch.int32
 _MOST_ROWS = 2**30 - 1  # of a sequence, whatever its table covers
 
 
-def _strides(t: torch.Tensor, count: int):
-    return (C.c_uint64 * count)(*t.stride()[:count])
+def _strides(t: torch.Tensor, count: int, each: int = 1):
+    return (C.c_uint64 * count)(*(each * s for s in t.stride()[:count]))
 
 
 @dataclass(frozen=True, eq=False)
 class KvCache:
     """Pages of keys and values: [pages, heads, page_rows, head_dim] each, in
     any order of the first three dimensions (rows contiguous, 16-byte aligned);
-    SQ8 caches carry f32 scales [pages, heads, page_rows].  A cache keeps the
-    tensors that it was made of."""
+    SQ8 caches carry f32 scales [pages, heads, page_rows].  MX4 caches have elements
+    of two dims, [pages, heads, page_rows, head_dim / 2] (the even dim in the low bits; head_dim
+    a multiple of 32), and carry float8_e8m0fnu scales [pages, heads, page_rows, head_dim / 32].
+    A cache keeps the tensors that it was made of."""
 
     keys: torch.Tensor
     values: torch.Tensor
@@ -57,29 +68,41 @@ class KvCache:
     def __post_init__(self):
         k, v = self.keys, self.values
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _TYPES:
-            raise ValueError("keys and values must be bf16, fp16 or int8 [pages, heads, page_rows, head_dim], alike")
+            raise ValueError("keys and values must be bf16, fp16, int8 or float4_e2m1fn_x2 [pages, heads, page_rows, "
+                             "head_dim], alike")
         if not k.is_cuda or k.device != v.device:
             raise ValueError("keys and values must be device tensors on one device")
         if k.stride(3) != 1 or v.stride(3) != 1:
             raise ValueError("rows must be contiguous")
+        each = 2 if k.dtype == MX4 else 1  # dims of an element
         n = N.KvCache(type=_TYPES[k.dtype], pages=k.shape[0], heads=k.shape[1], page_rows=k.shape[2],
-                      head_dim=k.shape[3], keys=k.data_ptr(), values=v.data_ptr(), key_strides=_strides(k, 3),
-                      value_strides=_strides(v, 3))
-        if k.dtype == torch.int8:
+                      head_dim=each * k.shape[3], keys=k.data_ptr(), values=v.data_ptr(),
+                      key_strides=_strides(k, 3, each), value_strides=_strides(v, 3, each))
+        if k.dtype in (torch.int8, MX4):
+            kind, name = (_SCALE, "MX4") if k.dtype == MX4 else (torch.float32, "SQ8")
+            shape = (*k.shape[:3], n.head_dim // 32) if k.dtype == MX4 else k.shape[:3]
             for s in (self.key_scales, self.value_scales):
-                if s is None or s.dtype != torch.float32 or s.shape != k.shape[:3] or s.device != k.device:
-                    raise ValueError("an SQ8 cache needs f32 scales [pages, heads, page_rows]")
+                if s is None or s.dtype != kind or s.shape != shape or s.device != k.device:
+                    raise ValueError(f"an {name} cache needs {kind} scales [pages, heads, page_rows"
+                                     + (", head_dim / 32]" if k.dtype == MX4 else "]"))
+                if k.dtype == MX4 and shape[3] > 1 and s.stride(3) != 1:
+                    raise ValueError("a row's scales must be contiguous")
             n.key_scales, n.value_scales = self.key_scales.data_ptr(), self.value_scales.data_ptr()
             n.key_scale_strides, n.value_scale_strides = _strides(self.key_scales, 3), _strides(self.value_scales, 3)
         elif self.key_scales is not None or self.value_scales is not None:
-            raise ValueError("only an SQ8 cache has scales")
+            raise ValueError("only SQ8 and MX4 caches have scales")
         object.__setattr__(self, "_native", n)
 
     @classmethod
     def allocate(cls, pages: int, heads: int, page_rows: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
                  device: str | torch.device = "cuda") -> "KvCache":
-        shape = (pages, heads, page_rows, head_dim)
+        if dtype == MX4 and head_dim % 32:
+            raise ValueError(f"head_dim {head_dim} of an MX4 cache is not a multiple of 32")
+        shape = (pages, heads, page_rows, head_dim // 2 if dtype == MX4 else head_dim)
         keys, values = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
+        if dtype == MX4:
+            return cls(keys, values, *(torch.empty((*shape[:3], head_dim // 32), dtype=_SCALE, device=device)
+                                       for _ in range(2)))
         if dtype != torch.int8:
             return cls(keys, values)
         return cls(keys, values, *(torch.empty(shape[:3], dtype=torch.float32, device=device) for _ in range(2)))
@@ -90,7 +113,7 @@ class KvCache:
 
     @property
     def head_dim(self) -> int:
-        return int(self.keys.shape[3])
+        return int(self._native.head_dim)
 
     @property
     def heads(self) -> int:
@@ -111,7 +134,7 @@ def _check(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device)
         raise ValueError(f"{name} must be {dtype} [{want}], got {t.dtype} {list(got)}")
     if t.get_device() != device.index:
         raise ValueError(f"{name} must be on {device}, not {t.device}")
-    if got[-1] > 1 and t.stride(-1) != 1:
+    if got[-1] > 1 and t.stride(-1) != 1 and t.numel():
         raise ValueError(f"the last dimension of {name} must be contiguous")
 
 
@@ -179,7 +202,7 @@ def append(cache: KvCache, page_table: torch.Tensor, starts: torch.Tensor, k: to
     _no_gradient(cache, k, v)
     seq = _sequences(cache, page_table, starts, None)
     dtype = cache.keys.dtype
-    if dtype == torch.int8:
+    if dtype in (torch.int8, MX4):
         dtype = k.dtype if k.dtype in _QUERY_TYPES else torch.bfloat16
     tokens = k.shape[0] if k.dim() else 0
     shape = (tokens, native.heads, native.head_dim)
@@ -210,7 +233,7 @@ def _attend(cache, q, page_table, lengths, max_length, scale, sinks, window, str
     kind = _QUERY_TYPES.get(q.dtype)
     if q.dim() != 3 or kind is None or q.device != dev:
         raise ValueError(f"q must be bf16 or fp16 [tokens, q_heads, head_dim] on {dev}")
-    if kind != native.type != N.KV_SQ8:
+    if kind != native.type and native.type not in (N.KV_SQ8, N.KV_MX4):
         raise ValueError(f"q is {q.dtype}, the cache {cache.keys.dtype}")
     tokens, heads, dim = q.shape
     if dim != native.head_dim or heads == 0 or heads % native.heads:
@@ -333,3 +356,148 @@ def evict(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tensor, weigh
                          0 if into is None else into.shape[1], rows, keep, sinks, recent, 0)
         N.check(N.load().tessa_kv_evict(C.byref(cache._native), C.byref(seq), C.byref(e), handle), "kv evict")
     return kept, new_lengths, new_weights
+
+
+def rotation_frequencies(dims: int, base: float = 10000.0, device: str | torch.device = "cuda") -> torch.Tensor:
+    """f64 [dims / 2]: base^(-2i / dims) radians for each position, for ``append_rotated``."""
+    return base ** (-torch.arange(0, dims, 2, dtype=torch.float64, device=device) / dims)
+
+
+def _places(slots: torch.Tensor, count: int | None, device) -> None:
+    _check(slots, "slots", torch.int64, (count,), device)
+
+
+def append_rotated(cache: KvCache, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                   slots: torch.Tensor, frequencies: torch.Tensor | None = None, q_weight: torch.Tensor | None = None,
+                   k_weight: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False,
+                   stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """Queries, normalized and rotated, [tokens, q_heads, head_dim] in q's type; keys likewise, and values as they
+    are, become the cache's rows ``slots`` (int64 [tokens]: page * page_rows + row, as ``plan`` gives them; others than
+    the cache has are not written; no two tokens may have the same one).
+
+    ``q_weight``, ``k_weight`` ([head_dim], q's type or f32): x * rsqrt(mean x^2 + eps) * weight
+    for each head; None: no norm.  ``frequencies`` (f64 [r / 2], r a multiple of 16; None: no rotation): pair i of the first r dims
+    turns by positions (int32 [tokens]) * frequencies[i] radians, dims (i, i + r / 2) or, ``interleaved``,
+    (2i, 2i + 1).  All of it in f32 (angles in 64 bits) and rounded once, so that the rows are
+    what ``append`` makes of the rounded ones.  A token with a negative position is of no sequence:
+    its queries come back as zeros and nothing of it is written."""
+    dev, native = cache.keys.device, cache._native
+    _no_gradient(cache, k, v)
+    _no_gradient(cache, q)
+    kind = _QUERY_TYPES.get(q.dtype)
+    if q.dim() != 3 or kind is None or q.device != dev:
+        raise ValueError(f"q must be bf16 or fp16 [tokens, q_heads, head_dim] on {dev}")
+    if kind != native.type and native.type not in (N.KV_SQ8, N.KV_MX4):
+        raise ValueError(f"q is {q.dtype}, the cache {cache.keys.dtype}")
+    tokens, heads, dim = q.shape
+    if dim != native.head_dim or heads == 0:
+        raise ValueError(f"q of {heads} heads x {dim} for a cache of {cache.heads} heads x {cache.head_dim}")
+    shape = (tokens, native.heads, dim)
+    for t, name in ((k, "k"), (v, "v")):
+        if t.dtype != q.dtype or t.shape != shape or t.device != dev:
+            raise ValueError(f"{name} must be {q.dtype} {list(shape)} on {dev}")
+    _check(positions, "positions", _INT, (tokens,), dev)
+    _places(slots, tokens, dev)
+    rotated = 0
+    if frequencies is not None:
+        _check(frequencies, "frequencies", torch.float64, (None,), dev)
+        rotated = 2 * frequencies.shape[0]
+        if rotated % 16 or rotated > dim:
+            raise ValueError(f"{rotated} rotated dims must be a multiple of 16 up to {dim}")
+    weight_type = q.dtype
+    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w is not None:
+            weight_type = w.dtype if w.dtype == torch.float32 else q.dtype
+            _check(w, name, weight_type, (dim,), dev)
+            _no_gradient(cache, w)
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise ValueError(f"q_weight is {q_weight.dtype}, k_weight {k_weight.dtype}")
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError(f"eps {eps} must be finite and not negative")
+    on, handle = _on(stream, dev, (*cache._tensors(), q, k, v, positions, slots, frequencies, q_weight, k_weight))
+    with on:
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        weights = [w if w is None or w.data_ptr() % 16 == 0 else w.clone() for w in (q_weight, k_weight)]
+        out = torch.empty(tokens, heads, dim, dtype=q.dtype, device=dev)
+        a = N.KvRotated(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q.stride()[:2], k.stride()[:2],
+                        v.stride()[:2], (heads * dim, dim), positions.data_ptr(), slots.data_ptr(),
+                        None if frequencies is None else frequencies.data_ptr(),
+                        *(None if w is None else w.data_ptr() for w in weights), tokens, kind,
+                        _VALUE_TYPES[weight_type], heads, rotated, int(interleaved), eps)
+        N.check(N.load().tessa_kv_append_rotated(C.byref(native), C.byref(a), handle), "kv append rotated")
+    return out
+
+
+def read(cache: KvCache, slots: torch.Tensor, dtype: torch.dtype | None = None, values: bool = True,
+         stream: torch.cuda.Stream | None = None):
+    """(keys, values) [n, heads, head_dim] of the cache's rows ``slots`` (int64 [n]: page * page_rows + row), zeros
+    where the cache has no such row.  ``dtype``: bf16, fp16 or f32 (default: the cache's own, f32 for SQ8, bf16 for
+    MX4, which holds each of its values).  ``values`` False: keys only, and None."""
+    dev, native = cache.keys.device, cache._native
+    _no_gradient(cache, slots)
+    _places(slots, None, dev)
+    if dtype is None:
+        own = cache.keys.dtype
+        dtype = torch.float32 if own == torch.int8 else torch.bfloat16 if own == MX4 else own
+    if dtype not in _VALUE_TYPES:
+        raise ValueError(f"rows are read as bf16, fp16 or f32, not {dtype}")
+    on, handle = _on(stream, dev, (*cache._tensors(), slots))
+    with on:
+        shape = (slots.shape[0], native.heads, native.head_dim)
+        k = torch.empty(shape, dtype=dtype, device=dev)
+        v = torch.empty(shape, dtype=dtype, device=dev) if values else None
+        a = N.KvRows(slots.data_ptr(), k.data_ptr(), v.data_ptr() if values else None, shape[0], _VALUE_TYPES[dtype], 0)
+        N.check(N.load().tessa_kv_read(C.byref(native), C.byref(a), handle), "kv read")
+    return k, v
+
+
+@dataclass(frozen=True, eq=False)
+class Plan:
+    """What a step does with its tokens (``plan``)."""
+
+    lengths: torch.Tensor    # int32 [batch]: rows of each sequence after the step
+    held: torch.Tensor       # int32 [batch]: pages of its table row that are its own
+    count: torch.Tensor      # int32 [1]: free pages
+    granted: torch.Tensor    # int32 [batch]: new rows that it got, all of them or none
+    offsets: torch.Tensor    # int32 [batch + 1]: first token of each sequence
+    positions: torch.Tensor  # int32 [tokens]: row of each token in its sequence, -1 where it got none
+    sequences: torch.Tensor  # int32 [tokens], -1 past the last token
+    slots: torch.Tensor      # int64 [tokens]: page * page_rows + row, -1 where the token got none
+
+
+def plan(page_rows: int, page_table: torch.Tensor, lengths: torch.Tensor, held: torch.Tensor, new: torch.Tensor,
+         free: torch.Tensor, count: torch.Tensor, tokens: int, stream: torch.cuda.Stream | None = None) -> Plan:
+    """The pages and places of a step in which sequence b gets ``new[b]`` rows, or ends (negative).
+
+    Sequence b has ``lengths[b]`` rows in the first ``held[b]`` pages of its row of ``page_table`` (int32 [batch,
+    columns]); ``free`` (int32 [pages]) is a stack of ``count`` (int32 [1]) page ids that nobody holds.  ``tokens``:
+    places of the step's tokens, which lie sequence by sequence; what is past the last is padding.
+
+    In the order of the sequences, pages that one holds and needs no more (it ends, or was evicted from) go
+    to the stack, then each that needs more gets them from its top, if what all up to it need is there.
+    One that does not get its pages, or whose rows would pass the table's columns or tokens ``tokens``, is
+    granted nothing: its tokens' places are -1 and its length stays (a prompt's attention of such tokens says
+    nothing).  The table and the stack are changed in place; the lengths, held pages and count that go with them are
+    the result's, and take the arguments' place in the next step."""
+    dev = lengths.device
+    if not lengths.is_cuda:
+        raise ValueError("lengths must be a device tensor")
+    if not 0 < page_rows <= 65536 or page_rows & (page_rows - 1):
+        raise ValueError(f"page_rows must be a power of two in 1..65536, got {page_rows}")
+    if not 0 <= tokens < 2**31:
+        raise ValueError(f"tokens {tokens} is outside 0..2^31 - 1")
+    _check(page_table, "page_table", _INT, (None, None), dev)
+    batch, columns = page_table.shape
+    for t, name, shape in ((lengths, "lengths", (batch,)), (held, "held", (batch,)), (new, "new", (batch,)),
+                           (free, "free", (None,)), (count, "count", (1,))):
+        _check(t, name, _INT, shape, dev)
+    on, handle = _on(stream, dev, (page_table, lengths, held, new, free, count))
+    with on:
+        slots = torch.empty(tokens, dtype=torch.int64, device=dev)
+        parts = torch.empty(4 * batch + 2 + 2 * tokens, dtype=_INT, device=dev).split(
+            [batch, batch, 1, batch, batch + 1, tokens, tokens])
+        a = N.KvStep(page_table.data_ptr(), page_table.stride(0) if batch > 1 else columns, lengths.data_ptr(),
+                     held.data_ptr(), new.data_ptr(), free.data_ptr(), count.data_ptr(), *(x.data_ptr() for x in parts),
+                     slots.data_ptr(), tokens, batch, columns, free.shape[0], page_rows)
+        N.check(N.load().tessa_kv_plan(C.byref(a), handle), "kv plan")
+    return Plan(*parts, slots)

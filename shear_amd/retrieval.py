@@ -71,7 +71,7 @@ class LongContext:
     head_dim: int
     max_rows: int                       # of a sequence, prompt and answer together
     page_rows: int = 64
-    dtype: torch.dtype = torch.bfloat16  # of the cache; torch.int8: SQ8 rows
+    dtype: torch.dtype = torch.bfloat16  # of the cache; torch.int8: SQ8 rows, KV.MX4: 4-bit rows
     sinks: int = 4                      # first rows that stay visible
     window: int = 256                   # last rows that stay visible
     found: int = 64                     # rows that each query head's search adds
@@ -123,10 +123,8 @@ class LongContext:
         self._indexed = list(self._rows)
         for b, n in enumerate(self._rows):
             rows = torch.arange(n, device="cuda")
-            pages, slots = self.table[b, rows // self.page_rows].long(), rows % self.page_rows
-            keys = self.cache.keys[pages, :, slots].float()
-            if self.cache.key_scales is not None:
-                keys *= self.cache.key_scales[pages, :, slots].unsqueeze(-1)
+            slots = self.table[b, rows // self.page_rows].long() * self.page_rows + rows % self.page_rows
+            keys = KV.read(self.cache, slots, torch.float32, values=False)[0]
             self.indexes.append([KeyIndex(keys[:, h]) for h in range(self.heads)])
 
     def find(self, q: torch.Tensor) -> torch.Tensor | None:
