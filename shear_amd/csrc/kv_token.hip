@@ -192,6 +192,15 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
     constexpr int kKLoads = kKWords / kKLoad;
     constexpr uint32_t kKDims = DP / 4 / kKLoads;      // dims of a lane's load, which four lanes share out
     constexpr int kMxGroups = DP / (int)kMxGroup;
+    // 4-bit rows: the next tile's loads are out while one is worked on, which costs few registers
+    constexpr bool kAhead = kMx4;
+    struct Tile {  // what a lane has of a tile's rows
+        KvWords<kKLoad> kw[2][kKLoads];
+        KvWords<kVWords> vw[8];
+        float scale;
+        uint32_t bytes[kMx4 ? (kMxGroups + 3) / 4 : 1];
+        uint32_t valid;  // rows that are there
+    };
     __shared__ __align__(16) uint32_t sh_place[kWaves][2][kTile];  // (read four at a time)
     __shared__ __align__(16) float sh_scale[kSq8 ? kWaves : 1][2][kTile];
     __shared__ __align__(16) float sh_group[kMx4 ? kWaves : 1][2][kMx4 ? kMxGroups : 1][kTile];  // scales of 32 dims
@@ -313,8 +322,11 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
 
     // row of the tile after next, page of the next tile: each load waits a whole step
     const uint32_t l32 = lane & 31u;
+    // the tile's row in place r of the instructions: 4-bit rows are half a cache line, so that a load of V, places j, 4 + j, 8 + j and
+    // 12 + j, takes neighbouring rows
+    auto row_in = [](uint32_t r) { return kMx4 ? (r & 16u) + 4u * (r & 3u) + (r >> 2 & 3u) : r; };
     auto row_of = [&](uint32_t tile) -> int32_t {
-        const uint32_t i = tile * kTile + l32;
+        const uint32_t i = tile * kTile + row_in(l32);
         return i < rows ? visible_row(vis, begin + i, list) : -1;
     };
     auto page_of = [&](int32_t row) -> int32_t { return row >= 0 ? table[(uint32_t)row >> c.page_shift] : -1; };
@@ -322,42 +334,42 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
     int32_t page = page_of(row);
     int32_t next_row = row_of(wave + kWaves);
 
-    for (uint32_t tile = wave; tile < tiles; tile += kWaves) {
+    // Starts the loads of a tile.
+    auto fetch = [&](uint32_t tile, Tile &x) {
         const uint32_t kplace = kv_place(c, c.keys, page, (uint32_t)row);
         const uint32_t vplace = kv_place(c, c.values, page, (uint32_t)row);
         const bool mine = kplace != kKvNoOffset;
-        const uint32_t valid = (uint32_t)__ballot(mine);  // lanes 32..63 repeat 0..31
+        x.valid = (uint32_t)__ballot(mine);  // lanes 32..63 repeat 0..31
         // a row's scales, by lanes 0..31 of the key, by lanes 32..63 of the value (its place: used after the rows' loads are out)
-        float scale = lane < kTile ? 0.0f : 1.0f;
+        x.scale = lane < kTile ? 0.0f : 1.0f;
         if constexpr (kSq8) {
             const KvArray &array = lane < kTile ? c.keys : c.values;
-            if (mine) scale = kv_row_scales(array)[kv_scale_place(c, array, page, (uint32_t)row, h)];
+            if (mine) x.scale = kv_row_scales(array)[kv_scale_place(c, array, page, (uint32_t)row, h)];
         }
         // MX4: a byte of each group, of the same rows by the same lanes (1 where there is no row: 0 * NaN would be NaN)
-        uint32_t bytes[kMx4 ? (kMxGroups + 3) / 4 : 1];
         if constexpr (kMx4) {
             const KvArray &array = lane < kTile ? c.keys : c.values;
             const uint8_t *at = kv_group_scales(array);
 #pragma unroll
-            for (int w = 0; w < (kMxGroups + 3) / 4; ++w) bytes[w] = 0x7f7f7f7fu;
+            for (int w = 0; w < (kMxGroups + 3) / 4; ++w) x.bytes[w] = 0x7f7f7f7fu;
             if (mine) {
                 at += kv_scale_place(c, array, page, (uint32_t)row, h);
                 if (c.scales_together) {  // as one word
-                    if constexpr (DP == 64) bytes[0] = *reinterpret_cast<const uint16_t *>(at);
-                    if constexpr (DP == 128) bytes[0] = *reinterpret_cast<const uint32_t *>(at);
+                    if constexpr (DP == 64) x.bytes[0] = *reinterpret_cast<const uint16_t *>(at);
+                    if constexpr (DP == 128) x.bytes[0] = *reinterpret_cast<const uint32_t *>(at);
                     if constexpr (DP == 256) {
                         const kv_u2 both = *reinterpret_cast<const kv_u2 *>(at);
-                        bytes[0] = both[0];
-                        bytes[kMxGroups / 4 - 1] = both[1];
+                        x.bytes[0] = both[0];
+                        x.bytes[kMxGroups / 4 - 1] = both[1];
                     }
                 } else {
 #pragma unroll
                     for (int w = 0; w < (kMxGroups + 3) / 4; ++w) {
-                        uint32_t x = 0;
+                        uint32_t word = 0;
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (4 * w + i < kMxGroups) x |= (uint32_t)at[kMxGroup * (4 * w + i) < c.dim ? 4 * w + i : 0] << (8 * i);
-                        bytes[w] = x;
+                            if (4 * w + i < kMxGroups) word |= (uint32_t)at[kMxGroup * (4 * w + i) < c.dim ? 4 * w + i : 0] << (8 * i);
+                        x.bytes[w] = word;
                     }
                 }
             }
@@ -369,18 +381,16 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
         next_row = row_of(tile + 2 * kWaves);
 
         // K: rows n and 16 + n
-        KvWords<kKLoad> kw[2][kKLoads];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const char *src = kbase + (uint64_t)sh_place[wave][0][16 * t + n] * 16u;
 #pragma unroll
             for (int s = 0; s < kKLoads; ++s) {
                 const uint32_t d = (uint32_t)s * 4u * kKDims + g * kKDims, there = d < c.dim ? d : 0u;
-                kw[t][s] = *reinterpret_cast<const KvWords<kKLoad> *>(src + (kMx4 ? there / 2u : kSq8 ? there : 2u * there));
+                x.kw[t][s] = *reinterpret_cast<const KvWords<kKLoad> *>(src + (kMx4 ? there / 2u : kSq8 ? there : 2u * there));
             }
         }
         // V: rows 16 (j / 4) + 4 g + j % 4
-        KvWords<kVWords> vw[8];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const kv_u4 place = *reinterpret_cast<const kv_u4 *>(&sh_place[wave][1][16 * t + 4 * g]);
@@ -388,19 +398,24 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
             for (int j = 0; j < 4; ++j) {
                 const char *src = vbase + (uint64_t)place[j] * 16u + vbyte;
                 if constexpr (kMx4 && kPer == 4)
-                    vw[4 * t + j].w[0] = *reinterpret_cast<const uint16_t *>(src);
+                    x.vw[4 * t + j].w[0] = *reinterpret_cast<const uint16_t *>(src);
                 else
-                    vw[4 * t + j] = *reinterpret_cast<const KvWords<kVWords> *>(src);
+                    x.vw[4 * t + j] = *reinterpret_cast<const KvWords<kVWords> *>(src);
             }
         }
+    };
+    auto attend = [&](uint32_t tile, Tile &here) {
+        auto &kw = here.kw;
+        auto &vw = here.vw;
+        const uint32_t valid = here.valid;
         if constexpr (kMx4) {
 #pragma unroll
             for (int i = 0; i < kMxGroups; ++i)
-                sh_group[wave][lane >> 5][i][l32] = kv_mx_scale(bytes[i / 4] >> (8 * (i & 3)) & 255u);
+                sh_group[wave][lane >> 5][i][l32] = kv_mx_scale(here.bytes[i / 4] >> (8 * (i & 3)) & 255u);
             kv_wave_sync();
         }
         if constexpr (kSq8) {
-            sh_scale[wave][lane >> 5][l32] = lane < kTile ? scale * p.scale_log2 : scale;
+            sh_scale[wave][lane >> 5][l32] = lane < kTile ? here.scale * p.scale_log2 : here.scale;
             kv_wave_sync();
         }
         if (!kMx4 && DP != c.dim) {  // (codes of 4 bits are) dims past the row meet zeros of Q and must be finite
@@ -443,10 +458,11 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
                 for (int i = 0; i < 4; ++i) x[t][i] = sacc[i] * ks[i];
             } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[t][i] = sacc[i] * p.scale_log2;
+                for (int i = 0; i < 4; ++i) x[t][i] = sacc[i] * (kMx4 ? 1.0f : p.scale_log2);
             }
         }
         if (valid != 0xffffffffu) {
+            asm volatile("");  // a branch: as selections it costs every tile 32 instructions
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -463,16 +479,18 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t r = 16 * t + 4 * g + i;
-                    if (head_ok && tile * kTile + r < rows) at[(uint64_t)r * p.group] = x[t][i];
+                    const uint32_t r = row_in(16 * t + 4 * g + i);
+                    if (head_ok && tile * kTile + r < rows) at[(uint64_t)r * p.group] = kMx4 ? x[t][i] * p.scale_log2 : x[t][i];
                 }
         }
-        float top = kKvNone;
+        // (4-bit rows: the scale comes with the difference from the maximum, one instruction for both)
+        float top = kMx4 ? -INFINITY : kKvNone;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, x[t][i]);
         top = kv_max16(top);
+        if constexpr (kMx4) top *= p.scale_log2;
         if (__any(top > m + kTop)) {
             const float higher = fmaxf(m, top - kLift);
             const float f = kv_exp2(m - higher);
@@ -491,11 +509,21 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
             if constexpr (kSq8) vs = *reinterpret_cast<const kv_f4 *>(&sh_scale[wave][1][16 * t + 4 * g]);
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
-                float w0 = kv_exp2(x[t][i] - m), w1 = kv_exp2(x[t][i + 1] - m);
+                float w0 = kv_exp2(kMx4 ? fmaf(x[t][i], p.scale_log2, -m) : x[t][i] - m);
+                float w1 = kv_exp2(kMx4 ? fmaf(x[t][i + 1], p.scale_log2, -m) : x[t][i + 1] - m);
                 l += w0 + w1;
                 if constexpr (kSq8) {
                     w0 *= vs[i];
                     w1 *= vs[i + 1];
+                }
+                if constexpr (kMx4) {  // cut, not rounded: three parts of 8 bits are all that f32 has
+                    constexpr uint32_t kUpper = 0x07060302u;  // the upper halves of both
+                    auto rest_of = [](float w) { return w - __uint_as_float(__float_as_uint(w) & 0xffff0000u); };
+                    const float r0 = rest_of(w0), r1 = rest_of(w1), y0 = rest_of(r0), y1 = rest_of(r1);
+                    hi[2 * t + i / 2] = __builtin_amdgcn_perm(__float_as_uint(w1), __float_as_uint(w0), kUpper);
+                    lo[2 * t + i / 2] = __builtin_amdgcn_perm(__float_as_uint(r1), __float_as_uint(r0), kUpper);
+                    least[2 * t + i / 2] = __builtin_amdgcn_perm(__float_as_uint(y1), __float_as_uint(y0), kUpper);
+                    continue;
                 }
                 const uint32_t r = P::pack(w0, w1);
                 hi[2 * t + i / 2] = r;
@@ -543,6 +571,24 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
                 rest[e] = P::mma16(a, lo, rest[e]);
             else
                 acc[e] = P::mma16(a, least, P::mma16(a, lo, acc[e]));
+        }
+    };
+    if constexpr (kAhead) {  // two by turns: in one set of registers moved on, each tile would wait for the next one's loads
+        Tile even, odd;
+        uint32_t tile = wave;
+        if (tile < tiles) fetch(tile, even);
+        for (; tile < tiles; tile += 2 * kWaves) {
+            if (tile + kWaves < tiles) fetch(tile + kWaves, odd);
+            attend(tile, even);
+            if (tile + kWaves >= tiles) break;
+            if (tile + 2 * kWaves < tiles) fetch(tile + 2 * kWaves, even);
+            attend(tile + kWaves, odd);
+        }
+    } else {
+        for (uint32_t tile = wave; tile < tiles; tile += kWaves) {
+            Tile here;
+            fetch(tile, here);
+            attend(tile, here);
         }
     }
     l = kv_sum16(l);
