@@ -86,8 +86,12 @@ tessa_status page_array(const tessa_kv_cache &k, const char *what, void *rows, c
     out.scale_page = out.scale_head = out.scale_row = 0;
     if (k.type == TESSA_KV_SQ8 || k.type == TESSA_KV_MX4) {
         if (!scales) KV_INVALID("kv cache: %s %s need scales", k.type == TESSA_KV_SQ8 ? "SQ8" : "MX4", what);
-        for (int i = 0; i < 3 && k.type == TESSA_KV_MX4; ++i)
+        double bytes = k.head_dim / 32;
+        for (int i = 0; i < 3 && k.type == TESSA_KV_MX4; ++i) {
             if (scale_strides[i] >= (1ull << 40)) KV_INVALID("kv cache: scale stride of %s", what);
+            bytes += (double)scale_strides[i] * (double)(counts[i] - 1);
+        }
+        if (bytes >= 4294967296.0) KV_UNSUPPORTED("kv cache: scales of %s span more than 4 GiB", what);
         out.scales = scales;
         out.scale_page = scale_strides[0];
         out.scale_head = scale_strides[1];

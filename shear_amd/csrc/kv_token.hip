@@ -88,6 +88,17 @@ __device__ __forceinline__ int32_t visible_row(const KvVisible &v, uint32_t i, c
     return r >= (int32_t)v.first && r < (int32_t)v.last_begin ? r : -1;
 }
 
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {
+    return (uint64_t)uniform((uint32_t)(x >> 32)) << 32 | uniform((uint32_t)x);
+}
+
+// x of the lane kBy before in a ring of 16.
+template <int kBy>
+__device__ __forceinline__ float turned(float x) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), 0x120 + kBy, 0xf, 0xf, true));
+}
+
 constexpr uint32_t kUnit = 128;  // rows: a tile for each wave
 
 __device__ __forceinline__ uint32_t units_of(const KvAttendParams &p, uint32_t b) {
@@ -173,16 +184,32 @@ __device__ __forceinline__ void find_sequence(const KvAttendParams &p, uint64_t 
     }
 }
 
+// Forms of the kernel over 4-bit rows.  A wave issues an instruction each 5 cycles at most and waits for its own
+// results, so two waves of a SIMD, all that the registers of kFormAny leave, take as long for the instructions
+// alone (70 us for the batch of 64 above, its rows in the cache) as the memory does (72), and 100 for both.
+//  * kFormWhole: 16 rows of a tile lie in one page, one after the other (all rows visible, pages of at
+//    least 16), so that their addresses are a scalar and a lane's constant.
+//  * kFormColumns4, kFormColumns8: besides, up to 4 or 8 query heads are repeated over the 16 columns of the
+//    instructions, and the parts of a weight (and of an fp16 query) have columns of their own, one or two products instead of
+//    three.  With the registers that this saves three waves fit a SIMD: the batch takes 80.5 us, the three long ones
+//    50.1 (two waves, each a tile ahead: 88.9 and 51.5).
+enum { kFormAny = 0, kFormWhole = 1, kFormColumns4 = 2, kFormColumns8 = 3 };
+// Waves of a SIMD, by registers.
+constexpr int token_waves(int dp, int form) { return dp == 256 ? (form == kFormColumns4 ? 2 : 1) : form >= kFormColumns4 ? 3 : 2; }
+
 // kDirect: one workgroup for each column of rows, which writes the result; else
 // workers and parts.
-template <typename T, int kRowsKind, int DP, bool kDirect>
-__global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(KvAttendParams p) {
+template <typename T, int kRowsKind, int DP, bool kDirect, int kForm>
+__global__ __launch_bounds__(kThreads, token_waves(DP, kForm)) void kv_token_kernel(KvAttendParams p) {
+    constexpr bool kWhole = kForm != kFormAny, kColumns = kForm >= kFormColumns4;
+    constexpr uint32_t kColumnHeads = kForm == kFormColumns4 ? 4 : kForm == kFormColumns8 ? 8 : 16;
     constexpr bool kSq8 = kRowsKind == kRowsSq8, kMx4 = kRowsKind == kRowsMx4;
     using E = KvElem<T>;
     using K = KvElem<std::conditional_t<kMx4, __bf16, T>>;  // of the logits' products
     using P = KvElem<std::conditional_t<kSq8 || kMx4, __bf16, T>>;  // of the weights and the values
     constexpr bool kHalf = !kSq8 && !kMx4 && std::is_same_v<T, _Float16>;  // fp16 weights
-    constexpr int kQueryParts = kMx4 && std::is_same_v<T, _Float16> ? 2 : 1;  // bf16 parts of an fp16 query, exactly
+    constexpr bool kSplitQuery = kMx4 && std::is_same_v<T, _Float16>;  // an fp16 query is two bf16 parts, exactly,
+    constexpr int kQueryParts = kSplitQuery && !kColumns ? 2 : 1;      // each a product (kColumns: of columns of its own)
     constexpr float kLift = kv_lift(kHalf, false), kTop = kv_top(kHalf), kRest = kHalf ? 4096.0f : 1.0f;
     constexpr int kSteps = DP / 32;                 // matrix instructions of 16 logits
     constexpr int kPer = DP / 16;                   // values of a row that a lane holds
@@ -192,8 +219,8 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
     constexpr int kKLoads = kKWords / kKLoad;
     constexpr uint32_t kKDims = DP / 4 / kKLoads;      // dims of a lane's load, which four lanes share out
     constexpr int kMxGroups = DP / (int)kMxGroup;
-    // 4-bit rows: the next tile's loads are out while one is worked on, which costs few registers
-    constexpr bool kAhead = kMx4;
+    // 4-bit rows: the next tiles' loads are out while one is worked on, which costs few registers
+    constexpr int kTurns = kMx4 && !kColumns ? 2 : 1;
     struct Tile {  // what a lane has of a tile's rows
         KvWords<kKLoad> kw[2][kKLoads];
         KvWords<kVWords> vw[8];
@@ -264,12 +291,21 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
     }
     bool again = false;
     while (unit < unit_end) {
+    if constexpr (kWhole) {  // the same for all lanes, which the compiler cannot see: scalar registers
+        b = uniform(b);
+        column = uniform(column);
+        unit = uniform(unit);
+        unit_end = uniform(unit_end);
+        line = uniform(line);
+    }
     const uint32_t h = column / blocks, first_q = (column - h * blocks) * 16u;
     const uint32_t heads = min(16u, p.group - first_q);
     const KvVisible vis = kv_visible(p, kv_length(c, b));
     const uint32_t units = (vis.count + kUnit - 1) / kUnit;
-    const uint32_t begin = kDirect ? 0u : (uint32_t)(unit - line) * kUnit;
-    const uint32_t end = kDirect ? vis.count : min(vis.count, begin + (uint32_t)min(unit_end - unit, (uint64_t)units) * kUnit);
+    const uint32_t begin0 = kDirect ? 0u : (uint32_t)(unit - line) * kUnit;
+    const uint32_t begin = kWhole ? uniform(begin0) : begin0;
+    const uint32_t end0 = kDirect ? vis.count : min(vis.count, begin + (uint32_t)min(unit_end - unit, (uint64_t)units) * kUnit);
+    const uint32_t end = kWhole ? uniform(end0) : end0;
     const uint32_t rows = end > begin ? end - begin : 0u;
     const uint32_t tiles = (rows + kTile - 1) / kTile;
     const int32_t *list = p.listed ? p.listed + ((uint64_t)b * c.heads + h) * p.listed_count : nullptr;
@@ -278,26 +314,28 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
     again = true;
 
     // Q operand: heads are columns; dims of step s as K's lanes hold them
-    const bool head_ok = n < heads;
+    const uint32_t my_head = n & (kColumnHeads - 1u);
+    const bool head_ok = my_head < heads;
     // beside the second sum of 256 dims the queries would not fit the registers (48 sequences of up to 4,100 rows,
     // 32 heads over 2 of 256 dims: 72 us, in registers with spills 77, bf16 65)
     constexpr bool kQueryInLds = kHalf && DP == 256;
     __shared__ kv_u4 sh_q[kQueryInLds ? kSteps : 1][64];
     kv_u4 qf[kQueryParts][kQueryInLds ? 1 : kSteps];
     {
-        const char *q = p.q + (uint64_t)b * p.q_token + (uint64_t)(h * p.group + first_q + (head_ok ? n : 0u)) * p.q_head;
+        const char *q = p.q + (uint64_t)b * p.q_token + (uint64_t)(h * p.group + first_q + (head_ok ? my_head : 0u)) * p.q_head;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             constexpr int kHere = kMx4 ? kKWords / kKLoads : kSq8 ? 2 : 1;  // steps of a load
             const uint32_t d = (uint32_t)(s / kHere) * 4u * kKDims + g * kKDims + (uint32_t)(s % kHere) * 8u;
             const kv_u4 zero = {0, 0, 0, 0};
             const kv_u4 x = head_ok && d < c.dim ? *reinterpret_cast<const kv_u4 *>(q + 2u * d) : zero;
-            if constexpr (kQueryParts == 2) {
+            if constexpr (kSplitQuery) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float lo = E::low(x[e]), hi = E::high(x[e]);
-                    qf[0][s][e] = K::pack(lo, hi);
-                    qf[1][s][e] = K::pack(lo - K::low(qf[0][s][e]), hi - K::high(qf[0][s][e]));
+                    const uint32_t first = K::pack(lo, hi), second = K::pack(lo - K::low(first), hi - K::high(first));
+                    qf[0][s][e] = kColumns && n >= 8u ? second : first;
+                    if constexpr (!kColumns) qf[1][s][e] = second;
                 }
             } else if constexpr (!kQueryInLds)
                 qf[0][s] = x;
@@ -312,6 +350,9 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
     const uint32_t vdim = n * kPer < c.dim ? n * kPer : 0u;
     const uint32_t vbyte = kMx4 ? vdim / 2u : kSq8 ? vdim : 2u * vdim;
 
+    // kColumns: what the parts after the first leave off (of 4 heads columns 12 .. 15 are left out)
+    const uint32_t first_cut = n >= kColumnHeads ? 0xffff0000u : 0u, second_cut = n >= 2u * kColumnHeads ? 0xffff0000u : 0u;
+    const uint32_t third_cut = n >= kColumnHeads ? 0xffffffffu : 0xffff0000u;
     float m = kKvNone, l = 0.0f;
     kv_f4 acc[kPer], rest[kHalf ? kPer : 1];
 #pragma unroll
@@ -330,12 +371,79 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
         return i < rows ? visible_row(vis, begin + i, list) : -1;
     };
     auto page_of = [&](int32_t row) -> int32_t { return row >= 0 ? table[(uint32_t)row >> c.page_shift] : -1; };
-    int32_t row = row_of(wave);
-    int32_t page = page_of(row);
-    int32_t next_row = row_of(wave + kWaves);
+    int32_t row = -1, page = -1, next_row = -1;
+    // kWhole: page of the lane's half of a tile; the lane's place in 16 rows
+    auto tile_page = [&](uint32_t tile) { return table[min(begin + tile * kTile + (l32 & 16u), end - 1u) >> c.page_shift]; };
+    uint32_t koffset[kWhole ? kKLoads : 1], voffset = 0, soffset = 0;
+    const uint8_t *sbase = nullptr;
+    const uint32_t wave0 = kWhole ? uniform(wave) : wave;
+    if constexpr (kWhole) {
+#pragma unroll
+        for (int s = 0; s < kKLoads; ++s) {
+            const uint32_t d = (uint32_t)s * 4u * kKDims + g * kKDims;
+            koffset[s] = row_in(n) * c.keys.row_units * 16u + (d < c.dim ? d : 0u) / 2u;
+        }
+        voffset = g * c.values.row_units * 16u + vbyte;
+        const KvArray &array = lane < kTile ? c.keys : c.values;
+        sbase = kv_group_scales(array);
+        soffset = h * (uint32_t)array.scale_head + (row_in(l32) & 15u) * (uint32_t)array.scale_row;
+        if (wave0 < tiles) page = tile_page(wave0);
+    } else {
+        row = row_of(wave);
+        page = page_of(row);
+        next_row = row_of(wave + kWaves);
+    }
 
+    // The scale bytes of a row's groups.
+    auto group_scales = [&](const uint8_t *at, uint32_t (&bytes)[kMx4 ? (kMxGroups + 3) / 4 : 1]) {
+        if (c.scales_together) {  // as one word
+            if constexpr (DP == 64) bytes[0] = *reinterpret_cast<const uint16_t *>(at);
+            if constexpr (DP == 128) bytes[0] = *reinterpret_cast<const uint32_t *>(at);
+            if constexpr (DP == 256) {
+                const kv_u2 both = *reinterpret_cast<const kv_u2 *>(at);
+                bytes[0] = both[0];
+                bytes[kMx4 ? kMxGroups / 4 - 1 : 0] = both[1];
+            }
+        } else {
+#pragma unroll
+            for (int w = 0; w < (kMxGroups + 3) / 4; ++w) {
+                uint32_t word = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (4 * w + i < kMxGroups) word |= (uint32_t)at[kMxGroup * (4 * w + i) < c.dim ? 4 * w + i : 0] << (8 * i);
+                bytes[kMx4 ? w : 0] = word;
+            }
+        }
+    };
     // Starts the loads of a tile.
-    auto fetch = [&](uint32_t tile, Tile &x) {
+    auto fetch = [&](uint32_t tile, Tile &x) __attribute__((always_inline)) {
+      if constexpr (kWhole) {
+        const uint32_t at = begin + tile * kTile, slots = 1u << c.page_shift;
+        const bool there = (uint32_t)page < c.pages;
+        x.valid = (uint32_t)__ballot(there && tile * kTile + row_in(l32) < rows);
+        const int32_t mine = there ? page : 0;  // row 0 of page 0 is there to read
+        uint32_t scales[2];                     // places of the halves' scales, of the lane's array
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const uint32_t id = (uint32_t)__builtin_amdgcn_readlane(mine, 16 * t), slot = (at + 16u * t) & (slots - 1u);
+            const char *k = kbase + (uint64_t)(id * c.keys.page_units + slot * c.keys.row_units) * 16u;
+            const char *v = vbase + (uint64_t)(id * c.values.page_units + slot * c.values.row_units) * 16u;
+            scales[t] = lane < kTile ? id * (uint32_t)c.keys.scale_page + slot * (uint32_t)c.keys.scale_row
+                                     : id * (uint32_t)c.values.scale_page + slot * (uint32_t)c.values.scale_row;
+#pragma unroll
+            for (int s = 0; s < kKLoads; ++s) x.kw[t][s] = *reinterpret_cast<const KvWords<kKLoad> *>(k + koffset[s]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const char *src = v + j * 4u * c.values.row_units * 16u + voffset;
+                if constexpr (kPer == 4)
+                    x.vw[4 * t + j].w[0] = *reinterpret_cast<const uint16_t *>(src);
+                else
+                    x.vw[4 * t + j] = *reinterpret_cast<const KvWords<kVWords> *>(src);
+            }
+        }
+        group_scales(sbase + (soffset + (l32 & 16u ? scales[1] : scales[0])), x.bytes);
+        if (tile + kWaves < tiles) page = tile_page(tile + kWaves);
+      } else {
         const uint32_t kplace = kv_place(c, c.keys, page, (uint32_t)row);
         const uint32_t vplace = kv_place(c, c.values, page, (uint32_t)row);
         const bool mine = kplace != kKvNoOffset;
@@ -354,24 +462,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
             for (int w = 0; w < (kMxGroups + 3) / 4; ++w) x.bytes[w] = 0x7f7f7f7fu;
             if (mine) {
                 at += kv_scale_place(c, array, page, (uint32_t)row, h);
-                if (c.scales_together) {  // as one word
-                    if constexpr (DP == 64) x.bytes[0] = *reinterpret_cast<const uint16_t *>(at);
-                    if constexpr (DP == 128) x.bytes[0] = *reinterpret_cast<const uint32_t *>(at);
-                    if constexpr (DP == 256) {
-                        const kv_u2 both = *reinterpret_cast<const kv_u2 *>(at);
-                        x.bytes[0] = both[0];
-                        x.bytes[kMxGroups / 4 - 1] = both[1];
-                    }
-                } else {
-#pragma unroll
-                    for (int w = 0; w < (kMxGroups + 3) / 4; ++w) {
-                        uint32_t word = 0;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (4 * w + i < kMxGroups) word |= (uint32_t)at[kMxGroup * (4 * w + i) < c.dim ? 4 * w + i : 0] << (8 * i);
-                        x.bytes[w] = word;
-                    }
-                }
+                group_scales(at, x.bytes);
             }
         }
         sh_place[wave][lane >> 5][l32] = mine ? (lane < kTile ? kplace : vplace) : 0u;  // row 0 of page 0 is there to read
@@ -403,12 +494,18 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
                     x.vw[4 * t + j] = *reinterpret_cast<const KvWords<kVWords> *>(src);
             }
         }
+      }
     };
-    auto attend = [&](uint32_t tile, Tile &here) {
+    auto attend = [&](uint32_t tile, Tile &here) __attribute__((always_inline)) {
         auto &kw = here.kw;
         auto &vw = here.vw;
         const uint32_t valid = here.valid;
         if constexpr (kMx4) {
+            if (kWhole && valid != 0xffffffffu) {  // what lies where no row is: 0 * NaN would be NaN
+                asm volatile("");
+#pragma unroll
+                for (int w = 0; w < (kMxGroups + 3) / 4; ++w) here.bytes[w] = valid >> l32 & 1u ? here.bytes[w] : 0x7f7f7f7fu;
+            }
 #pragma unroll
             for (int i = 0; i < kMxGroups; ++i)
                 sh_group[wave][lane >> 5][i][l32] = kv_mx_scale(here.bytes[i / 4] >> (8 * (i & 3)) & 255u);
@@ -459,6 +556,9 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[t][i] = sacc[i] * (kMx4 ? 1.0f : p.scale_log2);
+                if constexpr (kSplitQuery && kColumns)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[t][i] += turned<8>(x[t][i]);
             }
         }
         if (valid != 0xffffffffu) {
@@ -480,7 +580,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t r = row_in(16 * t + 4 * g + i);
-                    if (head_ok && tile * kTile + r < rows) at[(uint64_t)r * p.group] = kMx4 ? x[t][i] * p.scale_log2 : x[t][i];
+                    if (head_ok && n < kColumnHeads && tile * kTile + r < rows) at[(uint64_t)r * p.group] = kMx4 ? x[t][i] * p.scale_log2 : x[t][i];
                 }
         }
         // (4-bit rows: the scale comes with the difference from the maximum, one instruction for both)
@@ -502,7 +602,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
                 if constexpr (kHalf) rest[i] *= f;
             }
         }
-        kv_u4 hi, lo, least;
+        kv_u4 hi, lo = {0, 0, 0, 0}, least = {0, 0, 0, 0};
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             kv_f4 vs = {1, 1, 1, 1};
@@ -515,6 +615,21 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
                 if constexpr (kSq8) {
                     w0 *= vs[i];
                     w1 *= vs[i + 1];
+                }
+                if constexpr (kColumns) {  // the column's part
+                    auto rest_of = [](float w, uint32_t cut) { return w - __uint_as_float(__float_as_uint(w) & cut); };
+                    float r0 = rest_of(w0, first_cut), r1 = rest_of(w1, first_cut);
+                    if constexpr (kColumnHeads == 4) {
+                        r0 = rest_of(r0, second_cut);
+                        r1 = rest_of(r1, second_cut);
+                    }
+                    hi[2 * t + i / 2] = __builtin_amdgcn_perm(__float_as_uint(r1), __float_as_uint(r0), 0x07060302u);
+                    if constexpr (kColumnHeads == 8) {  // the third part beside the first, nothing beside the second
+                        r0 = rest_of(rest_of(r0, 0xffff0000u), third_cut);
+                        r1 = rest_of(rest_of(r1, 0xffff0000u), third_cut);
+                        lo[2 * t + i / 2] = __builtin_amdgcn_perm(__float_as_uint(r1), __float_as_uint(r0), 0x07060302u);
+                    }
+                    continue;
                 }
                 if constexpr (kMx4) {  // cut, not rounded: three parts of 8 bits are all that f32 has
                     constexpr uint32_t kUpper = 0x07060302u;  // the upper halves of both
@@ -552,8 +667,16 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
                     a0[j] = __builtin_amdgcn_perm(y, x, 0x05040100u);
                     a1[j] = __builtin_amdgcn_perm(y, x, 0x07060302u);
                 }
-                acc[e] = P::mma16(a0, least, P::mma16(a0, lo, P::mma16(a0, hi, acc[e])));
-                acc[e + 1] = P::mma16(a1, least, P::mma16(a1, lo, P::mma16(a1, hi, acc[e + 1])));
+                acc[e] = P::mma16(a0, hi, acc[e]);
+                acc[e + 1] = P::mma16(a1, hi, acc[e + 1]);
+                if constexpr (kColumnHeads >= 8) {
+                    acc[e] = P::mma16(a0, lo, acc[e]);
+                    acc[e + 1] = P::mma16(a1, lo, acc[e + 1]);
+                }
+                if constexpr (kColumnHeads == 16) {
+                    acc[e] = P::mma16(a0, least, acc[e]);
+                    acc[e + 1] = P::mma16(a1, least, acc[e + 1]);
+                }
             });
         }
 #pragma unroll
@@ -573,9 +696,9 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
                 acc[e] = P::mma16(a, least, P::mma16(a, lo, acc[e]));
         }
     };
-    if constexpr (kAhead) {  // two by turns: in one set of registers moved on, each tile would wait for the next one's loads
+    if constexpr (kTurns == 2) {  // by turns: in one set of registers moved on, each tile would wait for the next one's loads
         Tile even, odd;
-        uint32_t tile = wave;
+        uint32_t tile = wave0;
         if (tile < tiles) fetch(tile, even);
         for (; tile < tiles; tile += 2 * kWaves) {
             if (tile + kWaves < tiles) fetch(tile + kWaves, odd);
@@ -585,7 +708,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
             attend(tile + kWaves, odd);
         }
     } else {
-        for (uint32_t tile = wave; tile < tiles; tile += kWaves) {
+        for (uint32_t tile = wave; tile < tiles; tile += kWaves) {  // (wave0 would take scalar registers that are not left)
             Tile here;
             fetch(tile, here);
             attend(tile, here);
@@ -595,6 +718,17 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
     if constexpr (kHalf) {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) acc[i] += rest[i] * (1.0f / kRest);
+    }
+
+    if constexpr (kColumns) {  // the parts of a head
+#pragma unroll
+        for (int e = 0; e < kPer; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float y = kColumnHeads == 8 || n < 12u ? acc[e][i] : 0.0f;
+                y += turned<8>(y);
+                acc[e][i] = kColumnHeads == 8 ? y : y + turned<4>(y);
+            }
     }
 
     // join the waves: sums relative to the largest maximum
@@ -607,7 +741,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_token_kernel(K
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sh_ml[w][0][n]);
     const float f = kv_exp2(m - top);
-    if (head_ok) {
+    if (head_ok && n < kColumnHeads) {
         // the lane's values are dims kPer * 4 g .. of head n, in the order of the rows of the accumulators
         float *o = sh_out + ((uint64_t)wave * heads + n) * DP + kPer * 4 * g;
 #pragma unroll
@@ -893,14 +1027,33 @@ __global__ __launch_bounds__(kThreads) void kv_finish_kernel(KvAttendParams p, u
     }
 }
 
-template <typename T, int kRowsKind, int DP>
-int launch(const KvAttendParams &p, hipStream_t stream) {
+template <typename T, int kRowsKind, int DP, int kForm>
+int launch_form(const KvAttendParams &p, hipStream_t stream) {
     const size_t lds = (size_t)kWaves * (p.group < 16u ? p.group : 16u) * DP * sizeof(float);
-    auto *kernel = p.workers ? &kv_token_kernel<T, kRowsKind, DP, false> : &kv_token_kernel<T, kRowsKind, DP, true>;
+    auto *kernel = p.workers ? &kv_token_kernel<T, kRowsKind, DP, false, kForm> : &kv_token_kernel<T, kRowsKind, DP, true, kForm>;
     // 16 heads of 256 dims are 64 KiB, beside up to 10 KiB that the kernel has anyway: above the default limit
     if (lds > 32768 && ensure_lds_limit(reinterpret_cast<const void *>(kernel), (int)lds) != 0) return -1;
     kernel<<<p.workers ? dim3(p.workers) : dim3(p.columns, p.c.batch), kThreads, lds, stream>>>(p);
     return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+// The form that a call takes.
+int token_form(const KvAttendParams &p) {
+    // (16 rows within 2^28 bytes: their offsets are 32-bit)
+    if (!p.c.mx4 || p.window != 0xffffffffu || p.c.page_shift < 4u || p.c.keys.row_units > 1u << 20 || p.c.values.row_units > 1u << 20)
+        return kFormAny;
+    return p.group <= 4u ? kFormColumns4 : p.group <= 8u ? kFormColumns8 : kFormWhole;
+}
+
+template <typename T, int kRowsKind, int DP>
+int launch(const KvAttendParams &p, hipStream_t stream) {
+    if constexpr (kRowsKind == kRowsMx4) {
+        const int form = token_form(p);
+        if (form == kFormColumns4) return launch_form<T, kRowsKind, DP, kFormColumns4>(p, stream);
+        if (form == kFormColumns8) return launch_form<T, kRowsKind, DP, kFormColumns8>(p, stream);
+        if (form == kFormWhole) return launch_form<T, kRowsKind, DP, kFormWhole>(p, stream);
+    }
+    return launch_form<T, kRowsKind, DP, kFormAny>(p, stream);
 }
 
 template <typename T, int kRowsKind>
@@ -940,7 +1093,7 @@ void kv_token_split(KvAttendParams &p) {
     constexpr uint64_t kWhole = 512, kMostWhole = 2048, kWholeOfColumn = 8;
     p.columns = p.c.heads * ((p.group + 15u) / 16u);
     p.workers = 0;
-    const uint64_t most = (uint64_t)kv_compute_units() * (kv_padded_dim(p.c.dim) == 256 ? 1u : 2u);
+    const uint64_t most = (uint64_t)kv_compute_units() * token_waves((int)kv_padded_dim(p.c.dim), token_form(p));
     const uint64_t whole = kWholeOfColumn * p.columns * p.c.batch;
     if (p.max_visible <= (whole < kWhole ? kWhole : whole < kMostWhole ? whole : kMostWhole) && !p.weights) return;
     const uint64_t units = (uint64_t)(p.max_visible + kUnit - 1) / kUnit * p.columns * p.c.batch;
