@@ -454,6 +454,8 @@ tessa_status tessa_kv_append_rotated(const tessa_kv_cache *cache, const tessa_kv
         p.out = static_cast<char *>(t->out);
         p.out_token = b[0];
         p.out_head = b[1];
+        if (p.q_head > 0xffffffffull || p.k_head > 0xffffffffull || p.v_head > 0xffffffffull || p.out_head > 0xffffffffull)
+            KV_UNSUPPORTED("kv append rotated: heads lie more than 4 GiB apart");
         if (!t->positions || !t->slots) KV_INVALID("kv append rotated: null positions or slots");
         p.positions = t->positions;
         p.slots = t->slots;
