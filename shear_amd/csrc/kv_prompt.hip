@@ -92,15 +92,15 @@ __device__ __forceinline__ bool special_half(uint32_t x) {
 
 // Rows of a tile: at 256 dims of 16-bit rows half as many, for the registers' sake.  (Two
 // prompts of 4,096 tokens, 16 heads over 4 of 256: 549 us, with 64 rows and spills 1,390;
-// SQ8 609 with 64 rows, 742 with 32.)
-template <int kRowsKind, int DP>
+// SQ8 609 with 64 rows, 742 with 32.  fp16 queries over 4-bit rows spill with 64: 2,449, with 32 821.)
+template <typename T, int kRowsKind, int DP>
 constexpr uint32_t prompt_rows() {
-    return DP == 256 && kRowsKind == kRowsPlain ? 32u : 64u;
+    return DP == 256 && (kRowsKind == kRowsPlain || (kRowsKind == kRowsMx4 && !std::is_same_v<T, __bf16>)) ? 32u : 64u;
 }
 
-template <int kRowsKind, int DP>
+template <typename T, int kRowsKind, int DP>
 struct PromptLds {
-    static constexpr uint32_t kRows = prompt_rows<kRowsKind, DP>();
+    static constexpr uint32_t kRows = prompt_rows<T, kRowsKind, DP>();
     static constexpr bool kCodes = kRowsKind != kRowsPlain;
     alignas(16) char k[2][kRows * DP * 2];
     alignas(16) char v[2][kRows * DP * 2];
@@ -129,7 +129,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
     constexpr bool kRowScale = kSq8 || (kMx4 && !std::is_same_v<T, __bf16>);
     // (32 alike rows at the lift sum to 2^5 times it, below the top)
     constexpr float kLift = kv_lift(kHalf, true), kTop = kv_top(kHalf), kMost = kHalf ? 32768.0f : 1.0f;  // kMost = 2^kTop
-    using Lds = PromptLds<kRowsKind, DP>;
+    using Lds = PromptLds<T, kRowsKind, DP>;
     constexpr uint32_t kRows = Lds::kRows;
     constexpr int kSubs = (int)kRows / 32;       // 32 rows of logits each
     constexpr int kSteps = DP / 16;              // instructions along the dims
@@ -704,7 +704,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
 template <typename T, int kRowsKind, int DP, bool kWhole>
 int launch(const KvAttendParams &p, hipStream_t stream) {
     const uint32_t tiles = (uint32_t)(((uint64_t)p.max_new * p.group + kQueries - 1) / kQueries);
-    const int lds = (int)sizeof(PromptLds<kRowsKind, DP>);
+    const int lds = (int)sizeof(PromptLds<T, kRowsKind, DP>);
     auto *kernel = &kv_prompt_kernel<T, kRowsKind, DP, kWhole>;
     if (ensure_lds_limit(reinterpret_cast<const void *>(kernel), lds) != 0) return -1;
     kernel<<<tiles * p.chunks * p.c.heads * p.c.batch, kThreads, lds, stream>>>(p, tiles);
@@ -751,7 +751,13 @@ int launch_rows(const KvAttendParams &p, KvRows rows, hipStream_t stream) {
 //   2 x 256 tokens over 512 rows 20.8, 26.0 (not split); over 2,048 58.8, 49.8; over 4,096 121, 62
 void kv_prompt_split(KvAttendParams &p) {
     constexpr float kPartCost = 3e-6f, kJoinCost = 4.0f;  // us
-    const uint64_t tiles = ((uint64_t)p.max_new * p.group + kQueries - 1) / kQueries * p.c.heads * p.c.batch;
+    uint64_t tiles = ((uint64_t)p.max_new * p.group + kQueries - 1) / kQueries * p.c.heads * p.c.batch;
+    // 4-bit rows: no more than the tokens there are fill, which are fewer where prompts differ in length (5 of 30 to 301 tokens
+    // over a window of 1,500, 24 heads over 8 of 96 dims, fp16: 93 us in whole columns, 61 in two parts)
+    if (p.c.mx4) {
+        const uint64_t real = ((p.tokens * p.group + kQueries - 1) / kQueries + p.c.batch) * p.c.heads;
+        tiles = real < tiles ? real : tiles;
+    }
     const uint32_t visible = p.window == 0xffffffffu
                                  ? p.c.max_length
                                  : (uint32_t)min((uint64_t)p.c.max_length, (uint64_t)p.sinks + p.window + kQueries / p.group);

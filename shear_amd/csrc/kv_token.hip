@@ -298,7 +298,7 @@ __global__ __launch_bounds__(kThreads, token_waves(DP, kForm)) void kv_token_ker
         unit_end = uniform(unit_end);
         line = uniform(line);
     }
-    const uint32_t h = column / blocks, first_q = (column - h * blocks) * 16u;
+    const uint32_t h = kWhole ? uniform(column / blocks) : column / blocks, first_q = (column - h * blocks) * 16u;
     const uint32_t heads = min(16u, p.group - first_q);
     const KvVisible vis = kv_visible(p, kv_length(c, b));
     const uint32_t units = (vis.count + kUnit - 1) / kUnit;
