@@ -139,6 +139,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
     // loads of a thread, for K and for V each (MX4, 64 dims: of half of the threads)
     constexpr int kLoads = kRows * kPieces < (uint32_t)kThreads ? 1 : (int)(kRows * kPieces) / kThreads;
     constexpr uint32_t kRowsPer = kThreads / kPieces;  // rows of one load of the workgroup
+    constexpr bool kSomeThreads = kRowsPer > kRows;    // (threads past the tile load nothing)
     extern __shared__ __align__(16) char smem[];
     Lds &lds = *reinterpret_cast<Lds *>(smem);
 
@@ -277,8 +278,8 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
         for (int i = 0; i < kLoads; ++i) {
             const uint32_t r = (uint32_t)i * kRowsPer + load_row;
             const uint32_t row = r0 + r;
-            const bool there = row < length && r < kRows && (uint32_t)pages[i] < c.pages;
-            missing |= (uint32_t)(!there && row < length && r < kRows) << i;
+            const bool there = row < length && (!kSomeThreads || r < kRows) && (uint32_t)pages[i] < c.pages;
+            missing |= (uint32_t)(!there && row < length && (!kSomeThreads || r < kRows)) << i;
             const uint32_t slot = row & ((1u << c.page_shift) - 1u), page = (uint32_t)pages[i];
             const uint64_t kp = (uint64_t)(page * c.keys.page_units + slot * c.keys.row_units);
             const uint64_t vp = (uint64_t)(page * c.values.page_units + slot * c.values.row_units);

@@ -11,7 +11,7 @@ constexpr int kThreads = 256;
 constexpr int kFlight = 4;  // rows of a lane in flight
 
 // A lane's dims: 16 bytes of the output, so that a store is whole cache lines (f32 as 8 dims, two stores with gaps:
-// 72 us for 60,001 x 8 rows of 128, 245 MB; as 4 dims @@).
+// 72 us for 60,001 x 8 rows of 128, 245 MB; as 4 dims 57).
 template <typename Out>
 constexpr int kPer = 16 / (int)sizeof(Out);
 

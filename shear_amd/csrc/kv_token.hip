@@ -333,7 +333,9 @@ __global__ __launch_bounds__(kThreads, token_waves(DP, kForm)) void kv_token_ker
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float lo = E::low(x[e]), hi = E::high(x[e]);
-                    const uint32_t first = K::pack(lo, hi), second = K::pack(lo - K::low(first), hi - K::high(first));
+                    const uint32_t first = K::pack(lo, hi);
+                    auto rest_of = [](float w, float part) { return fabsf(w) < INFINITY ? w - part : 0.0f; };
+                    const uint32_t second = K::pack(rest_of(lo, K::low(first)), rest_of(hi, K::high(first)));
                     qf[0][s][e] = kColumns && n >= 8u ? second : first;
                     if constexpr (!kColumns) qf[1][s][e] = second;
                 }

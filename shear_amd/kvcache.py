@@ -31,6 +31,7 @@ import contextlib
 import ctypes as C
 import math
 from dataclasses import dataclass, field
+from typing import NamedTuple
 
 import torch
 
@@ -136,6 +137,11 @@ def _check(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device)
         raise ValueError(f"{name} must be on {device}, not {t.device}")
     if got[-1] > 1 and t.stride(-1) != 1 and t.numel():
         raise ValueError(f"the last dimension of {name} must be contiguous")
+
+
+def _is(t: torch.Tensor, dtype: torch.dtype, shape: tuple, index: int) -> bool:
+    """What ``_check`` asks for, as it mostly is: a small call's time is its checks'."""
+    return t.dtype is dtype and t.shape == shape and t.get_device() == index and t.is_contiguous()
 
 
 def _no_gradient(cache: KvCache, a: torch.Tensor, b: torch.Tensor | None = None) -> None:
@@ -363,10 +369,6 @@ def rotation_frequencies(dims: int, base: float = 10000.0, device: str | torch.d
     return base ** (-torch.arange(0, dims, 2, dtype=torch.float64, device=device) / dims)
 
 
-def _places(slots: torch.Tensor, count: int | None, device) -> None:
-    _check(slots, "slots", torch.int64, (count,), device)
-
-
 def append_rotated(cache: KvCache, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
                    slots: torch.Tensor, frequencies: torch.Tensor | None = None, q_weight: torch.Tensor | None = None,
                    k_weight: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False,
@@ -376,9 +378,9 @@ def append_rotated(cache: KvCache, q: torch.Tensor, k: torch.Tensor, v: torch.Te
     the cache has are not written; no two tokens may have the same one).
 
     ``q_weight``, ``k_weight`` ([head_dim], q's type or f32): x * rsqrt(mean x^2 + eps) * weight
-    for each head; None: no norm.  ``frequencies`` (f64 [r / 2], r a multiple of 16; None: no rotation): pair i of the first r dims
-    turns by positions (int32 [tokens]) * frequencies[i] radians, dims (i, i + r / 2) or, ``interleaved``,
-    (2i, 2i + 1).  All of it in f32 (angles in 64 bits) and rounded once, so that the rows are
+    for each head; None: no norm.  ``frequencies`` (f64 [r / 2], r a multiple of 16; None: no
+    rotation): pair i of the first r dims turns by positions (int32 [tokens]) *
+    frequencies[i] radians, dims (i, i + r / 2) or, ``interleaved``, (2i, 2i + 1).  All of it in f32 (angles in 64 bits) and rounded once, so that the rows are
     what ``append`` makes of the rounded ones.  A token with a negative position is of no sequence:
     its queries come back as zeros and nothing of it is written."""
     dev, native = cache.keys.device, cache._native
@@ -396,20 +398,25 @@ def append_rotated(cache: KvCache, q: torch.Tensor, k: torch.Tensor, v: torch.Te
     for t, name in ((k, "k"), (v, "v")):
         if t.dtype != q.dtype or t.shape != shape or t.device != dev:
             raise ValueError(f"{name} must be {q.dtype} {list(shape)} on {dev}")
-    _check(positions, "positions", _INT, (tokens,), dev)
-    _places(slots, tokens, dev)
+    index = dev.index
+    if not (_is(positions, _INT, (tokens,), index) and _is(slots, torch.int64, (tokens,), index)):
+        _check(positions, "positions", _INT, (tokens,), dev)
+        _check(slots, "slots", torch.int64, (tokens,), dev)
     rotated = 0
     if frequencies is not None:
         _check(frequencies, "frequencies", torch.float64, (None,), dev)
+        _no_gradient(cache, frequencies)
         rotated = 2 * frequencies.shape[0]
         if rotated % 16 or rotated > dim:
             raise ValueError(f"{rotated} rotated dims must be a multiple of 16 up to {dim}")
-    weight_type = q.dtype
-    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+    weight_type, weights = q.dtype, [0, 0]
+    for i, w in enumerate((q_weight, k_weight)):
         if w is not None:
-            weight_type = w.dtype if w.dtype == torch.float32 else q.dtype
-            _check(w, name, weight_type, (dim,), dev)
+            weight_type = w.dtype if w.dtype is torch.float32 else q.dtype
+            if not _is(w, weight_type, (dim,), index):
+                _check(w, "k_weight" if i else "q_weight", weight_type, (dim,), dev)
             _no_gradient(cache, w)
+            weights[i] = w.data_ptr()
     if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
         raise ValueError(f"q_weight is {q_weight.dtype}, k_weight {k_weight.dtype}")
     if not (eps >= 0.0 and math.isfinite(eps)):
@@ -417,13 +424,15 @@ def append_rotated(cache: KvCache, q: torch.Tensor, k: torch.Tensor, v: torch.Te
     on, handle = _on(stream, dev, (*cache._tensors(), q, k, v, positions, slots, frequencies, q_weight, k_weight))
     with on:
         q, k, v = _rows(q), _rows(k), _rows(v)
-        weights = [w if w is None or w.data_ptr() % 16 == 0 else w.clone() for w in (q_weight, k_weight)]
+        if weights[0] % 16 or weights[1] % 16:  # (clones start where an allocation does)
+            own = [None if w is None else w.clone() for w in (q_weight, k_weight)]
+            weights = [0 if w is None else w.data_ptr() for w in own]
         out = torch.empty(tokens, heads, dim, dtype=q.dtype, device=dev)
         a = N.KvRotated(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q.stride()[:2], k.stride()[:2],
                         v.stride()[:2], (heads * dim, dim), positions.data_ptr(), slots.data_ptr(),
                         None if frequencies is None else frequencies.data_ptr(),
-                        *(None if w is None else w.data_ptr() for w in weights), tokens, kind,
-                        _VALUE_TYPES[weight_type], heads, rotated, int(interleaved), eps)
+                        weights[0] or None, weights[1] or None, tokens, kind, _VALUE_TYPES[weight_type], heads, rotated,
+                        int(interleaved), eps)
         N.check(N.load().tessa_kv_append_rotated(C.byref(native), C.byref(a), handle), "kv append rotated")
     return out
 
@@ -435,7 +444,7 @@ def read(cache: KvCache, slots: torch.Tensor, dtype: torch.dtype | None = None, 
     MX4, which holds each of its values).  ``values`` False: keys only, and None."""
     dev, native = cache.keys.device, cache._native
     _no_gradient(cache, slots)
-    _places(slots, None, dev)
+    _check(slots, "slots", torch.int64, (None,), dev)
     if dtype is None:
         own = cache.keys.dtype
         dtype = torch.float32 if own == torch.int8 else torch.bfloat16 if own == MX4 else own
@@ -451,8 +460,7 @@ def read(cache: KvCache, slots: torch.Tensor, dtype: torch.dtype | None = None, 
     return k, v
 
 
-@dataclass(frozen=True, eq=False)
-class Plan:
+class Plan(NamedTuple):
     """What a step does with its tokens (``plan``)."""
 
     lengths: torch.Tensor    # int32 [batch]: rows of each sequence after the step
@@ -488,16 +496,23 @@ def plan(page_rows: int, page_table: torch.Tensor, lengths: torch.Tensor, held: 
         raise ValueError(f"tokens {tokens} is outside 0..2^31 - 1")
     _check(page_table, "page_table", _INT, (None, None), dev)
     batch, columns = page_table.shape
-    for t, name, shape in ((lengths, "lengths", (batch,)), (held, "held", (batch,)), (new, "new", (batch,)),
-                           (free, "free", (None,)), (count, "count", (1,))):
-        _check(t, name, _INT, shape, dev)
+    i, each = dev.index, (batch,)
+    if not (_is(lengths, _INT, each, i) and _is(held, _INT, each, i) and _is(new, _INT, each, i)
+            and _is(count, _INT, (1,), i)):
+        for t, name, shape in ((lengths, "lengths", each), (held, "held", each), (new, "new", each),
+                               (count, "count", (1,))):
+            _check(t, name, _INT, shape, dev)
+    _check(free, "free", _INT, (None,), dev)
     on, handle = _on(stream, dev, (page_table, lengths, held, new, free, count))
     with on:
         slots = torch.empty(tokens, dtype=torch.int64, device=dev)
-        parts = torch.empty(4 * batch + 2 + 2 * tokens, dtype=_INT, device=dev).split(
-            [batch, batch, 1, batch, batch + 1, tokens, tokens])
+        sizes = [batch, batch, 1, batch, batch + 1, tokens, tokens]
+        whole = torch.empty(4 * batch + 2 + 2 * tokens, dtype=_INT, device=dev)
+        at, parts = whole.data_ptr(), whole.split_with_sizes(sizes)
+        ints = (at, at + 4 * batch, at + 8 * batch, at + 8 * batch + 4, at + 12 * batch + 4, at + 16 * batch + 8,
+                at + 16 * batch + 8 + 4 * tokens)
         a = N.KvStep(page_table.data_ptr(), page_table.stride(0) if batch > 1 else columns, lengths.data_ptr(),
-                     held.data_ptr(), new.data_ptr(), free.data_ptr(), count.data_ptr(), *(x.data_ptr() for x in parts),
-                     slots.data_ptr(), tokens, batch, columns, free.shape[0], page_rows)
+                     held.data_ptr(), new.data_ptr(), free.data_ptr(), count.data_ptr(), *ints, slots.data_ptr(), tokens,
+                     batch, columns, free.shape[0], page_rows)
         N.check(N.load().tessa_kv_plan(C.byref(a), handle), "kv plan")
     return Plan(*parts, slots)

@@ -232,6 +232,25 @@ def test_token_large_logits_and_scales_far_apart(gpu, q_type):
                 assert abs(lh[b, i] - z) <= delta + 2.0**-21 * (abs(z) + 1)
 
 
+@pytest.mark.parametrize("q_type", [BF16, F16])
+@pytest.mark.parametrize("group,page", [(3, 16), (3, 8), (8, 16), (20, 16)])
+def test_queries_that_are_not_finite(gpu, q_type, group, page):
+    """An infinite query times keys of one sign is an infinite logit of that sign: of minus infinity nothing is left."""
+    lengths, dim = [200, 200, 200], 64
+    pool, g = pool4_with(lengths, 1, page, dim, q_type, 13)
+    kc, vc, ks, vs = pool.bytes()
+    kc &= 0x77  # no key is negative
+    kc |= 0x11  # or zero
+    q = normal(g, 3, group, dim, dtype=q_type)
+    q[0, 1, 5], q[1, 2, 7], q[2, 0, 40] = float("-inf"), float("inf"), float("nan")
+    out, lse = KV.attend_token(q, pool.cache, pool.table, lens(lengths))
+    assert (out[0, 1] == 0).all() and lse[0, 1] == -math.inf
+    assert out[1, 2].isnan().all() and out[2, 0].isnan().all()
+    rest = torch.ones((3, group), dtype=torch.bool, device="cuda")
+    rest[0, 1] = rest[1, 2] = rest[2, 0] = False
+    assert out[rest].isfinite().all() and lse[rest].isfinite().all()
+
+
 def test_token_strides_and_transposed_pages(gpu):
     lengths = [100, 257]
     pool, g = pool4_with(lengths, 4, 32, 128, BF16, 11, transposed=True)

@@ -194,7 +194,8 @@ def test_refusals(gpu):
                    dict(frequencies=f.float()), dict(frequencies=f[:4]), dict(frequencies=KV.rotation_frequencies(80)),
                    dict(q_weight=w.half()), dict(q_weight=w[:32]), dict(k_weight=w.float()), dict(eps=-1.0),
                    dict(eps=float("nan")), dict(q=q.detach().requires_grad_()), dict(k=k.detach().requires_grad_()),
-                   dict(q_weight=w.detach().requires_grad_())):
+                   dict(q_weight=w.detach().requires_grad_()),
+                   dict(frequencies=f.clone().requires_grad_())):
         with pytest.raises(ValueError):
             KV.append_rotated(**{**good, **change})
             pytest.fail(f"{change} was not refused")
