@@ -225,6 +225,7 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
     int32_t pages[kLoads];
     kv_u4 kr[kCodes ? kLoads : 1], vr[kCodes ? kLoads : 1];  // codes on their way to LDS
     float ks = 0.0f, vs = 1.0f;
+    const uint32_t kgroup = h * (uint32_t)c.keys.scale_head + load_piece, vgroup = h * (uint32_t)c.values.scale_head + load_piece;
     uint32_t kb[kMx4 ? kLoads : 1], vb[kMx4 ? kLoads : 1];  // scale bytes of the pieces
     bool special = false;  // some value or scale was replaced
     // some maximum is so large that its rounding is felt (from 2^23 on it would be binades of a
@@ -232,6 +233,14 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
     bool huge = false;
     constexpr float kHuge = 4194304.0f;  // 2^22, rounded to a quarter
 
+    // 4-bit rows: a piece becomes four of LDS, which a thread writes from its k_turn-th and v_turn-th on, so that 16 threads'
+    // writes meet all banks (a row's order of pieces alone left every fourth of them: two prompts of 4,096 tokens 170 us, so @@)
+    const uint32_t k_turn = DP == 256 ? load_piece >> 2 << 1 : 0u;
+    const uint32_t v_turn = (DP == 64 ? load_row >> 1 : DP == 128 ? load_row : (load_piece >> 2) + 2u * load_row) & 3u;
+    auto turned_by = [](kv_u4 x, uint32_t by) {
+        const kv_u4 y = by & 1u ? kv_u4{x[1], x[2], x[3], x[0]} : x;
+        return by & 2u ? kv_u4{y[2], y[3], y[0], y[1]} : y;
+    };
     // Page ids for a tile (past the end: those of the last row), read a tile before they are used.
     auto read_pages = [&](uint32_t it) {
         const uint32_t r0 = tile_row(min(it, last_it - 1u));
@@ -291,8 +300,9 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
             if constexpr (kMx4) {  // a piece is a group
                 kb[i] = vb[i] = 0u;
                 if (there && load_piece * kWide < c.dim) {
-                    kb[i] = kv_group_scales(c.keys)[kv_scale_place(c, c.keys, pages[i], row, h) + load_piece];
-                    vb[i] = kv_group_scales(c.values)[kv_scale_place(c, c.values, pages[i], row, h) + load_piece];
+                    // (scales span less than 4 GiB)
+                    kb[i] = kv_group_scales(c.keys)[kgroup + page * (uint32_t)c.keys.scale_page + slot * (uint32_t)c.keys.scale_row];
+                    vb[i] = kv_group_scales(c.values)[vgroup + page * (uint32_t)c.values.scale_page + slot * (uint32_t)c.values.scale_row];
                 }
             }
             if constexpr (kCodes) {
@@ -353,12 +363,13 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
                 if (bad) lds.marks[it & 3u][0] = 1u;
                 const float vscale = kv_mx_scale(bad ? 0x7fu : vb[i]);
                 if (r < kRows) {
+                    const kv_u4 kx = turned_by(kr[i], k_turn), vx = turned_by(vr[i], v_turn);
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const uint32_t to = 4u * load_piece + (uint32_t)w;
-                        *reinterpret_cast<kv_u4 *>(&lds.k[buf][r * DP * 2 + k_piece<DP>(r, to) * 16u]) = kv_mx_values<T>(kr[i][w], kscale);
-                        *reinterpret_cast<kv_u4 *>(&lds.v[buf][r * DP * 2 + v_piece<DP>(r, to) * 16u]) =
-                            kv_mx_values<V>(bad ? 0u : vr[i][w], vscale);
+                    for (uint32_t w = 0; w < 4; ++w) {
+                        const uint32_t kto = 4u * load_piece + ((w + k_turn) & 3u), vto = 4u * load_piece + ((w + v_turn) & 3u);
+                        *reinterpret_cast<kv_u4 *>(&lds.k[buf][r * DP * 2 + k_piece<DP>(r, kto) * 16u]) = kv_mx_values<T>(kx[w], kscale);
+                        *reinterpret_cast<kv_u4 *>(&lds.v[buf][r * DP * 2 + v_piece<DP>(r, vto) * 16u]) =
+                            kv_mx_values<V>(bad ? 0u : vx[w], vscale);
                     }
                 }
             }
