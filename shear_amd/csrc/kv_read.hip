@@ -11,22 +11,25 @@ constexpr int kThreads = 256;
 constexpr int kFlight = 4;  // rows of a lane in flight
 
 // A lane's dims: 16 bytes of the output, so that a store is whole cache lines (f32 as 8 dims, two stores with gaps:
-// 72 us for 60,001 x 8 rows of 128, 245 MB; as 4 dims 57).
+// 72 us for 60,001 x 8 rows of 128, 245 MB; as 4 dims 57, both through the caches).
 template <typename Out>
 constexpr int kPer = 16 / (int)sizeof(Out);
 
-template <typename Out>
-__device__ __forceinline__ void put(char *to, const float (&f)[kPer<Out>]) {
-    if constexpr (sizeof(Out) == 4) {
-        *reinterpret_cast<kv_f4 *>(to) = kv_f4{f[0], f[1], f[2], f[3]};
-    } else {
-        using E = KvElem<Out>;
-        *reinterpret_cast<kv_u4 *>(to) = kv_u4{E::pack(f[0], f[1]), E::pack(f[2], f[3]), E::pack(f[4], f[5]), E::pack(f[6], f[7])};
-    }
+// Results larger than all L2 caches together do not stay there anyway, and stores that do not pass through them are
+// faster (245 MB of f32 42.6 us, 6.5 TB/s, through them 57.7; 102 MB of bf16 and an append before it 27.5, 30.0).  Smaller ones are left
+// to whoever reads them next.
+constexpr uint64_t kStreamed = 32ull << 20;
+
+template <bool kStream>
+__device__ __forceinline__ void put(char *to, kv_u4 x) {
+    if constexpr (kStream)
+        __builtin_nontemporal_store(x, reinterpret_cast<kv_u4 *>(to));
+    else
+        *reinterpret_cast<kv_u4 *>(to) = x;
 }
 
 // T: a plain row's type.  Out: float, __bf16 or _Float16.
-template <typename T, int kRows, typename Out>
+template <typename T, int kRows, typename Out, bool kStream>
 __global__ __launch_bounds__(kThreads) void kv_read_kernel(KvReadParams p, uint32_t lanes_log2) {
     constexpr int kDims = kPer<Out>;
     constexpr int kBytes = kRows == kRowsPlain ? 2 * kDims : kRows == kRowsSq8 ? kDims : kDims / 2;  // of a lane's load
@@ -78,7 +81,7 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(KvReadParams p, uint3
         char *to = out + ((uint64_t)r * c.dim + d) * sizeof(Out);
         if constexpr (kRows == kRowsMx4 && sizeof(Out) == 2) {
             const kv_u4 y = kv_mx_values<Out>(x[j][0], scale[j]);
-            *reinterpret_cast<kv_u4 *>(to) = there[j] ? y : kv_u4{0, 0, 0, 0};
+            put<kStream>(to, there[j] ? y : kv_u4{0, 0, 0, 0});
         } else {
             float f[kDims];
             if constexpr (kRows == kRowsMx4) {
@@ -98,7 +101,12 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(KvReadParams p, uint3
             }
 #pragma unroll
             for (int e = 0; e < kDims; ++e) f[e] = there[j] ? f[e] : 0.0f;
-            put<Out>(to, f);
+            if constexpr (sizeof(Out) == 4) {
+                put<kStream>(to, __builtin_bit_cast(kv_u4, kv_f4{f[0], f[1], f[2], f[3]}));
+            } else {
+                using E = KvElem<Out>;
+                put<kStream>(to, kv_u4{E::pack(f[0], f[1]), E::pack(f[2], f[3]), E::pack(f[4], f[5]), E::pack(f[6], f[7])});
+            }
         }
     }
 }
@@ -108,7 +116,11 @@ int launch_out(const KvReadParams &p, hipStream_t stream) {
     uint32_t lanes_log2 = 1;
     while (((uint32_t)kPer<Out> << lanes_log2) < p.c.dim) ++lanes_log2;
     const uint32_t per = ((uint32_t)kThreads >> lanes_log2) * kFlight, rows = (uint32_t)p.count * p.c.heads;
-    kv_read_kernel<T, kRows, Out><<<dim3((rows + per - 1u) / per, p.v ? 2u : 1u), kThreads, 0, stream>>>(p, lanes_log2);
+    const dim3 grid((rows + per - 1u) / per, p.v ? 2u : 1u);
+    if ((uint64_t)rows * p.c.dim * sizeof(Out) * grid.y > kStreamed)
+        kv_read_kernel<T, kRows, Out, true><<<grid, kThreads, 0, stream>>>(p, lanes_log2);
+    else
+        kv_read_kernel<T, kRows, Out, false><<<grid, kThreads, 0, stream>>>(p, lanes_log2);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 

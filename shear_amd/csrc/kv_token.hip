@@ -80,6 +80,25 @@ struct alignas(16) KvWords<8> {
     uint32_t w[8];
 };
 
+// kOnce: rows that no other workgroup reads need no place in the caches.
+template <int N, bool kOnce>
+__device__ __forceinline__ KvWords<N> load_words(const char *from) {
+    if constexpr (!kOnce) {
+        return *reinterpret_cast<const KvWords<N> *>(from);
+    } else {
+        KvWords<N> x;
+        if constexpr (N == 1) {
+            x.w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t *>(from));
+        } else {
+            using V = uint32_t __attribute__((ext_vector_type(N)));
+            const V y = __builtin_nontemporal_load(reinterpret_cast<const V *>(from));
+#pragma unroll
+            for (int i = 0; i < N; ++i) x.w[i] = y[i];
+        }
+        return x;
+    }
+}
+
 // Row id of visible index i < v.count, or -1 (a place of the list that names no further row).
 __device__ __forceinline__ int32_t visible_row(const KvVisible &v, uint32_t i, const int32_t *list) {
     if (i < v.first) return (int32_t)i;
@@ -192,7 +211,8 @@ __device__ __forceinline__ void find_sequence(const KvAttendParams &p, uint64_t 
 //  * kFormColumns4, kFormColumns8: besides, up to 4 or 8 query heads are repeated over the 16 columns of the
 //    instructions, and the parts of a weight (and of an fp16 query) have columns of their own, one or two products instead of
 //    three.  With the registers that this saves three waves fit a SIMD: the batch takes 80.5 us, the three long ones
-//    50.1 (two waves, each a tile ahead: 88.9 and 51.5).
+//    50.1 (two waves, each a tile ahead: 88.9 and 51.5).  No other workgroup reads their rows, so these pass the caches by,
+//    which saves the batch 6 us and the long ones 4 (of 8 heads the keys alone: the values too, 2 us more).
 enum { kFormAny = 0, kFormWhole = 1, kFormColumns4 = 2, kFormColumns8 = 3 };
 // Waves of a SIMD, by registers.
 constexpr int token_waves(int dp, int form) { return dp == 256 ? (form == kFormColumns4 ? 2 : 1) : form >= kFormColumns4 ? 3 : 2; }
@@ -433,14 +453,14 @@ __global__ __launch_bounds__(kThreads, token_waves(DP, kForm)) void kv_token_ker
             scales[t] = lane < kTile ? id * (uint32_t)c.keys.scale_page + slot * (uint32_t)c.keys.scale_row
                                      : id * (uint32_t)c.values.scale_page + slot * (uint32_t)c.values.scale_row;
 #pragma unroll
-            for (int s = 0; s < kKLoads; ++s) x.kw[t][s] = *reinterpret_cast<const KvWords<kKLoad> *>(k + koffset[s]);
+            for (int s = 0; s < kKLoads; ++s) x.kw[t][s] = load_words<kKLoad, kColumns>(k + koffset[s]);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const char *src = v + j * 4u * c.values.row_units * 16u + voffset;
                 if constexpr (kPer == 4)
                     x.vw[4 * t + j].w[0] = *reinterpret_cast<const uint16_t *>(src);
                 else
-                    x.vw[4 * t + j] = *reinterpret_cast<const KvWords<kVWords> *>(src);
+                    x.vw[4 * t + j] = load_words<kVWords, kForm == kFormColumns4>(src);
             }
         }
         group_scales(sbase + (soffset + (l32 & 16u ? scales[1] : scales[0])), x.bytes);
