@@ -22,7 +22,8 @@
 // workgroup walks the rows of one 64-byte column of a (sequence, head) in order,
 // reading a batch of rows into registers, waiting for all of it, and writing:
 // what a batch writes lies before every source of the later ones.  Columns
-// are independent, which is where the parallelism comes from.
+// are independent, which is where the parallelism comes from.  SQ8 scales move with a row's first
+// piece, the scale byte of 32 dims with their piece, which is 16 bytes of 4-bit codes.
 #include "kernel_attr.h"
 #include "kv_device.h"
 

@@ -31,6 +31,10 @@
 //  * SQ8 rows become 16-bit whole numbers on the way into LDS, exactly; scales
 //    enter as in kv_token.hip, the weights in bf16, for fp16 queries as the sum of
 //    two parts (one alone would be rounded to 8 bits, the result to 11).
+//  * 4-bit rows become 16-bit values on the way into LDS: bf16 with their scales, exactly, and no factor is left for logits
+//    or weights.  For fp16 queries keys are fp16 relative to the largest scale of their row, which multiplies the
+//    logit; values stay bf16, under weights of two parts.  The two prompts above take 168 us, 84 vector
+//    instructions of a wave and tile more than 16-bit rows.
 //  * A row that only some queries see may hold infinities or NaN, which would
 //    reach the others as 0 * inf.  In tiles with a mask such values go to LDS as zeros,
 //    and come back at the end for the queries that see them.
@@ -234,7 +238,8 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void kv_prompt_kernel(
     constexpr float kHuge = 4194304.0f;  // 2^22, rounded to a quarter
 
     // 4-bit rows: a piece becomes four of LDS, which a thread writes from its k_turn-th and v_turn-th on, so that 16 threads'
-    // writes meet all banks (a row's order of pieces alone left every fourth of them: two prompts of 4,096 tokens 170 us, so @@)
+    // writes meet all banks (a row's order of pieces alone left every fourth of them: two prompts of 4,096 tokens of 256 dims
+    // 562 us, so 537; of 128 170 and 168)
     const uint32_t k_turn = DP == 256 ? load_piece >> 2 << 1 : 0u;
     const uint32_t v_turn = (DP == 64 ? load_row >> 1 : DP == 128 ? load_row : (load_piece >> 2) + 2u * load_row) & 3u;
     auto turned_by = [](kv_u4 x, uint32_t by) {

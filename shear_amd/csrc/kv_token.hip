@@ -21,6 +21,8 @@
 //   48 sequences of up to 4,100 rows, with weights   533 MB   115 + 14 us   4.1 TB/s
 //   8 of up to 40,000 SQ8 rows, with weights         522 MB   122 + 15 us   3.8 TB/s
 //   one of 131,071 rows                              268 MB    52 +  7 us   4.5 TB/s
+//   64 of up to 8,200 rows of 4 bits                 372 MB    75 +  9 us   4.4 TB/s
+//   3 of up to 131,071, 4 bits, 4 heads, weights     170 MB    49 + 16 us   2.6 TB/s
 //   16, 2,016 rows each of which 1,500 are listed     49 MB    17 +  5 us   2.3 TB/s
 // (a copy reaches 4.9 to 5.5 TB/s here).  The last is a chain of dependent
 // reads, length, list, page, row, and then only two units a workgroup.
@@ -45,6 +47,10 @@
 //    The key's scale multiplies the logit, the value's the weight, after l has
 //    summed it; O is formed in bf16 whatever q's type is, because the scales of
 //    a cache can lie further apart than fp16 reaches (a row of zeros has scale 1).
+//  * 4-bit rows: a conversion makes two codes and their group's scale two bf16 values, exactly.  Four lanes take the
+//    four quarters of a key's row (dims are then summed in an order of their own, the query's with them), so that a lane has
+//    one group.  The weight's three parts are cut, not rounded: 8 bits each are all that f32 has.
+//    fp16 queries are two bf16 parts, exactly.
 //  * A row that the table leaves without a page, and a place of the list that
 //    names no further visible row, weighs nothing; its values are replaced by zeros
 //    (0 * NaN would be NaN).
