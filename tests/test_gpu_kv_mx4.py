@@ -233,6 +233,64 @@ def test_token_large_logits_and_scales_far_apart(gpu, q_type):
 
 
 @pytest.mark.parametrize("q_type", [BF16, F16])
+@pytest.mark.parametrize("group,dim", [(4, 64), (5, 128), (8, 256), (9, 64), (33, 32)])
+def test_token_many_sequences(gpu, q_type, group, dim):
+    """Lines of more sequences than a workgroup has threads, many of them short or empty, some pages missing."""
+    g = np.random.default_rng(group)
+    lengths = g.integers(0, 90, 300).tolist()
+    lengths[5], lengths[100], lengths[299] = 2000, 0, 700
+    pool, g = pool4_with(lengths, 1, 16, dim, q_type, 17)
+    pool.table_host[5, 7] = pool.table_host[40] = -1
+    pool.table_host[299, 40:42] = 10**9
+    pool.table = torch.from_numpy(pool.table_host).cuda()
+    q = normal(g, len(lengths), group, dim, dtype=q_type, scale=2)
+    out, lse = KV.attend_token(q, pool.cache, pool.table, lens(lengths))
+    check_token(pool, lengths, q, out, lse, None, 0)
+    # lengths out of range: none, and clipped to max_length
+    clipped = [-3 if n < 30 else 2**31 - 1 if n > 1000 else n for n in lengths]
+    out, lse = KV.attend_token(q, pool.cache, pool.table, lens(clipped), max_length=1500)
+    check_token(pool, [0 if n < 30 else min(n, 1500) for n in lengths], q, out, lse, None, 0)
+
+
+@pytest.mark.parametrize("q_type", [BF16, F16])
+def test_keys_and_values_of_different_layouts(gpu, q_type):
+    lengths, heads, dim, page = [300, 77], 3, 96, 32
+    pool, g = pool4_with(lengths, heads, page, dim, q_type, 19)
+    c = pool.cache
+
+    def other(t):  # rows first, room between them
+        b = t.view(torch.uint8)
+        wide = torch.full((b.shape[0], b.shape[2], b.shape[1], b.shape[3] + 16), 0xff, dtype=torch.uint8, device="cuda")
+        y = wide[..., : b.shape[3]].transpose(1, 2)
+        y.copy_(b)
+        return y.view(t.dtype)
+
+    mixed = KV.KvCache(c.keys, other(c.values), other(c.key_scales), c.value_scales)
+    q, pq = normal(g, 2, 6, dim, dtype=q_type), normal(g, 150, 6, dim, dtype=q_type)
+    w = [torch.zeros((2, heads, 320), device="cuda") for _ in range(2)]
+    a = KV.attend_token(q, c, pool.table, lens(lengths), weights=w[0])
+    b = KV.attend_token(q, mixed, pool.table, lens(lengths), weights=w[1])
+    for x, y in zip((*a, w[0]), (*b, w[1])):
+        assert torch.equal(x, y)
+    for x, y in zip(KV.attend_prompt(pq, lens([0, 100, 150]), c, pool.table, lens(lengths)),
+                    KV.attend_prompt(pq, lens([0, 100, 150]), mixed, pool.table, lens(lengths))):
+        assert torch.equal(x, y)
+    slots = torch.arange(c.keys.shape[0] * page, device="cuda")
+    for x, y in zip(KV.read(c, slots), KV.read(mixed, slots)):
+        assert torch.equal(x.nan_to_num(nan=9.0), y.nan_to_num(nan=9.0))
+    k, v = normal(g, 2, heads, dim, dtype=q_type), normal(g, 2, heads, dim, dtype=q_type)
+    for cache in (c, mixed):
+        KV.append(cache, pool.table, lens([31, 5]), k, v)
+    for x, y in zip(KV.read(c, slots), KV.read(mixed, slots)):
+        assert torch.equal(x.nan_to_num(nan=9.0), y.nan_to_num(nan=9.0))
+    kept = [KV.evict(cache, pool.table, lens(lengths), w[0], 50, sinks=2, recent=9) for cache in (c, mixed)]
+    for x, y in zip(*kept):
+        assert torch.equal(x, y)
+    for x, y in zip(KV.read(c, slots), KV.read(mixed, slots)):
+        assert torch.equal(x.nan_to_num(nan=9.0), y.nan_to_num(nan=9.0))
+
+
+@pytest.mark.parametrize("q_type", [BF16, F16])
 @pytest.mark.parametrize("group,page", [(3, 16), (3, 8), (8, 16), (20, 16)])
 def test_queries_that_are_not_finite(gpu, q_type, group, page):
     """An infinite query times keys of one sign is an infinite logit of that sign: of minus infinity nothing is left."""

@@ -92,7 +92,8 @@ def test_positions_padding_and_slots_that_are_none(gpu, interleaved):
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("kind", [SQ8, KV.MX4])
 @pytest.mark.parametrize("dim,heads,kv", [(128, 8, 2), (64, 4, 4), (96, 5, 1), (256, 2, 2), (32, 1, 3)])
-def test_codes_are_those_of_the_rounded_rows(gpu, dtype, kind, dim, heads, kv):
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_codes_are_those_of_the_rounded_rows(gpu, dtype, kind, dim, heads, kv, interleaved):
     g = np.random.default_rng(dim)
     pages, page, n = 20, 16, 200
     q, k, v, positions, slots = tokens_of(g, n, heads, kv, dim, dtype, pages, page, 5000)
@@ -103,8 +104,7 @@ def test_codes_are_those_of_the_rounded_rows(gpu, dtype, kind, dim, heads, kv):
     for c in (codes, again):
         for t in c._tensors():
             t.view(torch.uint8).zero_()
-    a = KV.append_rotated(plain, q, k, v, positions, slots, f, w, w)
-    b = KV.append_rotated(codes, q, k, v, positions, slots, f, w, w)
+    a, b = (KV.append_rotated(c, q, k, v, positions, slots, f, w, w, interleaved=interleaved) for c in (plain, codes))
     assert torch.equal(a, b)
     # the rounded rows, appended one by one where their slots say
     real = (positions >= 0).nonzero().squeeze(-1)
