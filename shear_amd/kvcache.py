@@ -380,45 +380,47 @@ def append_rotated(cache: KvCache, q: torch.Tensor, k: torch.Tensor, v: torch.Te
     ``q_weight``, ``k_weight`` ([head_dim], q's type or f32): x * rsqrt(mean x^2 + eps) * weight
     for each head; None: no norm.  ``frequencies`` (f64 [r / 2], r a multiple of 16; None: no
     rotation): pair i of the first r dims turns by positions (int32 [tokens]) *
-    frequencies[i] radians, dims (i, i + r / 2) or, ``interleaved``, (2i, 2i + 1).  All of it in f32 (angles in 64 bits) and rounded once, so that the rows are
-    what ``append`` makes of the rounded ones.  A token with a negative position is of no sequence:
-    its queries come back as zeros and nothing of it is written."""
+    frequencies[i] radians, dims (i, i + r / 2) or, ``interleaved``, (2i, 2i + 1).  All of it in f32
+    (angles in 64 bits) and rounded once, so that the rows are what ``append`` makes of the rounded
+    ones.  A token with a negative position is of no sequence: its queries come back as zeros and
+    nothing of it is written."""
     dev, native = cache.keys.device, cache._native
-    _no_gradient(cache, k, v)
-    _no_gradient(cache, q)
-    kind = _QUERY_TYPES.get(q.dtype)
-    if q.dim() != 3 or kind is None or q.device != dev:
+    _no_gradient(cache, q, k)
+    index, dtype = dev.index, q.dtype
+    kind = _QUERY_TYPES.get(dtype)
+    if q.dim() != 3 or kind is None or q.get_device() != index:
         raise ValueError(f"q must be bf16 or fp16 [tokens, q_heads, head_dim] on {dev}")
     if kind != native.type and native.type not in (N.KV_SQ8, N.KV_MX4):
-        raise ValueError(f"q is {q.dtype}, the cache {cache.keys.dtype}")
+        raise ValueError(f"q is {dtype}, the cache {cache.keys.dtype}")
     tokens, heads, dim = q.shape
     if dim != native.head_dim or heads == 0:
         raise ValueError(f"q of {heads} heads x {dim} for a cache of {cache.heads} heads x {cache.head_dim}")
-    shape = (tokens, native.heads, dim)
+    shape, each = (tokens, native.heads, dim), (tokens,)
     for t, name in ((k, "k"), (v, "v")):
-        if t.dtype != q.dtype or t.shape != shape or t.device != dev:
-            raise ValueError(f"{name} must be {q.dtype} {list(shape)} on {dev}")
-    index = dev.index
-    if not (_is(positions, _INT, (tokens,), index) and _is(slots, torch.int64, (tokens,), index)):
-        _check(positions, "positions", _INT, (tokens,), dev)
-        _check(slots, "slots", torch.int64, (tokens,), dev)
-    rotated = 0
+        if t.dtype is not dtype or t.shape != shape or t.get_device() != index:
+            raise ValueError(f"{name} must be {dtype} {list(shape)} on {dev}")
+    if not (_is(positions, _INT, each, index) and _is(slots, torch.int64, each, index)):
+        _check(positions, "positions", _INT, each, dev)
+        _check(slots, "slots", torch.int64, each, dev)
+    rotated, turns = 0, None
     if frequencies is not None:
-        _check(frequencies, "frequencies", torch.float64, (None,), dev)
-        _no_gradient(cache, frequencies)
-        rotated = 2 * frequencies.shape[0]
+        if not _is(frequencies, torch.float64, (frequencies.numel(),), index):
+            _check(frequencies, "frequencies", torch.float64, (None,), dev)
+        rotated, turns = 2 * frequencies.shape[0], frequencies.data_ptr()
         if rotated % 16 or rotated > dim:
             raise ValueError(f"{rotated} rotated dims must be a multiple of 16 up to {dim}")
-    weight_type, weights = q.dtype, [0, 0]
+    weight_type, weights = dtype, [0, 0]
     for i, w in enumerate((q_weight, k_weight)):
         if w is not None:
-            weight_type = w.dtype if w.dtype is torch.float32 else q.dtype
+            weight_type = w.dtype if w.dtype is torch.float32 else dtype
             if not _is(w, weight_type, (dim,), index):
                 _check(w, "k_weight" if i else "q_weight", weight_type, (dim,), dev)
-            _no_gradient(cache, w)
             weights[i] = w.data_ptr()
     if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
         raise ValueError(f"q_weight is {q_weight.dtype}, k_weight {k_weight.dtype}")
+    for t in (v, frequencies, q_weight, k_weight):
+        if t is not None and t.requires_grad:
+            _no_gradient(cache, t)
     if not (eps >= 0.0 and math.isfinite(eps)):
         raise ValueError(f"eps {eps} must be finite and not negative")
     on, handle = _on(stream, dev, (*cache._tensors(), q, k, v, positions, slots, frequencies, q_weight, k_weight))
@@ -430,9 +432,8 @@ def append_rotated(cache: KvCache, q: torch.Tensor, k: torch.Tensor, v: torch.Te
         out = torch.empty(tokens, heads, dim, dtype=q.dtype, device=dev)
         a = N.KvRotated(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q.stride()[:2], k.stride()[:2],
                         v.stride()[:2], (heads * dim, dim), positions.data_ptr(), slots.data_ptr(),
-                        None if frequencies is None else frequencies.data_ptr(),
-                        weights[0] or None, weights[1] or None, tokens, kind, _VALUE_TYPES[weight_type], heads, rotated,
-                        int(interleaved), eps)
+                        turns, weights[0] or None, weights[1] or None, tokens, kind, _VALUE_TYPES[weight_type],
+                        heads, rotated, int(interleaved), eps)
         N.check(N.load().tessa_kv_append_rotated(C.byref(native), C.byref(a), handle), "kv append rotated")
     return out
 
@@ -494,15 +495,18 @@ def plan(page_rows: int, page_table: torch.Tensor, lengths: torch.Tensor, held: 
         raise ValueError(f"page_rows must be a power of two in 1..65536, got {page_rows}")
     if not 0 <= tokens < 2**31:
         raise ValueError(f"tokens {tokens} is outside 0..2^31 - 1")
-    _check(page_table, "page_table", _INT, (None, None), dev)
+    i = dev.index
+    if not (page_table.dim() == 2 and _is(page_table, _INT, page_table.shape, i)):
+        _check(page_table, "page_table", _INT, (None, None), dev)
     batch, columns = page_table.shape
-    i, each = dev.index, (batch,)
+    each = (batch,)
     if not (_is(lengths, _INT, each, i) and _is(held, _INT, each, i) and _is(new, _INT, each, i)
             and _is(count, _INT, (1,), i)):
         for t, name, shape in ((lengths, "lengths", each), (held, "held", each), (new, "new", each),
                                (count, "count", (1,))):
             _check(t, name, _INT, shape, dev)
-    _check(free, "free", _INT, (None,), dev)
+    if not _is(free, _INT, (free.numel(),), i):
+        _check(free, "free", _INT, (None,), dev)
     on, handle = _on(stream, dev, (page_table, lengths, held, new, free, count))
     with on:
         slots = torch.empty(tokens, dtype=torch.int64, device=dev)
@@ -512,7 +516,7 @@ def plan(page_rows: int, page_table: torch.Tensor, lengths: torch.Tensor, held: 
         ints = (at, at + 4 * batch, at + 8 * batch, at + 8 * batch + 4, at + 12 * batch + 4, at + 16 * batch + 8,
                 at + 16 * batch + 8 + 4 * tokens)
         a = N.KvStep(page_table.data_ptr(), page_table.stride(0) if batch > 1 else columns, lengths.data_ptr(),
-                     held.data_ptr(), new.data_ptr(), free.data_ptr(), count.data_ptr(), *ints, slots.data_ptr(), tokens,
-                     batch, columns, free.shape[0], page_rows)
+                     held.data_ptr(), new.data_ptr(), free.data_ptr(), count.data_ptr(), *ints, slots.data_ptr(),
+                     tokens, batch, columns, free.shape[0], page_rows)
         N.check(N.load().tessa_kv_plan(C.byref(a), handle), "kv plan")
     return Plan(*parts, slots)
