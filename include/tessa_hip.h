@@ -896,7 +896,7 @@ tessa_status tessa_graph_search_sq8(const int8_t *codes, const float *scales, ui
  * output capacities (max_leaf_count, max_leaf_rows) size the session's device
  * outputs.  wait blocks until the job is done and returns its status; the
  * result arrays stay valid until tessa_session_release(seq).  Other session
- * calls wait for a running job. */
+ * calls run after the jobs submitted before them, started or not. */
 typedef struct tessa_subtree_host_result {
     const uint32_t *leaf_row_ids;   /* pinned host, leaf_rows (resident rows) */
     const uint64_t *leaf_starts;    /* leaf_count */

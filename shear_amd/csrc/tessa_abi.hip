@@ -759,6 +759,26 @@ namespace {
 
 void stop_async(tessa_session *s);  // asynchronous submissions, below
 
+// A synchronous call's turn on the session: after the jobs submitted before it.
+// exec_mu alone does not give that order: between a submission and the moment
+// its worker wakes and takes exec_mu, a call would run ahead of the job, on the
+// rows of the upload before.  Jobs submitted during the wait are not waited for.
+struct SyncCall {
+    std::unique_lock<std::mutex> exec;
+    explicit SyncCall(tessa_session *s) {
+        {
+            std::unique_lock<std::mutex> lk(s->q_mu);
+            const uint64_t next = s->next_seq;
+            s->q_cv.wait(lk, [s, next] {
+                for (const auto &slot : s->slots)
+                    if (slot.state == 1 && slot.seq < next) return false;
+                return true;
+            });
+        }
+        exec = std::unique_lock<std::mutex>(s->exec_mu);
+    }
+};
+
 void free_sq8(tessa_session *s) {
     if (s->codes) (void)hipFree(s->codes);
     if (s->scales) (void)hipFree(s->scales);
@@ -886,7 +906,7 @@ static tessa_status tessa_session_upload_sq8_locked(tessa_session *s, const tess
 
 tessa_status tessa_session_upload_sq8(tessa_session *s, const tessa_sq8_view *host) {
     if (!s) return make_status(TESSA_ERR_INVALID_ARGUMENT, 0, "session is null");
-    std::lock_guard<std::mutex> lock(s->exec_mu);
+    SyncCall call(s);
     return tessa_session_upload_sq8_locked(s, host);
 }
 
@@ -955,7 +975,7 @@ tessa_status tessa_session_leaf_topk(tessa_session *s, const uint32_t *members, 
                                      uint32_t leaf_count, uint32_t k, uint32_t executor, uint32_t *out_ids,
                                      float *out_dists, uint64_t *counters, float *event_ms) {
     if (!s) return make_status(TESSA_ERR_INVALID_ARGUMENT, 0, "session is null");
-    std::lock_guard<std::mutex> lock(s->exec_mu);
+    SyncCall call(s);
     return tessa_session_leaf_topk_locked(s, members, member_offsets, member_counts, output_offsets, leaf_count, k,
                                           executor, out_ids, out_dists, counters, event_ms);
 }
@@ -1046,7 +1066,7 @@ tessa_status tessa_session_assign_replay(tessa_session *s, const uint32_t *membe
                                          const uint32_t *r_h, const uint64_t *output_offsets, uint32_t task_count,
                                          uint32_t *out_ids, float *out_dists, uint64_t *counters, float *event_ms) {
     if (!s) return make_status(TESSA_ERR_INVALID_ARGUMENT, 0, "session is null");
-    std::lock_guard<std::mutex> lock(s->exec_mu);
+    SyncCall call(s);
     return tessa_session_assign_replay_locked(s, members, leaders, member_offsets, member_counts, leader_offsets,
                                              leader_counts, r_h, output_offsets, task_count, out_ids, out_dists,
                                              counters, event_ms);
@@ -1371,7 +1391,7 @@ static tessa_status tessa_session_run_subtree_locked(tessa_session *s, const tes
 
 tessa_status tessa_session_run_subtree(tessa_session *s, const tessa_subtree_request *rq, tessa_subtree_output *out) {
     if (!s) return make_status(TESSA_ERR_INVALID_ARGUMENT, 0, "session is null");
-    std::lock_guard<std::mutex> lock(s->exec_mu);
+    SyncCall call(s);
     return tessa_session_run_subtree_locked(s, rq, out);
 }
 
@@ -1611,14 +1631,14 @@ static tessa_status tessa_session_partition_small_roots_locked(tessa_session *s,
 tessa_status tessa_session_partition_roots(tessa_session *s, const tessa_sq8_view *sq8, const tessa_roots_request *rq,
                                            tessa_roots_output *out) {
     if (!s) return make_status(TESSA_ERR_INVALID_ARGUMENT, 0, "session is null");
-    std::lock_guard<std::mutex> lock(s->exec_mu);
+    SyncCall call(s);
     return tessa_session_partition_roots_locked(s, sq8, rq, out);
 }
 
 tessa_status tessa_session_partition_small_roots(tessa_session *s, const tessa_sq8_view *sq8,
                                                  const tessa_roots_request *rq, tessa_roots_output *out) {
     if (!s) return make_status(TESSA_ERR_INVALID_ARGUMENT, 0, "session is null");
-    std::lock_guard<std::mutex> lock(s->exec_mu);
+    SyncCall call(s);
     return tessa_session_partition_small_roots_locked(s, sq8, rq, out);
 }
 
@@ -1875,7 +1895,7 @@ tessa_status tessa_session_wait(tessa_session *s, uint64_t seq, tessa_subtree_ho
 
 tessa_status tessa_session_set_assignment_capture(tessa_session *s, uint32_t min_members) {
     if (!s) return make_status(TESSA_ERR_INVALID_ARGUMENT, 0, "session is null");
-    std::lock_guard<std::mutex> lock(s->exec_mu);
+    SyncCall call(s);
     s->capture_min_members = min_members;
     s->capture.tasks.clear();
     s->capture.rows.clear();
@@ -1886,7 +1906,7 @@ tessa_status tessa_session_captured_assignments(tessa_session *s, tessa_captured
                                                 uint64_t task_capacity, uint32_t *ids, uint64_t id_capacity,
                                                 uint64_t *task_count, uint64_t *id_count) {
     if (!s || !task_count || !id_count) return make_status(TESSA_ERR_INVALID_ARGUMENT, 0, "capture: null argument");
-    std::lock_guard<std::mutex> lock(s->exec_mu);
+    SyncCall call(s);
     *task_count = s->capture.tasks.size();
     *id_count = s->capture.rows.size();
     if (!tasks && !ids) return ok_status();
