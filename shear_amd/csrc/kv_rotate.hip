@@ -141,12 +141,15 @@ __global__ __launch_bounds__(kThreads) void kv_rotate_kernel(KvRotateParams p, u
             f[place_of(db)] = float2{wb * cosine, wa * sine};
         }
     }
-    const uint32_t still = c.dim - 2u * p.half;  // dims that do not turn
+    // dims that do not turn, and those of the lanes past the row: an SQ8 row's scale is made of all its lanes, so these must be
+    // zeros and not what an earlier kernel left here
+    const uint32_t still = kDims - 2u * p.half;
     for (uint32_t i = t; i < n * still; i += kThreads) {
         const uint32_t k = i / still, at = 2u * p.half + i - k * still;
 #pragma unroll
         for (int kind = 0; kind < 2; ++kind)
-            sh_factor[(2u * k + kind) * kDims + place_of(at)] = float2{weight(kind ? p.k_weight : p.q_weight, at), 0.0f};
+            sh_factor[(2u * k + kind) * kDims + place_of(at)] =
+                float2{at < c.dim ? weight(kind ? p.k_weight : p.q_weight, at) : 0.0f, 0.0f};
     }
     __syncthreads();
     const bool turned = inside && d < 2u * p.half;
