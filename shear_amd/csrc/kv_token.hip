@@ -583,10 +583,13 @@ __global__ __launch_bounds__(kThreads, token_waves(DP, kForm)) void kv_token_ker
                 for (int i = 0; i < 4; ++i) x[t][i] = sacc[i] * ks[i];
             } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[t][i] = sacc[i] * (kMx4 ? 1.0f : p.scale_log2);
-                if constexpr (kSplitQuery && kColumns)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x[t][i] += turned<8>(x[t][i]);
+                for (int i = 0; i < 4; ++i) {
+                    float logit = sacc[i];
+                    if constexpr (kSplitQuery && kColumns) logit += turned<8>(logit);
+                    // rounded once: the maximum, the weights and the stored logits are of one number.  (With the scale in the weight's
+                    // own difference a large logit's rounding became a factor of its weight; 4-bit rows are no faster so.)
+                    x[t][i] = logit * p.scale_log2;
+                }
             }
         }
         if (valid != 0xffffffffu) {
@@ -608,17 +611,15 @@ __global__ __launch_bounds__(kThreads, token_waves(DP, kForm)) void kv_token_ker
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t r = row_in(16 * t + 4 * g + i);
-                    if (head_ok && n < kColumnHeads && tile * kTile + r < rows) at[(uint64_t)r * p.group] = kMx4 ? x[t][i] * p.scale_log2 : x[t][i];
+                    if (head_ok && n < kColumnHeads && tile * kTile + r < rows) at[(uint64_t)r * p.group] = x[t][i];
                 }
         }
-        // (4-bit rows: the scale comes with the difference from the maximum, one instruction for both)
-        float top = kMx4 ? -INFINITY : kKvNone;
+        float top = kKvNone;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, x[t][i]);
         top = kv_max16(top);
-        if constexpr (kMx4) top *= p.scale_log2;
         if (__any(top > m + kTop)) {
             const float higher = fmaxf(m, top - kLift);
             const float f = kv_exp2(m - higher);
@@ -637,8 +638,7 @@ __global__ __launch_bounds__(kThreads, token_waves(DP, kForm)) void kv_token_ker
             if constexpr (kSq8) vs = *reinterpret_cast<const kv_f4 *>(&sh_scale[wave][1][16 * t + 4 * g]);
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
-                float w0 = kv_exp2(kMx4 ? fmaf(x[t][i], p.scale_log2, -m) : x[t][i] - m);
-                float w1 = kv_exp2(kMx4 ? fmaf(x[t][i + 1], p.scale_log2, -m) : x[t][i + 1] - m);
+                float w0 = kv_exp2(x[t][i] - m), w1 = kv_exp2(x[t][i + 1] - m);
                 l += w0 + w1;
                 if constexpr (kSq8) {
                     w0 *= vs[i];
