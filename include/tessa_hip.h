@@ -1116,6 +1116,8 @@ tessa_status tessa_kv_read(const tessa_kv_cache *cache, const tessa_kv_rows *row
  *    need is there; else it gets no new rows.  Others that need none are served all the same.
  * new_lengths, new_held, new_count and granted say how it went; the table's new ids and the stack's are
  * written in place, and what lies past them is left as it was (ids past new_held are not the sequence's).
+ * Arrays that are written (the table, the stack and all results) share no memory with each other or with an argument; a
+ * step whose arrays overlap is refused.
  * For each of `tokens` places: the position (row) of the token, its sequence and its slot (page * page_rows + row of the
  * page); -1 past the last token, position and slot -1 too where the token was not granted. */
 typedef struct tessa_kv_step {

@@ -297,6 +297,44 @@ tessa_status attend(const tessa_kv_cache *cache, const tessa_kv_sequences *seq, 
     return fine();
 }
 
+// Whether the arrays of a step lie apart: workgroups read the arguments, and the table's held pages and the stack,
+// while others write, so what is written may share no memory with anything else.
+tessa_status apart(const tessa_kv_step &s) {
+    struct Array {
+        const char *name;
+        const void *at;
+        uint64_t bytes;
+    };
+    const uint64_t each = 4ull * s.batch, places = 4ull * s.tokens;
+    constexpr int kWritten = 9;
+    const Array arrays[] = {{"free", s.free, 4ull * s.pages},       {"new_lengths", s.new_lengths, each},
+                            {"new_held", s.new_held, each},         {"new_count", s.new_count, 4},
+                            {"granted", s.granted, each},           {"offsets", s.offsets, each + 4},
+                            {"positions", s.positions, places},     {"sequences", s.sequences, places},
+                            {"slots", s.slots, 2 * places},         {"lengths", s.lengths, each},
+                            {"held", s.held, each},                 {"fresh", s.fresh, each},
+                            {"count", s.count, 4}};
+    constexpr int kArrays = sizeof(arrays) / sizeof(arrays[0]);
+    const uintptr_t table = reinterpret_cast<uintptr_t>(s.table);
+    const uint64_t row = 4ull * s.columns, stride = 4ull * s.table_stride;
+    if (s.batch > 1 && s.table_stride >= (1ull << 40)) KV_INVALID("kv plan: table stride %llu", (unsigned long long)s.table_stride);
+    for (int i = 0; i < kArrays; ++i) {
+        const uintptr_t from = reinterpret_cast<uintptr_t>(arrays[i].at), to = from + arrays[i].bytes;
+        if (!arrays[i].bytes) continue;
+        for (int j = 0; j < i && j < kWritten; ++j) {
+            const uintptr_t other = reinterpret_cast<uintptr_t>(arrays[j].at);
+            if (from < other + arrays[j].bytes && other < to)
+                KV_INVALID("kv plan: %s overlap %s: results may not be the arguments", arrays[j].name, arrays[i].name);
+        }
+        if (!row) continue;
+        // (other arrays may lie between the table's rows) the first of them that ends behind the array's begin
+        const uint64_t first = from < table + row || s.batch <= 1 ? 0 : (from - table - row) / stride + 1;
+        if (first < s.batch && table + first * stride < to && from < table + first * stride + row)
+            KV_INVALID("kv plan: the table overlaps %s: results may not be the arguments", arrays[i].name);
+    }
+    return fine();
+}
+
 // The C boundary: nothing is thrown across it.
 template <typename F>
 tessa_status guarded(F &&f) {
@@ -513,8 +551,8 @@ tessa_status tessa_kv_plan(const tessa_kv_step *s, void *stream) {
         if (s->batch > 1 && s->table_stride < s->columns)
             KV_INVALID("kv plan: table stride %llu below %u columns", (unsigned long long)s->table_stride, s->columns);
         if (s->tokens && (!s->positions || !s->sequences || !s->slots)) KV_INVALID("kv plan: null pointer");
-        if ((s->batch && (s->new_lengths == s->lengths || s->new_held == s->held)) || s->new_count == s->count)
-            KV_INVALID("kv plan: results may not be the arguments");
+        const tessa_status st = apart(*s);
+        if (st.code) return st;
         KvPlanParams p;
         std::memset(&p, 0, sizeof(p));
         p.table = s->table;

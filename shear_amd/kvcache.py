@@ -486,8 +486,9 @@ def plan(page_rows: int, page_table: torch.Tensor, lengths: torch.Tensor, held: 
     to the stack, then each that needs more gets them from its top, if what all up to it need is there.
     One that does not get its pages, or whose rows would pass the table's columns or tokens ``tokens``, is
     granted nothing: its tokens' places are -1 and its length stays (a prompt's attention of such tokens says
-    nothing).  The table and the stack are changed in place; the lengths, held pages and count that go with them are
-    the result's, and take the arguments' place in the next step."""
+    nothing).  The table and the stack are changed in place, so they share no memory with each other or with other
+    arguments; the lengths, held pages and count that go with them are the result's, and take the arguments' place in the
+    next step."""
     dev = lengths.device
     if not lengths.is_cuda:
         raise ValueError("lengths must be a device tensor")
