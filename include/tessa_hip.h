@@ -1067,7 +1067,7 @@ tessa_status tessa_kv_evict(const tessa_kv_cache *cache, const tessa_kv_sequence
  *   (a, b) -> (a cos t - b sin t, a sin t + b cos t),  t = position * frequencies[i]
  * for the pairs i < rotated / 2 of dims (i, i + rotated / 2), or (2 i, 2 i + 1) with `interleaved`;
  * dims from `rotated` on stay.  t is formed in 64 bits, the rest in f32, rounded once to `type`.  q's rows go to `out`
- * (it may be q), k's and v's (v as it is) to row slots[token] % page_rows of page slots[token] / page_rows, as
+ * (it may be q, with q's strides, and shares no memory with q, k or v else), k's and v's (v as it is) to row slots[token] % page_rows of page slots[token] / page_rows, as
  * tessa_kv_append writes them.  A slot outside the cache is not written; a token whose position is
  * negative is of no sequence: nothing of it is written and its rows of `out` are zeros.  No two tokens may have the
  * same slot. */

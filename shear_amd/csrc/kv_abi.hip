@@ -492,6 +492,10 @@ tessa_status tessa_kv_append_rotated(const tessa_kv_cache *cache, const tessa_kv
         p.out = static_cast<char *>(t->out);
         p.out_token = b[0];
         p.out_head = b[1];
+        // (a row of out may be written before another workgroup has read its rows of k and v)
+        if (t->out == t->k || t->out == t->v) KV_INVALID("kv append rotated: out may be q, but not k or v");
+        if (t->out == t->q && (p.out_token != p.q_token || (t->q_heads > 1 && p.out_head != p.q_head)))
+            KV_INVALID("kv append rotated: out is q with other strides");
         if (p.q_head > 0xffffffffull || p.k_head > 0xffffffffull || p.v_head > 0xffffffffull || p.out_head > 0xffffffffull)
             KV_UNSUPPORTED("kv append rotated: heads lie more than 4 GiB apart");
         if (!t->positions || !t->slots) KV_INVALID("kv append rotated: null positions or slots");
