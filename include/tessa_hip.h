@@ -1093,7 +1093,7 @@ typedef struct tessa_kv_rotated {
 tessa_status tessa_kv_append_rotated(const tessa_kv_cache *cache, const tessa_kv_rotated *tokens, void *stream);
 
 /* Rows by place, as values of `type` (bf16, fp16 or f32): k and v (null: keys
- * only) get count x heads x head_dim values, contiguous, of row slots[i] % page_rows of page slots[i] /
+ * only), which may not overlap, get count x heads x head_dim values, contiguous, of row slots[i] % page_rows of page slots[i] /
  * page_rows; zeros where the slot is outside the cache. */
 typedef struct tessa_kv_rows {
     const int64_t *slots;

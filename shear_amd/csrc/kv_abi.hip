@@ -530,6 +530,9 @@ tessa_status tessa_kv_read(const tessa_kv_cache *cache, const tessa_kv_rows *r, 
             KV_UNSUPPORTED("kv read: %llu rows of %u heads", (unsigned long long)r->count, p.c.heads);
         if (!r->slots || !r->k) KV_INVALID("kv read: null pointer");
         if (!aligned16(r->k) || !aligned16(r->v)) KV_INVALID("kv read: k and v are not 16-byte aligned");
+        const uint64_t bytes = r->count * p.c.heads * p.c.dim * (r->type == TESSA_KV_F32 ? 4u : 2u);
+        const uintptr_t k = reinterpret_cast<uintptr_t>(r->k), v = reinterpret_cast<uintptr_t>(r->v);
+        if (v && k < v + bytes && v < k + bytes) KV_INVALID("kv read: k and v overlap");
         p.slots = r->slots;
         p.k = static_cast<char *>(r->k);
         p.v = static_cast<char *>(r->v);
