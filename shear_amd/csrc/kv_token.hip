@@ -212,22 +212,30 @@ __device__ __forceinline__ void find_sequence(const KvAttendParams &p, uint64_t 
 // Forms of the kernel over 4-bit rows.  A wave issues an instruction each 5 cycles at most and waits for its own
 // results, so two waves of a SIMD, all that the registers of kFormAny leave, take as long for the instructions
 // alone (70 us for the batch of 64 above, its rows in the cache) as the memory does (72), and 100 for both.
-//  * kFormWhole: 16 rows of a tile lie in one page, one after the other (all rows visible, pages of at
-//    least 16), so that their addresses are a scalar and a lane's constant.
-//  * kFormColumns4, kFormColumns8: besides, up to 4 or 8 query heads are repeated over the 16 columns of the
-//    instructions, and the parts of a weight (and of an fp16 query) have columns of their own, one or two products instead of
-//    three.  With the registers that this saves three waves fit a SIMD: the batch takes 80.5 us, the three long ones
-//    50.1 (two waves, each a tile ahead: 88.9 and 51.5).  No other workgroup reads their rows, so these pass the caches by,
-//    which saves the batch 6 us and the long ones 4 (of 8 heads the keys alone: the values too, 2 us more).
-enum { kFormAny = 0, kFormWhole = 1, kFormColumns4 = 2, kFormColumns8 = 3 };
+// Where 16 rows of a tile lie in one page, one after the other (all rows visible, pages of at least 16), addresses are a
+// scalar and a lane's constant, and up to 4 or 8 query heads are repeated over the 16 columns of the instructions, so that the
+// parts of a weight (and of an fp16 query) have columns of their own, one or two products instead of three.
+//  * kFormColumns4: with the registers that this saves three waves fit a SIMD (two at 256 dims).
+//  * kFormColumns8: likewise at 128 dims.
+// These pass the caches by (of 8 heads the keys alone: the values too cost 2 us).
+// Microseconds of a call, bf16, in columns and in kFormAny (a window that shows every row):
+//                                           64 dims       128 dims      256 dims
+//   64 sequences of up to 8,200 rows,  4 heads  65, 66    82, 92        81, 103 (32 sequences)
+//                                      8        74, 72    90, 100      128, 109
+//   3 of up to 131,071,                4        48, 50    60, 66       105, 133
+//                                      8        51, 50    64, 67       174, 136
+// Past 8 heads the scalar addresses alone took as long as kFormAny or up to a tenth longer.  Rows that no other workgroup
+// reads need no place in the caches: 64 sequences of 8,200 rows each 117 us, through the caches 126.  Sequences that share pages
+// read them from memory more often for it: 98 and 94 with all of them in common, 105 and 102 with half.
+enum { kFormAny = 0, kFormColumns4 = 1, kFormColumns8 = 2 };
 // Waves of a SIMD, by registers.
-constexpr int token_waves(int dp, int form) { return dp == 256 ? (form == kFormColumns4 ? 2 : 1) : form >= kFormColumns4 ? 3 : 2; }
+constexpr int token_waves(int dp, int form) { return dp == 256 ? (form != kFormAny ? 2 : 1) : form != kFormAny ? 3 : 2; }
 
 // kDirect: one workgroup for each column of rows, which writes the result; else
 // workers and parts.
 template <typename T, int kRowsKind, int DP, bool kDirect, int kForm>
 __global__ __launch_bounds__(kThreads, token_waves(DP, kForm)) void kv_token_kernel(KvAttendParams p) {
-    constexpr bool kWhole = kForm != kFormAny, kColumns = kForm >= kFormColumns4;
+    constexpr bool kColumns = kForm != kFormAny;
     constexpr uint32_t kColumnHeads = kForm == kFormColumns4 ? 4 : kForm == kFormColumns8 ? 8 : 16;
     constexpr bool kSq8 = kRowsKind == kRowsSq8, kMx4 = kRowsKind == kRowsMx4;
     using E = KvElem<T>;
@@ -317,21 +325,21 @@ __global__ __launch_bounds__(kThreads, token_waves(DP, kForm)) void kv_token_ker
     }
     bool again = false;
     while (unit < unit_end) {
-    if constexpr (kWhole) {  // the same for all lanes, which the compiler cannot see: scalar registers
+    if constexpr (kColumns) {  // the same for all lanes, which the compiler cannot see: scalar registers
         b = uniform(b);
         column = uniform(column);
         unit = uniform(unit);
         unit_end = uniform(unit_end);
         line = uniform(line);
     }
-    const uint32_t h = kWhole ? uniform(column / blocks) : column / blocks, first_q = (column - h * blocks) * 16u;
+    const uint32_t h = kColumns ? uniform(column / blocks) : column / blocks, first_q = (column - h * blocks) * 16u;
     const uint32_t heads = min(16u, p.group - first_q);
     const KvVisible vis = kv_visible(p, kv_length(c, b));
     const uint32_t units = (vis.count + kUnit - 1) / kUnit;
     const uint32_t begin0 = kDirect ? 0u : (uint32_t)(unit - line) * kUnit;
-    const uint32_t begin = kWhole ? uniform(begin0) : begin0;
+    const uint32_t begin = kColumns ? uniform(begin0) : begin0;
     const uint32_t end0 = kDirect ? vis.count : min(vis.count, begin + (uint32_t)min(unit_end - unit, (uint64_t)units) * kUnit);
-    const uint32_t end = kWhole ? uniform(end0) : end0;
+    const uint32_t end = kColumns ? uniform(end0) : end0;
     const uint32_t rows = end > begin ? end - begin : 0u;
     const uint32_t tiles = (rows + kTile - 1) / kTile;
     const int32_t *list = p.listed ? p.listed + ((uint64_t)b * c.heads + h) * p.listed_count : nullptr;
@@ -400,12 +408,12 @@ __global__ __launch_bounds__(kThreads, token_waves(DP, kForm)) void kv_token_ker
     };
     auto page_of = [&](int32_t row) -> int32_t { return row >= 0 ? table[(uint32_t)row >> c.page_shift] : -1; };
     int32_t row = -1, page = -1, next_row = -1;
-    // kWhole: page of the lane's half of a tile; the lane's place in 16 rows
+    // kColumns: page of the lane's half of a tile; the lane's place in 16 rows
     auto tile_page = [&](uint32_t tile) { return table[min(begin + tile * kTile + (l32 & 16u), end - 1u) >> c.page_shift]; };
-    uint32_t koffset[kWhole ? kKLoads : 1], voffset = 0, soffset = 0;
+    uint32_t koffset[kColumns ? kKLoads : 1], voffset = 0, soffset = 0;
     const uint8_t *sbase = nullptr;
-    const uint32_t wave0 = kWhole ? uniform(wave) : wave;
-    if constexpr (kWhole) {
+    const uint32_t wave0 = kColumns ? uniform(wave) : wave;
+    if constexpr (kColumns) {
 #pragma unroll
         for (int s = 0; s < kKLoads; ++s) {
             const uint32_t d = (uint32_t)s * 4u * kKDims + g * kKDims;
@@ -445,7 +453,7 @@ __global__ __launch_bounds__(kThreads, token_waves(DP, kForm)) void kv_token_ker
     };
     // Starts the loads of a tile.
     auto fetch = [&](uint32_t tile, Tile &x) __attribute__((always_inline)) {
-      if constexpr (kWhole) {
+      if constexpr (kColumns) {
         const uint32_t at = begin + tile * kTile, slots = 1u << c.page_shift;
         const bool there = (uint32_t)page < c.pages;
         x.valid = (uint32_t)__ballot(there && tile * kTile + row_in(l32) < rows);
@@ -529,7 +537,7 @@ __global__ __launch_bounds__(kThreads, token_waves(DP, kForm)) void kv_token_ker
         auto &vw = here.vw;
         const uint32_t valid = here.valid;
         if constexpr (kMx4) {
-            if (kWhole && valid != 0xffffffffu) {  // what lies where no row is: 0 * NaN would be NaN
+            if (kColumns && valid != 0xffffffffu) {  // what lies where no row is: 0 * NaN would be NaN
                 asm volatile("");
 #pragma unroll
                 for (int w = 0; w < (kMxGroups + 3) / 4; ++w) here.bytes[w] = valid >> l32 & 1u ? here.bytes[w] : 0x7f7f7f7fu;
@@ -1070,7 +1078,8 @@ int token_form(const KvAttendParams &p) {
     // (16 rows within 2^28 bytes: their offsets are 32-bit)
     if (!p.c.mx4 || p.window != 0xffffffffu || p.c.page_shift < 4u || p.c.keys.row_units > 1u << 20 || p.c.values.row_units > 1u << 20)
         return kFormAny;
-    return p.group <= 4u ? kFormColumns4 : p.group <= 8u ? kFormColumns8 : kFormWhole;
+    if (p.group <= 4u) return kFormColumns4;
+    return p.group <= 8u && kv_padded_dim(p.c.dim) == 128u ? kFormColumns8 : kFormAny;
 }
 
 template <typename T, int kRowsKind, int DP>
@@ -1078,8 +1087,8 @@ int launch(const KvAttendParams &p, hipStream_t stream) {
     if constexpr (kRowsKind == kRowsMx4) {
         const int form = token_form(p);
         if (form == kFormColumns4) return launch_form<T, kRowsKind, DP, kFormColumns4>(p, stream);
-        if (form == kFormColumns8) return launch_form<T, kRowsKind, DP, kFormColumns8>(p, stream);
-        if (form == kFormWhole) return launch_form<T, kRowsKind, DP, kFormWhole>(p, stream);
+        if constexpr (DP == 128)
+            if (form == kFormColumns8) return launch_form<T, kRowsKind, DP, kFormColumns8>(p, stream);
     }
     return launch_form<T, kRowsKind, DP, kFormAny>(p, stream);
 }
