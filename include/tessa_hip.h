@@ -941,7 +941,8 @@ uint32_t tessa_abi_version(void);
  * of fraction (0, 0.5, 1, 1.5, 2, 3, 4, 6), and for each 32 dims a byte e, value = 2^(e - 127) * code
  * (head_dim a multiple of 32).  e makes max|x| round to 6 at most: with max|x| = m 2^k, 1 <= m < 2, e is
  * 127 + k - 2, or one more from m = 1.75 on, held in 2..252; codes are the nearest, ties to the even code.  32 dims of which one is not
- * finite have e = 255 and are NaN.  Strides are between pages, heads and rows, in
+ * finite have e = 255 and are NaN.  (Rows from elsewhere may have e of 0 and 1 too; attention over e of 253 and 254, whose
+ * values pass f32's range, is not defined.)  Strides are between pages, heads and rows, in
  * elements (of 4 bits for MX4); rows are contiguous and 16-byte aligned.  Nothing here allocates,
  * waits for the device or keeps anything between calls: results are queued on
  * `stream`, scratch is the caller's, and the calls may be captured in a graph.

@@ -11,8 +11,8 @@ namespace tessa {
 // reciprocal: x * (1/scale), corrected once by its remainder (Markstein's method),
 // is the rounded quotient for every pair of 11-bit significands of the maximum and
 // of x (tests/test_kv_quotient.py goes through all of them; powers of two change
-// nothing in this range), at half the instructions: with a division each the
-// prompts above took 27 us.
+// nothing in this range), at half the instructions: with a division each, an append
+// of 4 prompts of up to 4,096 tokens, 8 heads of 128, took 27 us, so 21.
 constexpr uint32_t kQuickTop = 0x20000000u;
 
 // A lane's 8 values as SQ8: the codes, and the row's scale (a row of 2^lanes_log2 lanes).

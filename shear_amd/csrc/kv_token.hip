@@ -21,7 +21,7 @@
 //   48 sequences of up to 4,100 rows, with weights   533 MB   115 + 14 us   4.1 TB/s
 //   8 of up to 40,000 SQ8 rows, with weights         522 MB   122 + 15 us   3.8 TB/s
 //   one of 131,071 rows                              268 MB    52 +  7 us   4.5 TB/s
-//   64 of up to 8,200 rows of 4 bits                 372 MB    75 +  9 us   4.4 TB/s
+//   64 of up to 8,200 rows of 4 bits                 372 MB    76 +  9 us   4.4 TB/s
 //   3 of up to 131,071, 4 bits, 4 heads, weights     170 MB    49 + 16 us   2.6 TB/s
 //   16, 2,016 rows each of which 1,500 are listed     49 MB    17 +  5 us   2.3 TB/s
 // (a copy reaches 4.9 to 5.5 TB/s here).  The last is a chain of dependent

@@ -321,8 +321,8 @@ def attend_prompt(q: torch.Tensor, offsets: torch.Tensor, cache: KvCache, page_t
     new tokens of each sequence: tokens ``offsets[b]``..``offsets[b + 1]`` of q are
     its last rows, each seeing rows up to its own (with ``window``: the first
     ``sinks`` and its last ``window``).  Their keys and values are in the cache
-    already; ``offsets`` cover all tokens.  ``max_new``: no sequence has more new
-    tokens (default: all of them)."""
+    already; ``offsets`` cover all tokens (places past the last that they cover
+    are not written).  ``max_new``: no sequence has more new tokens (default: all of them)."""
     return _attend(cache, q, page_table, lengths, max_length, scale, sinks, window, stream, offsets=offsets,
                    max_new=max_new, prompt=True)
 
